@@ -14,6 +14,8 @@ DTYPE_F16, DTYPE_Q8, DTYPE_Q4 = 0, 1, 2
 WANT_LOGITS, WANT_HIDDEN, WANT_LABELS, WANT_LABELS_LSE = 0, 1, 2, 3
 SRC_NONE, SRC_RESIDENT, SRC_RAM, SRC_DISK, SRC_DECODED = 0, 1, 2, 3, 4
 ROLE_NONE, ROLE_OPT, ROLE_DECIDE = 0, 1, 2
+ELEM_F16, ELEM_BF16, ELEM_F32 = 0, 1, 2
+ROPE_HALF, ROPE_INTERLEAVED, ROPE_HEAD_HALF = 0, 1, 2
 
 
 class OmgError(RuntimeError):
@@ -41,6 +43,24 @@ class omg_config_t(C.Structure):
     _fields_ = [("vocab", C.c_uint32), ("d", C.c_uint32), ("layers", C.c_uint32), ("heads", C.c_uint32),
                 ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32), ("bos", C.c_uint32),
                 ("capacity", C.c_uint64), ("max_rows", C.c_uint64)]
+
+
+class omg_paged_kv(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("kv_heads", C.c_int), ("head_dim", C.c_int), ("page", C.c_int),
+                ("npages", C.c_int64), ("page_stride", C.c_int64), ("k", C.c_void_p), ("v", C.c_void_p)]
+
+
+class omg_paged_batch(C.Structure):
+    _fields_ = [("nseq", C.c_int64), ("t", C.c_int64), ("lens", C.c_void_p), ("table", C.c_void_p),
+                ("table_ld", C.c_int64), ("max_pages", C.c_int64), ("start", C.c_void_p),
+                ("prefix_table", C.c_void_p), ("prefix_len", C.c_int64)]
+
+
+class omg_kv_source(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("heads", C.c_int), ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p),
+                ("ld", C.c_int64), ("ldkv", C.c_int64), ("rope", C.c_void_p), ("rope_rows", C.c_int64),
+                ("rope_dims", C.c_int), ("rope_layout", C.c_int), ("positions", C.c_void_p), ("q_norm", C.c_void_p),
+                ("k_norm", C.c_void_p), ("v_norm", C.c_int), ("eps", C.c_float), ("q_scale", C.c_float)]
 
 
 class omg_laya_seq(C.Structure):
@@ -124,6 +144,8 @@ _SIGS = {
     "omg_dev_qkv_heads": (C.c_int, [_P, _P, C.c_int64, C.c_int64, _P, _P, _P, C.c_float, C.c_int64, _P, _P, _P,
                                     _P]),
     "omg_dev_attention_bi": (C.c_int, [_P, _P, _P, _P, C.c_int, C.c_int64, C.c_int64, C.c_int, _P, _P]),
+    "omg_dev_kv_append": (C.c_int, [C.POINTER(omg_paged_kv), C.POINTER(omg_paged_batch), C.POINTER(omg_kv_source), _P,
+                                    C.c_int64, _P]),
     "omg_laya_builder_new": (_P, [C.c_char_p]),
     "omg_laya_builder_push": (C.c_int, [_P, C.c_char_p, C.c_int, C.POINTER(C.c_int64), C.c_size_t, _P, C.c_size_t,
                                         _P, C.c_size_t]),

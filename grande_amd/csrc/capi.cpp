@@ -660,6 +660,36 @@ int omg_dev_attention_bi(const void* q16, const void* k16, const void* vt, const
     });
 }
 
+/* ---- carrying answers on token by token ---- */
+
+namespace {
+
+omg::PagedKv paged_kv(const omg_paged_kv* kv) {
+    if (!kv) omg::fail(omg::E_INVALID, "null paged cache");
+    return {kv->dtype,   kv->kv_heads, kv->head_dim,
+            kv->page,    kv->npages,   kv->page_stride ? kv->page_stride : int64_t(kv->kv_heads) * kv->page * kv->head_dim,
+            kv->k,       kv->v};
+}
+
+omg::PagedBatch paged_batch(const omg_paged_batch* b) {
+    if (!b) omg::fail(omg::E_INVALID, "null batch");
+    return {b->nseq, b->t, b->lens, b->table, b->table_ld, b->max_pages, b->start, b->prefix_table, b->prefix_len};
+}
+
+}  // namespace
+
+int omg_dev_kv_append(const omg_paged_kv* kv, const omg_paged_batch* b, const omg_kv_source* src, void* q_out,
+                      int64_t ldq, void* stream) {
+    return guard([&] {
+        if (!src) omg::fail(omg::E_INVALID, "null source");
+        const omg::KvSource s{src->dtype,     src->heads,       src->q,         src->k,      src->v,
+                              src->ld,        src->ldkv,        src->rope,      src->rope_rows, src->rope_dims,
+                              src->rope_layout, src->positions, src->q_norm,    src->k_norm, src->v_norm,
+                              src->eps,       src->q_scale};
+        omg::launch_kv_append(static_cast<hipStream_t>(stream), paged_kv(kv), paged_batch(b), s, q_out, ldq);
+    });
+}
+
 /* ---- the bidirectional encoder path ---- */
 
 omg_laya_builder* omg_laya_builder_new(const char* config_json) {

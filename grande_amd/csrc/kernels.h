@@ -301,4 +301,36 @@ void launch_attention(hipStream_t s, const AttnArgs& a, const int4* items, int64
 // The chunk merges of the split query tiles (after launch_attention).
 void launch_attention_merge(hipStream_t s, const AttnArgs& a, const int4* merges, int64_t nmerges, int nw);
 
+
+// ---- paged cache (paged.hip) ----
+// The C ABI's descriptions (include/omg_hip.h: omg_paged_kv,
+// omg_paged_batch, omg_kv_source) with their defaults filled in.
+constexpr int ELEM_F16 = 0, ELEM_BF16 = 1, ELEM_F32 = 2;
+struct PagedKv {
+    int dtype, kv_heads, head_dim, page;
+    int64_t npages, page_stride;
+    void *k, *v;
+};
+struct PagedBatch {
+    int64_t nseq, t;
+    const int32_t *lens, *table;
+    int64_t table_ld, max_pages;
+    const int32_t *start, *prefix_table;
+    int64_t prefix_len;
+};
+struct KvSource {
+    int dtype, heads;
+    const void *q, *k, *v;
+    int64_t ld, ldkv;
+    const float* rope;
+    int64_t rope_rows;
+    int rope_dims, rope_layout;
+    const int32_t* positions;
+    const float *q_norm, *k_norm;
+    int v_norm;
+    float eps, q_scale;
+};
+void launch_kv_append(hipStream_t s, const PagedKv& kv, const PagedBatch& b, const KvSource& src, void* q_out,
+                      int64_t ldq);
+
 }  // namespace omg

@@ -517,3 +517,50 @@ def attention_bi(q_ptr: int, k_ptr: int, vt_ptr: int, meta_ptr: int, heads: int,
                  out_ptr: int, stream: int | None = None) -> None:
     """The encoder path's attention kernel on device pointers."""
     L.check(L.lib().omg_dev_attention_bi(q_ptr, k_ptr, vt_ptr, meta_ptr, heads, t, tpad, window, out_ptr, stream))
+
+
+# ---- carrying answers on token by token: a paged K/V cache, on device pointers ----
+
+class PagedBatch(L.omg_paged_batch):
+    """The sequences of one step (omg_paged_batch): `tokens` new token rows
+    in all, int32 device arrays `lens` [nseq] (rows of each sequence in the
+    cache, the new ones included), `table` [nseq][table_ld] (its pages, the
+    first max_pages of each row in use), `start` [nseq + 1] (the token rows
+    of sequence s are start[s] .. start[s + 1]; None: one token each) and
+    `prefix_table` (the pages of the `prefix_len` rows that come before
+    every sequence)."""
+
+    def __init__(self, nseq: int, tokens: int, lens_ptr: int, table_ptr: int, max_pages: int,
+                 start_ptr: int | None = None, prefix_table_ptr: int | None = None, prefix_len: int = 0,
+                 table_ld: int = 0):
+        super().__init__(nseq, tokens, lens_ptr, table_ptr, table_ld or max_pages, max_pages, start_ptr,
+                         prefix_table_ptr, prefix_len)
+
+
+class KvSource(L.omg_kv_source):
+    """The rows an append takes (omg_kv_source): q heads at q_ptr, k and v
+    heads at k_ptr and v_ptr (None: left out), `ld` elements from token to
+    token (`ldkv` for k and v where it differs), with what happens to them
+    on the way: RMS norms, the rotation and the queries' scale."""
+
+    def __init__(self, dtype: int, heads: int, q_ptr: int | None, k_ptr: int | None, v_ptr: int | None, ld: int,
+                 ldkv: int = 0, *, rope: int | None = None, rope_rows: int = 0, rope_dims: int = 0,
+                 rope_layout: int = L.ROPE_HALF, positions: int | None = None, q_norm: int | None = None,
+                 k_norm: int | None = None, v_norm: bool = False, eps: float = 1e-6, q_scale: float = 1.0):
+        super().__init__(dtype, heads, q_ptr, k_ptr, v_ptr, ld, ldkv or ld, rope, rope_rows, rope_dims, rope_layout,
+                         positions, q_norm, k_norm, v_norm, eps, q_scale)
+
+
+class PagedKv(L.omg_paged_kv):
+    """A pool of K/V pages [npages][kv_heads][page][head_dim] at k_ptr and
+    v_ptr (omg_paged_kv).  The memory is the caller's."""
+
+    def __init__(self, k_ptr: int, v_ptr: int, npages: int, kv_heads: int, page: int, head_dim: int, dtype: int,
+                 page_stride: int = 0):
+        super().__init__(dtype, kv_heads, head_dim, page, npages, page_stride, k_ptr, v_ptr)
+
+    def append(self, batch: PagedBatch, src: KvSource, q_out_ptr: int | None = None, ldq: int = 0,
+               stream: int | None = None) -> None:
+        """omg_dev_kv_append: the step's keys and values into the cache, its
+        queries into q_out."""
+        L.check(L.lib().omg_dev_kv_append(self, batch, src, q_out_ptr, ldq, stream))

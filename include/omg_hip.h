@@ -312,6 +312,84 @@ int omg_dev_qkv_heads(const omg_weight *w, const void *x_f16, int64_t ldx, int64
 int omg_dev_attention_bi(const void *q16, const void *k16, const void *vt, const int32_t *meta, int heads, int64_t t,
                          int64_t tpad, int window, void *out_f16, void *stream);
 
+/* ---- carrying answers on token by token (no counterpart in the reference,
+ * whose answers are read at given positions) ----
+ * A paged K/V cache, the append that fills it and the attention that reads
+ * it, on device pointers, asynchronous on `stream` (NULL = the null stream)
+ * of the current device, which holds the buffers.  Nothing is allocated and
+ * nothing is kept between calls: every call can be captured into a HIP
+ * graph.  Element types of matrices and caches: */
+#define OMG_ELEM_F16 0
+#define OMG_ELEM_BF16 1
+#define OMG_ELEM_F32 2 /* sources and logits only, not caches */
+
+/* A pool of pages of K/V rows: row r (0 <= r < page) of KV head g on page p
+ * at element p * page_stride + (g * page + r) * head_dim of `k` and of `v`.
+ * head_dim 64, 128, 256 or 512; page 16, 32, 64, 128 or 256 rows;
+ * page_stride 0 = kv_heads * page * head_dim, else at least that and a
+ * multiple of 8; k and v 16-byte aligned. */
+typedef struct {
+    int dtype; /* OMG_ELEM_F16 or OMG_ELEM_BF16 */
+    int kv_heads, head_dim, page;
+    int64_t npages, page_stride;
+    void *k, *v;
+} omg_paged_kv;
+
+/* A batch of sequences with t new tokens in all, as int32 device arrays:
+ * sequence s has the token rows [start[s], start[s + 1]) (start NULL: row s,
+ * then t = nseq) and, these included, lens[s] rows of its own in the cache;
+ * row i is row i % page of page table[s * table_ld + i / page], for
+ * i / page < max_pages.  Its new tokens are the last of its rows.  All
+ * sequences follow a shared prefix of prefix_len rows on the pages
+ * prefix_table[i / page] (prefix_len 0: none): row i of a sequence has the
+ * position prefix_len + i.
+ *
+ * The device arrays are not checked before the launch.  What they name
+ * outside their arrays is left out: keys on a page outside [0, npages) or
+ * past max_pages are seen by no query and written by no append, and token
+ * rows that no sequence has (rows behind the last sequence's) leave their
+ * outputs as they were.  start must not descend.  Two sequences may share
+ * pages; a cache row that two tokens of one append name is left with the
+ * elements of either. */
+typedef struct {
+    int64_t nseq, t;
+    const int32_t *lens, *table;
+    int64_t table_ld, max_pages;
+    const int32_t *start;        /* [nseq + 1] or NULL */
+    const int32_t *prefix_table; /* [ceil(prefix_len / page)] */
+    int64_t prefix_len;
+} omg_paged_batch;
+
+/* What an append takes its rows from: for token row i, head h and column c
+ * element i * ld + h * head_dim + c of q (heads of them; NULL: no queries)
+ * and i * ldkv + h * head_dim + c of k and v (kv_heads of them; both NULL:
+ * no keys and values, a layer that reads another's cache).  Pointers 16-byte
+ * aligned, ld and ldkv whole 16 bytes. */
+#define OMG_ROPE_HALF 0        /* pairs (i, i + rope_dims / 2), i < rope_dims / 2 */
+#define OMG_ROPE_INTERLEAVED 1 /* pairs (2 i, 2 i + 1) */
+#define OMG_ROPE_HEAD_HALF 2   /* pairs (i, i + head_dim / 2), i < rope_dims / 2 */
+typedef struct {
+    int dtype, heads; /* OMG_ELEM_F32, or the cache's type */
+    const void *q, *k, *v;
+    int64_t ld, ldkv;
+    const float *rope; /* [rope_rows][rope_dims / 2] (cos, sin) pairs; NULL: no rotation */
+    int64_t rope_rows;
+    int rope_dims, rope_layout;  /* rope_dims a multiple of 16, at most head_dim */
+    const int32_t *positions;    /* [t] rows of the table; NULL: the tokens' positions */
+    const float *q_norm, *k_norm; /* [head_dim] RMS norm weights (any offset included); NULL: no norm */
+    int v_norm;                  /* != 0: v rows normed, without weights */
+    float eps, q_scale;
+} omg_kv_source;
+
+/* Per token: q heads normed, rotated, times q_scale into q_out (row stride
+ * ldq elements, a multiple of 8; the cache's type); k heads normed and
+ * rotated and v heads (normed) into the token's cache row.  f32 arithmetic,
+ * one rounding.  Positions outside the table count as its first or last
+ * row.  q_out may be the source's own q rows where type and stride are the
+ * same. */
+int omg_dev_kv_append(const omg_paged_kv *kv, const omg_paged_batch *b, const omg_kv_source *src, void *q_out,
+                      int64_t ldq, void *stream);
+
 /* ---- the bidirectional encoder path (crates/omg-wgpu/src/laya.rs) ----
  * An mmBERT / ModernBERT encoder with Laya's decision head: every question
  * is one sequence; a request's sequences run as one packed pass isolated by

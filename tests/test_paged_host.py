@@ -1,0 +1,71 @@
+"""What the paged-cache and sampling calls refuse before any launch: bad
+shapes, strides, alignments and types, on the host alone (the pointers are
+never followed)."""
+from __future__ import annotations
+
+import pytest
+
+import grande_amd as g
+
+P = 1 << 20  # an aligned address that is never followed
+
+
+def kv(**over):
+    a = dict(k_ptr=P, v_ptr=P, npages=8, kv_heads=2, page=16, head_dim=64, dtype=g.ELEM_F16)
+    a.update(over)
+    return g.PagedKv(**a)
+
+
+def batch(**over):
+    a = dict(nseq=3, tokens=3, lens_ptr=P, table_ptr=P, max_pages=4)
+    a.update(over)
+    return g.PagedBatch(**a)
+
+
+def source(**over):
+    a = dict(dtype=g.ELEM_F32, heads=4, q_ptr=P, k_ptr=P, v_ptr=P, ld=512)
+    a.update(over)
+    return g.KvSource(**a)
+
+
+BAD_KV = [(dict(dtype=g.ELEM_F32), "f16 or bf16"), (dict(head_dim=96), "head_dim"), (dict(kv_heads=0), "kv_heads"),
+          (dict(page=24), "page"), (dict(npages=0), "npages"), (dict(page_stride=64), "page_stride"),
+          (dict(page_stride=16 * 128 + 4), "page_stride"), (dict(k_ptr=P + 2), "aligned"), (dict(v_ptr=None), "aligned")]
+BAD_BATCH = [(dict(nseq=0), "nseq"), (dict(tokens=0), "nseq"), (dict(lens_ptr=None), "null"),
+             (dict(table_ptr=None), "null"), (dict(tokens=4), "t = nseq"), (dict(max_pages=0), "max_pages"),
+             (dict(table_ld=3), "max_pages"), (dict(prefix_len=-1), "prefix_len"), (dict(prefix_len=5), "prefix_table"),
+             (dict(max_pages=1 << 28), "max_pages")]
+
+
+@pytest.mark.parametrize("over,why", BAD_KV)
+def test_append_refuses_caches(over, why):
+    with pytest.raises(g.OmgError, match=why):
+        kv(**over).append(batch(), source(), P, 256)
+
+
+@pytest.mark.parametrize("over,why", BAD_BATCH)
+def test_append_refuses_batches(over, why):
+    with pytest.raises(g.OmgError, match=why):
+        kv().append(batch(**over), source(), P, 256)
+
+
+@pytest.mark.parametrize("over,q_out,ldq,why", [
+    (dict(dtype=g.ELEM_BF16), P, 256, "cache's type"), (dict(q_ptr=None, k_ptr=None, v_ptr=None), P, 256, "neither"),
+    (dict(v_ptr=None), P, 256, "together"), (dict(q_ptr=P + 4), P, 256, "aligned"), (dict(heads=0), P, 256, "heads"),
+    (dict(), None, 256, "q_out"), (dict(), P, 252, "ldq"), (dict(), P, 260, "ldq"), (dict(ld=255), P, 256, "ld"),
+    (dict(ld=514), P, 256, "ld"), (dict(ldkv=64), P, 256, "ldkv"), (dict(rope=P), P, 256, "rope table"),
+    (dict(rope=P, rope_rows=4, rope_dims=24), P, 256, "rope_dims"),
+    (dict(rope=P, rope_rows=4, rope_dims=80), P, 256, "rope_dims"),
+    (dict(rope=P, rope_rows=4, rope_dims=32, rope_layout=3), P, 256, "layout"),
+    (dict(rope=P + 8, rope_rows=4, rope_dims=32), P, 256, "aligned"), (dict(q_norm=P + 4), P, 256, "aligned")])
+def test_append_refuses_sources(over, q_out, ldq, why):
+    with pytest.raises(g.OmgError, match=why):
+        kv().append(batch(), source(**over), q_out, ldq)
+
+
+def test_append_refuses_null_descriptions():
+    import grande_amd._lib as L
+
+    for args in ((None, batch(), source()), (kv(), None, source()), (kv(), batch(), None)):
+        with pytest.raises(g.OmgError, match="null"):
+            L.check(L.lib().omg_dev_kv_append(*args, P, 256, None))
