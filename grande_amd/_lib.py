@@ -146,6 +146,9 @@ _SIGS = {
     "omg_dev_attention_bi": (C.c_int, [_P, _P, _P, _P, C.c_int, C.c_int64, C.c_int64, C.c_int, _P, _P]),
     "omg_dev_kv_append": (C.c_int, [C.POINTER(omg_paged_kv), C.POINTER(omg_paged_batch), C.POINTER(omg_kv_source), _P,
                                     C.c_int64, _P]),
+    "omg_dev_attention_shared_workspace": (C.c_int64, [C.POINTER(omg_paged_kv), C.POINTER(omg_paged_batch), C.c_int]),
+    "omg_dev_attention_shared": (C.c_int, [C.POINTER(omg_paged_kv), C.POINTER(omg_paged_batch), C.c_int, _P, C.c_int64,
+                                           _P, C.c_int64, _P, C.c_float, C.c_int, _P, C.c_size_t, _P]),
     "omg_laya_builder_new": (_P, [C.c_char_p]),
     "omg_laya_builder_push": (C.c_int, [_P, C.c_char_p, C.c_int, C.POINTER(C.c_int64), C.c_size_t, _P, C.c_size_t,
                                         _P, C.c_size_t]),
@@ -203,3 +206,10 @@ def handle(ptr):
     if not ptr:
         raise OmgError(E_INVALID, last_error())
     return ptr
+
+
+def size(n: int) -> int:
+    """A byte count of the C ABI, or its error."""
+    if n < 0:
+        raise OmgError(n, last_error())
+    return n

@@ -690,6 +690,22 @@ int omg_dev_kv_append(const omg_paged_kv* kv, const omg_paged_batch* b, const om
     });
 }
 
+int64_t omg_dev_attention_shared_workspace(const omg_paged_kv* kv, const omg_paged_batch* b, int heads) {
+    int64_t n = 0;
+    const int rc = guard([&] { n = omg::attention_shared_workspace(paged_kv(kv), paged_batch(b), heads); });
+    return rc == OMG_OK ? n : rc;
+}
+
+int omg_dev_attention_shared(const omg_paged_kv* kv, const omg_paged_batch* b, int heads, const void* q, int64_t ldq,
+                             void* out, int64_t ldo, float* lse, float scale, int window, void* workspace,
+                             size_t workspace_bytes, void* stream) {
+    return guard([&] {
+        const omg::SharedAttn x{heads, q, ldq, out, ldo, lse, scale, window};
+        omg::launch_attention_shared(static_cast<hipStream_t>(stream), paged_kv(kv), paged_batch(b), x, workspace,
+                                     workspace_bytes);
+    });
+}
+
 /* ---- the bidirectional encoder path ---- */
 
 omg_laya_builder* omg_laya_builder_new(const char* config_json) {

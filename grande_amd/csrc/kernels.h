@@ -333,4 +333,20 @@ struct KvSource {
 void launch_kv_append(hipStream_t s, const PagedKv& kv, const PagedBatch& b, const KvSource& src, void* q_out,
                       int64_t ldq);
 
+// Attention over the shared prefix and every sequence's own rows; its
+// workspace's size.
+struct SharedAttn {
+    int heads;
+    const void* q;
+    int64_t ldq;
+    void* out;
+    int64_t ldo;
+    float* lse;
+    float scale;
+    int window;
+};
+int64_t attention_shared_workspace(const PagedKv& kv, const PagedBatch& b, int heads);
+void launch_attention_shared(hipStream_t s, const PagedKv& kv, const PagedBatch& b, const SharedAttn& x,
+                             void* workspace, size_t bytes);
+
 }  // namespace omg

@@ -6,6 +6,12 @@
 
 namespace omg {
 
+// Host checks of the descriptions, shared by the calls that take them (paged.hip).
+bool aligned16(const void* p);
+int log2_of(int64_t n);  // the least s with 2^s >= n
+void check_kv(const PagedKv& kv, const char* who);
+void check_batch(const PagedBatch& b, const PagedKv& kv, const char* who);
+
 typedef __bf16 bf16_t;
 typedef bf16_t bf16x8 __attribute__((ext_vector_type(8)));
 

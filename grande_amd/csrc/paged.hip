@@ -156,8 +156,6 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
     }
 }
 
-namespace {
-
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 int log2_of(int64_t n) {
@@ -193,6 +191,8 @@ void check_batch(const PagedBatch& b, const PagedKv& kv, const char* who) {
     if (b.prefix_len < 0 || b.prefix_len > 0x3fffffff) fail(E_INVALID, w + ": prefix_len out of range");
     if (b.prefix_len > 0 && !b.prefix_table) fail(E_INVALID, w + ": null prefix_table");
 }
+
+namespace {
 
 template <typename S, typename T, int HD>
 void append_hd(hipStream_t s, AppendArgs a) {

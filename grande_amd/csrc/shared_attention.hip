@@ -1,0 +1,772 @@
+// Attention over a prefix that all sequences of a batch share and over each
+// sequence's own rows, both on pages of a K/V pool:
+//   out = sum_j p_j v_j / sum_j p_j,  p_j = 2^(c (s_j - m)),  s_j = q . k_j,
+// c = scale log2(e), m a running maximum of s, over the keys j that the
+// query sees.  Partial results over ranges of keys are joined by
+// (m, l = sum p, O = sum p v): O and l times 2^(c (m - max m)).
+//
+// Queries are rows (token, head) of one KV head, so that a tile of rows
+// takes every key and value it reads once for all of them: tiles of the
+// prefix hold rows of any sequences, tiles of a sequence's own keys its rows
+// alone.  Where sequences bring at least a wave of rows each (prompts,
+// questions) a tile runs through the prefix and then through the own keys
+// of the sequences it holds (`fused`); where they bring a few (a step of
+// decoding) the own keys have work items of their own, in the same launch.
+// Few tiles split the keys over work items; attention_join joins these.
+//
+// Tiles (MFMA shape = rows of a wave x keys):
+//   WAVES_ROWS 32: 4 waves x 32 rows, 32-key K and V tiles shared in LDS,
+//                  two buffers, the next tile's loads in flight;
+//   WAVES_ROWS 16: 4 waves x 16 rows, the same (head_dim 512, few rows);
+//   WAVES_KEYS:    16 rows, each wave takes every fourth 16-key tile into
+//                  LDS of its own; the waves join through LDS at the end.
+// Both products leave the query in the lane: S^T = K Q^T with the lane's
+// query as column, then O^T += V^T P^T, whose P^T operand is the lane's own
+// scores; V^T comes from row-major V by LDS transposing reads of 4 keys.
+//
+// K and V tiles come by buffer loads to LDS, 16 bytes a lane, from a
+// resource that ends with the last valid row of the page (rows behind it
+// and pages outside the pool arrive as zeros, so that nothing they hold
+// meets a probability of zero).  The 16-byte chunks of row r are XORed with
+// r (K: the 16 rows of an operand read on distinct banks) and with 2 r (V:
+// the 4 rows x 32 bytes of a transposing read).
+#include <algorithm>
+#include <climits>
+#include <string>
+
+#include "common.h"
+#include "kern_common.h"
+#include "paged.h"
+
+namespace omg {
+
+namespace {
+
+enum Tile { WAVES_KEYS = 0, WAVES_16 = 1, WAVES_32 = 2 };
+
+struct Plan {
+    int tile;       // Tile of the prefix / fused items
+    bool fused;     // own keys in the prefix items' tiles
+    bool whole;     // fused and not split: prefix and own keys in one item
+    int ntile, np, chunk_p;            // prefix: row tiles, splits, keys per split
+    int64_t own_tiles;                 // bound of the sequences' 16-row tiles (not fused)
+    int os, chunk_o;                   // own keys: splits, keys per split
+    __host__ __device__ int64_t slots() const { return whole ? 1 : np + os; }
+};
+
+struct Args {
+    PagedKv kv;
+    PagedBatch b;
+    SharedAttn x;
+    Plan p;
+    int hpg, page_shift;
+    int64_t max_len;           // rows a table reaches
+    int64_t prefix_blocks;     // (a multiple of 8)
+    float c;                   // scale log2(e)
+    float* part_o;             // [slots][t * heads][head_dim], null: results go out
+    float2* part_ml;           // [slots][t * heads] (c m, l)
+};
+
+typedef __attribute__((address_space(3))) void* lds_ptr;
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef short short8v __attribute__((ext_vector_type(8)));
+
+__device__ inline floatx16 mfma32(half8 a, half8 b, floatx16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ inline floatx16 mfma32(bf16x8 a, bf16x8 b, floatx16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ inline floatx4 mfma16(half8 a, half8 b, floatx4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ inline floatx4 mfma16(bf16x8 a, bf16x8 b, floatx4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+typedef bf16_t bf16x4 __attribute__((ext_vector_type(4)));
+__device__ inline floatx4 mfma16k16(half4 a, half4 b, floatx4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, c, 0, 0, 0);
+}
+__device__ inline floatx4 mfma16k16(bf16x4 a, bf16x4 b, floatx4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(short4v, a), __builtin_bit_cast(short4v, b), c,
+                                                     0, 0, 0);
+}
+
+// V rows r .. r + 3 of this lane's 16-lane group, one column a lane: lane i
+// of the group gives the address of row i / 4, columns 4 (i % 4) .. + 3 and
+// gets column i of the four rows.
+template <typename T>
+__device__ inline short4v read_tr(const T* p) {
+    typedef __attribute__((address_space(3))) short4v* ptr;
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(p));
+}
+
+template <typename T, int D, int TILE>
+struct Core {
+    static constexpr int RW = TILE == WAVES_32 ? 32 : 16;      // rows of a wave
+    static constexpr int KT = TILE == WAVES_KEYS ? 16 : 32;    // keys of a tile
+    static constexpr int KS = RW == 32 ? 16 : 32;              // head dims per MFMA of K Q^T
+    static constexpr int NS = D / KS, NC = D / RW;
+    static constexpr int NB = KT / RW < 1 ? 1 : KT / RW;       // score blocks
+    static constexpr int SR = RW == 32 ? 16 : 4;               // scores of a lane per block
+    static constexpr int CH = D / 8;                           // 16-byte chunks of a row
+    typedef typename Vec8<T>::type frag;
+    typedef std::conditional_t<RW == 32, floatx16, floatx4> acc;
+
+    frag q[NS];
+    acc o[NC];
+    float m, l;  // running maximum of the raw scores; the lane's share of sum p
+
+    static __device__ int swz_k(int row) { return CH >= 16 ? row & 15 : row & 7; }
+    static __device__ int swz_v(int row) { return CH >= 16 ? (row & 7) << 1 : (row & 3) << 1; }
+    // The tile's key of score r of block j.
+    static __device__ int key_of(int lane, int j, int r) {
+        return RW == 32 ? 8 * (r / 4) + 4 * (lane / 32) + r % 4 : 16 * j + 4 * (lane / 16) + r;
+    }
+    static __device__ float row_max(float v) {
+        if constexpr (RW == 32) {
+            const uint32_t u = __builtin_bit_cast(uint32_t, v);
+            const auto p = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+            return fmaxf(__builtin_bit_cast(float, uint32_t(p[0])), __builtin_bit_cast(float, uint32_t(p[1])));
+        } else {
+            return max_lanes_16_32(v);
+        }
+    }
+    static __device__ float row_sum(float v) {
+        if constexpr (RW == 32) {
+            const uint32_t u = __builtin_bit_cast(uint32_t, v);
+            const auto p = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+            return __builtin_bit_cast(float, uint32_t(p[0])) + __builtin_bit_cast(float, uint32_t(p[1]));
+        } else {
+            return sum_lanes_16_32(v);
+        }
+    }
+
+    __device__ void init(const T* row, int lane) {
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            frag z{};
+            q[s] = row ? *reinterpret_cast<const frag*>(row + s * KS + 8 * (lane / RW)) : z;
+        }
+#pragma unroll
+        for (int i = 0; i < NC; ++i)
+#pragma unroll
+            for (int r = 0; r < SR; ++r) o[i][r] = 0.0f;
+        m = -INFINITY;
+        l = 0.0f;
+    }
+
+    // One tile whose first key is k0; the lane's query sees the keys lo ..
+    // hi - 1 that are not in `bad` (a bit per key of the tile).
+    __device__ void tile(const T* K, const T* V, int lane, int k0, bool full, int lo, int hi, uint32_t bad, float c) {
+        acc s[NB];
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+            for (int r = 0; r < SR; ++r) s[j][r] = 0.0f;
+        const int kr = lane % RW;
+#pragma unroll
+        for (int st = 0; st < NS; ++st)
+#pragma unroll
+            for (int j = 0; j < NB; ++j) {
+                const int row = j * RW + kr, ch = (st * (KS / 8) + lane / RW) ^ swz_k(row);
+                const frag kf = *reinterpret_cast<const frag*>(K + row * D + ch * 8);
+                if constexpr (RW == 32)
+                    s[j] = mfma32(kf, q[st], s[j]);
+                else
+                    s[j] = mfma16(kf, q[st], s[j]);
+            }
+        if (!full) {
+#pragma unroll
+            for (int j = 0; j < NB; ++j)
+#pragma unroll
+                for (int r = 0; r < SR; ++r) {
+                    const int kk = key_of(lane, j, r), key = k0 + kk;
+                    const bool see = key >= lo && key < hi && !(bad >> kk & 1u);
+                    s[j][r] = see ? s[j][r] : -INFINITY;
+                }
+        }
+        float mt = s[0][0];
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+            for (int r = 0; r < SR; ++r) mt = fmaxf(mt, s[j][r]);
+        mt = row_max(mt);
+        // The maximum moves where a row's scores pass it by more than 2^8 in
+        // p: p and l stay far from f16's and f32's ends either way.
+        if (__any((mt - m) * c > 8.0f || (m == -INFINITY && mt > m))) {
+            const float mn = fmaxf(m, mt);
+            const float al = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * c);
+            m = mn;
+            l *= al;
+#pragma unroll
+            for (int i = 0; i < NC; ++i)
+#pragma unroll
+                for (int r = 0; r < SR; ++r) o[i][r] *= al;
+        }
+        const float mc = m == -INFINITY ? 0.0f : m * c;
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+            for (int r = 0; r < SR; ++r) {
+                const float p = __builtin_amdgcn_exp2f(fmaf(s[j][r], c, -mc));
+                s[j][r] = p;
+                sum += p;
+            }
+        l += sum;
+        const int i16 = lane % 16, g16 = lane / 16;
+        if constexpr (RW == 32) {
+            // (two 16-key steps; the lane's keys of step j: 16 j + 4 h + 0 .. 3 and + 8)
+#pragma unroll
+            for (int j = 0; j < KT / 16; ++j) {
+                frag pf;
+#pragma unroll
+                for (int r = 0; r < 8; ++r) pf[r] = T(s[0][8 * j + r]);
+                const int r0 = 16 * j + 4 * (g16 / 2) + i16 / 4;
+#pragma unroll
+                for (int i = 0; i < NC; ++i) {
+                    const int ch = 4 * i + 2 * (g16 % 2) + (i16 % 4) / 2, e = 4 * (i16 % 2);
+                    union {
+                        short4v h[2];
+                        frag f;
+                    } v;
+                    v.h[0] = read_tr(V + r0 * D + (ch ^ swz_v(r0)) * 8 + e);
+                    v.h[1] = read_tr(V + (r0 + 8) * D + (ch ^ swz_v(r0 + 8)) * 8 + e);
+                    o[i] = mfma32(v.f, pf, o[i]);
+                }
+            }
+        } else if constexpr (KT == 32) {
+            frag pf;
+#pragma unroll
+            for (int r = 0; r < 8; ++r) pf[r] = T(s[r / 4][r % 4]);
+            const int r0 = 4 * g16 + i16 / 4;
+#pragma unroll
+            for (int i = 0; i < NC; ++i) {
+                const int ch = 2 * i + (i16 % 4) / 2, e = 4 * (i16 % 2);
+                union {
+                    short4v h[2];
+                    frag f;
+                } v;
+                v.h[0] = read_tr(V + r0 * D + (ch ^ swz_v(r0)) * 8 + e);
+                v.h[1] = read_tr(V + (r0 + 16) * D + (ch ^ swz_v(r0 + 16)) * 8 + e);
+                o[i] = mfma16(v.f, pf, o[i]);
+            }
+        } else {
+            typedef T frag4 __attribute__((ext_vector_type(4)));
+            frag4 pf;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) pf[r] = T(s[0][r]);
+            const int r0 = 4 * g16 + i16 / 4;
+#pragma unroll
+            for (int i = 0; i < NC; ++i) {
+                const int ch = 2 * i + (i16 % 4) / 2, e = 4 * (i16 % 2);
+                const short4v v = read_tr(V + r0 * D + (ch ^ swz_v(r0)) * 8 + e);
+                o[i] = mfma16k16(__builtin_bit_cast(frag4, v), pf, o[i]);
+            }
+        }
+    }
+    // The lane's four consecutive head dims of output quad (i, rr).
+    static constexpr int QUADS = SR / 4;
+    static __device__ int dim_of(int lane, int i, int rr) {
+        return RW == 32 ? 32 * i + 8 * rr + 4 * (lane / 32) : 16 * i + 4 * (lane / 16);
+    }
+};
+
+// Where a row's result of slot `slot` goes: the partials, or the output.
+template <typename T>
+struct Sink {
+    const Args& a;
+    int64_t row;    // tok * heads + head
+    int64_t out;    // tok * ldo + head * D
+    int64_t slot;
+    __device__ void stats(float cm, float l) const {
+        if (a.part_o)
+            a.part_ml[slot * a.b.t * a.x.heads + row] = make_float2(cm, l);
+        else if (a.x.lse)
+            a.x.lse[row] = l == 0.0f ? -INFINITY : (cm + __builtin_amdgcn_logf(l)) * 0.69314718055994531f;
+    }
+    template <int D>
+    __device__ void quad(int dim, float4 v, float l) const {
+        if (a.part_o) {
+            if (l != 0.0f)
+                *reinterpret_cast<float4*>(a.part_o + (slot * a.b.t * a.x.heads + row) * D + dim) = v;
+        } else {
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            typedef T vec4 __attribute__((ext_vector_type(4)));
+            *reinterpret_cast<vec4*>(static_cast<T*>(a.x.out) + out + dim) =
+                vec4{T(v.x * inv), T(v.y * inv), T(v.z * inv), T(v.w * inv)};
+        }
+    }
+};
+
+// A value that is the same in every lane, in a scalar register.
+__device__ inline int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+constexpr int NW = 4;
+
+// The keys of one work item's segments, tile by tile, through LDS.
+template <typename T, int D, int TILE>
+struct Stream {
+    typedef Core<T, D, TILE> C;
+    static constexpr bool KEYS = TILE == WAVES_KEYS;
+    static constexpr int KT = C::KT;
+    static constexpr int TILE_ELEMS = KT * D;
+    static constexpr int INS = TILE_ELEMS * 2 / 1024 / (KEYS ? 1 : NW);  // 1 KiB loads per wave for K, and for V
+    static_assert(INS >= 1, "a wave loads at least 1 KiB of a tile");
+
+    const Args& a;
+    int g, wave, lane;
+    T* smem;  // KEYS: [wave][K, V], else [2 buffers][K, V]
+
+    __device__ T* buf(int which) const { return smem + int64_t(KEYS ? wave : which) * 2 * TILE_ELEMS; }
+
+    __device__ void issue(int k0, int klim, T* dst, int p0, int p1) const {
+        // A wave's rows lie in one 16-row half of the tile, so in one page.
+        const int hf = !KEYS && wave >= NW / 2 ? 1 : 0;
+        const int p = hf ? p1 : p0, kk = k0 + 16 * hf;
+        const bool ok = unsigned(p) < unsigned(a.kv.npages);
+        int rows = klim - kk;
+        rows = rows < 0 ? 0 : rows > 16 ? 16 : rows;
+        const int bytes = ok ? rows * D * 2 : 0;
+        const int64_t off = (ok ? p : 0) * a.kv.page_stride + (int64_t(g) * a.kv.page + (kk & (a.kv.page - 1))) * D;
+        const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<T*>(static_cast<const T*>(a.kv.k) + off), (short)0, bytes, 0x00020000);
+        const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<T*>(static_cast<const T*>(a.kv.v) + off), (short)0, bytes, 0x00020000);
+#pragma unroll
+        for (int i = 0; i < INS; ++i) {
+            const int piece = (KEYS ? 0 : wave * INS) + i;
+            const int slot = piece * WAVE + lane, row = slot / C::CH, pc = slot % C::CH;
+            const uint32_t ko = uint32_t(((row & 15) * D + (pc ^ C::swz_k(row)) * 8) * 2);
+            const uint32_t vo = uint32_t(((row & 15) * D + (pc ^ C::swz_v(row)) * 8) * 2);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds_ptr)(dst + piece * 512), 16, ko, 0, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds_ptr)(dst + TILE_ELEMS + piece * 512), 16, vo, 0, 0, 0);
+        }
+    }
+
+    // Keys kb .. ke - 1 (kb a multiple of 32; rows from klim on do not
+    // exist) on the pages table[0 .. plast]; the lane's query sees [lo, hi).
+    // Every wave of the workgroup calls it with the same kb and ke.
+    __device__ void run(C& core, const int32_t* table, int plast, int kb, int ke, int klim, bool valid, int lo,
+                        int hi) const {
+        kb = uni(kb), ke = uni(ke), klim = uni(klim);
+        const int step = KEYS ? NW * KT : KT;
+        int k0 = kb + (KEYS ? wave * KT : 0);
+        const int shift = a.page_shift;
+        auto fetch = [&](int k) {
+            int i = (k + 16 * (lane & 1)) >> shift;
+            return table[i > plast ? plast : i];
+        };
+        if (k0 >= ke) return;  // (no barrier below where waves differ in k0)
+        int pn = fetch(k0);
+        if constexpr (!KEYS) __syncthreads();  // the buffers may still be read for the segment before
+        int p0 = __builtin_amdgcn_readlane(pn, 0), p1 = __builtin_amdgcn_readlane(pn, 1);
+        if constexpr (!KEYS) issue(k0, klim, buf(0), p0, p1);
+        int which = 0;
+        if (!KEYS && k0 + step < ke) pn = fetch(k0 + step);
+        for (; k0 < ke; k0 += step, which ^= 1) {
+            if constexpr (KEYS) {
+                issue(k0, klim, buf(0), p0, p1);
+                if (k0 + step < ke) pn = fetch(k0 + step);
+            }
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            if constexpr (!KEYS) __syncthreads();
+            uint32_t bad = unsigned(p0) < unsigned(a.kv.npages) ? 0u : 0xffffu;
+            if (KT == 32 && unsigned(p1) >= unsigned(a.kv.npages)) bad |= 0xffff0000u;
+            p0 = __builtin_amdgcn_readlane(pn, 0), p1 = __builtin_amdgcn_readlane(pn, 1);
+            if (!KEYS && k0 + step < ke) {
+                issue(k0 + step, klim, buf(which ^ 1), p0, p1);
+                if (k0 + 2 * step < ke) pn = fetch(k0 + 2 * step);
+            }
+            if (__ballot(valid && lo < k0 + KT && hi > k0)) {
+                const bool full = bad == 0 && __all(!valid || (lo <= k0 && hi >= k0 + KT));
+                const T* K = buf(which);
+                core.tile(K, K + TILE_ELEMS, lane, k0, full, lo, hi, bad, a.c);
+            }
+            if constexpr (KEYS) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        }
+    }
+};
+
+__device__ inline int imin(int a, int b) { return a < b ? a : b; }
+__device__ inline int imax(int a, int b) { return a > b ? a : b; }
+
+// A lane's query row.
+struct Row {
+    bool valid;
+    int64_t tok;
+    int head, seq, own;  // own: its row in the sequence's cache rows
+};
+
+// The results of a wave's rows (not KEYS).
+template <typename T, int D, int TILE>
+__device__ inline void emit(const Args& a, Core<T, D, TILE>& core, const Row& r, int lane, int64_t slot) {
+    typedef Core<T, D, TILE> C;
+    const float l = C::row_sum(core.l);
+    if (!r.valid) return;
+    const Sink<T> out{a, r.tok * a.x.heads + r.head, r.tok * a.x.ldo + int64_t(r.head) * D, slot};
+    if (lane < C::RW) out.stats(core.m == -INFINITY ? -INFINITY : core.m * a.c, l);
+#pragma unroll
+    for (int i = 0; i < C::NC; ++i)
+#pragma unroll
+        for (int rr = 0; rr < C::QUADS; ++rr)
+            out.template quad<D>(C::dim_of(lane, i, rr),
+                                 make_float4(core.o[i][4 * rr], core.o[i][4 * rr + 1], core.o[i][4 * rr + 2],
+                                             core.o[i][4 * rr + 3]),
+                                 l);
+}
+
+// The four waves' results for the same 16 rows, joined through LDS.
+template <typename T, int D>
+__device__ inline void emit_keys(const Args& a, Core<T, D, WAVES_KEYS>& core, const Row& r, int lane, int wave,
+                                 int64_t slot, float* smem) {
+    typedef Core<T, D, WAVES_KEYS> C;
+    const float l = C::row_sum(core.l);
+    __syncthreads();  // every wave is done with its tiles
+    float* ml = smem + NW * 16 * D;  // [NW][16] c m, then l
+    float* mine = smem + wave * 16 * D;
+#pragma unroll
+    for (int i = 0; i < C::NC; ++i)
+        *reinterpret_cast<floatx4*>(mine + ((i * 4 + lane / 16) * 16 + lane % 16) * 4) = core.o[i];
+    if (lane < 16) {
+        ml[wave * 16 + lane] = core.m == -INFINITY ? -INFINITY : core.m * a.c;
+        ml[64 + wave * 16 + lane] = l;
+    }
+    __syncthreads();
+    float cm = -INFINITY, w[NW], sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < NW; ++k) cm = fmaxf(cm, ml[k * 16 + lane % 16]);
+#pragma unroll
+    for (int k = 0; k < NW; ++k) {
+        const float x = ml[k * 16 + lane % 16];
+        w[k] = x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x - cm);
+        sum += w[k] * ml[64 + k * 16 + lane % 16];
+    }
+    if (!r.valid) return;
+    const Sink<T> out{a, r.tok * a.x.heads + r.head, r.tok * a.x.ldo + int64_t(r.head) * D, slot};
+    if (wave == 0 && lane < 16) out.stats(cm, sum);
+    for (int c4 = wave * 4 + lane / 16; c4 < D / 4; c4 += NW * 4) {
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int k = 0; k < NW; ++k) {
+            const float4 x = *reinterpret_cast<const float4*>(smem + k * 16 * D + (c4 * 16 + lane % 16) * 4);
+            v.x += w[k] * x.x, v.y += w[k] * x.y, v.z += w[k] * x.z, v.w += w[k] * x.w;
+        }
+        out.template quad<D>(4 * c4, v, sum);
+    }
+}
+
+template <typename T, int D, int TILE>
+__global__ __launch_bounds__(NW * 64, D == 512 ? 1 : 2) void attention_shared_kernel(Args a) {
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem_raw[];
+    T* smem = reinterpret_cast<T*>(smem_raw);
+    const int tid = int(threadIdx.x), lane = tid % WAVE;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
+    const int G = a.kv.kv_heads, H = a.x.heads, hpg = a.hpg, P = int(a.b.prefix_len), w = a.x.window;
+    const int cap = int(a.max_len);
+
+    // The sequence of token `tok`, known to lie in [s0, s1].
+    auto seq_in = [&](int64_t tok, int64_t s0, int64_t s1) {
+        while (s0 < s1) {
+            const int64_t mid = (s0 + s1) / 2;
+            if (a.b.start[mid + 1] <= tok)
+                s0 = mid + 1;
+            else
+                s1 = mid;
+        }
+        return s0;
+    };
+    auto place = [&](Row& r, int64_t s0, int64_t s1) {
+        r.seq = 0, r.own = 0;
+        if (!r.valid) return;
+        if (a.b.start) {
+            const int64_t s = seq_in(r.tok, s0, s1);
+            r.valid = s < a.b.nseq && r.tok >= a.b.start[0];
+            if (!r.valid) return;
+            r.seq = int(s);
+            r.own = a.b.lens[s] - int(a.b.start[s + 1] - r.tok);
+        } else {
+            r.seq = int(r.tok);
+            r.own = a.b.lens[r.tok] - 1;
+        }
+    };
+
+    if (int64_t(blockIdx.x) < a.prefix_blocks) {
+        typedef Core<T, D, TILE> C;
+        constexpr int M = TILE == WAVES_KEYS ? 16 : NW * C::RW;
+        // Consecutive workgroups go to the 8 XCDs in turn: each XCD takes a
+        // run of items, whose tiles share their keys in its L2.
+        const int64_t nsplit = a.p.whole ? 1 : a.p.np + (a.p.fused ? a.p.os : 0);
+        const int64_t items = int64_t(a.p.ntile) * G * nsplit;
+        const int64_t item = (blockIdx.x % 8) * (a.prefix_blocks / 8) + blockIdx.x / 8;
+        if (item >= items) return;
+        const int tile = int(item % a.p.ntile);
+        const int split = uni(int(item / a.p.ntile % nsplit)), g = uni(int(item / a.p.ntile / nsplit));
+        const int64_t rows = a.b.t * hpg, row0 = int64_t(tile) * M;
+        const int64_t R = row0 + (TILE == WAVES_KEYS ? 0 : wave * C::RW) + lane % C::RW;
+        Row r{R < rows, R / hpg, int(g * hpg + R % hpg), 0, 0};
+        const int64_t tok0 = row0 / hpg, tok1 = ((row0 + M < rows ? row0 + M : rows) - 1) / hpg;
+        int64_t s0 = tok0, s1 = tok1;
+        if (a.b.start) {
+            s0 = count_le(a.b.start, a.b.nseq, tok0, lane);
+            s1 = count_le(a.b.start, a.b.nseq, tok1, lane);
+        }
+        place(r, s0, s1);
+        C core;
+        core.init(r.valid ? static_cast<const T*>(a.x.q) + r.tok * a.x.ldq + int64_t(r.head) * D : nullptr, lane);
+        const Stream<T, D, TILE> st{a, g, wave, lane, smem};
+        if (a.p.whole || split < a.p.np) {
+            int kb = a.p.whole ? 0 : split * a.p.chunk_p, ke = a.p.whole ? P : imin(P, kb + a.p.chunk_p);
+            const int lo = w > 0 ? imax(0, P + r.own - w + 1) : 0;
+            if (w > 0) {
+                // the first key that any of the workgroup's rows sees
+                __shared__ int first;
+                if (tid == 0) first = INT_MAX;
+                __syncthreads();
+                if (r.valid) atomicMin(&first, lo);
+                __syncthreads();
+                kb = imax(kb, first == INT_MAX ? ke : first / 32 * 32);
+            }
+            if (kb < ke) st.run(core, a.b.prefix_table, (P - 1) >> a.page_shift, kb, ke, P, r.valid, lo, P);
+        }
+        if (a.p.fused && (a.p.whole || split >= a.p.np)) {
+            const int ob = a.p.whole ? 0 : (split - a.p.np) * a.p.chunk_o;
+            const int oe = a.p.whole ? cap : imin(cap, ob + a.p.chunk_o);
+            for (int64_t s = s0; s <= s1 && s < a.b.nseq; ++s) {
+                // the sequence's tokens of this tile and the keys they see
+                const int64_t b0 = a.b.start ? a.b.start[s] : s, b1 = a.b.start ? a.b.start[s + 1] : s + 1;
+                const int64_t ta = b0 > tok0 ? b0 : tok0, tb = b1 - 1 < tok1 ? b1 - 1 : tok1;
+                if (ta > tb) continue;
+                const int len = a.b.lens[s];
+                const int ra = len - int(b1 - ta), rb = len - int(b1 - tb);
+                const int kb = imax(ob, w > 0 ? imax(0, ra - w + 1) / 32 * 32 : 0);
+                const int ke = imin(oe, rb + 1);
+                if (kb >= ke) continue;
+                const bool here = r.valid && r.seq == int(s);
+                const int lo = here ? (w > 0 ? imax(0, r.own - w + 1) : 0) : 0;
+                const int hi = here ? imin(r.own + 1, cap) : 0;
+                st.run(core, a.b.table + s * a.b.table_ld, int(a.b.max_pages) - 1, kb, ke, imin(len, cap), r.valid, lo,
+                       hi);
+            }
+        }
+        if constexpr (TILE == WAVES_KEYS)
+            emit_keys<T, D>(a, core, r, lane, wave, split, reinterpret_cast<float*>(smem_raw));
+        else
+            emit<T, D, TILE>(a, core, r, lane, split);
+        return;
+    }
+
+    // Own keys of one sequence: 16 of its rows.
+    typedef Core<T, D, WAVES_KEYS> C;
+    const int64_t item = int64_t(blockIdx.x) - a.prefix_blocks;
+    const int split = uni(int(item % a.p.os)), g = uni(int(item / a.p.os % G));
+    const int64_t i = item / a.p.os / G;
+    const int per = (hpg + 15) / 16;  // tiles of a single token
+    int64_t s, tile, b0, b1;
+    if (a.b.start) {
+        // Tile i is of the sequence with start[s] hpg / 16 + s <= i: these
+        // bounds leave ceil(rows / 16) tiles for every sequence.
+        int64_t lo = 0, n = a.b.nseq;
+        while (n > 0) {
+            const int64_t step = (n + WAVE - 1) / WAVE, k = lo + (lane + 1) * step;
+            const int64_t at = k <= lo + n ? k : lo + n;
+            const int cnt = __popcll(__ballot(k <= lo + n && int64_t(a.b.start[at]) * hpg / 16 + at <= i));
+            const int64_t rest = n - cnt * step;
+            lo += cnt * step;
+            n = rest < step - 1 ? rest : step - 1;
+        }
+        s = lo;
+        if (s >= a.b.nseq) return;
+        b0 = a.b.start[s], b1 = a.b.start[s + 1];
+        tile = i - (b0 * hpg / 16 + s);
+    } else {
+        s = i / per, tile = i % per;
+        b0 = s, b1 = s + 1;
+    }
+    if (tile < 0 || tile * 16 >= (b1 - b0) * hpg) return;
+    const int64_t R = tile * 16 + lane % 16;
+    Row r{R < (b1 - b0) * hpg, b0 + R / hpg, int(g * hpg + R % hpg), int(s), 0};
+    r.valid = r.valid && r.tok >= 0 && r.tok < a.b.t;
+    const int len = a.b.lens[s];
+    r.own = len - int(b1 - r.tok);
+    C core;
+    core.init(r.valid ? static_cast<const T*>(a.x.q) + r.tok * a.x.ldq + int64_t(r.head) * D : nullptr, lane);
+    // the keys that the tile's first and last tokens see
+    const int64_t last = (tile * 16 + 15 < (b1 - b0) * hpg ? tile * 16 + 15 : (b1 - b0) * hpg - 1) / hpg;
+    const int ra = len - int(b1 - b0 - tile * 16 / hpg), rb = len - int(b1 - b0 - last);
+    const int kb = imax(split * a.p.chunk_o, w > 0 ? imax(0, ra - w + 1) / 32 * 32 : 0);
+    const int ke = imin(imin(cap, (split + 1) * a.p.chunk_o), rb + 1);
+    const Stream<T, D, WAVES_KEYS> st{a, g, wave, lane, smem};
+    if (kb < ke)
+        st.run(core, a.b.table + s * a.b.table_ld, int(a.b.max_pages) - 1, kb, ke, imin(len, cap), r.valid,
+               w > 0 ? imax(0, r.own - w + 1) : 0, imin(r.own + 1, cap));
+    emit_keys<T, D>(a, core, r, lane, wave, a.p.np + split, reinterpret_cast<float*>(smem_raw));
+}
+
+// out = sum_i w_i O_i / sum_i w_i l_i, w_i = 2^(c m_i - max): one wave per
+// (token, head), D / 64 values a lane.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void attention_join_kernel(Args a) {
+    constexpr int E = D / WAVE;
+    const int lane = int(threadIdx.x) % WAVE;
+    const int64_t rows = a.b.t * a.x.heads;
+    const int64_t row = int64_t(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(int(threadIdx.x) / WAVE);
+    if (row >= rows) return;
+    const int64_t tok = row / a.x.heads, head = row - tok * a.x.heads;
+    if (token_row(a.b, tok, lane).seq < 0) return;
+    const int slots = int(a.p.slots());
+    float cm = -INFINITY;
+    for (int i = lane; i < slots; i += WAVE) cm = fmaxf(cm, a.part_ml[i * rows + row].x);
+    cm = wave_max(cm);
+    float l = 0.0f, v[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = 0.0f;
+    for (int i0 = 0; i0 < slots; i0 += WAVE) {
+        float wl = 0.0f;
+        if (i0 + lane < slots) {
+            const float2 ml = a.part_ml[(i0 + lane) * rows + row];
+            wl = ml.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(ml.x - cm);
+            l += wl * ml.y;
+        }
+        const int n = slots - i0 < WAVE ? slots - i0 : WAVE;
+#pragma unroll 4
+        for (int i = 0; i < n; ++i) {
+            const float f = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wl), i));
+            if (f == 0.0f) continue;  // (its O was not written)
+            const float* o = a.part_o + (int64_t(i0 + i) * rows + row) * D + lane * E;
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[e] += f * o[e];
+        }
+    }
+    l = wave_sum(l);
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    T* out = static_cast<T*>(a.x.out) + tok * a.x.ldo + head * D + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; ++e) out[e] = T(v[e] * inv);
+    if (lane == 0 && a.x.lse) a.x.lse[row] = l == 0.0f ? -INFINITY : (cm + __builtin_amdgcn_logf(l)) * 0.69314718055994531f;
+}
+
+int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+
+// Work items fill the chip's 256 CUs twice (head_dim 512: once, by LDS)
+// where the keys are long enough to be split.
+Plan plan(const PagedKv& kv, const PagedBatch& b, int heads) {
+    Plan p{};
+    const int64_t hpg = heads / kv.kv_heads, rows = b.t * hpg, max_len = b.max_pages * kv.page, P = b.prefix_len;
+    const int64_t target = kv.head_dim == 512 ? 256 : 512;
+    p.fused = rows >= 32 * b.nseq;
+    if (!p.fused && rows <= 16)
+        p.tile = WAVES_KEYS;
+    else
+        p.tile = rows <= 64 || kv.head_dim == 512 ? WAVES_16 : WAVES_32;
+    const int64_t M = p.tile == WAVES_KEYS ? 16 : p.tile == WAVES_16 ? 64 : 128;
+    p.ntile = int((rows + M - 1) / M);
+    const int64_t base = p.ntile * int64_t(kv.kv_heads);
+    auto splits = [&](int64_t keys, int64_t items, int64_t least, int& n, int& chunk) {
+        int64_t k = std::min(std::max<int64_t>(1, target / std::max<int64_t>(1, items)), (keys + least - 1) / least);
+        k = std::max<int64_t>(1, std::min<int64_t>(k, 64));
+        chunk = int(up((keys + k - 1) / k, 32));
+        n = int((keys + chunk - 1) / chunk);
+    };
+    p.os = 1, p.chunk_o = int(std::min<int64_t>(up(max_len, 32), INT_MAX / 2));
+    if (p.fused) {
+        p.whole = base * 2 >= target;
+        if (!p.whole) {
+            if (P > 0) splits(P, base, 256, p.np, p.chunk_p);
+            splits(max_len, base, 256, p.os, p.chunk_o);
+        }
+        return p;
+    }
+    if (P > 0) splits(P, base, 256, p.np, p.chunk_p);
+    const int64_t per = (hpg + 15) / 16;
+    p.own_tiles = b.start ? rows / 16 + b.nseq : b.nseq * per;
+    splits(max_len, p.own_tiles * kv.kv_heads, 256, p.os, p.chunk_o);
+    return p;
+}
+
+void check(const PagedKv& kv, const PagedBatch& b, int heads) {
+    check_kv(kv, "attention_shared");
+    check_batch(b, kv, "attention_shared");
+    if (heads <= 0 || heads > 4096 || heads % kv.kv_heads)
+        fail(E_INVALID, "attention_shared: heads must be a multiple of kv_heads, at most 4096");
+}
+
+int64_t part_bytes(const Plan& p, const PagedKv& kv, const PagedBatch& b, int heads) {
+    const int64_t n = p.slots();
+    return n <= 1 ? 0 : n * b.t * heads * (kv.head_dim * 4 + 8);
+}
+
+template <typename T, int D>
+void launch_d(hipStream_t s, const Args& a, unsigned blocks) {
+    // tiles: 2 buffers x 32 keys, or 4 waves x 16 keys, of K and V; the
+    // waves' join: 4 x 16 rows of f32 and their statistics
+    constexpr unsigned lds = 4 * 32 * D * 2 + 2 * NW * 16 * 4;
+    auto go = [&](auto kernel) {
+        OMG_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                    int(lds)));
+        kernel<<<dim3(blocks), dim3(NW * 64), lds, s>>>(a);
+    };
+    if (a.p.tile == WAVES_KEYS)
+        go(attention_shared_kernel<T, D, WAVES_KEYS>);
+    else if (a.p.tile == WAVES_16)
+        go(attention_shared_kernel<T, D, WAVES_16>);
+    else if constexpr (D < 512)
+        go(attention_shared_kernel<T, D, WAVES_32>);
+    OMG_HIP(hipGetLastError());
+    if (a.part_o) {
+        attention_join_kernel<T, D><<<dim3(unsigned((a.b.t * a.x.heads + 3) / 4)), dim3(256), 0, s>>>(a);
+        OMG_HIP(hipGetLastError());
+    }
+}
+
+template <typename T>
+void launch_t(hipStream_t s, const Args& a, unsigned blocks) {
+    switch (a.kv.head_dim) {
+        case 64: return launch_d<T, 64>(s, a, blocks);
+        case 128: return launch_d<T, 128>(s, a, blocks);
+        case 256: return launch_d<T, 256>(s, a, blocks);
+        default: return launch_d<T, 512>(s, a, blocks);
+    }
+}
+
+}  // namespace
+
+int64_t attention_shared_workspace(const PagedKv& kv, const PagedBatch& b, int heads) {
+    check(kv, b, heads);
+    return part_bytes(plan(kv, b, heads), kv, b, heads);
+}
+
+void launch_attention_shared(hipStream_t s, const PagedKv& kv, const PagedBatch& b, const SharedAttn& x,
+                             void* workspace, size_t bytes) {
+    check(kv, b, x.heads);
+    const int64_t width = int64_t(x.heads) * kv.head_dim;
+    if (!x.q || !x.out || !aligned16(x.q) || !aligned16(x.out))
+        fail(E_INVALID, "attention_shared: q and out must be 16-byte aligned device pointers");
+    if (x.ldq < width || x.ldq % 8 || x.ldo < width || x.ldo % 8)
+        fail(E_INVALID, "attention_shared: ldq and ldo must hold the heads and be multiples of 8");
+    if (!(x.scale > 0.0f) || x.scale > 1e30f) fail(E_INVALID, "attention_shared: scale must be positive and finite");
+    if (x.window < 0) fail(E_INVALID, "attention_shared: window must not be negative");
+    Args a{};
+    a.kv = kv, a.b = b, a.x = x;
+    a.p = plan(kv, b, x.heads);
+    a.hpg = x.heads / kv.kv_heads;
+    a.page_shift = log2_of(kv.page);
+    a.max_len = b.max_pages * kv.page;
+    a.c = x.scale * 1.4426950408889634f;
+    const int64_t need = part_bytes(a.p, kv, b, x.heads);
+    if (int64_t(bytes) < need)
+        fail(E_CAPACITY, "attention_shared: the workspace needs " + std::to_string(need) + " bytes");
+    if (need) {
+        if (!workspace || !aligned16(workspace)) fail(E_INVALID, "attention_shared: the workspace must be 16-byte aligned");
+        a.part_o = static_cast<float*>(workspace);
+        a.part_ml = reinterpret_cast<float2*>(a.part_o + a.p.slots() * b.t * x.heads * kv.head_dim);
+    }
+    const int64_t nsplit = a.p.whole ? 1 : a.p.np + (a.p.fused ? a.p.os : 0);
+    a.prefix_blocks = up(int64_t(a.p.ntile) * kv.kv_heads * nsplit, 8);
+    const int64_t blocks = a.prefix_blocks + (a.p.fused ? 0 : a.p.own_tiles * kv.kv_heads * a.p.os);
+    if (blocks > INT_MAX) fail(E_CAPACITY, "attention_shared: too many work items");
+    kv.dtype == ELEM_F16 ? launch_t<half_t>(s, a, unsigned(blocks)) : launch_t<bf16_t>(s, a, unsigned(blocks));
+}
+
+}  // namespace omg

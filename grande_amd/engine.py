@@ -564,3 +564,15 @@ class PagedKv(L.omg_paged_kv):
         """omg_dev_kv_append: the step's keys and values into the cache, its
         queries into q_out."""
         L.check(L.lib().omg_dev_kv_append(self, batch, src, q_out_ptr, ldq, stream))
+
+    def attention_workspace(self, batch: PagedBatch, heads: int) -> int:
+        """Bytes of workspace that `attention` needs for batches of these sizes."""
+        return L.size(L.lib().omg_dev_attention_shared_workspace(self, batch, heads))
+
+    def attention(self, batch: PagedBatch, heads: int, q_ptr: int, ldq: int, out_ptr: int, ldo: int, scale: float, *,
+                  window: int = 0, lse: int | None = None, workspace: int | None = None, workspace_bytes: int = 0,
+                  stream: int | None = None) -> None:
+        """omg_dev_attention_shared: the step's queries over the shared
+        prefix and their sequences' own rows."""
+        L.check(L.lib().omg_dev_attention_shared(self, batch, heads, q_ptr, ldq, out_ptr, ldo, lse, scale, window,
+                                                 workspace, workspace_bytes, stream))

@@ -390,6 +390,30 @@ typedef struct {
 int omg_dev_kv_append(const omg_paged_kv *kv, const omg_paged_batch *b, const omg_kv_source *src, void *q_out,
                       int64_t ldq, void *stream);
 
+/* Attention of the batch's token rows (`heads` query heads, heads a multiple
+ * of kv_heads; row i, head h at q + i * ldq + h * head_dim) over the cache:
+ * a token sees the whole shared prefix and its sequence's own rows up to its
+ * own, of these (window > 0) the ones less than `window` positions back.
+ *   out = softmax(scale * q . k) v, lse = log(sum exp(scale * q . k))
+ * out (row stride ldo) has the cache's type, lse [t][heads] f32 (may be
+ * NULL); a token that sees no key gets zeros and -infinity.  The prefix's
+ * keys and values are read once for a tile of query rows, whatever
+ * sequences these belong to.  What stands in cache rows that nobody sees
+ * does not matter, unless another query of the call sees it: a value that
+ * is infinite or NaN there may reach queries that do not see its row.
+ * scale positive; q and out 16-byte aligned, ldq and ldo multiples of 8.
+ * f32 sums; the softmax's probabilities are rounded to the cache's type for
+ * their product with the values.
+ *
+ * workspace: omg_dev_attention_shared_workspace bytes (a function of the
+ * shapes alone: nseq, t, max_pages, prefix_len, heads and the cache's;
+ * negative: an OMG_E_* status), 16-byte aligned, this call's own until it
+ * has run. */
+int64_t omg_dev_attention_shared_workspace(const omg_paged_kv *kv, const omg_paged_batch *b, int heads);
+int omg_dev_attention_shared(const omg_paged_kv *kv, const omg_paged_batch *b, int heads, const void *q, int64_t ldq,
+                             void *out, int64_t ldo, float *lse, float scale, int window, void *workspace,
+                             size_t workspace_bytes, void *stream);
+
 /* ---- the bidirectional encoder path (crates/omg-wgpu/src/laya.rs) ----
  * An mmBERT / ModernBERT encoder with Laya's decision head: every question
  * is one sequence; a request's sequences run as one packed pass isolated by

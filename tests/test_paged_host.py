@@ -69,3 +69,40 @@ def test_append_refuses_null_descriptions():
     for args in ((None, batch(), source()), (kv(), None, source()), (kv(), batch(), None)):
         with pytest.raises(g.OmgError, match="null"):
             L.check(L.lib().omg_dev_kv_append(*args, P, 256, None))
+
+
+def attend(k=None, b=None, heads=4, q=P, ldq=256, out=P, ldo=256, scale=0.125, window=0, lse=None, workspace=P,
+           workspace_bytes=1 << 40):
+    (k or kv()).attention(b or batch(), heads, q, ldq, out, ldo, scale, window=window, lse=lse, workspace=workspace,
+                          workspace_bytes=workspace_bytes)
+
+
+@pytest.mark.parametrize("over,why", BAD_KV)
+def test_attention_refuses_caches(over, why):
+    with pytest.raises(g.OmgError, match=why):
+        attend(k=kv(**over))
+
+
+@pytest.mark.parametrize("over,why", BAD_BATCH)
+def test_attention_refuses_batches(over, why):
+    with pytest.raises(g.OmgError, match=why):
+        attend(b=batch(**over))
+
+
+@pytest.mark.parametrize("over,why", [
+    (dict(heads=3), "heads"), (dict(heads=0), "heads"), (dict(q=None), "q and out"), (dict(out=P + 2), "q and out"),
+    (dict(ldq=248), "ldq"), (dict(ldq=260), "ldq"), (dict(ldo=255), "ldo"), (dict(scale=0.0), "scale"),
+    (dict(scale=-1.0), "scale"), (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"),
+    (dict(window=-1), "window"), (dict(b=batch(prefix_table_ptr=P, prefix_len=900), workspace_bytes=16), "workspace needs"),
+    (dict(b=batch(prefix_table_ptr=P, prefix_len=900), workspace=None), "workspace must"),
+    (dict(b=batch(prefix_table_ptr=P, prefix_len=900), workspace=P + 8), "workspace must")])
+def test_attention_refuses_arguments(over, why):
+    with pytest.raises(g.OmgError, match=why):
+        attend(**over)
+
+
+def test_workspace_is_refused_or_sized():
+    assert kv().attention_workspace(batch(), 4) == 0  # one item a row: no partial results
+    assert kv().attention_workspace(batch(prefix_table_ptr=P, prefix_len=900), 4) > 0
+    with pytest.raises(g.OmgError, match="heads"):
+        kv().attention_workspace(batch(), 3)
