@@ -63,6 +63,12 @@ class omg_kv_source(C.Structure):
                 ("k_norm", C.c_void_p), ("v_norm", C.c_int), ("eps", C.c_float), ("q_scale", C.c_float)]
 
 
+class omg_sample_args(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("rows", C.c_int64), ("vocab", C.c_int64), ("ld", C.c_int64),
+                ("logits", C.c_void_p), ("u", C.c_void_p), ("temperature", C.c_void_p), ("top_k", C.c_void_p),
+                ("top_p", C.c_void_p), ("min_p", C.c_void_p), ("tokens", C.c_void_p), ("logprob", C.c_void_p)]
+
+
 class omg_laya_seq(C.Structure):
     _fields_ = [("ids", C.POINTER(C.c_uint32)), ("nids", C.c_size_t), ("markers", C.POINTER(C.c_uint32)),
                 ("nmarkers", C.c_size_t), ("qtype", C.c_int)]
@@ -149,6 +155,8 @@ _SIGS = {
     "omg_dev_attention_shared_workspace": (C.c_int64, [C.POINTER(omg_paged_kv), C.POINTER(omg_paged_batch), C.c_int]),
     "omg_dev_attention_shared": (C.c_int, [C.POINTER(omg_paged_kv), C.POINTER(omg_paged_batch), C.c_int, _P, C.c_int64,
                                            _P, C.c_int64, _P, C.c_float, C.c_int, _P, C.c_size_t, _P]),
+    "omg_dev_sample_workspace": (C.c_int64, [C.c_int64, C.c_int64]),
+    "omg_dev_sample": (C.c_int, [C.POINTER(omg_sample_args), _P, C.c_size_t, _P]),
     "omg_laya_builder_new": (_P, [C.c_char_p]),
     "omg_laya_builder_push": (C.c_int, [_P, C.c_char_p, C.c_int, C.POINTER(C.c_int64), C.c_size_t, _P, C.c_size_t,
                                         _P, C.c_size_t]),

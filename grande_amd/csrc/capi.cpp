@@ -706,6 +706,21 @@ int omg_dev_attention_shared(const omg_paged_kv* kv, const omg_paged_batch* b, i
     });
 }
 
+int64_t omg_dev_sample_workspace(int64_t rows, int64_t vocab) {
+    int64_t n = 0;
+    const int rc = guard([&] { n = omg::sample_workspace(rows, vocab); });
+    return rc == OMG_OK ? n : rc;
+}
+
+int omg_dev_sample(const omg_sample_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+    return guard([&] {
+        if (!a) omg::fail(omg::E_INVALID, "null arguments");
+        const omg::SampleArgs s{a->dtype,       a->rows,  a->vocab, a->ld,    a->logits, a->u,
+                                a->temperature, a->top_k, a->top_p, a->min_p, a->tokens, a->logprob};
+        omg::launch_sample(static_cast<hipStream_t>(stream), s, workspace, workspace_bytes);
+    });
+}
+
 /* ---- the bidirectional encoder path ---- */
 
 omg_laya_builder* omg_laya_builder_new(const char* config_json) {

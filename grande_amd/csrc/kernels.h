@@ -349,4 +349,18 @@ int64_t attention_shared_workspace(const PagedKv& kv, const PagedBatch& b, int h
 void launch_attention_shared(hipStream_t s, const PagedKv& kv, const PagedBatch& b, const SharedAttn& x,
                              void* workspace, size_t bytes);
 
+// ---- sampling (sample.hip) ----
+struct SampleArgs {  // omg_sample_args
+    int dtype;
+    int64_t rows, vocab, ld;
+    const void* logits;
+    const float *u, *temperature;
+    const int32_t* top_k;
+    const float *top_p, *min_p;
+    int32_t* tokens;
+    float* logprob;
+};
+int64_t sample_workspace(int64_t rows, int64_t vocab);
+void launch_sample(hipStream_t s, const SampleArgs& a, void* workspace, size_t bytes);
+
 }  // namespace omg

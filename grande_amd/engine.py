@@ -576,3 +576,20 @@ class PagedKv(L.omg_paged_kv):
         prefix and their sequences' own rows."""
         L.check(L.lib().omg_dev_attention_shared(self, batch, heads, q_ptr, ldq, out_ptr, ldo, lse, scale, window,
                                                  workspace, workspace_bytes, stream))
+
+
+def sample_workspace(rows: int, vocab: int) -> int:
+    """Bytes of workspace that `sample` needs."""
+    return L.size(L.lib().omg_dev_sample_workspace(rows, vocab))
+
+
+def sample(logits_ptr: int, dtype: int, rows: int, vocab: int, ld: int, u_ptr: int, tokens_ptr: int,
+           logprob_ptr: int | None = None, *, temperature: int | None = None, top_k: int | None = None,
+           top_p: int | None = None, min_p: int | None = None, workspace: int | None = None,
+           workspace_bytes: int = 0, stream: int | None = None) -> None:
+    """omg_dev_sample: the next token of each row of logits, drawn with the
+    random numbers at u_ptr; the parameters are device arrays of a value per
+    row (temperature, top_p and min_p f32, top_k int32) or None."""
+    a = L.omg_sample_args(dtype, rows, vocab, ld, logits_ptr, u_ptr, temperature, top_k, top_p, min_p, tokens_ptr,
+                          logprob_ptr)
+    L.check(L.lib().omg_dev_sample(a, workspace, workspace_bytes, stream))

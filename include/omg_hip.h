@@ -414,6 +414,41 @@ int omg_dev_attention_shared(const omg_paged_kv *kv, const omg_paged_batch *b, i
                              void *out, int64_t ldo, float *lse, float scale, int window, void *workspace,
                              size_t workspace_bytes, void *stream);
 
+/* The next token of each row of logits (row r, token i at logits[r * ld + i];
+ * dtype OMG_ELEM_F32, F16 or BF16; any ld from vocab up), drawn with the
+ * given random number u[r] in [0, 1).  With z the row, M its maximum and
+ * w_i = exp((z_i - M) / temperature):
+ *   1. top_k: the k largest z stay (ties: the lowest indexes first);
+ *   2. top_p: of these, largest first, a token stays while the mass before
+ *      it is under top_p times the mass of all of step 1 (the first always);
+ *   3. min_p: of these, tokens with w_i >= min_p stay (the largest always);
+ *   4. the token is the first kept one, in index order, whose running mass
+ *      exceeds u times the mass of all kept tokens.
+ * logprob (may be NULL) is log(w_token / mass of the kept).  Each parameter
+ * is a device array of a value per row, or NULL (off): temperature (NULL:
+ * 1; <= 0 or NaN: the first largest z, logprob 0), top_k (<= 0: off), top_p
+ * (>= 1 or NaN: off), min_p (<= 0 or NaN: off).  u outside [0, 1) counts as
+ * the nearest inside, NaN as 0.
+ * Masked tokens are -infinity or NaN and are never drawn; a row with nothing
+ * else gives token -1 and logprob -infinity.  Masses are 64-bit fixed-point
+ * sums of w rounded to 2^-42, so a token under 2^-43 of the largest is not
+ * drawn, and the result does not depend on the order of the sums.
+ * vocab up to 2^20.  workspace: omg_dev_sample_workspace bytes (negative: an
+ * OMG_E_* status), 16-byte aligned, this call's own until it has run. */
+int64_t omg_dev_sample_workspace(int64_t rows, int64_t vocab);
+typedef struct {
+    int dtype;
+    int64_t rows, vocab, ld;
+    const void *logits;
+    const float *u;
+    const float *temperature;
+    const int32_t *top_k;
+    const float *top_p, *min_p;
+    int32_t *tokens;
+    float *logprob;
+} omg_sample_args;
+int omg_dev_sample(const omg_sample_args *a, void *workspace, size_t workspace_bytes, void *stream);
+
 /* ---- the bidirectional encoder path (crates/omg-wgpu/src/laya.rs) ----
  * An mmBERT / ModernBERT encoder with Laya's decision head: every question
  * is one sequence; a request's sequences run as one packed pass isolated by

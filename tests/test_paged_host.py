@@ -106,3 +106,21 @@ def test_workspace_is_refused_or_sized():
     assert kv().attention_workspace(batch(prefix_table_ptr=P, prefix_len=900), 4) > 0
     with pytest.raises(g.OmgError, match="heads"):
         kv().attention_workspace(batch(), 3)
+
+
+@pytest.mark.parametrize("over,why", [
+    (dict(dtype=7), "f32, f16 or bf16"), (dict(rows=0), "rows"), (dict(vocab=0), "vocab"),
+    (dict(vocab=(1 << 20) + 1, ld=1 << 21), "vocab"), (dict(ld=99), "ld"), (dict(logits_ptr=None), "null"),
+    (dict(u_ptr=None), "null"), (dict(tokens_ptr=None), "null"), (dict(logits_ptr=P + 2), "aligned")])
+def test_sample_refuses(over, why):
+    a = dict(logits_ptr=P, dtype=g.ELEM_F32, rows=3, vocab=100, ld=100, u_ptr=P, tokens_ptr=P)
+    a.update(over)
+    with pytest.raises(g.OmgError, match=why):
+        g.sample(**a, workspace=P, workspace_bytes=1 << 40)
+
+
+def test_sample_workspace_is_refused_or_sized():
+    assert g.sample_workspace(3, 100) >= 0
+    for rows, vocab in ((0, 10), (3, 0), (3, (1 << 20) + 1)):
+        with pytest.raises(g.OmgError):
+            g.sample_workspace(rows, vocab)
