@@ -1,12 +1,26 @@
 // Sampling the next token from rows of logits (omg_dev_sample).
 //
-// A token is kept or not by its place in the order (z descending, index
-// ascending), so what a filter keeps is a threshold: every z above it and
-// the first `ties` tokens equal to it.  Masses are sums of
-//   W(z) = round(2^42 exp((z - max) / T)),
-// whole numbers that add up the same in any order (at most 2^20 of them, so
-// 2^62): the histograms' atomics and the split of a row over threads leave
-// no trace in the result.  exp is taken in 64 bits.
+// A filter keeps the first n tokens in the order (z descending, index
+// ascending), so a cut is one item (z's key, index): what comes before it
+// stays.  Masses are whole numbers W(z) = round(2^42 exp((z - max) / T)),
+// at most 2^20 of them: they add up to the same in any order, so neither
+// atomics nor the split of a row over threads leave a trace in the result.
+// exp is taken in 64 bits: a token's border in the running mass is met by a
+// random number closer than f32's error in one row of a few hundred.
+//
+// A row costs one read where it is short: up to 32 * 1,024 logits it lies in
+// the registers of one workgroup (sample_short).  Longer rows are read once
+// by the whole chip (sample_stats: per 2,048 logits the maximum, its index
+// and, where the row's filters need it, the sum of exp; per 16 the maximum),
+// then one workgroup a row finishes (sample_long).  Both look for a
+// threshold that few logits pass but all that can be kept do, from the
+// maxima of small groups: the k-th largest of these maxima has k logits at
+// or above it; min_p's threshold is its own; for top_p alone a guess is
+// taken and proved by the mass above it.  The logits above it are gathered
+// into a list in LDS, where the exact cuts and the drawn token are found by
+// comparing all pairs (up to 256) or by histograms over the items' digits.
+// Rows whose kept tokens do not fit the list run the same digits over the
+// whole row.
 #include <string>
 
 #include "common.h"
@@ -17,33 +31,98 @@ namespace omg {
 
 namespace {
 
-constexpr int NT = 1024;  // threads of a row's workgroup
-constexpr int DIG = 2048; // histogram bins: the key's digits are 11, 11 and 10 bits
+constexpr int NT = 1024;          // threads of a row's workgroup
+constexpr int NWAVE = NT / WAVE;
+constexpr int CHUNK = 2048;       // logits of a wave of sample_stats
+constexpr int GROUP = 16;         // logits of a group maximum there
+constexpr int CAP = 8192;         // items of the list
+constexpr int BINS = 2048;
+constexpr int PAIRS = NT / 4;     // items compared pair by pair: four threads each
+constexpr int SEG = 256;          // consecutive logits a wave takes at once
+constexpr int IDX_BITS = 20;      // vocab <= 2^20
+constexpr uint32_t IDX_MASK = (1u << IDX_BITS) - 1;
+constexpr double ONE = 4398046511104.0;  // 2^42
 
-// Order-preserving bits of a logit; 0 for masked ones (-infinity, NaN).
-// (z + 0 makes -0 the 0 it equals.)
+// A logit as it is ordered: masked ones (-infinity, NaN) -infinity, -0 the 0 it equals.
+__device__ inline float clean(float z) { return z > -INFINITY ? z + 0.0f : -INFINITY; }
+// Order-preserving bits of a clean logit; 0 for masked ones.
 __device__ inline uint32_t key_of(float z) {
-    if (!(z > -INFINITY)) return 0;
-    const uint32_t u = __builtin_bit_cast(uint32_t, z + 0.0f);
-    return u & 0x80000000u ? ~u : u | 0x80000000u;
+    const uint32_t u = __builtin_bit_cast(uint32_t, z);
+    return z == -INFINITY ? 0 : u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 __device__ inline float value_of(uint32_t k) {
     return __builtin_bit_cast(float, k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
+// An item: larger comes first.
+__device__ inline uint64_t item_of(float z, uint32_t i) {
+    return uint64_t(key_of(z)) << IDX_BITS | (IDX_MASK - i);
+}
+__device__ inline float item_value(uint64_t it) { return value_of(uint32_t(it >> IDX_BITS)); }
+__device__ inline uint32_t item_index(uint64_t it) { return IDX_MASK - (uint32_t(it) & IDX_MASK); }
 
-// What stays of a row: keys above `key`, and the first `ties` equal to it.
-struct Cut {
-    uint32_t key;
-    uint64_t ties;
+// exp(x) for -40 < x <= 0: x = n ln 2 + f, |f| <= ln 2 / 2, the series of
+// exp f to f^12 (its rest is below 2^-52), times 2^n.
+__device__ inline double exp_small(double x) {
+    const double n = rint(x * 1.4426950408889634);
+    double f = fma(n, -0.69314718055994529, x);
+    f = fma(n, -2.3190468138462996e-17, f);
+    double p = 1.0 / 479001600.0;
+    p = fma(p, f, 1.0 / 39916800.0);
+    p = fma(p, f, 1.0 / 3628800.0);
+    p = fma(p, f, 1.0 / 362880.0);
+    p = fma(p, f, 1.0 / 40320.0);
+    p = fma(p, f, 1.0 / 5040.0);
+    p = fma(p, f, 1.0 / 720.0);
+    p = fma(p, f, 1.0 / 120.0);
+    p = fma(p, f, 1.0 / 24.0);
+    p = fma(p, f, 1.0 / 6.0);
+    p = fma(p, f, 0.5);
+    p = fma(p, f, 1.0);
+    p = fma(p, f, 1.0);
+    return __builtin_amdgcn_ldexp(p, int(n));
+}
+
+// exp((z - max) / T) of a clean logit: 1 at the maximum, whatever it is, 0
+// where it is masked or far under 2^-43.
+struct Weigh {
+    double max, inv_t;
+    __device__ double operator()(float z) const {
+        const double d = double(z) - max;
+        if (z == -INFINITY) return 0.0;
+        if (!(d < 0.0)) return 1.0;
+        const double x = d * inv_t;
+        return x > -40.0 ? exp_small(x) : 0.0;
+    }
+    __device__ uint64_t mass(float z) const { return fixed((*this)(z)); }
+    // (2^52 + v rounds v to a whole number in its low bits)
+    static __device__ uint64_t fixed(double w) {
+        return __builtin_bit_cast(uint64_t, fma(w, ONE, 4503599627370496.0)) & 0xfffffffffffffull;
+    }
 };
 
-struct Shared {
-    uint64_t hist[DIG];
-    uint64_t part[NT / WAVE], part2[NT / WAVE];
-    uint64_t found, before;
-    uint32_t bin;
-    uint32_t kmax, kfirst;
+// A row's settings; filters that are off have their neutral value.
+struct Settings {
+    bool greedy;
+    int64_t k;      // 0: off
+    float p;        // >= 1: off
+    double least;   // 0: off
+    double inv_t;
+    float t;
+    __device__ bool need_sum() const { return !greedy && k == 0 && (p < 1.0f || least == 0.0); }
 };
+__device__ inline Settings settings_of(const SampleArgs& a, int64_t r) {
+    Settings s;
+    s.t = a.temperature ? a.temperature[r] : 1.0f;
+    s.greedy = !(s.t > 0.0f);
+    s.inv_t = s.greedy ? 0.0 : 1.0 / double(s.t);
+    const int64_t k = a.top_k ? int64_t(a.top_k[r]) : 0;
+    s.k = k > 0 && k < a.vocab ? k : 0;
+    const float p = a.top_p ? a.top_p[r] : 1.0f;
+    s.p = p < 1.0f ? p : 1.0f;
+    const float m = a.min_p ? a.min_p[r] : 0.0f;
+    s.least = m > 0.0f ? (m < 1.0f ? double(m) : 1.0) : 0.0;
+    return s;
+}
 
 __device__ inline uint64_t wave_sum_u64(uint64_t v) {
 #pragma unroll
@@ -59,200 +138,697 @@ __device__ inline uint64_t wave_scan_u64(uint64_t v, int lane) {  // inclusive
     return v;
 }
 
-template <typename T>
-struct RowOf {
-    const T* z;
-    int64_t n;
-    double max, inv_t;  // (inv_t unused for an infinite maximum)
-    __device__ uint32_t key(int64_t i) const { return key_of(float(z[i])); }
-    // exp((z - max) / T): 1 at the maximum, whatever it is
-    __device__ double weight(uint32_t k) const {
-        if (k == 0) return 0.0;
-        const double d = double(value_of(k)) - max;
-        if (!(d < 0.0)) return 1.0;  // (infinity - infinity)
-        const double x = d * inv_t;
-        return x > -40.0 ? exp(x) : 0.0;
-    }
-    __device__ uint64_t mass(uint32_t k) const { return uint64_t(rint(weight(k) * 4398046511104.0)); }
+struct Shared {
+    uint64_t item[CAP];   // the list; without one, the masses of the row's segments
+    uint64_t mass[CAP];   // (top bit: under min_p)
+    uint64_t hist[BINS];
+    uint64_t part[NWAVE];
+    uint64_t before, in_bin, total;
+    uint32_t bin, kmax, kfirst;
+    int count;
 };
+constexpr uint64_t UNDER = uint64_t(1) << 63;
 
-// Sum of v over the workgroup, in every thread.
-__device__ inline uint64_t block_sum(uint64_t v, uint64_t* part) {
-    const int lane = int(threadIdx.x) % WAVE, wave = int(threadIdx.x) / WAVE;
+__device__ inline uint64_t block_sum(uint64_t v, Shared& sm) {
     v = wave_sum_u64(v);
     __syncthreads();
-    if (lane == 0) part[wave] = v;
+    if (threadIdx.x % WAVE == 0) sm.part[threadIdx.x / WAVE] = v;
     __syncthreads();
     uint64_t s = 0;
-    for (int i = 0; i < NT / WAVE; ++i) s += part[i];
+#pragma unroll
+    for (int i = 0; i < NWAVE; ++i) s += sm.part[i];
     return s;
 }
 
-// The element at which the running sum, over keys from the largest down,
-// first reaches `target` (at least 1): `what` gives each key's share (a count
-// of one, or its mass) and `limit` the keys that take part.  Returns its key
-// and how many of the keys equal to it are needed.
-template <typename T, typename F>
-__device__ Cut find_cut(const RowOf<T>& row, Shared& sm, uint64_t target, const Cut& limit, F&& what) {
-    uint32_t prefix = 0;
-    uint64_t before = 0;
-    for (int level = 0; level < 3; ++level) {
-        const int shift = level == 0 ? 21 : level == 1 ? 10 : 0, bits = level == 2 ? 10 : 11;
-        __syncthreads();
-        for (int i = threadIdx.x; i < DIG; i += NT) sm.hist[i] = 0;
-        __syncthreads();
-        for (int64_t i = threadIdx.x; i < row.n; i += NT) {
-            const uint32_t k = row.key(i);
-            if (k <= limit.key || (level > 0 && (k >> (shift + bits)) != prefix)) continue;
-            atomicAdd(reinterpret_cast<unsigned long long*>(&sm.hist[(k >> shift) & ((1u << bits) - 1)]),
-                      static_cast<unsigned long long>(what(k)));
-        }
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            if (limit.key && limit.ties && (level == 0 || (limit.key >> (shift + bits)) == prefix))
-                sm.hist[(limit.key >> shift) & ((1u << bits) - 1)] += limit.ties * what(limit.key);
-            uint64_t run = before;
-            uint32_t b = (1u << bits) - 1;
-            for (;; --b) {
-                if (run + sm.hist[b] >= target || b == 0) break;
-                run += sm.hist[b];
-            }
-            sm.bin = b;
-            sm.before = run;
-        }
-        __syncthreads();
-        prefix = (prefix << bits) | sm.bin;
-        before = sm.before;
+// The bin at which the running sum over h[0 .. n), in ascending or (DOWN)
+// descending order, first reaches `target`; the last one in order if it
+// never does.  Sets sm.bin, sm.before (the sum before it), sm.in_bin and
+// sm.total.
+template <bool DOWN>
+__device__ inline void pick(const uint64_t* h, int n, uint64_t target, Shared& sm) {
+    const int tid = int(threadIdx.x), lane = tid % WAVE, wave = tid / WAVE;
+    const int per = (n + NT - 1) / NT;
+    __syncthreads();
+    uint64_t own = 0;
+    for (int i = 0; i < per; ++i) {
+        const int j = tid * per + i;
+        if (j < n) own += h[DOWN ? n - 1 - j : j];
     }
-    const uint64_t one = what(prefix);
-    return {prefix, one ? (target - before + one - 1) / one : 1};
+    const uint64_t scan = wave_scan_u64(own, lane);
+    if (lane == WAVE - 1) sm.part[wave] = scan;
+    __syncthreads();
+    uint64_t base = 0, total = 0;
+#pragma unroll
+    for (int i = 0; i < NWAVE; ++i) {
+        if (i < wave) base += sm.part[i];
+        total += sm.part[i];
+    }
+    uint64_t run = base + scan - own;
+    const bool never = total < target;
+    if (tid == 0) sm.total = total;
+    for (int i = 0; i < per; ++i) {
+        const int j = tid * per + i;
+        if (j >= n) break;
+        const uint64_t x = h[DOWN ? n - 1 - j : j];
+        if (never ? j == n - 1 : run < target && run + x >= target) {
+            sm.bin = uint32_t(DOWN ? n - 1 - j : j);
+            sm.before = run;
+            sm.in_bin = x;
+        }
+        run += x;
+    }
+    __syncthreads();
 }
 
+__device__ inline void clear(uint64_t* h, int n) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += NT) h[i] = 0;
+    __syncthreads();
+}
+__device__ inline void add(uint64_t* h, uint64_t v) {
+    atomicAdd(reinterpret_cast<unsigned long long*>(h), static_cast<unsigned long long>(v));
+}
+
+// The item at which the running share, over the items >= limit from the
+// first on, first reaches `target` (>= 1); an item that takes in all of them
+// if it never does.  src(f) calls f(item, i) for the thread's items;
+// share(item, i) is an item's count or mass.
+template <typename S, typename F>
+__device__ uint64_t find_cut(S&& src, Shared& sm, uint64_t target, uint64_t limit, F&& share) {
+    constexpr int digits[5] = {11, 11, 10, 10, 10};
+    uint64_t prefix = 0, before = 0;
+    int shift = 52;
+    for (int level = 0; level < 5; ++level) {
+        const int bits = digits[level];
+        shift -= bits;
+        clear(sm.hist, 1 << bits);
+        src([&](uint64_t it, int i) {
+            if (it < limit || (it >> (shift + bits)) != prefix) return;
+            const uint64_t v = share(it, i);
+            if (v) add(&sm.hist[(it >> shift) & ((1u << bits) - 1)], v);
+        });
+        pick<true>(sm.hist, 1 << bits, target - before, sm);
+        prefix = prefix << bits | sm.bin;
+        before += sm.before;
+        if (before + sm.in_bin <= target) break;  // the whole bin stays
+    }
+    const uint64_t cut = prefix << shift;
+    return cut > limit ? cut : limit;
+}
+
+// A row that is worked on as a whole: each(f) calls f(z, index) for the
+// thread's logits, SEG consecutive ones a wave; segment(s, f) for a lane's of
+// segment s (in lane order).
+template <typename T, int E>
+struct RegisterRow {
+    float z[E];
+    int64_t n;
+    __device__ uint32_t index(int j) const { return uint32_t(((j / 4) * NT + threadIdx.x) * 4 + j % 4); }
+    __device__ void load(const T* p, int64_t vocab) {
+        n = vocab;
+        const bool wide = reinterpret_cast<uintptr_t>(p) % (4 * sizeof(T)) == 0;
+#pragma unroll
+        for (int j = 0; j < E; j += 4) {
+            const int64_t i = index(j);
+            if (wide && i + 4 <= n) {
+                typedef T vec __attribute__((ext_vector_type(4)));
+                const vec v = *reinterpret_cast<const vec*>(p + i);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) z[j + c] = float(v[c]);
+            } else {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) z[j + c] = i + c < n ? float(p[i + c]) : -INFINITY;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < E; ++j) z[j] = clean(z[j]);
+    }
+    template <typename F>
+    __device__ void each(F&& f) const {
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+            if (z[j] != -INFINITY) f(z[j], index(j));
+    }
+    __device__ int segments() const { return E / 4 * NWAVE; }
+    // m(z, i) summed over each segment into out[]
+    template <typename F>
+    __device__ void sums(uint64_t* out, F&& m) const {
+        const int lane = int(threadIdx.x) % WAVE, wave = int(threadIdx.x) / WAVE;
+#pragma unroll
+        for (int j = 0; j < E; j += 4) {
+            uint64_t v = 0;
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                if (z[j + c] != -INFINITY) v += m(z[j + c], index(j + c));
+            v = wave_sum_u64(v);
+            if (lane == 0) out[j / 4 * NWAVE + wave] = v;
+        }
+    }
+};
+
 template <typename T>
-__global__ __launch_bounds__(NT) void sample_kernel(SampleArgs a) {
+struct MemoryRow {
+    const T* p;
+    int64_t n;
+    template <typename F>
+    __device__ void each(F&& f) const {
+        for (int64_t i = threadIdx.x; i < n; i += NT) {
+            const float z = clean(float(p[i]));
+            if (z != -INFINITY) f(z, uint32_t(i));
+        }
+    }
+    __device__ int segments() const { return int((n + SEG - 1) / SEG); }
+    template <typename F>
+    __device__ void sums(uint64_t* out, F&& m) const {
+        const int lane = int(threadIdx.x) % WAVE, wave = int(threadIdx.x) / WAVE;
+        for (int s = wave; s < segments(); s += NWAVE) {
+            uint64_t v = 0;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const int64_t i = int64_t(s) * SEG + lane * 4 + c;
+                const float z = i < n ? clean(float(p[i])) : -INFINITY;
+                if (z != -INFINITY) v += m(z, uint32_t(i));
+            }
+            v = wave_sum_u64(v);
+            if (lane == 0) out[s] = v;
+        }
+    }
+};
+
+struct Result {
+    int32_t* token;
+    float* logprob;
+    Weigh w;
+    __device__ void write(float z, uint32_t i, uint64_t total) const {
+        *token = int32_t(i);
+        const double d = double(z) - w.max;
+        if (logprob) *logprob = float((d < 0.0 ? d * w.inv_t : 0.0) - log(double(total) / ONE));
+    }
+};
+
+// The first running mass that exceeds u * total.
+__device__ inline uint64_t goal(float u, uint64_t total) {
+    const double t = (u > 0.0f ? (u < 1.0f ? double(u) : 1.0) : 0.0) * double(total);
+    const uint64_t g = uint64_t(t) + 1;
+    return g < total ? g : total;
+}
+// top_p's: the running mass at which p * total is reached.
+__device__ inline uint64_t share_of(float p, uint64_t total) {
+    const double t = ceil(double(p) * double(total));
+    const uint64_t g = t < 1.0 ? 1 : uint64_t(t);
+    return g < total ? g : total;
+}
+
+// The drawn logit of one segment: `target` into the masses m(z, i) of its
+// logits (its last with a mass where rounding leaves them short of it).
+template <typename T, typename F>
+__device__ inline void draw_in(const T* p, int64_t n, int64_t first, int count, uint64_t target, uint64_t total,
+                               const Result& out, F&& m) {
+    if (threadIdx.x >= WAVE) return;
+    const int lane = int(threadIdx.x);
+    uint64_t run = 0;
+    float drawn = 0.0f;
+    int64_t index = -1;
+    for (int at = 0; at < count; at += WAVE) {
+        const int64_t i = first + at + lane;
+        const float z = at + lane < count && i < n ? clean(float(p[i])) : -INFINITY;
+        const uint64_t v = z != -INFINITY ? m(z, uint32_t(i)) : 0;
+        const uint64_t scan = run + wave_scan_u64(v, lane);
+        const uint64_t some = __ballot(v > 0), hit = __ballot(v > 0 && scan >= target);
+        if (some) {
+            const int l = hit ? __builtin_ctzll(hit) : 63 - __builtin_clzll(some);
+            drawn = __shfl(z, l, WAVE);
+            index = first + at + l;
+        }
+        if (hit) break;
+        run = __shfl(scan, WAVE - 1, WAVE);
+    }
+    if (lane == 0 && index >= 0) out.write(drawn, uint32_t(index), total);
+}
+
+// The exact cuts and the draw over the whole row.
+template <typename T, typename R>
+__device__ void finish_row(const R& row, const T* p, const Settings& s, float u, Shared& sm, const Result& out) {
+    const Weigh& w = out.w;
+    auto items = [&](auto&& f) { row.each([&](float z, uint32_t i) { f(item_of(z, i), 0); }); };
+    uint64_t cut = 1;  // every unmasked item
+    if (s.k) cut = find_cut(items, sm, uint64_t(s.k), cut, [](uint64_t, int) { return uint64_t(1); });
+    if (s.p < 1.0f) {
+        uint64_t own = 0;
+        row.each([&](float z, uint32_t i) {
+            if (item_of(z, i) >= cut) own += w.mass(z);
+        });
+        const uint64_t total = block_sum(own, sm);
+        cut = find_cut(items, sm, share_of(s.p, total), cut, [&](uint64_t it, int) { return w.mass(item_value(it)); });
+    }
+    auto kept = [&](float z, uint32_t i) -> uint64_t {
+        if (item_of(z, i) < cut) return 0;
+        const double x = w(z);
+        return x >= s.least ? Weigh::fixed(x) : 0;
+    };
+    __syncthreads();
+    row.sums(sm.item, kept);
+    const int ns = row.segments();
+    uint64_t own = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < ns; i += NT) own += sm.item[i];
+    const uint64_t total = block_sum(own, sm), target = goal(u, total);
+    pick<false>(sm.item, ns, target, sm);
+    draw_in(p, row.n, int64_t(sm.bin) * SEG, SEG, target - sm.before, total, out, kept);
+}
+
+// The exact cuts and the draw over the list's n items (every item that can
+// be kept is there); `row_mass`: the mass that top_p is a share of, unless
+// top_k is on.
+__device__ void finish_list(int n, const Settings& s, float u, uint64_t row_mass, Shared& sm, const Result& out) {
+    const Weigh& w = out.w;
+    const int tid = int(threadIdx.x);
+    __syncthreads();
+    for (int i = tid; i < n; i += NT) {
+        const double x = w(item_value(sm.item[i]));
+        sm.mass[i] = Weigh::fixed(x) | (x >= s.least ? 0 : UNDER);
+    }
+    __syncthreads();
+    if (n <= PAIRS) {
+        // Four threads an item: its place, the mass before it; the mass of
+        // what stays; the running mass in index order.
+        const int e = tid / 4, part = tid % 4;
+        const uint64_t mine = e < n ? sm.item[e] : 0, mass = e < n ? sm.mass[e] : 0;
+        uint64_t place = 0, before = 0, all = 0;
+        for (int j = part; j < n; j += 4) {
+            const bool first = sm.item[j] > mine;
+            place += first;
+            if (first) before += sm.mass[j] & ~UNDER;
+        }
+        place += __shfl_xor(place, 1, WAVE), before += __shfl_xor(before, 1, WAVE);
+        place += __shfl_xor(place, 2, WAVE), before += __shfl_xor(before, 2, WAVE);
+        bool keep = e < n && (s.k == 0 || place < uint64_t(s.k));
+        if (s.p < 1.0f) {
+            all = row_mass;
+            if (s.k) all = block_sum(part == 0 && keep ? mass & ~UNDER : 0, sm);
+            keep = keep && before < share_of(s.p, all);
+        }
+        keep = keep && !(mass & UNDER);
+        __syncthreads();
+        if (part == 0 && e < n) sm.hist[e] = keep ? mass : 0;
+        __syncthreads();
+        uint64_t run = 0, total = 0;
+        const uint32_t at = item_index(mine);
+        for (int j = part; j < n; j += 4) {
+            const uint64_t m = sm.hist[j];
+            total += m;
+            if (item_index(sm.item[j]) <= at) run += m;
+        }
+        run += __shfl_xor(run, 1, WAVE), total += __shfl_xor(total, 1, WAVE);
+        run += __shfl_xor(run, 2, WAVE), total += __shfl_xor(total, 2, WAVE);
+        const uint64_t target = goal(u, total);
+        if (part == 0 && keep && mass > 0 && run >= target && run - mass < target)
+            out.write(item_value(mine), at, total);
+        return;
+    }
+    auto items = [&](auto&& f) {
+        for (int i = tid; i < n; i += NT) f(sm.item[i], i);
+    };
+    uint64_t cut = 1;
+    if (s.k) cut = find_cut(items, sm, uint64_t(s.k), cut, [](uint64_t, int) { return uint64_t(1); });
+    if (s.p < 1.0f) {
+        uint64_t all = row_mass;
+        if (s.k) {
+            uint64_t own = 0;
+            items([&](uint64_t it, int i) { own += it >= cut ? sm.mass[i] & ~UNDER : 0; });
+            all = block_sum(own, sm);
+        }
+        cut = find_cut(items, sm, share_of(s.p, all), cut, [&](uint64_t, int i) { return sm.mass[i] & ~UNDER; });
+    }
+    // the draw: the digits of the index, 10 and 10 bits
+    uint64_t own = 0;
+    items([&](uint64_t it, int i) { own += it >= cut && !(sm.mass[i] & UNDER) ? sm.mass[i] : 0; });
+    const uint64_t total = block_sum(own, sm);
+    uint64_t target = goal(u, total);
+    uint32_t high = 0;
+    for (int level = 0; level < 2; ++level) {
+        clear(sm.hist, 1024);
+        items([&](uint64_t it, int i) {
+            const uint32_t at = item_index(it);
+            if (it < cut || (sm.mass[i] & UNDER) || sm.mass[i] == 0 || (level == 1 && at >> 10 != high)) return;
+            add(&sm.hist[level == 0 ? at >> 10 : at & 1023], sm.mass[i]);
+        });
+        pick<false>(sm.hist, 1024, target, sm);
+        target -= sm.before;
+        if (level == 0) high = sm.bin;
+    }
+    const uint32_t at = high << 10 | sm.bin;
+    items([&](uint64_t it, int) {
+        if (item_index(it) == at) out.write(item_value(it), at, total);
+    });
+}
+
+// Counts of group maxima by their distance from the row's maximum, in bins
+// of T / 64 or 1/32, whichever is narrower.  A threshold is a bin's far edge
+// (with a slack for the rounding of the bins).
+struct Scale {
+    float max, per;  // bins per unit of z
+    bool whole;      // what lies past the last bin has no mass
+    __device__ Scale(float m, float t) : max(m) {
+        const float f = 64.0f / t;
+        per = f > 32.0f ? (f < 1e30f ? f : 1e30f) : 32.0f;
+        whole = float(BINS - 1) > 30.5f * t * per;  // e^-29.9 < 2^-43
+    }
+    __device__ int bin(float z) const {
+        const float x = (max - z) * per;
+        return x < float(BINS - 1) ? int(x) : BINS - 1;  // (NaN, infinity - infinity: the last)
+    }
+};
+
+// Gathers into the list the row's logits that lie in bins 0 .. last, by
+// gather(f): f(z, i) is called for all of them at least.  The count may pass
+// CAP: then the list does not hold them all.
+template <typename G>
+__device__ inline int gather(Shared& sm, G&& each, int last, const Scale& sc) {
+    __syncthreads();
+    if (threadIdx.x == 0) sm.count = 0;
+    __syncthreads();
+    each([&](float z, uint32_t i) {
+        if (sc.bin(z) <= last) {
+            const int at = atomicAdd(&sm.count, 1);
+            if (at < CAP) sm.item[at] = item_of(z, i);
+        }
+    });
+    __syncthreads();
+    return sm.count;
+}
+
+// The list that holds every token that the filters can keep, if one can be
+// had: its length, or -1.  maxima(f) calls f(z) for the maxima of the
+// thread's groups, each(last bin, f) for the logits of the groups that reach
+// that bin.
+template <typename Q, typename G>
+__device__ int make_list(const Settings& s, const Scale& sc, Shared& sm, uint64_t row_mass, const Weigh& w, Q&& maxima,
+                         G&& each) {
+    if (!(sc.max < INFINITY)) return -1;
+    if (s.least > 0.0 && s.k == 0) {
+        // z >= max + T log(min_p), and a bin to spare
+        const float far = float(-log(s.least) * double(s.t)) * sc.per + 1.0f;
+        const int last = far < float(BINS - 2) ? int(far) + 1 : BINS - 1;
+        if (last == BINS - 1) return -1;
+        const int n = gather(sm, [&](auto&& f) { each(last, f); }, last, sc);
+        return n <= CAP ? n : -1;
+    }
+    clear(sm.hist, BINS);
+    maxima([&](float z) {
+        if (z != -INFINITY) add(&sm.hist[sc.bin(z)], 1);
+    });
+    if (s.k) {
+        pick<false>(sm.hist, BINS, uint64_t(s.k), sm);
+        int last = int(sm.bin);
+        if (last == BINS - 1) {
+            if (!sc.whole) return -1;
+            last = BINS - 2;  // (all that have a mass)
+        }
+        const int n = gather(sm, [&](auto&& f) { each(last, f); }, last, sc);
+        return n <= CAP ? n : -1;
+    }
+    // top_p alone: the groups that hold some 100 tokens, then some 5,000
+    const uint64_t target = share_of(s.p, row_mass);
+    for (int guess = 0; guess < 2; ++guess) {
+        pick<false>(sm.hist, BINS, guess == 0 ? 96 : 3072, sm);
+        int last = int(sm.bin);
+        if (last == BINS - 1) {
+            if (!sc.whole) return -1;
+            last = BINS - 2;
+        }
+        const int n = gather(sm, [&](auto&& f) { each(last, f); }, last, sc);
+        if (n > CAP) return -1;
+        uint64_t own = 0;
+        for (int i = threadIdx.x; i < n; i += NT) own += w.mass(item_value(sm.item[i]));
+        if (block_sum(own, sm) >= target) return n;
+    }
+    return -1;
+}
+
+__device__ inline void nothing_left(const Result& out) {
+    *out.token = -1;
+    if (out.logprob) *out.logprob = -INFINITY;
+}
+
+// Rows of at most E * NT logits: one workgroup a row, the row in registers.
+template <typename T, int E>
+__global__ __launch_bounds__(NT) void sample_short(SampleArgs a) {
     __shared__ Shared sm;
     const int64_t r = blockIdx.x;
-    const int tid = int(threadIdx.x), lane = tid % WAVE, wave = tid / WAVE;
-    RowOf<T> row{static_cast<const T*>(a.logits) + r * a.ld, a.vocab, 0.0, 0.0};
-    const float temp = a.temperature ? a.temperature[r] : 1.0f;
-
-    // The maximum and its first index.
+    const int tid = int(threadIdx.x);
+    const T* p = static_cast<const T*>(a.logits) + r * a.ld;
+    RegisterRow<T, E> row;
+    row.load(p, a.vocab);
+    const Settings s = settings_of(a, r);
+    const float u = a.u[r];
     if (tid == 0) sm.kmax = 0, sm.kfirst = 0xffffffffu;
+    float zmax = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < E; ++j) zmax = fmaxf(zmax, row.z[j]);
+    const float wmax = wave_max(zmax);
     __syncthreads();
-    uint32_t kmax = 0, at = 0xffffffffu;
-    for (int64_t i = tid; i < row.n; i += NT) {
-        const uint32_t k = row.key(i);
-        if (k > kmax) kmax = k, at = uint32_t(i);
+    if (tid % WAVE == 0) atomicMax(&sm.kmax, key_of(wmax));
+    __syncthreads();
+    const uint32_t kmax = sm.kmax;
+    Result out{a.tokens + r, a.logprob ? a.logprob + r : nullptr, {double(value_of(kmax)), s.inv_t}};
+    if (kmax == 0) {
+        if (tid == 0) nothing_left(out);
+        return;
     }
-    atomicMax(&sm.kmax, kmax);
-    __syncthreads();
-    if (kmax == sm.kmax) atomicMin(&sm.kfirst, at);
-    __syncthreads();
-    kmax = sm.kmax;
-    if (kmax == 0 || !(temp > 0.0f)) {
+    const float top = value_of(kmax);
+    if (s.greedy) {
+        if (zmax == top) {
+#pragma unroll
+            for (int j = E - 1; j >= 0; --j)
+                if (row.z[j] == top) atomicMin(&sm.kfirst, row.index(j));
+        }
+        __syncthreads();
         if (tid == 0) {
-            a.tokens[r] = kmax == 0 ? -1 : int32_t(sm.kfirst);
-            if (a.logprob) a.logprob[r] = kmax == 0 ? -INFINITY : 0.0f;
+            *out.token = int32_t(sm.kfirst);
+            if (out.logprob) *out.logprob = 0.0f;
         }
         return;
     }
-    row.max = double(value_of(kmax));
-    row.inv_t = 1.0 / double(temp);
-
-    Cut cut{0, 0};  // everything that is not masked
-    const int64_t k = a.top_k ? int64_t(a.top_k[r]) : 0;
-    if (k > 0 && k < row.n) cut = find_cut(row, sm, uint64_t(k), cut, [](uint32_t) { return uint64_t(1); });
-    const float p = a.top_p ? a.top_p[r] : 1.0f;
-    if (p < 1.0f) {
-        uint64_t own = 0;
-        for (int64_t i = tid; i < row.n; i += NT) {
-            const uint32_t q = row.key(i);
-            if (q > cut.key) own += row.mass(q);
+    const Scale sc(top, s.t);
+    int n = -1;
+    if (s.k || s.p < 1.0f || s.least > 0.0) {
+        uint64_t total = 0;
+        if (s.need_sum()) {
+            uint64_t own = 0;
+            row.each([&](float z, uint32_t) { own += out.w.mass(z); });
+            total = block_sum(own, sm);
         }
-        const uint64_t total = block_sum(own, sm.part) + (cut.key ? cut.ties * row.mass(cut.key) : 0);
-        const double want = ceil(double(p) * double(total));
-        const uint64_t target = want < 1.0 ? 1 : uint64_t(want);
-        cut = find_cut(row, sm, target < total ? target : total, cut,
-                       [&](uint32_t q) { return row.mass(q); });
+        n = make_list(
+            s, sc, sm, total, out.w,
+            [&](auto&& f) {
+#pragma unroll
+                for (int j = 0; j < E; j += 8) {
+                    float m = row.z[j];
+#pragma unroll
+                    for (int c = 1; c < 8; ++c) m = fmaxf(m, row.z[j + c]);
+                    f(m);
+                }
+            },
+            [&](int last, auto&& f) {
+                if (sc.bin(zmax) > last || zmax == -INFINITY) return;
+                row.each(f);
+            });
+        if (n >= 0) {
+            finish_list(n, s, u, total, sm, out);
+            return;
+        }
     }
-    const float mp = a.min_p ? a.min_p[r] : 0.0f;
-    const double least = mp > 0.0f ? (mp < 1.0f ? double(mp) : 1.0) : 0.0;
+    finish_row(row, p, s, u, sm, out);
+}
 
-    // The kept masses in index order: ranges of the row, one per wave, then
-    // the range that holds the drawn token in 16 again, down to one element
-    // a lane.
-    auto kept_mass = [&](uint32_t q) -> uint64_t {
-        return least > 0.0 && row.weight(q) < least ? 0 : row.mass(q);
-    };
-    const uint64_t tie_mass = cut.key ? kept_mass(cut.key) : 0;
-    int64_t lo = 0, n = row.n;
-    uint64_t ties_before = 0, target = 0, total = 0;
-    for (int level = 0;; ++level) {
-        const int64_t span = (n + NT / WAVE - 1) / (NT / WAVE);
-        const int64_t b = lo + wave * span, e = b + span < lo + n ? b + span : lo + n;
-        uint64_t above = 0, ties = 0;
-        for (int64_t i = b + lane; i < e; i += WAVE) {
-            const uint32_t q = row.key(i);
-            if (q > cut.key) above += kept_mass(q);
-            if (q == cut.key && cut.key) ++ties;
+// What sample_stats leaves of a long row's 2,048 logits.
+struct Chunk {
+    float max;
+    uint32_t first;  // index of the first maximum
+    double sum;      // of exp((z - max) / T), where need_sum()
+};
+
+template <typename T, int VEC>
+__global__ __launch_bounds__(256) void sample_stats(SampleArgs a, Chunk* chunks, float* groups, int64_t nchunk) {
+    constexpr int L = CHUNK / WAVE / VEC, G = GROUP / VEC;  // loads of a lane; lanes of a group
+    const int lane = int(threadIdx.x) % WAVE;
+    const int64_t id = int64_t(blockIdx.x) * 4 + int(threadIdx.x) / WAVE;
+    if (id >= a.rows * nchunk) return;
+    const int64_t r = id / nchunk, c = id - r * nchunk;
+    const T* p = static_cast<const T*>(a.logits) + r * a.ld;
+    float z[L][VEC];
+#pragma unroll
+    for (int j = 0; j < L; ++j) {
+        const int64_t i = c * CHUNK + (j * WAVE + lane) * VEC;
+        if (i + VEC <= a.vocab) {
+            typedef T vec __attribute__((ext_vector_type(VEC)));
+            const vec v = *reinterpret_cast<const vec*>(p + i);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) z[j][e] = float(v[e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) z[j][e] = i + e < a.vocab ? float(p[i + e]) : -INFINITY;
         }
-        above = wave_sum_u64(above);
-        ties = wave_sum_u64(ties);
-        __syncthreads();
-        if (lane == 0) sm.part[wave] = above, sm.part2[wave] = ties;
-        __syncthreads();
-        // every thread runs over the 16 ranges
-        auto range_mass = [&](int i, uint64_t& seen) {
-            const uint64_t left = cut.ties > seen ? cut.ties - seen : 0;
-            const uint64_t use = sm.part2[i] < left ? sm.part2[i] : left;
-            seen += sm.part2[i];
-            return sm.part[i] + use * tie_mass;
-        };
-        if (level == 0) {
-            uint64_t seen = 0;
-            for (int i = 0; i < NT / WAVE; ++i) total += range_mass(i, seen);
-            const float u = a.u[r];
-            const double t = (u > 0.0f ? (u < 1.0f ? double(u) : 1.0) : 0.0) * double(total);
-            target = uint64_t(t) + 1;  // the first running mass > u total
-            if (target > total) target = total;
+    }
+    const Settings s = settings_of(a, r);
+    float top = -INFINITY;
+    float* gr = groups + r * nchunk * (CHUNK / GROUP) + c * (CHUNK / GROUP);
+#pragma unroll
+    for (int j = 0; j < L; ++j) {
+        float m = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            z[j][e] = clean(z[j][e]);
+            m = fmaxf(m, z[j][e]);
         }
-        uint64_t seen = ties_before, run = 0;
-        int pick = 0;
-        for (; pick < NT / WAVE; ++pick) {
-            const uint64_t s0 = seen;
-            const uint64_t m = range_mass(pick, seen);
-            if (run + m >= target) {
-                seen = s0;
-                break;
+        top = fmaxf(top, m);
+#pragma unroll
+        for (int o = 1; o < G; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, WAVE));
+        if (lane % G == 0) gr[(j * WAVE + lane) / G] = m;
+    }
+    top = wave_max(top);
+    uint32_t first = 0xffffffffu;
+#pragma unroll
+    for (int j = L - 1; j >= 0; --j)
+#pragma unroll
+        for (int e = VEC - 1; e >= 0; --e)
+            if (z[j][e] == top) first = uint32_t(c * CHUNK + (j * WAVE + lane) * VEC + e);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        const uint32_t x = __shfl_xor(first, o, WAVE);
+        first = x < first ? x : first;
+    }
+    double sum = 0.0;
+    if (s.need_sum() && top > -INFINITY) {
+        const Weigh w{double(top), s.inv_t};
+#pragma unroll
+        for (int j = 0; j < L; ++j)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) sum += w(z[j][e]);
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, WAVE);
+    }
+    if (lane == 0) chunks[id] = Chunk{top, first, sum};
+}
+
+template <typename T>
+__global__ __launch_bounds__(NT) void sample_long(SampleArgs a, const Chunk* chunks, const float* groups,
+                                                  int64_t nchunk) {
+    __shared__ Shared sm;
+    const int64_t r = blockIdx.x;
+    const int tid = int(threadIdx.x);
+    const Settings s = settings_of(a, r);
+    const float u = a.u[r];
+    chunks += r * nchunk;
+    groups += r * nchunk * (CHUNK / GROUP);
+    const MemoryRow<T> row{static_cast<const T*>(a.logits) + r * a.ld, a.vocab};
+    if (tid == 0) sm.kmax = 0, sm.kfirst = 0xffffffffu;
+    __syncthreads();
+    const Chunk mine = tid < nchunk ? chunks[tid] : Chunk{-INFINITY, 0xffffffffu, 0.0};  // (nchunk <= NT)
+    const float wmax = wave_max(mine.max);
+    if (tid % WAVE == 0) atomicMax(&sm.kmax, key_of(wmax));
+    __syncthreads();
+    const uint32_t kmax = sm.kmax;
+    const float top = value_of(kmax);
+    Result out{a.tokens + r, a.logprob ? a.logprob + r : nullptr, {double(top), s.inv_t}};
+    if (kmax == 0) {
+        if (tid == 0) nothing_left(out);
+        return;
+    }
+    if (s.greedy) {
+        if (mine.max == top) atomicMin(&sm.kfirst, mine.first);
+        __syncthreads();
+        if (tid == 0) {
+            *out.token = int32_t(sm.kfirst);
+            if (out.logprob) *out.logprob = 0.0f;
+        }
+        return;
+    }
+    uint64_t own = 0, total = 0;
+    if (s.need_sum()) {
+        // (a chunk has a mass where one of its logits has)
+        const double x = out.w(mine.max);
+        if (Weigh::fixed(x)) own = uint64_t(rint(mine.sum * x * ONE));
+        total = block_sum(own, sm);
+    }
+    if (s.k == 0 && s.p >= 1.0f && s.least == 0.0) {
+        sm.hist[tid] = own;
+        const uint64_t target = goal(u, total);
+        pick<false>(sm.hist, NT, target, sm);
+        const int64_t c = sm.bin;
+        const uint64_t left = target - sm.before;
+        // the chunk's segments, then the segment
+        const MemoryRow<T> part{row.p + c * CHUNK, a.vocab - c * CHUNK < CHUNK ? a.vocab - c * CHUNK : CHUNK};
+        auto mass = [&](float z, uint32_t) { return out.w.mass(z); };
+        __syncthreads();
+        part.sums(sm.item, mass);
+        pick<false>(sm.item, part.segments(), left, sm);
+        // (the chunk's sum and its logits' masses differ by their rounding:
+        // past the end is the last logit with a mass)
+        int seg = int(sm.bin);
+        uint64_t target2 = left > sm.before ? left - sm.before : 1;
+        if (sm.total < left) {
+            while (seg > 0 && sm.item[seg] == 0) --seg;
+            target2 = sm.item[seg];
+        }
+        draw_in(row.p, a.vocab, c * CHUNK + int64_t(seg) * SEG, SEG, target2, total, out, mass);
+        return;
+    }
+    const Scale sc(top, s.t);
+    const int64_t ngroup = (a.vocab + GROUP - 1) / GROUP;
+    const int n = make_list(
+        s, sc, sm, total, out.w,
+        [&](auto&& f) {
+            for (int64_t g = tid; g < ngroup; g += NT) f(groups[g]);
+        },
+        [&](int last, auto&& f) {
+            for (int64_t g = tid; g < ngroup; g += NT) {
+                const float m = groups[g];
+                if (m == -INFINITY || sc.bin(m) > last) continue;
+                for (int64_t i = g * GROUP; i < (g + 1) * GROUP && i < a.vocab; ++i) {
+                    const float z = clean(float(row.p[i]));
+                    if (z != -INFINITY) f(z, uint32_t(i));
+                }
             }
-            run += m;
-        }
-        target -= run;
-        ties_before = seen;
-        lo += pick * span;
-        n = n - pick * span < span ? n - pick * span : span;
-        if (n <= WAVE) break;
-    }
-    if (wave == 0) {
-        const uint32_t q = lane < n ? row.key(lo + lane) : 0;
-        const uint64_t mine = q == cut.key && cut.key ? 1 : 0;
-        const uint64_t rank = ties_before + wave_scan_u64(mine, lane);
-        const uint64_t m = q > cut.key ? kept_mass(q) : mine && rank <= cut.ties ? tie_mass : 0;
-        const uint64_t run = wave_scan_u64(m, lane);
-        const uint64_t hit = __ballot(run >= target && m > 0);
-        if (hit && lane == __builtin_ctzll(hit)) {
-            a.tokens[r] = int32_t(lo + lane);
-            const double d = double(value_of(q)) - row.max;
-            if (a.logprob) a.logprob[r] = float((d < 0.0 ? d * row.inv_t : 0.0) - log(double(total) / 4398046511104.0));
-        }
-    }
+        });
+    if (n >= 0)
+        finish_list(n, s, u, total, sm, out);
+    else
+        finish_row(row, row.p, s, u, sm, out);
 }
 
 void check(const SampleArgs& a) {
     if (a.dtype != ELEM_F32 && a.dtype != ELEM_F16 && a.dtype != ELEM_BF16)
         fail(E_INVALID, "sample: logits must be f32, f16 or bf16");
     if (a.rows <= 0 || a.rows > (1 << 24)) fail(E_INVALID, "sample: rows must be 1 to 2^24");
-    if (a.vocab <= 0 || a.vocab > (1 << 20)) fail(E_INVALID, "sample: vocab must be 1 to 2^20");
+    if (a.vocab <= 0 || a.vocab > (1 << IDX_BITS)) fail(E_INVALID, "sample: vocab must be 1 to 2^20");
+}
+
+constexpr int64_t SHORT = 32 * NT;
+int64_t chunks_of(int64_t vocab) { return (vocab + CHUNK - 1) / CHUNK; }
+
+template <typename T>
+void launch(hipStream_t s, const SampleArgs& a, void* workspace) {
+    const dim3 grid{unsigned(a.rows)}, block{NT};
+    if (a.vocab <= 8 * NT) {
+        sample_short<T, 8><<<grid, block, 0, s>>>(a);
+    } else if (a.vocab <= SHORT) {
+        sample_short<T, 32><<<grid, block, 0, s>>>(a);
+    } else {
+        const int64_t nchunk = chunks_of(a.vocab);
+        Chunk* chunks = static_cast<Chunk*>(workspace);
+        float* groups = reinterpret_cast<float*>(chunks + a.rows * nchunk);
+        const dim3 wide{unsigned((a.rows * nchunk + 3) / 4)};
+        constexpr int VEC = 16 / int(sizeof(T));
+        if (reinterpret_cast<uintptr_t>(a.logits) % 16 == 0 && a.ld % VEC == 0)
+            sample_stats<T, VEC><<<wide, dim3(256), 0, s>>>(a, chunks, groups, nchunk);
+        else
+            sample_stats<T, 1><<<wide, dim3(256), 0, s>>>(a, chunks, groups, nchunk);
+        OMG_HIP(hipGetLastError());
+        sample_long<T><<<grid, block, 0, s>>>(a, chunks, groups, nchunk);
+    }
+    OMG_HIP(hipGetLastError());
 }
 
 }  // namespace
@@ -261,23 +837,25 @@ int64_t sample_workspace(int64_t rows, int64_t vocab) {
     SampleArgs a{};
     a.rows = rows, a.vocab = vocab;
     check(a);
-    return 0;
+    return vocab <= SHORT ? 0 : rows * chunks_of(vocab) * int64_t(sizeof(Chunk) + CHUNK / GROUP * 4);
 }
 
 void launch_sample(hipStream_t s, const SampleArgs& a, void* workspace, size_t bytes) {
+    const int64_t need = sample_workspace(a.rows, a.vocab);
     check(a);
     if (a.ld < a.vocab) fail(E_INVALID, "sample: ld must hold the vocabulary");
     if (!a.logits || !a.u || !a.tokens) fail(E_INVALID, "sample: null logits, u or tokens");
     if (reinterpret_cast<uintptr_t>(a.logits) % (a.dtype == ELEM_F32 ? 4 : 2))
         fail(E_INVALID, "sample: logits must be aligned to their type");
-    const dim3 grid{unsigned(a.rows)}, block{NT};
+    if (int64_t(bytes) < need) fail(E_CAPACITY, "sample: the workspace needs " + std::to_string(need) + " bytes");
+    if (need && (!workspace || !aligned16(workspace)))
+        fail(E_INVALID, "sample: the workspace must be 16-byte aligned");
     if (a.dtype == ELEM_F32)
-        sample_kernel<float><<<grid, block, 0, s>>>(a);
+        launch<float>(s, a, workspace);
     else if (a.dtype == ELEM_F16)
-        sample_kernel<half_t><<<grid, block, 0, s>>>(a);
+        launch<half_t>(s, a, workspace);
     else
-        sample_kernel<bf16_t><<<grid, block, 0, s>>>(a);
-    OMG_HIP(hipGetLastError());
+        launch<bf16_t>(s, a, workspace);
 }
 
 }  // namespace omg

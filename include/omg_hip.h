@@ -430,9 +430,10 @@ int omg_dev_attention_shared(const omg_paged_kv *kv, const omg_paged_batch *b, i
  * (>= 1 or NaN: off), min_p (<= 0 or NaN: off).  u outside [0, 1) counts as
  * the nearest inside, NaN as 0.
  * Masked tokens are -infinity or NaN and are never drawn; a row with nothing
- * else gives token -1 and logprob -infinity.  Masses are 64-bit fixed-point
- * sums of w rounded to 2^-42, so a token under 2^-43 of the largest is not
- * drawn, and the result does not depend on the order of the sums.
+ * else gives token -1 and logprob -infinity.  Masses are sums of w rounded
+ * to 2^-42 (the whole mass of a row of more than 32,768 tokens: sums of w in
+ * 64 bits), so a token under 2^-43 of the largest is not drawn, and the same
+ * call gives the same tokens.
  * vocab up to 2^20.  workspace: omg_dev_sample_workspace bytes (negative: an
  * OMG_E_* status), 16-byte aligned, this call's own until it has run. */
 int64_t omg_dev_sample_workspace(int64_t rows, int64_t vocab);

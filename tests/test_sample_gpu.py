@@ -57,8 +57,8 @@ def draw(z, u, temp=None, k=None, p=None, mp=None, dtype="f32", pad=0, logprob=T
     rows, vocab = z.shape
     buf = torch.full((rows, vocab + pad), 1e4, dtype=TYPES[dtype], device="cuda")
     buf[:, :vocab] = torch.as_tensor(z).to(TYPES[dtype])
-    ud = torch.as_tensor(np.asarray(u, np.float32)).cuda()
-    par = {n: torch.as_tensor(np.asarray(v, t)).cuda() for n, v, t in
+    ud = torch.as_tensor(np.array(u, np.float32)).cuda()
+    par = {n: torch.as_tensor(np.array(v, t)).cuda() for n, v, t in
            (("temperature", temp, np.float32), ("top_k", k, np.int32), ("top_p", p, np.float32),
             ("min_p", mp, np.float32)) if v is not None}
     tok = torch.full((rows + 1,), -7, dtype=torch.int32, device="cuda")
