@@ -21,6 +21,7 @@
 // comparing all pairs (up to 256) or by histograms over the items' digits.
 // Rows whose kept tokens do not fit the list run the same digits over the
 // whole row.
+#include <algorithm>
 #include <string>
 
 #include "common.h"
@@ -236,6 +237,23 @@ __device__ uint64_t find_cut(S&& src, Shared& sm, uint64_t target, uint64_t limi
     return cut > limit ? cut : limit;
 }
 
+// Counts of group maxima by their distance from the row's maximum, in bins
+// of T / 64 or 1/32, whichever is narrower.  A threshold is a bin's far edge
+// (with a slack for the rounding of the bins).
+struct Scale {
+    float max, per;  // bins per unit of z
+    bool whole;      // what lies past the last bin has no mass
+    __device__ Scale(float m, float t) : max(m) {
+        const float f = 64.0f / t;
+        per = f > 32.0f ? (f < 1e30f ? f : 1e30f) : 32.0f;
+        whole = float(BINS - 1) > 30.5f * t * per;  // e^-29.9 < 2^-43
+    }
+    __device__ int bin(float z) const {
+        const float x = (max - z) * per;
+        return x < float(BINS - 1) ? int(x) : BINS - 1;  // (NaN, infinity - infinity: the last)
+    }
+};
+
 // A row that is worked on as a whole: each(f) calls f(z, index) for the
 // thread's logits, SEG consecutive ones a wave; segment(s, f) for a lane's of
 // segment s (in lane order).
@@ -244,24 +262,35 @@ struct RegisterRow {
     float z[E];
     int64_t n;
     __device__ uint32_t index(int j) const { return uint32_t(((j / 4) * NT + threadIdx.x) * 4 + j % 4); }
+    // Every load is issued before the first use: addresses past the row are
+    // moved into it and their values masked.
     __device__ void load(const T* p, int64_t vocab) {
         n = vocab;
-        const bool wide = reinterpret_cast<uintptr_t>(p) % (4 * sizeof(T)) == 0;
+        const bool wide = reinterpret_cast<uintptr_t>(p) % (4 * sizeof(T)) == 0 && n >= 4;
+        if (wide) {
+            typedef T vec __attribute__((ext_vector_type(4)));
+            vec v[E / 4];
 #pragma unroll
-        for (int j = 0; j < E; j += 4) {
-            const int64_t i = index(j);
-            if (wide && i + 4 <= n) {
-                typedef T vec __attribute__((ext_vector_type(4)));
-                const vec v = *reinterpret_cast<const vec*>(p + i);
-#pragma unroll
-                for (int c = 0; c < 4; ++c) z[j + c] = float(v[c]);
-            } else {
-#pragma unroll
-                for (int c = 0; c < 4; ++c) z[j + c] = i + c < n ? float(p[i + c]) : -INFINITY;
+            for (int j = 0; j < E; j += 4) {
+                const int64_t i = index(j);
+                v[j / 4] = *reinterpret_cast<const vec*>(p + (i + 4 <= n ? i : 0));
             }
-        }
+            const int64_t tail = n & ~int64_t(3);
+            float rest[3];
 #pragma unroll
-        for (int j = 0; j < E; ++j) z[j] = clean(z[j]);
+            for (int c = 0; c < 3; ++c) rest[c] = float(p[tail + c < n ? tail + c : n - 1]);
+#pragma unroll
+            for (int j = 0; j < E; ++j) {
+                const int64_t i = index(j);
+                const float last = j % 4 < 3 && i < n ? rest[j % 4 < 3 ? j % 4 : 0] : -INFINITY;
+                z[j] = clean(i - j % 4 + 4 <= n ? float(v[j / 4][j % 4]) : last);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < E; ++j) z[j] = float(p[index(j) < n ? index(j) : n - 1]);
+#pragma unroll
+            for (int j = 0; j < E; ++j) z[j] = index(j) < n ? clean(z[j]) : -INFINITY;
+        }
     }
     template <typename F>
     __device__ void each(F&& f) const {
@@ -366,37 +395,6 @@ __device__ inline void draw_in(const T* p, int64_t n, int64_t first, int count, 
     if (lane == 0 && index >= 0) out.write(drawn, uint32_t(index), total);
 }
 
-// The exact cuts and the draw over the whole row.
-template <typename T, typename R>
-__device__ void finish_row(const R& row, const T* p, const Settings& s, float u, Shared& sm, const Result& out) {
-    const Weigh& w = out.w;
-    auto items = [&](auto&& f) { row.each([&](float z, uint32_t i) { f(item_of(z, i), 0); }); };
-    uint64_t cut = 1;  // every unmasked item
-    if (s.k) cut = find_cut(items, sm, uint64_t(s.k), cut, [](uint64_t, int) { return uint64_t(1); });
-    if (s.p < 1.0f) {
-        uint64_t own = 0;
-        row.each([&](float z, uint32_t i) {
-            if (item_of(z, i) >= cut) own += w.mass(z);
-        });
-        const uint64_t total = block_sum(own, sm);
-        cut = find_cut(items, sm, share_of(s.p, total), cut, [&](uint64_t it, int) { return w.mass(item_value(it)); });
-    }
-    auto kept = [&](float z, uint32_t i) -> uint64_t {
-        if (item_of(z, i) < cut) return 0;
-        const double x = w(z);
-        return x >= s.least ? Weigh::fixed(x) : 0;
-    };
-    __syncthreads();
-    row.sums(sm.item, kept);
-    const int ns = row.segments();
-    uint64_t own = 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < ns; i += NT) own += sm.item[i];
-    const uint64_t total = block_sum(own, sm), target = goal(u, total);
-    pick<false>(sm.item, ns, target, sm);
-    draw_in(p, row.n, int64_t(sm.bin) * SEG, SEG, target - sm.before, total, out, kept);
-}
-
 // The exact cuts and the draw over the list's n items (every item that can
 // be kept is there); `row_mass`: the mass that top_p is a share of, unless
 // top_k is on.
@@ -483,23 +481,6 @@ __device__ void finish_list(int n, const Settings& s, float u, uint64_t row_mass
     });
 }
 
-// Counts of group maxima by their distance from the row's maximum, in bins
-// of T / 64 or 1/32, whichever is narrower.  A threshold is a bin's far edge
-// (with a slack for the rounding of the bins).
-struct Scale {
-    float max, per;  // bins per unit of z
-    bool whole;      // what lies past the last bin has no mass
-    __device__ Scale(float m, float t) : max(m) {
-        const float f = 64.0f / t;
-        per = f > 32.0f ? (f < 1e30f ? f : 1e30f) : 32.0f;
-        whole = float(BINS - 1) > 30.5f * t * per;  // e^-29.9 < 2^-43
-    }
-    __device__ int bin(float z) const {
-        const float x = (max - z) * per;
-        return x < float(BINS - 1) ? int(x) : BINS - 1;  // (NaN, infinity - infinity: the last)
-    }
-};
-
 // Gathers into the list the row's logits that lie in bins 0 .. last, by
 // gather(f): f(z, i) is called for all of them at least.  The count may pass
 // CAP: then the list does not hold them all.
@@ -520,8 +501,8 @@ __device__ inline int gather(Shared& sm, G&& each, int last, const Scale& sc) {
 
 // The list that holds every token that the filters can keep, if one can be
 // had: its length, or -1.  maxima(f) calls f(z) for the maxima of the
-// thread's groups, each(last bin, f) for the logits of the groups that reach
-// that bin.
+// thread's groups, each(last bin, f), called by the whole workgroup, f(z, i)
+// for the logits of the groups that reach that bin.
 template <typename Q, typename G>
 __device__ int make_list(const Settings& s, const Scale& sc, Shared& sm, uint64_t row_mass, const Weigh& w, Q&& maxima,
                          G&& each) {
@@ -564,6 +545,90 @@ __device__ int make_list(const Settings& s, const Scale& sc, Shared& sm, uint64_
         if (block_sum(own, sm) >= target) return n;
     }
     return -1;
+}
+
+// The cut over a whole row, found from the sums of `share` by bins of the
+// distance from the maximum (in sm.hist): the first items at which the
+// running share reaches `target` lie in one bin, whose items are gathered,
+// each(bin, f) calling f(z, i) for all logits of that bin at least.
+template <typename R, typename G, typename F>
+__device__ uint64_t cut_by_bins(const R& row, const Scale& sc, Shared& sm, uint64_t target, G&& each, F&& share) {
+    pick<false>(sm.hist, BINS, target, sm);
+    const int bin = int(sm.bin);
+    const uint64_t left = target - sm.before;
+    __syncthreads();
+    if (threadIdx.x == 0) sm.count = 0;
+    __syncthreads();
+    each(bin, [&](float z, uint32_t i) {
+        if (sc.bin(z) == bin) {
+            const int at = atomicAdd(&sm.count, 1);
+            if (at < CAP) sm.item[at] = item_of(z, i);
+        }
+    });
+    __syncthreads();
+    const int n = sm.count;
+    if (n <= CAP) {
+        auto items = [&](auto&& f) {
+            for (int i = threadIdx.x; i < n; i += NT) f(sm.item[i], i);
+        };
+        const uint64_t edge = find_cut(items, sm, left, 1, [&](uint64_t it, int) { return share(item_value(it)); });
+        // (the edge may lie below the bin: the last item of the bin above it)
+        __syncthreads();
+        if (threadIdx.x == 0) sm.before = ~uint64_t(0);
+        __syncthreads();
+        items([&](uint64_t it, int) {
+            if (it >= edge) atomicMin(reinterpret_cast<unsigned long long*>(&sm.before), static_cast<unsigned long long>(it));
+        });
+        __syncthreads();
+        const uint64_t cut = sm.before;
+        __syncthreads();
+        return cut == ~uint64_t(0) ? 1 : cut;  // (nothing in the last bin: all stay)
+    }
+    auto items = [&](auto&& f) { row.each([&](float z, uint32_t i) { f(item_of(z, i), 0); }); };
+    return find_cut(items, sm, target, 1, [&](uint64_t it, int) { return share(item_value(it)); });
+}
+
+// The exact cuts and the draw over the whole row.
+template <typename T, typename R>
+__device__ void finish_row(const R& row, const T* p, const Settings& s, float u, const Scale& sc, Shared& sm,
+                           const Result& out) {
+    const Weigh& w = out.w;
+    uint64_t cut = 1;  // every unmasked item
+    auto any = [&](int, auto&& f) { row.each(f); };
+    auto count = [](float) { return uint64_t(1); };
+    if (s.k) {
+        clear(sm.hist, BINS);
+        row.each([&](float z, uint32_t) { add(&sm.hist[sc.bin(z)], 1); });
+        cut = cut_by_bins(row, sc, sm, uint64_t(s.k), any, count);
+    }
+    if (s.p < 1.0f) {
+        clear(sm.hist, BINS);
+        uint64_t own = 0;
+        row.each([&](float z, uint32_t i) {
+            if (item_of(z, i) < cut) return;
+            const uint64_t m = w.mass(z);
+            own += m;
+            if (m) add(&sm.hist[sc.bin(z)], m);
+        });
+        const uint64_t total = block_sum(own, sm);
+        // (a mass of top_k's cut that lies past top_p's is not reached)
+        const uint64_t c = cut_by_bins(row, sc, sm, share_of(s.p, total), any, [&](float z) { return w.mass(z); });
+        cut = c > cut ? c : cut;
+    }
+    auto kept = [&](float z, uint32_t i) -> uint64_t {
+        if (item_of(z, i) < cut) return 0;
+        const double x = w(z);
+        return x >= s.least ? Weigh::fixed(x) : 0;
+    };
+    __syncthreads();
+    row.sums(sm.item, kept);
+    const int ns = row.segments();
+    uint64_t own = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < ns; i += NT) own += sm.item[i];
+    const uint64_t total = block_sum(own, sm), target = goal(u, total);
+    pick<false>(sm.item, ns, target, sm);
+    draw_in(p, row.n, int64_t(sm.bin) * SEG, SEG, target - sm.before, total, out, kept);
 }
 
 __device__ inline void nothing_left(const Result& out) {
@@ -639,7 +704,7 @@ __global__ __launch_bounds__(NT) void sample_short(SampleArgs a) {
             return;
         }
     }
-    finish_row(row, p, s, u, sm, out);
+    finish_row(row, p, s, u, sc, sm, out);
 }
 
 // What sample_stats leaves of a long row's 2,048 logits.
@@ -712,18 +777,91 @@ __global__ __launch_bounds__(256) void sample_stats(SampleArgs a, Chunk* chunks,
     if (lane == 0) chunks[id] = Chunk{top, first, sum};
 }
 
+// Long rows whose kept tokens do not fit a list, between the kernels.
+struct Pending {
+    uint64_t cut;       // the first item that goes
+    uint32_t kmax;
+    uint32_t step;      // 0: done; 1: the cut is to be found; 2: the draw
+    uint32_t arrived[2];
+};
+struct Workspace {
+    Chunk* chunks;      // [rows][nchunk]
+    float* groups;      // [rows][nchunk * CHUNK / GROUP]
+    Pending* pending;   // [rows]
+    uint64_t* hist;     // [rows][BINS]
+    uint64_t* segs;     // [rows][nchunk * CHUNK / SEG]
+    int64_t nchunk;
+    Workspace from(int64_t r) const {
+        Workspace w = *this;
+        w.chunks += r * nchunk, w.groups += r * nchunk * (CHUNK / GROUP), w.pending += r;
+        w.hist += r * BINS, w.segs += r * nchunk * (CHUNK / SEG);
+        return w;
+    }
+};
+
+constexpr int PER = 16;  // logits of a thread of the wide kernels
+constexpr int PART = PER * NT;
+
+// The logits of the groups of GROUP whose maxima reach bin `last`: the
+// groups' numbers are collected first, so that four threads a group read
+// them, two groups at a time in flight.
+template <typename T, typename F>
+__device__ inline void each_of_groups(const T* p, int64_t n, const float* groups, const Scale& sc, int last, Shared& sm,
+                                      F&& f) {
+    uint32_t* ids = reinterpret_cast<uint32_t*>(sm.mass);
+    constexpr int MOST = int(sizeof(sm.mass) / 4);  // (a row has up to 2^16 groups)
+    const int64_t ngroup = (n + GROUP - 1) / GROUP;
+    const bool wide = reinterpret_cast<uintptr_t>(p) % (4 * sizeof(T)) == 0;
+    for (int64_t g0 = 0; g0 < ngroup; g0 += MOST) {
+        const int64_t g1 = g0 + MOST < ngroup ? g0 + MOST : ngroup;
+        __syncthreads();
+        if (threadIdx.x == 0) sm.bin = 0;
+        __syncthreads();
+        for (int64_t g = g0 + threadIdx.x; g < g1; g += NT) {
+            const float m = groups[g];
+            if (m != -INFINITY && sc.bin(m) <= last) ids[atomicAdd(&sm.bin, 1u)] = uint32_t(g);
+        }
+        __syncthreads();
+        const int count = int(sm.bin);
+        for (int k = int(threadIdx.x) / 4; k < count; k += NT / 2) {
+            const int k2 = k + NT / 4;
+            const int64_t i0 = int64_t(ids[k]) * GROUP + threadIdx.x % 4 * 4;
+            const int64_t i1 = k2 < count ? int64_t(ids[k2]) * GROUP + threadIdx.x % 4 * 4 : i0;
+            float z[8];
+            if (wide && i0 + 4 <= n && i1 + 4 <= n) {
+                typedef T vec __attribute__((ext_vector_type(4)));
+                const vec v0 = *reinterpret_cast<const vec*>(p + i0), v1 = *reinterpret_cast<const vec*>(p + i1);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) z[c] = float(v0[c]), z[4 + c] = float(v1[c]);
+            } else {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    z[c] = i0 + c < n ? float(p[i0 + c]) : -INFINITY;
+                    z[4 + c] = i1 + c < n ? float(p[i1 + c]) : -INFINITY;
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const float x = clean(z[c]), y = clean(z[4 + c]);
+                if (x != -INFINITY) f(x, uint32_t(i0 + c));
+                if (k2 < count && y != -INFINITY) f(y, uint32_t(i1 + c));
+            }
+        }
+    }
+    __syncthreads();
+}
+
 template <typename T>
-__global__ __launch_bounds__(NT) void sample_long(SampleArgs a, const Chunk* chunks, const float* groups,
-                                                  int64_t nchunk) {
+__global__ __launch_bounds__(NT) void sample_long(SampleArgs a, Workspace ws) {
     __shared__ Shared sm;
-    const int64_t r = blockIdx.x;
+    const int64_t r = blockIdx.x, nchunk = ws.nchunk;
     const int tid = int(threadIdx.x);
     const Settings s = settings_of(a, r);
     const float u = a.u[r];
-    chunks += r * nchunk;
-    groups += r * nchunk * (CHUNK / GROUP);
+    const Chunk* chunks = ws.chunks + r * nchunk;
+    const float* groups = ws.groups + r * nchunk * (CHUNK / GROUP);
     const MemoryRow<T> row{static_cast<const T*>(a.logits) + r * a.ld, a.vocab};
-    if (tid == 0) sm.kmax = 0, sm.kfirst = 0xffffffffu;
+    if (tid == 0) sm.kmax = 0, sm.kfirst = 0xffffffffu, ws.pending[r].step = 0;
     __syncthreads();
     const Chunk mine = tid < nchunk ? chunks[tid] : Chunk{-INFINITY, 0xffffffffu, 0.0};  // (nchunk <= NT)
     const float wmax = wave_max(mine.max);
@@ -782,20 +920,132 @@ __global__ __launch_bounds__(NT) void sample_long(SampleArgs a, const Chunk* chu
         [&](auto&& f) {
             for (int64_t g = tid; g < ngroup; g += NT) f(groups[g]);
         },
-        [&](int last, auto&& f) {
-            for (int64_t g = tid; g < ngroup; g += NT) {
-                const float m = groups[g];
-                if (m == -INFINITY || sc.bin(m) > last) continue;
-                for (int64_t i = g * GROUP; i < (g + 1) * GROUP && i < a.vocab; ++i) {
-                    const float z = clean(float(row.p[i]));
-                    if (z != -INFINITY) f(z, uint32_t(i));
-                }
-            }
-        });
-    if (n >= 0)
+        [&](int last, auto&& f) { each_of_groups(row.p, row.n, groups, sc, last, sm, f); });
+    if (n >= 0) {
         finish_list(n, s, u, total, sm, out);
-    else
-        finish_row(row, row.p, s, u, sm, out);
+        return;
+    }
+    if (s.k) {
+        finish_row(row, row.p, s, u, sc, sm, out);
+        return;
+    }
+    for (int i = tid; i < BINS; i += NT) ws.hist[r * BINS + i] = 0;
+    if (tid == 0) ws.pending[r] = Pending{1, kmax, s.p < 1.0f ? 1u : 2u, {0, 0}};
+}
+
+// Whether this workgroup is the last of its row's to arrive; what the others
+// wrote before is then visible to it.
+__device__ inline bool last_of(uint32_t* arrived, Shared& sm) {
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) sm.count = int(atomicAdd(arrived, 1u));
+    __syncthreads();
+    const bool last = sm.count == int(gridDim.x) - 1;
+    __threadfence();
+    __syncthreads();
+    return last;
+}
+__device__ inline uint64_t load_shared(const uint64_t* p) {  // written by other workgroups of this launch
+    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+template <typename T>
+struct PartRow {
+    float z[PER];
+    int64_t first;
+    __device__ uint32_t index(int j) const { return uint32_t(first + ((j / 4) * NT + threadIdx.x) * 4 + j % 4); }
+    __device__ void load(const T* p, int64_t n) {
+#pragma unroll
+        for (int j = 0; j < PER; ++j) z[j] = float(p[index(j) < n ? index(j) : n - 1]);
+#pragma unroll
+        for (int j = 0; j < PER; ++j) z[j] = index(j) < n ? clean(z[j]) : -INFINITY;
+    }
+};
+
+// The masses of pending rows by bins; the last workgroup of a row finds
+// top_p's cut.
+template <typename T>
+__global__ __launch_bounds__(NT) void sample_bins(SampleArgs a, Workspace ws) {
+    const int64_t r = blockIdx.y;
+    Pending& pd = ws.pending[r];
+    if (pd.step != 1) return;
+    __shared__ Shared sm;
+    const int tid = int(threadIdx.x);
+    const Settings s = settings_of(a, r);
+    const MemoryRow<T> row{static_cast<const T*>(a.logits) + r * a.ld, a.vocab};
+    const float top = value_of(pd.kmax);
+    const Weigh w{double(top), s.inv_t};
+    const Scale sc(top, s.t);
+    PartRow<T> part;
+    part.first = int64_t(blockIdx.x) * PART;
+    part.load(row.p, row.n);
+    clear(sm.hist, BINS);
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const uint64_t m = w.mass(part.z[j]);
+        if (m) add(&sm.hist[sc.bin(part.z[j])], m);
+    }
+    __syncthreads();
+    uint64_t* hist = ws.hist + r * BINS;
+    for (int i = tid; i < BINS; i += NT)
+        if (sm.hist[i]) add(hist + i, sm.hist[i]);
+    if (!last_of(&pd.arrived[0], sm)) return;
+    uint64_t own = 0;
+    for (int i = tid; i < BINS; i += NT) {
+        sm.hist[i] = load_shared(hist + i);
+        own += sm.hist[i];
+    }
+    const uint64_t total = block_sum(own, sm);
+    const float* groups = ws.groups + r * ws.nchunk * (CHUNK / GROUP);
+    const uint64_t cut = cut_by_bins(
+        row, sc, sm, share_of(s.p, total),
+        [&](int bin, auto&& f) { each_of_groups(row.p, row.n, groups, sc, bin, sm, f); },
+        [&](float z) { return w.mass(z); });
+    if (tid == 0) pd.cut = cut, pd.step = 2;
+}
+
+// The kept masses of pending rows by segments; the last workgroup of a row
+// draws.
+template <typename T>
+__global__ __launch_bounds__(NT) void sample_draw(SampleArgs a, Workspace ws) {
+    const int64_t r = blockIdx.y;
+    Pending& pd = ws.pending[r];
+    if (pd.step != 2) return;
+    __shared__ Shared sm;
+    const int tid = int(threadIdx.x);
+    const Settings s = settings_of(a, r);
+    const T* p = static_cast<const T*>(a.logits) + r * a.ld;
+    const Result out{a.tokens + r, a.logprob ? a.logprob + r : nullptr, {double(value_of(pd.kmax)), s.inv_t}};
+    const uint64_t cut = pd.cut;
+    auto kept = [&](float z, uint32_t i) -> uint64_t {
+        if (item_of(z, i) < cut) return 0;
+        const double x = out.w(z);
+        return x >= s.least ? Weigh::fixed(x) : 0;
+    };
+    PartRow<T> part;
+    part.first = int64_t(blockIdx.x) * PART;
+    part.load(p, a.vocab);
+    const int64_t ns = ws.nchunk * (CHUNK / SEG);
+    uint64_t* segs = ws.segs + r * ns;
+#pragma unroll
+    for (int j = 0; j < PER; j += 4) {
+        uint64_t v = 0;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+            if (part.z[j + c] != -INFINITY) v += kept(part.z[j + c], part.index(j + c));
+        v = wave_sum_u64(v);
+        const int64_t seg = part.first / SEG + j / 4 * NWAVE + tid / WAVE;
+        if (tid % WAVE == 0 && seg < ns) __hip_atomic_store(segs + seg, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    if (!last_of(&pd.arrived[1], sm)) return;
+    uint64_t own = 0;
+    for (int i = tid; i < ns; i += NT) {
+        sm.item[i] = load_shared(segs + i);
+        own += sm.item[i];
+    }
+    const uint64_t total = block_sum(own, sm), target = goal(a.u[r], total);
+    pick<false>(sm.item, int(ns), target, sm);
+    draw_in(p, a.vocab, int64_t(sm.bin) * SEG, SEG, target - sm.before, total, out, kept);
 }
 
 void check(const SampleArgs& a) {
@@ -803,6 +1053,18 @@ void check(const SampleArgs& a) {
         fail(E_INVALID, "sample: logits must be f32, f16 or bf16");
     if (a.rows <= 0 || a.rows > (1 << 24)) fail(E_INVALID, "sample: rows must be 1 to 2^24");
     if (a.vocab <= 0 || a.vocab > (1 << IDX_BITS)) fail(E_INVALID, "sample: vocab must be 1 to 2^20");
+}
+
+template <typename T>
+SampleArgs rows_from(SampleArgs a, int64_t r) {
+    a.logits = static_cast<const T*>(a.logits) + r * a.ld;
+    a.u += r, a.tokens += r;
+    if (a.logprob) a.logprob += r;
+    if (a.temperature) a.temperature += r;
+    if (a.top_k) a.top_k += r;
+    if (a.top_p) a.top_p += r;
+    if (a.min_p) a.min_p += r;
+    return a;
 }
 
 constexpr int64_t SHORT = 32 * NT;
@@ -817,16 +1079,33 @@ void launch(hipStream_t s, const SampleArgs& a, void* workspace) {
         sample_short<T, 32><<<grid, block, 0, s>>>(a);
     } else {
         const int64_t nchunk = chunks_of(a.vocab);
-        Chunk* chunks = static_cast<Chunk*>(workspace);
-        float* groups = reinterpret_cast<float*>(chunks + a.rows * nchunk);
+        Workspace ws;
+        ws.nchunk = nchunk;
+        ws.chunks = static_cast<Chunk*>(workspace);
+        ws.hist = reinterpret_cast<uint64_t*>(ws.chunks + a.rows * nchunk);
+        ws.segs = ws.hist + a.rows * BINS;
+        ws.pending = reinterpret_cast<Pending*>(ws.segs + a.rows * nchunk * (CHUNK / SEG));
+        ws.groups = reinterpret_cast<float*>(ws.pending + a.rows);
         const dim3 wide{unsigned((a.rows * nchunk + 3) / 4)};
         constexpr int VEC = 16 / int(sizeof(T));
         if (reinterpret_cast<uintptr_t>(a.logits) % 16 == 0 && a.ld % VEC == 0)
-            sample_stats<T, VEC><<<wide, dim3(256), 0, s>>>(a, chunks, groups, nchunk);
+            sample_stats<T, VEC><<<wide, dim3(256), 0, s>>>(a, ws.chunks, ws.groups, nchunk);
         else
-            sample_stats<T, 1><<<wide, dim3(256), 0, s>>>(a, chunks, groups, nchunk);
+            sample_stats<T, 1><<<wide, dim3(256), 0, s>>>(a, ws.chunks, ws.groups, nchunk);
         OMG_HIP(hipGetLastError());
-        sample_long<T><<<grid, block, 0, s>>>(a, chunks, groups, nchunk);
+        sample_long<T><<<grid, block, 0, s>>>(a, ws);
+        if (a.top_p || a.min_p) {
+            OMG_HIP(hipGetLastError());
+            for (int64_t r = 0; r < a.rows; r += 65535) {  // (a grid's second size)
+                const dim3 parts{unsigned((a.vocab + PART - 1) / PART), unsigned(std::min<int64_t>(65535, a.rows - r))};
+                const SampleArgs b = rows_from<T>(a, r);
+                const Workspace wr = ws.from(r);
+                if (a.top_p) sample_bins<T><<<parts, block, 0, s>>>(b, wr);
+                OMG_HIP(hipGetLastError());
+                sample_draw<T><<<parts, block, 0, s>>>(b, wr);
+                OMG_HIP(hipGetLastError());
+            }
+        }
     }
     OMG_HIP(hipGetLastError());
 }
@@ -837,7 +1116,10 @@ int64_t sample_workspace(int64_t rows, int64_t vocab) {
     SampleArgs a{};
     a.rows = rows, a.vocab = vocab;
     check(a);
-    return vocab <= SHORT ? 0 : rows * chunks_of(vocab) * int64_t(sizeof(Chunk) + CHUNK / GROUP * 4);
+    static_assert(sizeof(Pending) % 8 == 0 && sizeof(Chunk) % 16 == 0, "the workspace's arrays are aligned");
+    return vocab <= SHORT ? 0
+                          : rows * (chunks_of(vocab) * int64_t(sizeof(Chunk) + CHUNK / SEG * 8 + CHUNK / GROUP * 4) +
+                                    BINS * 8 + int64_t(sizeof(Pending)));
 }
 
 void launch_sample(hipStream_t s, const SampleArgs& a, void* workspace, size_t bytes) {

@@ -95,7 +95,8 @@ def logits(rng, rows, vocab, likely=20):
 
 FILTERS = [dict(), dict(temp=0.7, k=40, p=0.95), dict(temp=0.7, k=40), dict(p=0.9), dict(temp=1.5, p=0.999),
            dict(temp=0.01, p=0.5), dict(mp=0.05), dict(temp=1.3, mp=0.2, p=0.8), dict(k=1), dict(k=700, p=0.97, mp=0.001),
-           dict(temp=1.6, k=5000, p=0.9), dict(temp=0.0), dict(temp=30.0, p=0.7), dict(temp=30.0, k=4000)]
+           dict(temp=1.6, k=5000, p=0.9), dict(temp=0.0), dict(temp=30.0, p=0.7), dict(temp=30.0, k=4000),
+           dict(temp=2.0, mp=1e-6), dict(temp=1.5, p=0.97, mp=1e-4), dict(temp=1.0, p=0.95)]
 
 
 @pytest.mark.parametrize("vocab", [1, 2, 63, 64, 65, 1000, 1023, 4097, 25_000, 32_769, 70_001, 262_144])
