@@ -8,19 +8,27 @@
 // exp is taken in 64 bits: a token's border in the running mass is met by a
 // random number closer than f32's error in one row of a few hundred.
 //
-// A row costs one read where it is short: up to 32 * 1,024 logits it lies in
-// the registers of one workgroup (sample_short).  Longer rows are read once
-// by the whole chip (sample_stats: per 2,048 logits the maximum, its index
-// and, where the row's filters need it, the sum of exp; per 16 the maximum),
-// then one workgroup a row finishes (sample_long).  Both look for a
+// Rows of up to 32,768 logits take one workgroup each (sample_short), which
+// reads them once from memory and again from its L2.  Longer rows are read
+// once by the whole chip (sample_stats: per 2,048 logits the maximum, its
+// index and, where the row's filters need it, the sum of exp; per 16 the
+// maximum), then one workgroup a row finishes (sample_long).  Both look for a
 // threshold that few logits pass but all that can be kept do, from the
-// maxima of small groups: the k-th largest of these maxima has k logits at
-// or above it; min_p's threshold is its own; for top_p alone a guess is
-// taken and proved by the mass above it.  The logits above it are gathered
-// into a list in LDS, where the exact cuts and the drawn token are found by
+// maxima of groups of 16: the k-th largest of these maxima has k logits at or
+// above it; min_p's threshold is its own; for top_p alone a guess is taken
+// and proved by the mass above it.  The logits above it are gathered into a
+// list in LDS, where the exact cuts and the drawn token are found by
 // comparing all pairs (up to 256) or by histograms over the items' digits.
-// Rows whose kept tokens do not fit the list run the same digits over the
-// whole row.
+// Where the kept tokens do not fit the list, the row's masses are summed by
+// bins of their distance from the maximum, which leaves one bin's logits to
+// order exactly, and the kept masses by segments in index order: by the
+// row's workgroup, or for long rows by the whole chip (sample_bins,
+// sample_draw).
+//
+// The code of a pass is kept short (rolled loops over memory, not a row in
+// registers): a workgroup that runs through it once waits for instructions
+// more than for data; a row of 25,000 held in 32 registers a thread took 14.5
+// us for its maximum alone, and 14 more for each unrolled pass of exp.
 #include <algorithm>
 #include <string>
 
@@ -40,6 +48,7 @@ constexpr int CAP = 8192;         // items of the list
 constexpr int BINS = 2048;
 constexpr int PAIRS = NT / 4;     // items compared pair by pair: four threads each
 constexpr int SEG = 256;          // consecutive logits a wave takes at once
+constexpr int64_t SHORT = 32 * NT;  // logits of a row that one workgroup takes alone
 constexpr int IDX_BITS = 20;      // vocab <= 2^20
 constexpr uint32_t IDX_MASK = (1u << IDX_BITS) - 1;
 constexpr double ONE = 4398046511104.0;  // 2^42
@@ -61,38 +70,36 @@ __device__ inline uint64_t item_of(float z, uint32_t i) {
 __device__ inline float item_value(uint64_t it) { return value_of(uint32_t(it >> IDX_BITS)); }
 __device__ inline uint32_t item_index(uint64_t it) { return IDX_MASK - (uint32_t(it) & IDX_MASK); }
 
-// exp(x) for -40 < x <= 0: x = n ln 2 + f, |f| <= ln 2 / 2, the series of
-// exp f to f^12 (its rest is below 2^-52), times 2^n.
-__device__ inline double exp_small(double x) {
-    const double n = rint(x * 1.4426950408889634);
-    double f = fma(n, -0.69314718055994529, x);
-    f = fma(n, -2.3190468138462996e-17, f);
-    double p = 1.0 / 479001600.0;
-    p = fma(p, f, 1.0 / 39916800.0);
-    p = fma(p, f, 1.0 / 3628800.0);
-    p = fma(p, f, 1.0 / 362880.0);
-    p = fma(p, f, 1.0 / 40320.0);
-    p = fma(p, f, 1.0 / 5040.0);
-    p = fma(p, f, 1.0 / 720.0);
-    p = fma(p, f, 1.0 / 120.0);
-    p = fma(p, f, 1.0 / 24.0);
-    p = fma(p, f, 1.0 / 6.0);
-    p = fma(p, f, 0.5);
-    p = fma(p, f, 1.0);
-    p = fma(p, f, 1.0);
-    return __builtin_amdgcn_ldexp(p, int(n));
-}
-
 // exp((z - max) / T) of a clean logit: 1 at the maximum, whatever it is, 0
-// where it is masked or far under 2^-43.
+// where it is masked.  With t = (z - max) log2(e) / T = n + f, |f| <= 1/2:
+// the series of 2^f = exp(f ln 2) to the 11th power (its rest is below
+// 2^-46), its exponent raised by n.
 struct Weigh {
     double max, inv_t;
     __device__ double operator()(float z) const {
-        const double d = double(z) - max;
-        if (z == -INFINITY) return 0.0;
-        if (!(d < 0.0)) return 1.0;
-        const double x = d * inv_t;
-        return x > -40.0 ? exp_small(x) : 0.0;
+        constexpr double WHOLE = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number
+        double t = (double(z) - max) * (inv_t * 1.4426950408889634);
+        t = fmax(t, -1000.0);  // (and NaN, from -infinity / infinity, to -1000)
+        const double shifted = t + WHOLE, f = t - (shifted - WHOLE);
+        constexpr double L = 0.69314718055994531;
+        constexpr double c2 = L * L / 2, c3 = c2 * L / 3, c4 = c3 * L / 4, c5 = c4 * L / 5, c6 = c5 * L / 6,
+                         c7 = c6 * L / 7, c8 = c7 * L / 8, c9 = c8 * L / 9, c10 = c9 * L / 10, c11 = c10 * L / 11;
+        double p = c11;
+        p = fma(p, f, c10);
+        p = fma(p, f, c9);
+        p = fma(p, f, c8);
+        p = fma(p, f, c7);
+        p = fma(p, f, c6);
+        p = fma(p, f, c5);
+        p = fma(p, f, c4);
+        p = fma(p, f, c3);
+        p = fma(p, f, c2);
+        p = fma(p, f, L);
+        p = fma(p, f, 1.0);
+        const uint64_t n = __builtin_bit_cast(uint64_t, shifted);  // (its low bits: n)
+        const double w = __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, p) + (n << 52));
+        // an infinite maximum leaves NaN and 2^-1000 above: its equals weigh 1
+        return max < INFINITY ? w : z < INFINITY ? 0.0 : 1.0;
     }
     __device__ uint64_t mass(float z) const { return fixed((*this)(z)); }
     // (2^52 + v rounds v to a whole number in its low bits)
@@ -216,11 +223,11 @@ __device__ inline void add(uint64_t* h, uint64_t v) {
 // share(item, i) is an item's count or mass.
 template <typename S, typename F>
 __device__ uint64_t find_cut(S&& src, Shared& sm, uint64_t target, uint64_t limit, F&& share) {
-    constexpr int digits[5] = {11, 11, 10, 10, 10};
     uint64_t prefix = 0, before = 0;
     int shift = 52;
+#pragma unroll 1
     for (int level = 0; level < 5; ++level) {
-        const int bits = digits[level];
+        const int bits = level < 2 ? 11 : 10;
         shift -= bits;
         clear(sm.hist, 1 << bits);
         src([&](uint64_t it, int i) {
@@ -255,92 +262,69 @@ struct Scale {
 };
 
 // A row that is worked on as a whole: each(f) calls f(z, index) for the
-// thread's logits, SEG consecutive ones a wave; segment(s, f) for a lane's of
-// segment s (in lane order).
-template <typename T, int E>
-struct RegisterRow {
-    float z[E];
-    int64_t n;
-    __device__ uint32_t index(int j) const { return uint32_t(((j / 4) * NT + threadIdx.x) * 4 + j % 4); }
-    // Every load is issued before the first use: addresses past the row are
-    // moved into it and their values masked.
-    __device__ void load(const T* p, int64_t vocab) {
-        n = vocab;
-        const bool wide = reinterpret_cast<uintptr_t>(p) % (4 * sizeof(T)) == 0 && n >= 4;
-        if (wide) {
-            typedef T vec __attribute__((ext_vector_type(4)));
-            vec v[E / 4];
-#pragma unroll
-            for (int j = 0; j < E; j += 4) {
-                const int64_t i = index(j);
-                v[j / 4] = *reinterpret_cast<const vec*>(p + (i + 4 <= n ? i : 0));
-            }
-            const int64_t tail = n & ~int64_t(3);
-            float rest[3];
-#pragma unroll
-            for (int c = 0; c < 3; ++c) rest[c] = float(p[tail + c < n ? tail + c : n - 1]);
-#pragma unroll
-            for (int j = 0; j < E; ++j) {
-                const int64_t i = index(j);
-                const float last = j % 4 < 3 && i < n ? rest[j % 4 < 3 ? j % 4 : 0] : -INFINITY;
-                z[j] = clean(i - j % 4 + 4 <= n ? float(v[j / 4][j % 4]) : last);
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < E; ++j) z[j] = float(p[index(j) < n ? index(j) : n - 1]);
-#pragma unroll
-            for (int j = 0; j < E; ++j) z[j] = index(j) < n ? clean(z[j]) : -INFINITY;
-        }
-    }
-    template <typename F>
-    __device__ void each(F&& f) const {
-#pragma unroll
-        for (int j = 0; j < E; ++j)
-            if (z[j] != -INFINITY) f(z[j], index(j));
-    }
-    __device__ int segments() const { return E / 4 * NWAVE; }
-    // m(z, i) summed over each segment into out[]
-    template <typename F>
-    __device__ void sums(uint64_t* out, F&& m) const {
-        const int lane = int(threadIdx.x) % WAVE, wave = int(threadIdx.x) / WAVE;
-#pragma unroll
-        for (int j = 0; j < E; j += 4) {
-            uint64_t v = 0;
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-                if (z[j + c] != -INFINITY) v += m(z[j + c], index(j + c));
-            v = wave_sum_u64(v);
-            if (lane == 0) out[j / 4 * NWAVE + wave] = v;
-        }
-    }
-};
-
+// thread's logits, sums(out, m) leaves the sums of m(z, index) over segments
+// of SEG.
 template <typename T>
-struct MemoryRow {
+struct Row {
     const T* p;
     int64_t n;
+    bool wide;  // four elements at once are aligned
+    __device__ Row(const T* row, int64_t vocab)
+        : p(row), n(vocab), wide(reinterpret_cast<uintptr_t>(row) % (4 * sizeof(T)) == 0 && vocab >= 4) {}
+    // The four logits from i (a multiple of 4) on, masked behind the row, in
+    // two steps, so that a caller's loads can be under way together.
+    typedef T vec __attribute__((ext_vector_type(4)));
+    __device__ vec load(int64_t i) const {
+        if (wide) return *reinterpret_cast<const vec*>(p + (i + 4 <= n ? i : 0));
+        vec v;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) v[c] = p[i + c < n ? i + c : 0];
+        return v;
+    }
+    __device__ void four(vec v, int64_t i, float* z) const {
+        if (i < n && i + 4 > n) {
+#pragma unroll
+            for (int c = 0; c < 3; ++c) v[c] = p[i + c < n ? i + c : 0];
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) z[c] = i + c < n ? clean(float(v[c])) : -INFINITY;
+    }
+    // f(z, i) for the four logits z of each of the thread's turns, the next
+    // two turns' loads under way; every thread makes the same turns.
+    template <typename F>
+    __device__ void turns(F&& f) const {
+        int64_t i = int64_t(threadIdx.x) * 4;
+        vec v0 = load(i), v1 = load(i + NT * 4);
+#pragma unroll 1
+        for (int64_t base = 0; base < n; base += NT * 8, i += NT * 8) {
+            const vec w0 = load(i + NT * 8), w1 = load(i + NT * 12);
+            float z[4];
+            four(v0, i, z);
+            f(z, i);
+            four(v1, i + NT * 4, z);
+            f(z, i + NT * 4);
+            v0 = w0, v1 = w1;
+        }
+    }
     template <typename F>
     __device__ void each(F&& f) const {
-        for (int64_t i = threadIdx.x; i < n; i += NT) {
-            const float z = clean(float(p[i]));
-            if (z != -INFINITY) f(z, uint32_t(i));
-        }
+        turns([&](const float* z, int64_t i) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                if (z[c] != -INFINITY) f(z[c], uint32_t(i + c));
+        });
     }
     __device__ int segments() const { return int((n + SEG - 1) / SEG); }
     template <typename F>
     __device__ void sums(uint64_t* out, F&& m) const {
-        const int lane = int(threadIdx.x) % WAVE, wave = int(threadIdx.x) / WAVE;
-        for (int s = wave; s < segments(); s += NWAVE) {
+        turns([&](const float* z, int64_t i) {
             uint64_t v = 0;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const int64_t i = int64_t(s) * SEG + lane * 4 + c;
-                const float z = i < n ? clean(float(p[i])) : -INFINITY;
-                if (z != -INFINITY) v += m(z, uint32_t(i));
-            }
+            for (int c = 0; c < 4; ++c)
+                if (z[c] != -INFINITY) v += m(z[c], uint32_t(i + c));
             v = wave_sum_u64(v);
-            if (lane == 0) out[s] = v;
-        }
+            if (threadIdx.x % WAVE == 0 && i < n) out[i / SEG] = v;
+        });
     }
 };
 
@@ -348,6 +332,10 @@ struct Result {
     int32_t* token;
     float* logprob;
     Weigh w;
+    __device__ void certain(uint32_t i) const {
+        *token = int32_t(i);
+        if (logprob) *logprob = 0.0f;
+    }
     __device__ void write(float z, uint32_t i, uint64_t total) const {
         *token = int32_t(i);
         const double d = double(z) - w.max;
@@ -481,85 +469,125 @@ __device__ void finish_list(int n, const Settings& s, float u, uint64_t row_mass
     });
 }
 
-// Gathers into the list the row's logits that lie in bins 0 .. last, by
-// gather(f): f(z, i) is called for all of them at least.  The count may pass
-// CAP: then the list does not hold them all.
-template <typename G>
-__device__ inline int gather(Shared& sm, G&& each, int last, const Scale& sc) {
+// The logits of the groups of GROUP whose maxima reach bin `last`: the
+// groups' numbers are collected first, so that four threads a group read
+// them, two groups at a time in flight.
+template <typename T, typename F>
+__device__ inline void each_of_groups(const Row<T>& row, const float* groups, const Scale& sc, int last, Shared& sm,
+                                      F&& f) {
+    uint32_t* ids = reinterpret_cast<uint32_t*>(sm.mass);
+    constexpr int MOST = int(sizeof(sm.mass) / 4);  // (a row has up to 2^16 groups)
+    const int ngroup = int((row.n + GROUP - 1) / GROUP);
+#pragma unroll 1
+    for (int g0 = 0; g0 < ngroup; g0 += MOST) {
+        const int g1 = g0 + MOST < ngroup ? g0 + MOST : ngroup;
+        __syncthreads();
+        if (threadIdx.x == 0) sm.bin = 0;
+        __syncthreads();
+        const int lane = int(threadIdx.x) % WAVE;
+        for (int g = g0 + int(threadIdx.x); g - lane < g1; g += NT) {
+            const float m = g < g1 ? groups[g] : -INFINITY;
+            const bool in = m != -INFINITY && sc.bin(m) <= last;
+            const uint64_t some = __ballot(in);
+            uint32_t at = 0;
+            if (lane == 0 && some) at = atomicAdd(&sm.bin, uint32_t(__popcll(some)));
+            at = __builtin_amdgcn_readfirstlane(at);
+            if (in) ids[at + __popcll(some & ((uint64_t(1) << lane) - 1))] = uint32_t(g);
+        }
+        __syncthreads();
+        const int count = int(sm.bin);
+#pragma unroll 1
+        for (int k = int(threadIdx.x) / 4; k < count; k += NT / 2) {
+            const int k2 = k + NT / 4;
+            const int64_t i0 = int64_t(ids[k]) * GROUP + threadIdx.x % 4 * 4;
+            const int64_t i1 = k2 < count ? int64_t(ids[k2]) * GROUP + threadIdx.x % 4 * 4 : row.n;
+            const auto v0 = row.load(i0), v1 = row.load(i1);
+            float z[8];
+            row.four(v0, i0, z);
+            row.four(v1, i1, z + 4);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                if (z[c] != -INFINITY) f(z[c], uint32_t(i0 + c));
+                if (z[4 + c] != -INFINITY) f(z[4 + c], uint32_t(i1 + c));
+            }
+        }
+    }
+    __syncthreads();
+}
+
+// Gathers into the list the row's logits that lie in bins 0 .. last.  The
+// count may pass CAP: then the list does not hold them all.
+template <typename T>
+__device__ inline int gather(const Row<T>& row, const float* groups, const Scale& sc, int last, Shared& sm) {
     __syncthreads();
     if (threadIdx.x == 0) sm.count = 0;
     __syncthreads();
-    each([&](float z, uint32_t i) {
+    each_of_groups(row, groups, sc, last, sm, [&](float z, uint32_t i) {
         if (sc.bin(z) <= last) {
             const int at = atomicAdd(&sm.count, 1);
             if (at < CAP) sm.item[at] = item_of(z, i);
         }
     });
-    __syncthreads();
     return sm.count;
 }
 
 // The list that holds every token that the filters can keep, if one can be
-// had: its length, or -1.  maxima(f) calls f(z) for the maxima of the
-// thread's groups, each(last bin, f), called by the whole workgroup, f(z, i)
-// for the logits of the groups that reach that bin.
-template <typename Q, typename G>
-__device__ int make_list(const Settings& s, const Scale& sc, Shared& sm, uint64_t row_mass, const Weigh& w, Q&& maxima,
-                         G&& each) {
+// had: its length, or -1.  groups: the maxima of the row's groups.
+template <typename T>
+__device__ int make_list(const Settings& s, const Scale& sc, Shared& sm, uint64_t row_mass, const Row<T>& row,
+                         const float* groups, const Weigh& w) {
     if (!(sc.max < INFINITY)) return -1;
-    if (s.least > 0.0 && s.k == 0) {
-        // z >= max + T log(min_p), and a bin to spare
-        const float far = float(-log(s.least) * double(s.t)) * sc.per + 1.0f;
-        const int last = far < float(BINS - 2) ? int(far) + 1 : BINS - 1;
-        if (last == BINS - 1) return -1;
-        const int n = gather(sm, [&](auto&& f) { each(last, f); }, last, sc);
-        return n <= CAP ? n : -1;
-    }
-    clear(sm.hist, BINS);
-    maxima([&](float z) {
-        if (z != -INFINITY) add(&sm.hist[sc.bin(z)], 1);
-    });
-    if (s.k) {
-        pick<false>(sm.hist, BINS, uint64_t(s.k), sm);
-        int last = int(sm.bin);
-        if (last == BINS - 1) {
-            if (!sc.whole) return -1;
-            last = BINS - 2;  // (all that have a mass)
+    const bool by_p = s.k == 0 && s.least == 0.0;
+    if (s.k || by_p) {
+        clear(sm.hist, BINS);
+        const int ngroup = int((row.n + GROUP - 1) / GROUP);
+#pragma unroll 4
+        for (int g = threadIdx.x; g < ngroup; g += NT) {
+            const float m = groups[g];
+            if (m != -INFINITY) add(&sm.hist[sc.bin(m)], 1);
         }
-        const int n = gather(sm, [&](auto&& f) { each(last, f); }, last, sc);
-        return n <= CAP ? n : -1;
     }
-    // top_p alone: the groups that hold some 100 tokens, then some 5,000
-    const uint64_t target = share_of(s.p, row_mass);
+    // top_p alone: the groups that hold some 100 tokens, then some 4,000
+    const uint64_t want = by_p ? share_of(s.p, row_mass) : 0;
+#pragma unroll 1
     for (int guess = 0; guess < 2; ++guess) {
-        pick<false>(sm.hist, BINS, guess == 0 ? 96 : 3072, sm);
-        int last = int(sm.bin);
-        if (last == BINS - 1) {
-            if (!sc.whole) return -1;
-            last = BINS - 2;
+        int last;
+        if (s.k || by_p) {
+            pick<false>(sm.hist, BINS, s.k ? uint64_t(s.k) : guess == 0 ? 96 : 3072, sm);
+            last = int(sm.bin);
+            if (last == BINS - 1) {
+                if (!sc.whole) return -1;
+                last = BINS - 2;  // (all that have a mass)
+            }
+        } else {
+            // z >= max + T log(min_p), and a bin to spare
+            const float far = float(-log(s.least) * double(s.t)) * sc.per + 1.0f;
+            last = far < float(BINS - 2) ? int(far) + 1 : BINS - 1;
+            if (last == BINS - 1) return -1;
         }
-        const int n = gather(sm, [&](auto&& f) { each(last, f); }, last, sc);
+        const int n = gather(row, groups, sc, last, sm);
         if (n > CAP) return -1;
+        if (!by_p) return n;
         uint64_t own = 0;
         for (int i = threadIdx.x; i < n; i += NT) own += w.mass(item_value(sm.item[i]));
-        if (block_sum(own, sm) >= target) return n;
+        if (block_sum(own, sm) >= want) return n;
     }
     return -1;
 }
 
 // The cut over a whole row, found from the sums of `share` by bins of the
 // distance from the maximum (in sm.hist): the first items at which the
-// running share reaches `target` lie in one bin, whose items are gathered,
-// each(bin, f) calling f(z, i) for all logits of that bin at least.
-template <typename R, typename G, typename F>
-__device__ uint64_t cut_by_bins(const R& row, const Scale& sc, Shared& sm, uint64_t target, G&& each, F&& share) {
+// running share reaches `target` lie in one bin, whose items are gathered and
+// ordered.
+template <typename T, typename F>
+__device__ uint64_t cut_by_bins(const Row<T>& row, const Scale& sc, Shared& sm, uint64_t target, F&& share) {
     pick<false>(sm.hist, BINS, target, sm);
     const int bin = int(sm.bin);
     const uint64_t left = target - sm.before;
     __syncthreads();
     if (threadIdx.x == 0) sm.count = 0;
     __syncthreads();
-    each(bin, [&](float z, uint32_t i) {
+    row.each([&](float z, uint32_t i) {
         if (sc.bin(z) == bin) {
             const int at = atomicAdd(&sm.count, 1);
             if (at < CAP) sm.item[at] = item_of(z, i);
@@ -589,17 +617,15 @@ __device__ uint64_t cut_by_bins(const R& row, const Scale& sc, Shared& sm, uint6
 }
 
 // The exact cuts and the draw over the whole row.
-template <typename T, typename R>
-__device__ void finish_row(const R& row, const T* p, const Settings& s, float u, const Scale& sc, Shared& sm,
+template <typename T>
+__device__ void finish_row(const Row<T>& row, const Settings& s, float u, const Scale& sc, Shared& sm,
                            const Result& out) {
     const Weigh& w = out.w;
     uint64_t cut = 1;  // every unmasked item
-    auto any = [&](int, auto&& f) { row.each(f); };
-    auto count = [](float) { return uint64_t(1); };
     if (s.k) {
         clear(sm.hist, BINS);
         row.each([&](float z, uint32_t) { add(&sm.hist[sc.bin(z)], 1); });
-        cut = cut_by_bins(row, sc, sm, uint64_t(s.k), any, count);
+        cut = cut_by_bins(row, sc, sm, uint64_t(s.k), [](float) { return uint64_t(1); });
     }
     if (s.p < 1.0f) {
         clear(sm.hist, BINS);
@@ -612,7 +638,7 @@ __device__ void finish_row(const R& row, const T* p, const Settings& s, float u,
         });
         const uint64_t total = block_sum(own, sm);
         // (a mass of top_k's cut that lies past top_p's is not reached)
-        const uint64_t c = cut_by_bins(row, sc, sm, share_of(s.p, total), any, [&](float z) { return w.mass(z); });
+        const uint64_t c = cut_by_bins(row, sc, sm, share_of(s.p, total), [&](float z) { return w.mass(z); });
         cut = c > cut ? c : cut;
     }
     auto kept = [&](float z, uint32_t i) -> uint64_t {
@@ -628,7 +654,7 @@ __device__ void finish_row(const R& row, const T* p, const Settings& s, float u,
     for (int i = threadIdx.x; i < ns; i += NT) own += sm.item[i];
     const uint64_t total = block_sum(own, sm), target = goal(u, total);
     pick<false>(sm.item, ns, target, sm);
-    draw_in(p, row.n, int64_t(sm.bin) * SEG, SEG, target - sm.before, total, out, kept);
+    draw_in(row.p, row.n, int64_t(sm.bin) * SEG, SEG, target - sm.before, total, out, kept);
 }
 
 __device__ inline void nothing_left(const Result& out) {
@@ -636,47 +662,47 @@ __device__ inline void nothing_left(const Result& out) {
     if (out.logprob) *out.logprob = -INFINITY;
 }
 
-// Rows of at most E * NT logits: one workgroup a row, the row in registers.
-template <typename T, int E>
+// Rows of at most SHORT logits: one workgroup a row.
+template <typename T>
 __global__ __launch_bounds__(NT) void sample_short(SampleArgs a) {
     __shared__ Shared sm;
+    __shared__ float groups[SHORT / GROUP];
     const int64_t r = blockIdx.x;
     const int tid = int(threadIdx.x);
-    const T* p = static_cast<const T*>(a.logits) + r * a.ld;
-    RegisterRow<T, E> row;
-    row.load(p, a.vocab);
+    const Row<T> row(static_cast<const T*>(a.logits) + r * a.ld, a.vocab);
     const Settings s = settings_of(a, r);
     const float u = a.u[r];
     if (tid == 0) sm.kmax = 0, sm.kfirst = 0xffffffffu;
     float zmax = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < E; ++j) zmax = fmaxf(zmax, row.z[j]);
+    uint32_t first = 0xffffffffu;
+    row.turns([&](const float* z, int64_t i) {
+        float m = fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3]));
+        if (m > zmax) {
+            zmax = m;
+            first = uint32_t(i) + (z[0] == m ? 0 : z[1] == m ? 1 : z[2] == m ? 2 : 3);
+        }
+        m = fmaxf(m, dpp_f32<0xb1>(m));  // (four lanes of a quad: a group)
+        m = fmaxf(m, dpp_f32<0x4e>(m));
+        if (tid % 4 == 0 && i < a.vocab) groups[i / GROUP] = m;
+    });
     const float wmax = wave_max(zmax);
     __syncthreads();
     if (tid % WAVE == 0) atomicMax(&sm.kmax, key_of(wmax));
     __syncthreads();
     const uint32_t kmax = sm.kmax;
-    Result out{a.tokens + r, a.logprob ? a.logprob + r : nullptr, {double(value_of(kmax)), s.inv_t}};
+    const float top = value_of(kmax);
+    const Result out{a.tokens + r, a.logprob ? a.logprob + r : nullptr, {double(top), s.inv_t}};
     if (kmax == 0) {
         if (tid == 0) nothing_left(out);
         return;
     }
-    const float top = value_of(kmax);
     if (s.greedy) {
-        if (zmax == top) {
-#pragma unroll
-            for (int j = E - 1; j >= 0; --j)
-                if (row.z[j] == top) atomicMin(&sm.kfirst, row.index(j));
-        }
+        if (zmax == top) atomicMin(&sm.kfirst, first);
         __syncthreads();
-        if (tid == 0) {
-            *out.token = int32_t(sm.kfirst);
-            if (out.logprob) *out.logprob = 0.0f;
-        }
+        if (tid == 0) out.certain(sm.kfirst);
         return;
     }
     const Scale sc(top, s.t);
-    int n = -1;
     if (s.k || s.p < 1.0f || s.least > 0.0) {
         uint64_t total = 0;
         if (s.need_sum()) {
@@ -684,27 +710,13 @@ __global__ __launch_bounds__(NT) void sample_short(SampleArgs a) {
             row.each([&](float z, uint32_t) { own += out.w.mass(z); });
             total = block_sum(own, sm);
         }
-        n = make_list(
-            s, sc, sm, total, out.w,
-            [&](auto&& f) {
-#pragma unroll
-                for (int j = 0; j < E; j += 8) {
-                    float m = row.z[j];
-#pragma unroll
-                    for (int c = 1; c < 8; ++c) m = fmaxf(m, row.z[j + c]);
-                    f(m);
-                }
-            },
-            [&](int last, auto&& f) {
-                if (sc.bin(zmax) > last || zmax == -INFINITY) return;
-                row.each(f);
-            });
+        const int n = make_list(s, sc, sm, total, row, groups, out.w);
         if (n >= 0) {
             finish_list(n, s, u, total, sm, out);
             return;
         }
     }
-    finish_row(row, p, s, u, sc, sm, out);
+    finish_row(row, s, u, sc, sm, out);
 }
 
 // What sample_stats leaves of a long row's 2,048 logits.
@@ -799,57 +811,7 @@ struct Workspace {
     }
 };
 
-constexpr int PER = 16;  // logits of a thread of the wide kernels
-constexpr int PART = PER * NT;
-
-// The logits of the groups of GROUP whose maxima reach bin `last`: the
-// groups' numbers are collected first, so that four threads a group read
-// them, two groups at a time in flight.
-template <typename T, typename F>
-__device__ inline void each_of_groups(const T* p, int64_t n, const float* groups, const Scale& sc, int last, Shared& sm,
-                                      F&& f) {
-    uint32_t* ids = reinterpret_cast<uint32_t*>(sm.mass);
-    constexpr int MOST = int(sizeof(sm.mass) / 4);  // (a row has up to 2^16 groups)
-    const int64_t ngroup = (n + GROUP - 1) / GROUP;
-    const bool wide = reinterpret_cast<uintptr_t>(p) % (4 * sizeof(T)) == 0;
-    for (int64_t g0 = 0; g0 < ngroup; g0 += MOST) {
-        const int64_t g1 = g0 + MOST < ngroup ? g0 + MOST : ngroup;
-        __syncthreads();
-        if (threadIdx.x == 0) sm.bin = 0;
-        __syncthreads();
-        for (int64_t g = g0 + threadIdx.x; g < g1; g += NT) {
-            const float m = groups[g];
-            if (m != -INFINITY && sc.bin(m) <= last) ids[atomicAdd(&sm.bin, 1u)] = uint32_t(g);
-        }
-        __syncthreads();
-        const int count = int(sm.bin);
-        for (int k = int(threadIdx.x) / 4; k < count; k += NT / 2) {
-            const int k2 = k + NT / 4;
-            const int64_t i0 = int64_t(ids[k]) * GROUP + threadIdx.x % 4 * 4;
-            const int64_t i1 = k2 < count ? int64_t(ids[k2]) * GROUP + threadIdx.x % 4 * 4 : i0;
-            float z[8];
-            if (wide && i0 + 4 <= n && i1 + 4 <= n) {
-                typedef T vec __attribute__((ext_vector_type(4)));
-                const vec v0 = *reinterpret_cast<const vec*>(p + i0), v1 = *reinterpret_cast<const vec*>(p + i1);
-#pragma unroll
-                for (int c = 0; c < 4; ++c) z[c] = float(v0[c]), z[4 + c] = float(v1[c]);
-            } else {
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    z[c] = i0 + c < n ? float(p[i0 + c]) : -INFINITY;
-                    z[4 + c] = i1 + c < n ? float(p[i1 + c]) : -INFINITY;
-                }
-            }
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const float x = clean(z[c]), y = clean(z[4 + c]);
-                if (x != -INFINITY) f(x, uint32_t(i0 + c));
-                if (k2 < count && y != -INFINITY) f(y, uint32_t(i1 + c));
-            }
-        }
-    }
-    __syncthreads();
-}
+constexpr int PART = 16 * NT;  // logits of a workgroup of the wide kernels
 
 template <typename T>
 __global__ __launch_bounds__(NT) void sample_long(SampleArgs a, Workspace ws) {
@@ -860,7 +822,7 @@ __global__ __launch_bounds__(NT) void sample_long(SampleArgs a, Workspace ws) {
     const float u = a.u[r];
     const Chunk* chunks = ws.chunks + r * nchunk;
     const float* groups = ws.groups + r * nchunk * (CHUNK / GROUP);
-    const MemoryRow<T> row{static_cast<const T*>(a.logits) + r * a.ld, a.vocab};
+    const Row<T> row(static_cast<const T*>(a.logits) + r * a.ld, a.vocab);
     if (tid == 0) sm.kmax = 0, sm.kfirst = 0xffffffffu, ws.pending[r].step = 0;
     __syncthreads();
     const Chunk mine = tid < nchunk ? chunks[tid] : Chunk{-INFINITY, 0xffffffffu, 0.0};  // (nchunk <= NT)
@@ -877,10 +839,7 @@ __global__ __launch_bounds__(NT) void sample_long(SampleArgs a, Workspace ws) {
     if (s.greedy) {
         if (mine.max == top) atomicMin(&sm.kfirst, mine.first);
         __syncthreads();
-        if (tid == 0) {
-            *out.token = int32_t(sm.kfirst);
-            if (out.logprob) *out.logprob = 0.0f;
-        }
+        if (tid == 0) out.certain(sm.kfirst);
         return;
     }
     uint64_t own = 0, total = 0;
@@ -897,7 +856,7 @@ __global__ __launch_bounds__(NT) void sample_long(SampleArgs a, Workspace ws) {
         const int64_t c = sm.bin;
         const uint64_t left = target - sm.before;
         // the chunk's segments, then the segment
-        const MemoryRow<T> part{row.p + c * CHUNK, a.vocab - c * CHUNK < CHUNK ? a.vocab - c * CHUNK : CHUNK};
+        const Row<T> part(row.p + c * CHUNK, a.vocab - c * CHUNK < CHUNK ? a.vocab - c * CHUNK : CHUNK);
         auto mass = [&](float z, uint32_t) { return out.w.mass(z); };
         __syncthreads();
         part.sums(sm.item, mass);
@@ -914,19 +873,13 @@ __global__ __launch_bounds__(NT) void sample_long(SampleArgs a, Workspace ws) {
         return;
     }
     const Scale sc(top, s.t);
-    const int64_t ngroup = (a.vocab + GROUP - 1) / GROUP;
-    const int n = make_list(
-        s, sc, sm, total, out.w,
-        [&](auto&& f) {
-            for (int64_t g = tid; g < ngroup; g += NT) f(groups[g]);
-        },
-        [&](int last, auto&& f) { each_of_groups(row.p, row.n, groups, sc, last, sm, f); });
+    const int n = make_list(s, sc, sm, total, row, groups, out.w);
     if (n >= 0) {
         finish_list(n, s, u, total, sm, out);
         return;
     }
     if (s.k) {
-        finish_row(row, row.p, s, u, sc, sm, out);
+        finish_row(row, s, u, sc, sm, out);
         return;
     }
     for (int i = tid; i < BINS; i += NT) ws.hist[r * BINS + i] = 0;
@@ -934,14 +887,18 @@ __global__ __launch_bounds__(NT) void sample_long(SampleArgs a, Workspace ws) {
 }
 
 // Whether this workgroup is the last of its row's to arrive; what the others
-// wrote before is then visible to it.
+// wrote before is then visible to it.  (One thread fences for all, ordered
+// with them by the barriers: a fence writes back and invalidates the L2, and
+// one by every wave took 300 us of a 16.8 million logits' pass.)
 __device__ inline bool last_of(uint32_t* arrived, Shared& sm) {
-    __threadfence();
     __syncthreads();
-    if (threadIdx.x == 0) sm.count = int(atomicAdd(arrived, 1u));
+    if (threadIdx.x == 0) {
+        __threadfence();
+        sm.count = int(atomicAdd(arrived, 1u));
+        __threadfence();
+    }
     __syncthreads();
     const bool last = sm.count == int(gridDim.x) - 1;
-    __threadfence();
     __syncthreads();
     return last;
 }
@@ -949,18 +906,11 @@ __device__ inline uint64_t load_shared(const uint64_t* p) {  // written by other
     return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-template <typename T>
-struct PartRow {
-    float z[PER];
-    int64_t first;
-    __device__ uint32_t index(int j) const { return uint32_t(first + ((j / 4) * NT + threadIdx.x) * 4 + j % 4); }
-    __device__ void load(const T* p, int64_t n) {
-#pragma unroll
-        for (int j = 0; j < PER; ++j) z[j] = float(p[index(j) < n ? index(j) : n - 1]);
-#pragma unroll
-        for (int j = 0; j < PER; ++j) z[j] = index(j) < n ? clean(z[j]) : -INFINITY;
-    }
-};
+// The logits of this workgroup's part of a row.
+__device__ inline int64_t part_size(int64_t n) {
+    const int64_t left = n - int64_t(blockIdx.x) * PART;
+    return left < PART ? left : PART;
+}
 
 // The masses of pending rows by bins; the last workgroup of a row finds
 // top_p's cut.
@@ -972,19 +922,16 @@ __global__ __launch_bounds__(NT) void sample_bins(SampleArgs a, Workspace ws) {
     __shared__ Shared sm;
     const int tid = int(threadIdx.x);
     const Settings s = settings_of(a, r);
-    const MemoryRow<T> row{static_cast<const T*>(a.logits) + r * a.ld, a.vocab};
+    const Row<T> row(static_cast<const T*>(a.logits) + r * a.ld, a.vocab);
     const float top = value_of(pd.kmax);
     const Weigh w{double(top), s.inv_t};
     const Scale sc(top, s.t);
-    PartRow<T> part;
-    part.first = int64_t(blockIdx.x) * PART;
-    part.load(row.p, row.n);
     clear(sm.hist, BINS);
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-        const uint64_t m = w.mass(part.z[j]);
-        if (m) add(&sm.hist[sc.bin(part.z[j])], m);
-    }
+    const Row<T> part(row.p + int64_t(blockIdx.x) * PART, part_size(row.n));
+    part.each([&](float z, uint32_t) {
+        const uint64_t m = w.mass(z);
+        if (m) add(&sm.hist[sc.bin(z)], m);
+    });
     __syncthreads();
     uint64_t* hist = ws.hist + r * BINS;
     for (int i = tid; i < BINS; i += NT)
@@ -996,11 +943,7 @@ __global__ __launch_bounds__(NT) void sample_bins(SampleArgs a, Workspace ws) {
         own += sm.hist[i];
     }
     const uint64_t total = block_sum(own, sm);
-    const float* groups = ws.groups + r * ws.nchunk * (CHUNK / GROUP);
-    const uint64_t cut = cut_by_bins(
-        row, sc, sm, share_of(s.p, total),
-        [&](int bin, auto&& f) { each_of_groups(row.p, row.n, groups, sc, bin, sm, f); },
-        [&](float z) { return w.mass(z); });
+    const uint64_t cut = cut_by_bins(row, sc, sm, share_of(s.p, total), [&](float z) { return w.mass(z); });
     if (tid == 0) pd.cut = cut, pd.step = 2;
 }
 
@@ -1022,21 +965,15 @@ __global__ __launch_bounds__(NT) void sample_draw(SampleArgs a, Workspace ws) {
         const double x = out.w(z);
         return x >= s.least ? Weigh::fixed(x) : 0;
     };
-    PartRow<T> part;
-    part.first = int64_t(blockIdx.x) * PART;
-    part.load(p, a.vocab);
-    const int64_t ns = ws.nchunk * (CHUNK / SEG);
+    const int64_t first = int64_t(blockIdx.x) * PART, ns = ws.nchunk * (CHUNK / SEG);
     uint64_t* segs = ws.segs + r * ns;
-#pragma unroll
-    for (int j = 0; j < PER; j += 4) {
-        uint64_t v = 0;
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-            if (part.z[j + c] != -INFINITY) v += kept(part.z[j + c], part.index(j + c));
-        v = wave_sum_u64(v);
-        const int64_t seg = part.first / SEG + j / 4 * NWAVE + tid / WAVE;
-        if (tid % WAVE == 0 && seg < ns) __hip_atomic_store(segs + seg, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
+    const Row<T> part(p + first, part_size(a.vocab));
+    // (the segments of a part end with the row, the row's with its chunks)
+    part.sums(sm.item, [&](float z, uint32_t i) { return kept(z, uint32_t(first) + i); });
+    __syncthreads();
+    for (int i = tid; i < PART / SEG && first / SEG + i < ns; i += NT)
+        __hip_atomic_store(segs + first / SEG + i, i < part.segments() ? sm.item[i] : 0, __ATOMIC_RELAXED,
+                           __HIP_MEMORY_SCOPE_AGENT);
     if (!last_of(&pd.arrived[1], sm)) return;
     uint64_t own = 0;
     for (int i = tid; i < ns; i += NT) {
@@ -1067,16 +1004,13 @@ SampleArgs rows_from(SampleArgs a, int64_t r) {
     return a;
 }
 
-constexpr int64_t SHORT = 32 * NT;
 int64_t chunks_of(int64_t vocab) { return (vocab + CHUNK - 1) / CHUNK; }
 
 template <typename T>
 void launch(hipStream_t s, const SampleArgs& a, void* workspace) {
     const dim3 grid{unsigned(a.rows)}, block{NT};
-    if (a.vocab <= 8 * NT) {
-        sample_short<T, 8><<<grid, block, 0, s>>>(a);
-    } else if (a.vocab <= SHORT) {
-        sample_short<T, 32><<<grid, block, 0, s>>>(a);
+    if (a.vocab <= SHORT) {
+        sample_short<T><<<grid, block, 0, s>>>(a);
     } else {
         const int64_t nchunk = chunks_of(a.vocab);
         Workspace ws;
