@@ -21,14 +21,17 @@
 // comparing all pairs (up to 256) or by histograms over the items' digits.
 // Where the kept tokens do not fit the list, the row's masses are summed by
 // bins of their distance from the maximum, which leaves one bin's logits to
-// order exactly, and the kept masses by segments in index order: by the
-// row's workgroup, or for long rows by the whole chip (sample_bins,
-// sample_draw).
+// order exactly, and the kept masses by segments in index order: by one
+// workgroup a row (sample_row), or, where a long row's top_p or min_p keeps
+// them, by the whole chip (sample_bins, sample_draw).
 //
-// The code of a pass is kept short (rolled loops over memory, not a row in
-// registers): a workgroup that runs through it once waits for instructions
-// more than for data; a row of 25,000 held in 32 registers a thread took 14.5
-// us for its maximum alone, and 14 more for each unrolled pass of exp.
+// What bounds the kernels of one workgroup a row is its CU: 64 lanes a cycle
+// (150 lane instructions a nanosecond) and a microsecond for every trip to
+// memory that the next step waits for.  So passes over a row compare raw
+// logits with a threshold and take keys, bins and masses of the few that
+// pass, and their loops are rolled: a row of 25,000 held in registers, 32 a
+// thread, took 14.5 us for its maximum and 14 for a pass of exp, waiting for
+// instructions; this form takes 5.
 #include <algorithm>
 #include <string>
 
@@ -43,43 +46,58 @@ namespace {
 constexpr int NT = 1024;          // threads of a row's workgroup
 constexpr int NWAVE = NT / WAVE;
 constexpr int CHUNK = 2048;       // logits of a wave of sample_stats
-constexpr int GROUP = 16;         // logits of a group maximum there
+constexpr int GROUP = 16;         // logits of a group maximum
+constexpr int SHORT = 32 * NT;    // logits of a row that one workgroup takes alone
 constexpr int CAP = 8192;         // items of the list
 constexpr int BINS = 2048;
 constexpr int PAIRS = NT / 4;     // items compared pair by pair: four threads each
 constexpr int SEG = 256;          // consecutive logits a wave takes at once
-constexpr int64_t SHORT = 32 * NT;  // logits of a row that one workgroup takes alone
+constexpr int PART = 16 * NT;     // logits of a workgroup of the wide kernels
 constexpr int IDX_BITS = 20;      // vocab <= 2^20
 constexpr uint32_t IDX_MASK = (1u << IDX_BITS) - 1;
 constexpr double ONE = 4398046511104.0;  // 2^42
 
-// A logit as it is ordered: masked ones (-infinity, NaN) -infinity, -0 the 0 it equals.
-__device__ inline float clean(float z) { return z > -INFINITY ? z + 0.0f : -INFINITY; }
-// Order-preserving bits of a clean logit; 0 for masked ones.
+// Order-preserving bits of a logit that is not masked (above -infinity); -0
+// is the 0 it equals.
 __device__ inline uint32_t key_of(float z) {
-    const uint32_t u = __builtin_bit_cast(uint32_t, z);
-    return z == -INFINITY ? 0 : u & 0x80000000u ? ~u : u | 0x80000000u;
+    const uint32_t u = __builtin_bit_cast(uint32_t, z + 0.0f);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 __device__ inline float value_of(uint32_t k) {
     return __builtin_bit_cast(float, k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 // An item: larger comes first.
-__device__ inline uint64_t item_of(float z, uint32_t i) {
-    return uint64_t(key_of(z)) << IDX_BITS | (IDX_MASK - i);
-}
+__device__ inline uint64_t item_of(float z, int i) { return uint64_t(key_of(z)) << IDX_BITS | (IDX_MASK - uint32_t(i)); }
 __device__ inline float item_value(uint64_t it) { return value_of(uint32_t(it >> IDX_BITS)); }
-__device__ inline uint32_t item_index(uint64_t it) { return IDX_MASK - (uint32_t(it) & IDX_MASK); }
+__device__ inline int item_index(uint64_t it) { return int(IDX_MASK - (uint32_t(it) & IDX_MASK)); }
 
-// exp((z - max) / T) of a clean logit: 1 at the maximum, whatever it is, 0
-// where it is masked.  With t = (z - max) log2(e) / T = n + f, |f| <= 1/2:
-// the series of 2^f = exp(f ln 2) to the 11th power (its rest is below
-// 2^-46), its exponent raised by n.
+// The items from the first on to an item, as logits compare: larger ones, and
+// its equals up to its index.  Without one: all that are not masked.
+struct Cut {
+    float z = -INFINITY;
+    int i = 0;
+    __device__ bool keeps(float x, int at) const { return x > z || (x == z && at <= i && z > -INFINITY); }
+    static __device__ Cut at(uint64_t item) {
+        Cut c;
+        if (uint32_t(item >> IDX_BITS) > 0x007fffffu) c.z = item_value(item), c.i = item_index(item);  // (-infinity's key)
+        return c;
+    }
+};
+
+// exp((z - max) / T): 1 at the maximum, whatever it is, nothing where z is
+// masked.  With t = (z - max) log2(e) / T = n + f, |f| <= 1/2: the series of
+// 2^f = exp(f ln 2) to the 11th power (its rest is below 2^-46), its exponent
+// raised by n.
 struct Weigh {
-    double max, inv_t;
+    double max, per;  // log2(e) / T
+    bool infinite;
+    __device__ Weigh(float m, double inv_t)
+        : max(double(m)), per(inv_t * 1.4426950408889634), infinite(m == INFINITY) {}
     __device__ double operator()(float z) const {
+        if (infinite) return z == INFINITY ? 1.0 : 0.0;
         constexpr double WHOLE = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number
-        double t = (double(z) - max) * (inv_t * 1.4426950408889634);
-        t = fmax(t, -1000.0);  // (and NaN, from -infinity / infinity, to -1000)
+        // (NaN, and what is far below every mass, to 2^-1000)
+        const double t = fmax((double(z) - max) * per, -1000.0);
         const double shifted = t + WHOLE, f = t - (shifted - WHOLE);
         constexpr double L = 0.69314718055994531;
         constexpr double c2 = L * L / 2, c3 = c2 * L / 3, c4 = c3 * L / 4, c5 = c4 * L / 5, c6 = c5 * L / 6,
@@ -96,10 +114,9 @@ struct Weigh {
         p = fma(p, f, c2);
         p = fma(p, f, L);
         p = fma(p, f, 1.0);
-        const uint64_t n = __builtin_bit_cast(uint64_t, shifted);  // (its low bits: n)
-        const double w = __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, p) + (n << 52));
-        // an infinite maximum leaves NaN and 2^-1000 above: its equals weigh 1
-        return max < INFINITY ? w : z < INFINITY ? 0.0 : 1.0;
+        const uint64_t b = __builtin_bit_cast(uint64_t, p);
+        const uint32_t n = uint32_t(__builtin_bit_cast(uint64_t, shifted));  // (its low bits: n)
+        return __builtin_bit_cast(double, uint64_t(uint32_t(b >> 32) + (n << 20)) << 32 | uint32_t(b));
     }
     __device__ uint64_t mass(float z) const { return fixed((*this)(z)); }
     // (2^52 + v rounds v to a whole number in its low bits)
@@ -132,84 +149,105 @@ __device__ inline Settings settings_of(const SampleArgs& a, int64_t r) {
     return s;
 }
 
-__device__ inline uint64_t wave_sum_u64(uint64_t v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, WAVE);
+// Sums over the wave by DPP (a shuffle goes through LDS, a hundred cycles a
+// step): lanes without a source add 0.
+template <int CTRL, int ROWS>
+__device__ inline uint64_t dpp_u64(uint64_t v) {
+    const uint32_t lo = uint32_t(__builtin_amdgcn_update_dpp(0, int(uint32_t(v)), CTRL, ROWS, 0xf, true));
+    const uint32_t hi = uint32_t(__builtin_amdgcn_update_dpp(0, int(uint32_t(v >> 32)), CTRL, ROWS, 0xf, true));
+    return uint64_t(hi) << 32 | lo;
+}
+__device__ inline uint64_t row_scan_u64(uint64_t v) {  // inclusive, in each 16 lanes
+    v += dpp_u64<0x111, 0xf>(v);  // row_shr 1, 2, 4, 8
+    v += dpp_u64<0x112, 0xf>(v);
+    v += dpp_u64<0x114, 0xf>(v);
+    v += dpp_u64<0x118, 0xf>(v);
     return v;
 }
-__device__ inline uint64_t wave_scan_u64(uint64_t v, int lane) {  // inclusive
-#pragma unroll
-    for (int o = 1; o < WAVE; o <<= 1) {
-        const uint64_t x = __shfl_up(v, o, WAVE);
-        if (lane >= o) v += x;
-    }
+__device__ inline uint64_t wave_scan_u64(uint64_t v) {  // inclusive
+    v = row_scan_u64(v);
+    v += dpp_u64<0x142, 0xa>(v);  // row_bcast 15: into rows 1 and 3
+    v += dpp_u64<0x143, 0xc>(v);  // row_bcast 31: into rows 2 and 3
     return v;
+}
+__device__ inline uint64_t quad_sum_u64(uint64_t v) {  // over four lanes, in each
+    v += dpp_u64<0xb1, 0xf>(v);
+    v += dpp_u64<0x4e, 0xf>(v);
+    return v;
+}
+__device__ inline uint64_t lane_u64(uint64_t v, int lane) {
+    const uint32_t lo = uint32_t(__builtin_amdgcn_readlane(int(uint32_t(v)), lane));
+    const uint32_t hi = uint32_t(__builtin_amdgcn_readlane(int(uint32_t(v >> 32)), lane));
+    return uint64_t(hi) << 32 | lo;
 }
 
-struct Shared {
-    uint64_t item[CAP];   // the list; without one, the masses of the row's segments
-    uint64_t mass[CAP];   // (top bit: under min_p)
-    uint64_t hist[BINS];
+struct Common {
     uint64_t part[NWAVE];
-    uint64_t before, in_bin, total;
-    uint32_t bin, kmax, kfirst;
-    int count;
+    uint64_t before, in_bin, total, found;
+    uint32_t bin, kmax, kfirst, count;
 };
-constexpr uint64_t UNDER = uint64_t(1) << 63;
+struct Shared : Common {
+    uint64_t item[CAP];   // the list; without one, the masses of the row's segments
+    uint64_t mass[CAP];   // kept masses; before, the numbers of the groups to read
+    uint64_t hist[BINS];
+    uint64_t edge[PAIRS]; // items of one bin
+};
+struct DrawShared : Common {
+    uint64_t item[(1 << IDX_BITS) / SEG];  // the masses of the row's segments
+};
+__device__ inline int wave_id() { return __builtin_amdgcn_readfirstlane(int(threadIdx.x) / WAVE); }
 
-__device__ inline uint64_t block_sum(uint64_t v, Shared& sm) {
-    v = wave_sum_u64(v);
+// Sum of v over the workgroup, in every thread.
+__device__ inline uint64_t block_sum(uint64_t v, Common& sm) {
+    const int lane = int(threadIdx.x) % WAVE;
+    v = wave_scan_u64(v);
     __syncthreads();
-    if (threadIdx.x % WAVE == 0) sm.part[threadIdx.x / WAVE] = v;
+    if (lane == WAVE - 1) sm.part[wave_id()] = v;
     __syncthreads();
-    uint64_t s = 0;
-#pragma unroll
-    for (int i = 0; i < NWAVE; ++i) s += sm.part[i];
-    return s;
+    return lane_u64(row_scan_u64(sm.part[lane % NWAVE]), NWAVE - 1);
 }
 
 // The bin at which the running sum over h[0 .. n), in ascending or (DOWN)
 // descending order, first reaches `target`; the last one in order if it
 // never does.  Sets sm.bin, sm.before (the sum before it), sm.in_bin and
-// sm.total.
+// sm.total.  n up to 4 NT.
 template <bool DOWN>
-__device__ inline void pick(const uint64_t* h, int n, uint64_t target, Shared& sm) {
-    const int tid = int(threadIdx.x), lane = tid % WAVE, wave = tid / WAVE;
+__device__ inline void pick(const uint64_t* h, int n, uint64_t target, Common& sm) {
+    const int tid = int(threadIdx.x), lane = tid % WAVE, wave = wave_id();
     const int per = (n + NT - 1) / NT;
     __syncthreads();
-    uint64_t own = 0;
-    for (int i = 0; i < per; ++i) {
+    uint64_t x[4], own = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
         const int j = tid * per + i;
-        if (j < n) own += h[DOWN ? n - 1 - j : j];
+        x[i] = i < per && j < n ? h[DOWN ? n - 1 - j : j] : 0;
+        own += x[i];
     }
-    const uint64_t scan = wave_scan_u64(own, lane);
+    const uint64_t scan = wave_scan_u64(own);
     if (lane == WAVE - 1) sm.part[wave] = scan;
     __syncthreads();
-    uint64_t base = 0, total = 0;
-#pragma unroll
-    for (int i = 0; i < NWAVE; ++i) {
-        if (i < wave) base += sm.part[i];
-        total += sm.part[i];
-    }
-    uint64_t run = base + scan - own;
+    const uint64_t waves = row_scan_u64(sm.part[lane % NWAVE]);
+    const uint64_t total = lane_u64(waves, NWAVE - 1);
+    uint64_t run = (wave ? lane_u64(waves, wave - 1) : 0) + scan - own;
     const bool never = total < target;
     if (tid == 0) sm.total = total;
-    for (int i = 0; i < per; ++i) {
-        const int j = tid * per + i;
-        if (j >= n) break;
-        const uint64_t x = h[DOWN ? n - 1 - j : j];
-        if (never ? j == n - 1 : run < target && run + x >= target) {
-            sm.bin = uint32_t(DOWN ? n - 1 - j : j);
-            sm.before = run;
-            sm.in_bin = x;
+    if (never ? tid == (n - 1) / per : run < target && run + own >= target) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int j = tid * per + i;
+            if (i < per && (never ? j == n - 1 : run < target && run + x[i] >= target)) {
+                sm.bin = uint32_t(DOWN ? n - 1 - j : j);
+                sm.before = run;
+                sm.in_bin = x[i];
+            }
+            run += x[i];
         }
-        run += x;
     }
     __syncthreads();
 }
 
+// (h's last readers are past a barrier)
 __device__ inline void clear(uint64_t* h, int n) {
-    __syncthreads();
     for (int i = threadIdx.x; i < n; i += NT) h[i] = 0;
     __syncthreads();
 }
@@ -217,39 +255,28 @@ __device__ inline void add(uint64_t* h, uint64_t v) {
     atomicAdd(reinterpret_cast<unsigned long long*>(h), static_cast<unsigned long long>(v));
 }
 
-// The item at which the running share, over the items >= limit from the
-// first on, first reaches `target` (>= 1); an item that takes in all of them
-// if it never does.  src(f) calls f(item, i) for the thread's items;
-// share(item, i) is an item's count or mass.
-template <typename S, typename F>
-__device__ uint64_t find_cut(S&& src, Shared& sm, uint64_t target, uint64_t limit, F&& share) {
-    uint64_t prefix = 0, before = 0;
-    int shift = 52;
-#pragma unroll 1
-    for (int level = 0; level < 5; ++level) {
-        const int bits = level < 2 ? 11 : 10;
-        shift -= bits;
-        clear(sm.hist, 1 << bits);
-        src([&](uint64_t it, int i) {
-            if (it < limit || (it >> (shift + bits)) != prefix) return;
-            const uint64_t v = share(it, i);
-            if (v) add(&sm.hist[(it >> shift) & ((1u << bits) - 1)], v);
-        });
-        pick<true>(sm.hist, 1 << bits, target - before, sm);
-        prefix = prefix << bits | sm.bin;
-        before += sm.before;
-        if (before + sm.in_bin <= target) break;  // the whole bin stays
-    }
-    const uint64_t cut = prefix << shift;
-    return cut > limit ? cut : limit;
+// A place in a list for each of the lane's `own` entries, by one atomic of
+// the wave.
+__device__ inline int places(uint32_t* count, int own) {
+    int scan = own;
+    scan += __builtin_amdgcn_update_dpp(0, scan, 0x111, 0xf, 0xf, true);
+    scan += __builtin_amdgcn_update_dpp(0, scan, 0x112, 0xf, 0xf, true);
+    scan += __builtin_amdgcn_update_dpp(0, scan, 0x114, 0xf, 0xf, true);
+    scan += __builtin_amdgcn_update_dpp(0, scan, 0x118, 0xf, 0xf, true);
+    scan += __builtin_amdgcn_update_dpp(0, scan, 0x142, 0xa, 0xf, true);
+    scan += __builtin_amdgcn_update_dpp(0, scan, 0x143, 0xc, 0xf, true);
+    const int all = __builtin_amdgcn_readlane(scan, WAVE - 1);
+    uint32_t at = 0;
+    if (all && threadIdx.x % WAVE == 0) at = atomicAdd(count, uint32_t(all));
+    return __builtin_amdgcn_readfirstlane(int(at)) + scan - own;
 }
 
-// Counts of group maxima by their distance from the row's maximum, in bins
-// of T / 64 or 1/32, whichever is narrower.  A threshold is a bin's far edge
-// (with a slack for the rounding of the bins).
+
+// Bins of the distance from the row's maximum, T / 64 or 1/32 wide, whichever
+// is narrower.
 struct Scale {
     float max, per;  // bins per unit of z
-    bool whole;      // what lies past the last bin has no mass
+    bool whole;      // what lies in the last bin has no mass
     __device__ Scale(float m, float t) : max(m) {
         const float f = 64.0f / t;
         per = f > 32.0f ? (f < 1e30f ? f : 1e30f) : 32.0f;
@@ -259,44 +286,48 @@ struct Scale {
         const float x = (max - z) * per;
         return x < float(BINS - 1) ? int(x) : BINS - 1;  // (NaN, infinity - infinity: the last)
     }
+    // A logit below all that lie in bins 0 .. last, however the bins rounded.
+    __device__ float under(int last) const {
+        const float x = max - float(last + 1) / per * 1.00001f;
+        return x - fabsf(x) * 1e-6f - 1e-37f;
+    }
 };
 
-// A row that is worked on as a whole: each(f) calls f(z, index) for the
-// thread's logits, sums(out, m) leaves the sums of m(z, index) over segments
-// of SEG.
+// A row of logits: raw, masked ones as they stand (NaN, -infinity).
 template <typename T>
 struct Row {
     const T* p;
-    int64_t n;
+    int n;
     bool wide;  // four elements at once are aligned
-    __device__ Row(const T* row, int64_t vocab)
-        : p(row), n(vocab), wide(reinterpret_cast<uintptr_t>(row) % (4 * sizeof(T)) == 0 && vocab >= 4) {}
-    // The four logits from i (a multiple of 4) on, masked behind the row, in
-    // two steps, so that a caller's loads can be under way together.
     typedef T vec __attribute__((ext_vector_type(4)));
-    __device__ vec load(int64_t i) const {
+    __device__ Row(const T* row, int64_t vocab)
+        : p(row), n(int(vocab)), wide(reinterpret_cast<uintptr_t>(row) % (4 * sizeof(T)) == 0 && vocab >= 4) {}
+    // The four logits from i (a multiple of 4) on, -infinity behind the row,
+    // in two steps, so that a caller's loads can be under way together.
+    __device__ vec load(int i) const {
         if (wide) return *reinterpret_cast<const vec*>(p + (i + 4 <= n ? i : 0));
         vec v;
 #pragma unroll
         for (int c = 0; c < 4; ++c) v[c] = p[i + c < n ? i + c : 0];
         return v;
     }
-    __device__ void four(vec v, int64_t i, float* z) const {
-        if (i < n && i + 4 > n) {
+    __device__ void four(vec v, int i, float* z) const {
 #pragma unroll
-            for (int c = 0; c < 3; ++c) v[c] = p[i + c < n ? i + c : 0];
+        for (int c = 0; c < 4; ++c) z[c] = float(v[c]);
+        if (i + 4 > n) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) z[c] = i + c < n ? float(p[i + c]) : -INFINITY;
         }
-#pragma unroll
-        for (int c = 0; c < 4; ++c) z[c] = i + c < n ? clean(float(v[c])) : -INFINITY;
     }
     // f(z, i) for the four logits z of each of the thread's turns, the next
-    // two turns' loads under way; every thread makes the same turns.
+    // two turns' loads under way; every thread makes the same turns, a wave
+    // takes SEG consecutive logits in each.
     template <typename F>
     __device__ void turns(F&& f) const {
-        int64_t i = int64_t(threadIdx.x) * 4;
+        int i = int(threadIdx.x) * 4;
         vec v0 = load(i), v1 = load(i + NT * 4);
 #pragma unroll 1
-        for (int64_t base = 0; base < n; base += NT * 8, i += NT * 8) {
+        for (int base = 0; base < n; base += NT * 8, i += NT * 8) {
             const vec w0 = load(i + NT * 8), w1 = load(i + NT * 12);
             float z[4];
             four(v0, i, z);
@@ -306,24 +337,16 @@ struct Row {
             v0 = w0, v1 = w1;
         }
     }
-    template <typename F>
-    __device__ void each(F&& f) const {
-        turns([&](const float* z, int64_t i) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-                if (z[c] != -INFINITY) f(z[c], uint32_t(i + c));
-        });
-    }
-    __device__ int segments() const { return int((n + SEG - 1) / SEG); }
+    __device__ int segments() const { return (n + SEG - 1) / SEG; }
+    // Sums of m(z, i) over the row's segments.
     template <typename F>
     __device__ void sums(uint64_t* out, F&& m) const {
-        turns([&](const float* z, int64_t i) {
+        turns([&](const float* z, int i) {
             uint64_t v = 0;
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
-                if (z[c] != -INFINITY) v += m(z[c], uint32_t(i + c));
-            v = wave_sum_u64(v);
-            if (threadIdx.x % WAVE == 0 && i < n) out[i / SEG] = v;
+            for (int c = 0; c < 4; ++c) v += m(z[c], i + c);
+            v = wave_scan_u64(v);
+            if (threadIdx.x % WAVE == WAVE - 1 && i - (WAVE - 1) * 4 < n) out[i / SEG] = v;
         });
     }
 };
@@ -332,14 +355,17 @@ struct Result {
     int32_t* token;
     float* logprob;
     Weigh w;
-    __device__ void certain(uint32_t i) const {
-        *token = int32_t(i);
-        if (logprob) *logprob = 0.0f;
+    double inv_t;
+    __device__ Result(const SampleArgs& a, int64_t r, float max, const Settings& s)
+        : token(a.tokens + r), logprob(a.logprob ? a.logprob + r : nullptr), w(max, s.inv_t), inv_t(s.inv_t) {}
+    __device__ void certain(int i) const {
+        *token = i;
+        if (logprob) *logprob = i < 0 ? -INFINITY : 0.0f;
     }
-    __device__ void write(float z, uint32_t i, uint64_t total) const {
-        *token = int32_t(i);
+    __device__ void write(float z, int i, uint64_t total) const {
+        *token = i;
         const double d = double(z) - w.max;
-        if (logprob) *logprob = float((d < 0.0 ? d * w.inv_t : 0.0) - log(double(total) / ONE));
+        if (logprob) *logprob = float((d < 0.0 ? d * inv_t : 0.0) - log(double(total) / ONE));
     }
 };
 
@@ -359,323 +385,440 @@ __device__ inline uint64_t share_of(float p, uint64_t total) {
 // The drawn logit of one segment: `target` into the masses m(z, i) of its
 // logits (its last with a mass where rounding leaves them short of it).
 template <typename T, typename F>
-__device__ inline void draw_in(const T* p, int64_t n, int64_t first, int count, uint64_t target, uint64_t total,
-                               const Result& out, F&& m) {
+__device__ inline void draw_in(const Row<T>& row, int first, uint64_t target, uint64_t total, const Result& out, F&& m) {
     if (threadIdx.x >= WAVE) return;
-    const int lane = int(threadIdx.x);
-    uint64_t run = 0;
-    float drawn = 0.0f;
-    int64_t index = -1;
-    for (int at = 0; at < count; at += WAVE) {
-        const int64_t i = first + at + lane;
-        const float z = at + lane < count && i < n ? clean(float(p[i])) : -INFINITY;
-        const uint64_t v = z != -INFINITY ? m(z, uint32_t(i)) : 0;
-        const uint64_t scan = run + wave_scan_u64(v, lane);
-        const uint64_t some = __ballot(v > 0), hit = __ballot(v > 0 && scan >= target);
-        if (some) {
-            const int l = hit ? __builtin_ctzll(hit) : 63 - __builtin_clzll(some);
-            drawn = __shfl(z, l, WAVE);
-            index = first + at + l;
-        }
-        if (hit) break;
-        run = __shfl(scan, WAVE - 1, WAVE);
+    const int lane = int(threadIdx.x), i = first + lane * 4;
+    float z[4];
+    row.four(row.load(i), i, z);
+    uint64_t v[4], own = 0;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        v[c] = m(z[c], i + c);
+        own += v[c];
     }
-    if (lane == 0 && index >= 0) out.write(drawn, uint32_t(index), total);
+    const uint64_t scan = wave_scan_u64(own);
+    const uint64_t some = __ballot(own > 0), hit = __ballot(own > 0 && scan >= target);
+    if (!some || lane != (hit ? __builtin_ctzll(hit) : 63 - __builtin_clzll(some))) return;
+    uint64_t run = scan - own;
+    float drawn = 0.0f;
+    int at = -1;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        const bool here = v[c] > 0 && (at < 0 || run < target);
+        if (here) drawn = z[c], at = i + c;
+        run += v[c];
+    }
+    out.write(drawn, at, total);
+}
+
+// The item at which the running share, over the items from the first on,
+// first reaches `target` (>= 1); 0 if it never does, or an item below all
+// that do.  items(f) calls f(z, i) for the thread's items; masses: an item's
+// share is its mass, else one.
+template <typename S>
+__device__ uint64_t find_cut(S&& items, Shared& sm, uint64_t target, bool masses, const Weigh& w) {
+    uint64_t prefix = 0, before = 0;
+    int shift = 52;
+#pragma unroll 1
+    for (int level = 0; level < 5; ++level) {
+        const int bits = level < 2 ? 11 : 10;
+        shift -= bits;
+        clear(sm.hist, 1 << bits);
+        items([&](float z, int i) {
+            const uint64_t it = item_of(z, i);
+            if ((it >> (shift + bits)) != prefix) return;
+            const uint64_t v = masses ? w.mass(z) : 1;
+            if (v) add(&sm.hist[(it >> shift) & ((1u << bits) - 1)], v);
+        });
+        pick<true>(sm.hist, 1 << bits, target - before, sm);
+        prefix = prefix << bits | sm.bin;
+        before += sm.before;
+        if (before + sm.in_bin <= target) break;  // the whole bin stays
+    }
+    return prefix << shift;
+}
+
+// The cut at which the running share reaches `target`, the shares' sums by
+// bins in sm.hist: the items of the bin where it does are collected, in
+// room[0 .. most), and compared pair by pair.
+template <typename S>
+__device__ Cut cut_by_bins(S&& items, const Scale& sc, Shared& sm, uint64_t* room, int most, uint64_t target,
+                           bool masses, const Weigh& w) {
+    const int tid = int(threadIdx.x);
+    pick<false>(sm.hist, BINS, target, sm);
+    const int bin = int(sm.bin);
+    const uint64_t left = target - sm.before;
+    if (sm.total < target) return Cut();
+    __syncthreads();
+    if (tid == 0) sm.count = 0, sm.found = 0;
+    __syncthreads();
+    const float low = bin < BINS - 1 ? sc.under(bin) : -INFINITY;  // (the last holds all further ones)
+    items([&](float z, int i) {
+        if (z >= low && sc.bin(z) == bin) {
+            const uint32_t at = atomicAdd(&sm.count, 1u);
+            if (int(at) < most) room[at] = item_of(z, i);
+        }
+    });
+    __syncthreads();
+    const int n = int(sm.count);
+    if (n > PAIRS) {
+        // Half-precision logits are equal by the hundred: the digits decide,
+        // over the room or, past it, over all items.
+        const bool fits = n <= most;
+        auto some = [&](auto&& f) {
+            if (fits) {
+#pragma unroll 1
+                for (int i = tid; i < n; i += NT) f(item_value(room[i]), item_index(room[i]));
+            } else {
+                items(f);
+            }
+        };
+        const uint64_t edge = find_cut(some, sm, fits ? left : target, masses, w);
+        if (!fits) return Cut::at(edge);
+        // (the edge may lie below the bin: the last item of the bin above it)
+        if (tid == 0) sm.found = ~uint64_t(0);
+        __syncthreads();
+        for (int i = tid; i < n; i += NT)
+            if (room[i] >= edge)
+                atomicMin(reinterpret_cast<unsigned long long*>(&sm.found), static_cast<unsigned long long>(room[i]));
+        __syncthreads();
+        return Cut::at(sm.found);
+    }
+    const int e = tid / 4, lane4 = tid % 4;
+    if (e < n) {
+        const uint64_t mine = room[e];
+        uint64_t run = 0;
+        for (int j = lane4; j < n; j += 4) {
+            const uint64_t it = room[j];
+            if (it >= mine) run += masses ? w.mass(item_value(it)) : 1;
+        }
+        run = quad_sum_u64(run);
+        const uint64_t own = masses ? w.mass(item_value(mine)) : 1;
+        if (lane4 == 0 && own && run >= left && run - own < left) sm.found = mine;
+    }
+    __syncthreads();
+    return Cut::at(sm.found);
+}
+
+// The cuts of top_k and top_p over items, whose shares are summed by bins
+// first; row_mass: the mass that top_p is a share of where it is known (0:
+// it is summed here).
+template <typename S>
+__device__ Cut cuts(S&& items, const Settings& s, const Scale& sc, uint64_t row_mass, Shared& sm, uint64_t* room,
+                    int most, const Weigh& w) {
+    Cut cut;
+#pragma unroll 1
+    for (int step = s.k ? 0 : 1; step < (s.p < 1.0f ? 2 : 1); ++step) {
+        const bool masses = step == 1;
+        clear(sm.hist, BINS);
+        uint64_t own = 0;
+        items([&](float z, int i) {
+            if (!cut.keeps(z, i)) return;
+            const uint64_t v = masses ? w.mass(z) : 1;
+            own += v;
+            if (v) add(&sm.hist[sc.bin(z)], v);
+        });
+        uint64_t target = uint64_t(s.k);
+        if (masses) {
+            const uint64_t total = block_sum(own, sm);
+            target = share_of(s.p, row_mass && !s.k ? row_mass : total);
+        }
+        const Cut c = cut_by_bins(items, sc, sm, room, most, target, masses, w);
+        if (c.z > cut.z || (c.z == cut.z && c.i < cut.i)) cut = c;
+    }
+    return cut;
 }
 
 // The exact cuts and the draw over the list's n items (every item that can
 // be kept is there); `row_mass`: the mass that top_p is a share of, unless
 // top_k is on.
-__device__ void finish_list(int n, const Settings& s, float u, uint64_t row_mass, Shared& sm, const Result& out) {
+__device__ void finish_list(int n, const Settings& s, float u, uint64_t row_mass, const Scale& sc, Shared& sm,
+                            const Result& out) {
     const Weigh& w = out.w;
     const int tid = int(threadIdx.x);
-    __syncthreads();
-    for (int i = tid; i < n; i += NT) {
-        const double x = w(item_value(sm.item[i]));
-        sm.mass[i] = Weigh::fixed(x) | (x >= s.least ? 0 : UNDER);
-    }
-    __syncthreads();
     if (n <= PAIRS) {
         // Four threads an item: its place, the mass before it; the mass of
         // what stays; the running mass in index order.
         const int e = tid / 4, part = tid % 4;
-        const uint64_t mine = e < n ? sm.item[e] : 0, mass = e < n ? sm.mass[e] : 0;
-        uint64_t place = 0, before = 0, all = 0;
+        const uint64_t mine = e < n ? sm.item[e] : 0;
+        const double x = e < n ? w(item_value(mine)) : 0.0;
+        const uint64_t mass = Weigh::fixed(x);
+        if (part == 0 && e < n) sm.mass[e] = mass;
+        __syncthreads();
+        uint64_t place = 0, before = 0;
         for (int j = part; j < n; j += 4) {
-            const bool first = sm.item[j] > mine;
-            place += first;
-            if (first) before += sm.mass[j] & ~UNDER;
+            if (sm.item[j] > mine) before += sm.mass[j], ++place;
         }
-        place += __shfl_xor(place, 1, WAVE), before += __shfl_xor(before, 1, WAVE);
-        place += __shfl_xor(place, 2, WAVE), before += __shfl_xor(before, 2, WAVE);
+        place = quad_sum_u64(place), before = quad_sum_u64(before);
         bool keep = e < n && (s.k == 0 || place < uint64_t(s.k));
         if (s.p < 1.0f) {
-            all = row_mass;
-            if (s.k) all = block_sum(part == 0 && keep ? mass & ~UNDER : 0, sm);
+            const uint64_t all = s.k ? block_sum(part == 0 && keep ? mass : 0, sm) : row_mass;
             keep = keep && before < share_of(s.p, all);
         }
-        keep = keep && !(mass & UNDER);
-        __syncthreads();
+        keep = keep && x >= s.least;
         if (part == 0 && e < n) sm.hist[e] = keep ? mass : 0;
         __syncthreads();
         uint64_t run = 0, total = 0;
-        const uint32_t at = item_index(mine);
+        const int at = item_index(mine);
         for (int j = part; j < n; j += 4) {
             const uint64_t m = sm.hist[j];
             total += m;
             if (item_index(sm.item[j]) <= at) run += m;
         }
-        run += __shfl_xor(run, 1, WAVE), total += __shfl_xor(total, 1, WAVE);
-        run += __shfl_xor(run, 2, WAVE), total += __shfl_xor(total, 2, WAVE);
+        run = quad_sum_u64(run), total = quad_sum_u64(total);
         const uint64_t target = goal(u, total);
         if (part == 0 && keep && mass > 0 && run >= target && run - mass < target)
             out.write(item_value(mine), at, total);
         return;
     }
     auto items = [&](auto&& f) {
-        for (int i = tid; i < n; i += NT) f(sm.item[i], i);
+#pragma unroll 1
+        for (int i = tid; i < n; i += NT) f(item_value(sm.item[i]), item_index(sm.item[i]));
     };
-    uint64_t cut = 1;
-    if (s.k) cut = find_cut(items, sm, uint64_t(s.k), cut, [](uint64_t, int) { return uint64_t(1); });
-    if (s.p < 1.0f) {
-        uint64_t all = row_mass;
-        if (s.k) {
-            uint64_t own = 0;
-            items([&](uint64_t it, int i) { own += it >= cut ? sm.mass[i] & ~UNDER : 0; });
-            all = block_sum(own, sm);
-        }
-        cut = find_cut(items, sm, share_of(s.p, all), cut, [&](uint64_t, int i) { return sm.mass[i] & ~UNDER; });
-    }
-    // the draw: the digits of the index, 10 and 10 bits
+    const Cut cut = cuts(items, s, sc, row_mass, sm, sm.edge, PAIRS, w);
+    // the kept masses, then the draw: the digits of the index, 10 and 10 bits
     uint64_t own = 0;
-    items([&](uint64_t it, int i) { own += it >= cut && !(sm.mass[i] & UNDER) ? sm.mass[i] : 0; });
+#pragma unroll 1
+    for (int i = tid; i < n; i += NT) {
+        const float z = item_value(sm.item[i]);
+        const double x = w(z);
+        const uint64_t m = cut.keeps(z, item_index(sm.item[i])) && x >= s.least ? Weigh::fixed(x) : 0;
+        sm.mass[i] = m;
+        own += m;
+    }
     const uint64_t total = block_sum(own, sm);
     uint64_t target = goal(u, total);
-    uint32_t high = 0;
+    int high = 0;
+#pragma unroll 1
     for (int level = 0; level < 2; ++level) {
         clear(sm.hist, 1024);
-        items([&](uint64_t it, int i) {
-            const uint32_t at = item_index(it);
-            if (it < cut || (sm.mass[i] & UNDER) || sm.mass[i] == 0 || (level == 1 && at >> 10 != high)) return;
-            add(&sm.hist[level == 0 ? at >> 10 : at & 1023], sm.mass[i]);
-        });
+#pragma unroll 1
+        for (int i = tid; i < n; i += NT) {
+            const int at = item_index(sm.item[i]);
+            if (sm.mass[i] && (level == 0 || at >> 10 == high)) add(&sm.hist[level == 0 ? at >> 10 : at & 1023], sm.mass[i]);
+        }
         pick<false>(sm.hist, 1024, target, sm);
         target -= sm.before;
-        if (level == 0) high = sm.bin;
+        if (level == 0) high = int(sm.bin);
     }
-    const uint32_t at = high << 10 | sm.bin;
-    items([&](uint64_t it, int) {
-        if (item_index(it) == at) out.write(item_value(it), at, total);
-    });
+    const int at = high << 10 | int(sm.bin);
+    for (int i = tid; i < n; i += NT)
+        if (item_index(sm.item[i]) == at) out.write(item_value(sm.item[i]), at, total);
 }
 
-// The logits of the groups of GROUP whose maxima reach bin `last`: the
-// groups' numbers are collected first, so that four threads a group read
-// them, two groups at a time in flight.
-template <typename T, typename F>
-__device__ inline void each_of_groups(const Row<T>& row, const float* groups, const Scale& sc, int last, Shared& sm,
-                                      F&& f) {
+// Gathers into the list the row's logits from `low` up, by the groups whose
+// maxima reach it: the groups' numbers are collected first, so that four
+// threads a group read them, two groups at a time in flight.  The count may
+// pass CAP: then the list does not hold them all.
+template <typename T>
+__device__ int gather(const Row<T>& row, const float* groups, float low, Shared& sm) {
     uint32_t* ids = reinterpret_cast<uint32_t*>(sm.mass);
     constexpr int MOST = int(sizeof(sm.mass) / 4);  // (a row has up to 2^16 groups)
-    const int ngroup = int((row.n + GROUP - 1) / GROUP);
+    static_assert(MOST == 16 * NT, "a turn over the groups' maxima fills the room for their numbers");
+    const int ngroup = (row.n + GROUP - 1) / GROUP, tid = int(threadIdx.x);
+    __syncthreads();
+    if (tid == 0) sm.count = 0;
 #pragma unroll 1
     for (int g0 = 0; g0 < ngroup; g0 += MOST) {
-        const int g1 = g0 + MOST < ngroup ? g0 + MOST : ngroup;
         __syncthreads();
-        if (threadIdx.x == 0) sm.bin = 0;
-        __syncthreads();
-        const int lane = int(threadIdx.x) % WAVE;
-        for (int g = g0 + int(threadIdx.x); g - lane < g1; g += NT) {
-            const float m = g < g1 ? groups[g] : -INFINITY;
-            const bool in = m != -INFINITY && sc.bin(m) <= last;
-            const uint64_t some = __ballot(in);
-            uint32_t at = 0;
-            if (lane == 0 && some) at = atomicAdd(&sm.bin, uint32_t(__popcll(some)));
-            at = __builtin_amdgcn_readfirstlane(at);
-            if (in) ids[at + __popcll(some & ((uint64_t(1) << lane) - 1))] = uint32_t(g);
+        if (tid == 0) sm.bin = 0;
+        // (four maxima a load, four loads under way)
+        float4 m[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int g = g0 + (j * NT + tid) * 4;
+            m[j] = *reinterpret_cast<const float4*>(groups + (g < ngroup ? g : 0));
         }
         __syncthreads();
-        const int count = int(sm.bin);
+        uint32_t in = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int g = g0 + (j * NT + tid) * 4;
+            const uint32_t b = uint32_t(m[j].x >= low) | uint32_t(m[j].y >= low) << 1 | uint32_t(m[j].z >= low) << 2 |
+                               uint32_t(m[j].w >= low) << 3;
+            const int live = ngroup - g;  // (the room behind the last group's maximum)
+            in |= (live >= 4 ? b : live > 0 ? b & ((1u << live) - 1) : 0u) << (4 * j);
+        }
+        int at = places(&sm.bin, __popc(in));
+        for (uint32_t left = in; left; left &= left - 1) {
+            const int b = __builtin_ctz(left);
+            ids[at++] = uint32_t(g0 + (b / 4 * NT + tid) * 4 + b % 4);
+        }
+        __syncthreads();
+        const int count = int(sm.bin), turns = (count + NT / 2 - 1) / (NT / 2);
 #pragma unroll 1
-        for (int k = int(threadIdx.x) / 4; k < count; k += NT / 2) {
-            const int k2 = k + NT / 4;
-            const int64_t i0 = int64_t(ids[k]) * GROUP + threadIdx.x % 4 * 4;
-            const int64_t i1 = k2 < count ? int64_t(ids[k2]) * GROUP + threadIdx.x % 4 * 4 : row.n;
+        for (int t = 0; t < turns; ++t) {
+            const int k = t * (NT / 2) + tid / 4, k2 = k + NT / 4;
+            const int i0 = k < count ? int(ids[k]) * GROUP + tid % 4 * 4 : row.n;
+            const int i1 = k2 < count ? int(ids[k2]) * GROUP + tid % 4 * 4 : row.n;
             const auto v0 = row.load(i0), v1 = row.load(i1);
             float z[8];
             row.four(v0, i0, z);
             row.four(v1, i1, z + 4);
+            uint32_t pass = 0;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                if (z[c] != -INFINITY) f(z[c], uint32_t(i0 + c));
-                if (z[4 + c] != -INFINITY) f(z[4 + c], uint32_t(i1 + c));
-            }
+            for (int c = 0; c < 8; ++c) pass |= uint32_t(z[c] >= low) << c;
+            int to = places(&sm.count, __popc(pass));
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+                if (pass >> c & 1) {
+                    if (to < CAP) sm.item[to] = item_of(z[c], (c < 4 ? i0 : i1) + c % 4);
+                    ++to;
+                }
         }
     }
     __syncthreads();
+    return int(sm.count);
 }
 
-// Gathers into the list the row's logits that lie in bins 0 .. last.  The
-// count may pass CAP: then the list does not hold them all.
-template <typename T>
-__device__ inline int gather(const Row<T>& row, const float* groups, const Scale& sc, int last, Shared& sm) {
+// From the counts of `units` maxima by bins, each of as many logits: the bin
+// down to which the logits' mass is estimated to reach `target`, and their
+// number (sm.found).  With c of the maxima at or above a threshold there are
+// about -units log(1 - c / units) logits there.
+__device__ inline int guess_bin(int units, uint64_t target, const Scale& sc, Shared& sm, const Weigh& w) {
+    static_assert(BINS == 2 * NT, "two bins a thread");
+    const int tid = int(threadIdx.x);
     __syncthreads();
-    if (threadIdx.x == 0) sm.count = 0;
+    const uint64_t x0 = sm.hist[2 * tid], x1 = sm.hist[2 * tid + 1];
+    const uint64_t scan = wave_scan_u64(x0 + x1);
+    if (tid % WAVE == WAVE - 1) sm.part[wave_id()] = scan;
     __syncthreads();
-    each_of_groups(row, groups, sc, last, sm, [&](float z, uint32_t i) {
-        if (sc.bin(z) <= last) {
-            const int at = atomicAdd(&sm.count, 1);
-            if (at < CAP) sm.item[at] = item_of(z, i);
-        }
-    });
-    return sm.count;
+    const uint64_t waves = row_scan_u64(sm.part[tid % NWAVE]);
+    const uint64_t c2 = (wave_id() ? lane_u64(waves, wave_id() - 1) : 0) + scan, c1 = c2 - x1, c0 = c1 - x0;
+    auto logits = [&](uint64_t c) {  // (saturated: more than any list holds)
+        const float rest = 1.0f - float(c) / float(units);
+        return rest > 0.0f ? -float(units) * __logf(rest) : 1e7f;
+    };
+    const float n0 = logits(c0), n1 = logits(c1), n2 = logits(c2);
+    auto share = [&](float n, int bin) {
+        return uint64_t(n > 0.0f ? double(n) * double(w.mass(sc.max - float(bin + 1) / sc.per)) : 0.0);
+    };
+    sm.hist[2 * tid] = share(n1 - n0, 2 * tid);
+    sm.hist[2 * tid + 1] = share(n2 - n1, 2 * tid + 1);
+    pick<false>(sm.hist, BINS, target, sm);
+    const int bin = int(sm.bin);
+    if (tid == bin / 2) sm.found = sm.total < target ? ~uint64_t(0) : uint64_t(bin % 2 ? n2 : n1);
+    __syncthreads();
+    return bin;
 }
 
 // The list that holds every token that the filters can keep, if one can be
-// had: its length, or -1.  groups: the maxima of the row's groups.
+// had: its length, or -1.  groups: the maxima of the row's groups; chunk: the
+// thread's of its nchunk chunks (0: none are kept).
 template <typename T>
 __device__ int make_list(const Settings& s, const Scale& sc, Shared& sm, uint64_t row_mass, const Row<T>& row,
-                         const float* groups, const Weigh& w) {
-    if (!(sc.max < INFINITY)) return -1;
+                         const float* groups, float chunk, int nchunk, const Weigh& w) {
     const bool by_p = s.k == 0 && s.least == 0.0;
-    if (s.k || by_p) {
-        clear(sm.hist, BINS);
-        const int ngroup = int((row.n + GROUP - 1) / GROUP);
-#pragma unroll 4
-        for (int g = threadIdx.x; g < ngroup; g += NT) {
-            const float m = groups[g];
-            if (m != -INFINITY) add(&sm.hist[sc.bin(m)], 1);
-        }
-    }
-    // top_p alone: the groups that hold some 100 tokens, then some 4,000
+    const int ngroup = (row.n + GROUP - 1) / GROUP;
+    // top_p alone: a threshold with a little more mass above it by estimate,
+    // then with more; at last the whole row, if it fits.
     const uint64_t want = by_p ? share_of(s.p, row_mass) : 0;
 #pragma unroll 1
-    for (int guess = 0; guess < 2; ++guess) {
-        int last;
-        if (s.k || by_p) {
-            pick<false>(sm.hist, BINS, s.k ? uint64_t(s.k) : guess == 0 ? 96 : 3072, sm);
-            last = int(sm.bin);
-            if (last == BINS - 1) {
-                if (!sc.whole) return -1;
-                last = BINS - 2;  // (all that have a mass)
+    for (int guess = w.infinite ? 2 : 0;; ++guess) {
+        int last = -1;
+        if (guess == 2) {
+            // (everything)
+        } else if (s.k || by_p) {
+            // The coarsest maxima of which k are fewer than half: fewer
+            // maxima to count, and hardly more logits above the k-th.
+            const int k = s.k ? int(s.k) : ngroup >= 8192 ? ngroup / 8 : ngroup;
+            clear(sm.hist, BINS);
+            if (2 * k <= nchunk && s.k) {
+                if (chunk > -INFINITY) add(&sm.hist[sc.bin(chunk)], 1);
+            } else {
+                const bool fours = 2 * k <= ngroup / 4;
+#pragma unroll 2
+                for (int g = int(threadIdx.x) * 4; g < ngroup; g += NT * 4) {
+                    const float4 m = *reinterpret_cast<const float4*>(groups + g);
+                    float x[4] = {m.x, g + 1 < ngroup ? m.y : -INFINITY, g + 2 < ngroup ? m.z : -INFINITY,
+                                  g + 3 < ngroup ? m.w : -INFINITY};
+                    if (fours) {
+                        x[0] = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+                        if (x[0] > -INFINITY) add(&sm.hist[sc.bin(x[0])], 1);
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < 4; ++c)
+                            if (x[c] > -INFINITY) add(&sm.hist[sc.bin(x[c])], 1);
+                    }
+                }
+            }
+            if (s.k) {
+                pick<false>(sm.hist, BINS, uint64_t(k), sm);
+                last = int(sm.bin);
+            } else {
+                const uint64_t rest = row_mass > want ? row_mass - want : 0;
+                last = guess_bin(k < ngroup ? ngroup / 4 : ngroup, want + (guess == 0 ? rest / 4 : rest / 4 * 3), sc,
+                                 sm, w);
+                if (sm.found > CAP * 7 / 8) {
+                    if (row.n > CAP) return -1;
+                    last = BINS - 1;
+                }
             }
         } else {
             // z >= max + T log(min_p), and a bin to spare
             const float far = float(-log(s.least) * double(s.t)) * sc.per + 1.0f;
             last = far < float(BINS - 2) ? int(far) + 1 : BINS - 1;
-            if (last == BINS - 1) return -1;
         }
-        const int n = gather(row, groups, sc, last, sm);
+        if (last == BINS - 1) last = sc.whole ? BINS - 2 : -1;  // (all that have a mass)
+        const bool all = last < 0;
+        if (all && row.n > CAP) return -1;
+        const int n = gather(row, groups, all ? -3.4028235e38f : sc.under(last), sm);
+        if (n <= CAP && (all || !by_p)) return n;
         if (n > CAP) return -1;
-        if (!by_p) return n;
         uint64_t own = 0;
+#pragma unroll 1
         for (int i = threadIdx.x; i < n; i += NT) own += w.mass(item_value(sm.item[i]));
         if (block_sum(own, sm) >= want) return n;
     }
-    return -1;
 }
 
-// The cut over a whole row, found from the sums of `share` by bins of the
-// distance from the maximum (in sm.hist): the first items at which the
-// running share reaches `target` lie in one bin, whose items are gathered and
-// ordered.
-template <typename T, typename F>
-__device__ uint64_t cut_by_bins(const Row<T>& row, const Scale& sc, Shared& sm, uint64_t target, F&& share) {
-    pick<false>(sm.hist, BINS, target, sm);
-    const int bin = int(sm.bin);
-    const uint64_t left = target - sm.before;
-    __syncthreads();
-    if (threadIdx.x == 0) sm.count = 0;
-    __syncthreads();
-    row.each([&](float z, uint32_t i) {
-        if (sc.bin(z) == bin) {
-            const int at = atomicAdd(&sm.count, 1);
-            if (at < CAP) sm.item[at] = item_of(z, i);
-        }
-    });
-    __syncthreads();
-    const int n = sm.count;
-    if (n <= CAP) {
-        auto items = [&](auto&& f) {
-            for (int i = threadIdx.x; i < n; i += NT) f(sm.item[i], i);
-        };
-        const uint64_t edge = find_cut(items, sm, left, 1, [&](uint64_t it, int) { return share(item_value(it)); });
-        // (the edge may lie below the bin: the last item of the bin above it)
-        __syncthreads();
-        if (threadIdx.x == 0) sm.before = ~uint64_t(0);
-        __syncthreads();
-        items([&](uint64_t it, int) {
-            if (it >= edge) atomicMin(reinterpret_cast<unsigned long long*>(&sm.before), static_cast<unsigned long long>(it));
-        });
-        __syncthreads();
-        const uint64_t cut = sm.before;
-        __syncthreads();
-        return cut == ~uint64_t(0) ? 1 : cut;  // (nothing in the last bin: all stay)
+// Rows whose kept tokens do not fit a list, between the kernels.
+enum Step : uint32_t { DONE = 0, TO_CUT, TO_DRAW, TO_FINISH };
+struct Pending {
+    Cut cut;
+    float max;
+    uint32_t step;
+    uint32_t arrived[2];
+    uint32_t pad[2];
+};
+// What sample_stats leaves of a long row's 2,048 logits.
+struct Chunk {
+    float max;
+    uint32_t first;  // index of the first maximum
+    double sum;      // of exp((z - max) / T), where need_sum()
+};
+struct Workspace {
+    Pending* pending;   // [rows]
+    Chunk* chunks;      // [rows][nchunk] (this and what follows: long rows)
+    float* groups;      // [rows][nchunk * CHUNK / GROUP]
+    uint64_t* hist;     // [rows][BINS]
+    uint64_t* segs;     // [rows][nchunk * CHUNK / SEG]
+    int64_t nchunk;
+    Workspace from(int64_t r) const {
+        Workspace w = *this;
+        w.pending += r, w.chunks += r * nchunk, w.groups += r * nchunk * (CHUNK / GROUP);
+        w.hist += r * BINS, w.segs += r * nchunk * (CHUNK / SEG);
+        return w;
     }
-    auto items = [&](auto&& f) { row.each([&](float z, uint32_t i) { f(item_of(z, i), 0); }); };
-    return find_cut(items, sm, target, 1, [&](uint64_t it, int) { return share(item_value(it)); });
-}
-
-// The exact cuts and the draw over the whole row.
-template <typename T>
-__device__ void finish_row(const Row<T>& row, const Settings& s, float u, const Scale& sc, Shared& sm,
-                           const Result& out) {
-    const Weigh& w = out.w;
-    uint64_t cut = 1;  // every unmasked item
-    if (s.k) {
-        clear(sm.hist, BINS);
-        row.each([&](float z, uint32_t) { add(&sm.hist[sc.bin(z)], 1); });
-        cut = cut_by_bins(row, sc, sm, uint64_t(s.k), [](float) { return uint64_t(1); });
-    }
-    if (s.p < 1.0f) {
-        clear(sm.hist, BINS);
-        uint64_t own = 0;
-        row.each([&](float z, uint32_t i) {
-            if (item_of(z, i) < cut) return;
-            const uint64_t m = w.mass(z);
-            own += m;
-            if (m) add(&sm.hist[sc.bin(z)], m);
-        });
-        const uint64_t total = block_sum(own, sm);
-        // (a mass of top_k's cut that lies past top_p's is not reached)
-        const uint64_t c = cut_by_bins(row, sc, sm, share_of(s.p, total), [&](float z) { return w.mass(z); });
-        cut = c > cut ? c : cut;
-    }
-    auto kept = [&](float z, uint32_t i) -> uint64_t {
-        if (item_of(z, i) < cut) return 0;
-        const double x = w(z);
-        return x >= s.least ? Weigh::fixed(x) : 0;
-    };
-    __syncthreads();
-    row.sums(sm.item, kept);
-    const int ns = row.segments();
-    uint64_t own = 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < ns; i += NT) own += sm.item[i];
-    const uint64_t total = block_sum(own, sm), target = goal(u, total);
-    pick<false>(sm.item, ns, target, sm);
-    draw_in(row.p, row.n, int64_t(sm.bin) * SEG, SEG, target - sm.before, total, out, kept);
-}
-
-__device__ inline void nothing_left(const Result& out) {
-    *out.token = -1;
-    if (out.logprob) *out.logprob = -INFINITY;
-}
+};
 
 // Rows of at most SHORT logits: one workgroup a row.
 template <typename T>
-__global__ __launch_bounds__(NT) void sample_short(SampleArgs a) {
+__global__ __launch_bounds__(NT) void sample_short(SampleArgs a, Workspace ws) {
     __shared__ Shared sm;
-    __shared__ float groups[SHORT / GROUP];
+    __shared__ __attribute__((aligned(16))) float groups[SHORT / GROUP];
     const int64_t r = blockIdx.x;
     const int tid = int(threadIdx.x);
     const Row<T> row(static_cast<const T*>(a.logits) + r * a.ld, a.vocab);
     const Settings s = settings_of(a, r);
     const float u = a.u[r];
-    if (tid == 0) sm.kmax = 0, sm.kfirst = 0xffffffffu;
+    if (tid == 0) {
+        sm.kmax = 0, sm.kfirst = 0xffffffffu;
+        if (ws.pending) ws.pending[r].step = DONE;
+    }
     float zmax = -INFINITY;
     uint32_t first = 0xffffffffu;
-    row.turns([&](const float* z, int64_t i) {
+    row.turns([&](const float* z, int i) {
         float m = fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3]));
         if (m > zmax) {
             zmax = m;
@@ -683,88 +826,89 @@ __global__ __launch_bounds__(NT) void sample_short(SampleArgs a) {
         }
         m = fmaxf(m, dpp_f32<0xb1>(m));  // (four lanes of a quad: a group)
         m = fmaxf(m, dpp_f32<0x4e>(m));
-        if (tid % 4 == 0 && i < a.vocab) groups[i / GROUP] = m;
+        if (tid % 4 == 0 && i < SHORT) groups[i / GROUP] = m > -INFINITY ? m : -INFINITY;
     });
     const float wmax = wave_max(zmax);
     __syncthreads();
-    if (tid % WAVE == 0) atomicMax(&sm.kmax, key_of(wmax));
+    if (tid % WAVE == 0 && wmax > -INFINITY) atomicMax(&sm.kmax, key_of(wmax));
     __syncthreads();
-    const uint32_t kmax = sm.kmax;
-    const float top = value_of(kmax);
-    const Result out{a.tokens + r, a.logprob ? a.logprob + r : nullptr, {double(top), s.inv_t}};
+    const uint32_t kmax = __builtin_amdgcn_readfirstlane(sm.kmax);
+    const float top = kmax ? value_of(kmax) : -INFINITY;
+    const Result out(a, r, top, s);
     if (kmax == 0) {
-        if (tid == 0) nothing_left(out);
+        if (tid == 0) out.certain(-1);
         return;
     }
     if (s.greedy) {
         if (zmax == top) atomicMin(&sm.kfirst, first);
         __syncthreads();
-        if (tid == 0) out.certain(sm.kfirst);
+        if (tid == 0) out.certain(int(sm.kfirst));
         return;
     }
-    const Scale sc(top, s.t);
-    if (s.k || s.p < 1.0f || s.least > 0.0) {
-        uint64_t total = 0;
-        if (s.need_sum()) {
-            uint64_t own = 0;
-            row.each([&](float z, uint32_t) { own += out.w.mass(z); });
-            total = block_sum(own, sm);
-        }
-        const int n = make_list(s, sc, sm, total, row, groups, out.w);
-        if (n >= 0) {
-            finish_list(n, s, u, total, sm, out);
+    auto mass = [&](float z, int) { return out.w.mass(z); };
+    uint64_t total = 0;
+    if (s.need_sum()) {
+        row.sums(sm.item, mass);
+        __syncthreads();
+        total = block_sum(tid < row.segments() ? sm.item[tid] : 0, sm);
+        if (s.p >= 1.0f) {  // no filter
+            const uint64_t target = goal(u, total);
+            pick<false>(sm.item, row.segments(), target, sm);
+            draw_in(row, int(sm.bin) * SEG, target - sm.before, total, out, mass);
             return;
         }
     }
-    finish_row(row, s, u, sc, sm, out);
+    const Scale sc(top, s.t);
+    const int n = make_list(s, sc, sm, total, row, groups, -INFINITY, 0, out.w);
+    if (n >= 0)
+        finish_list(n, s, u, total, sc, sm, out);
+    else if (tid == 0)
+        ws.pending[r] = Pending{Cut(), top, TO_FINISH, {0, 0}, {0, 0}};
 }
 
-// What sample_stats leaves of a long row's 2,048 logits.
-struct Chunk {
-    float max;
-    uint32_t first;  // index of the first maximum
-    double sum;      // of exp((z - max) / T), where need_sum()
-};
-
 template <typename T, int VEC>
-__global__ __launch_bounds__(256) void sample_stats(SampleArgs a, Chunk* chunks, float* groups, int64_t nchunk) {
+__global__ __launch_bounds__(256) void sample_stats(SampleArgs a, Workspace ws) {
     constexpr int L = CHUNK / WAVE / VEC, G = GROUP / VEC;  // loads of a lane; lanes of a group
     const int lane = int(threadIdx.x) % WAVE;
-    const int64_t id = int64_t(blockIdx.x) * 4 + int(threadIdx.x) / WAVE;
+    const int64_t nchunk = ws.nchunk, id = int64_t(blockIdx.x) * 4 + wave_id();
     if (id >= a.rows * nchunk) return;
     const int64_t r = id / nchunk, c = id - r * nchunk;
-    const T* p = static_cast<const T*>(a.logits) + r * a.ld;
+    const T* p = static_cast<const T*>(a.logits) + r * a.ld + c * CHUNK;
+    const int n = int(a.vocab - c * CHUNK < CHUNK ? a.vocab - c * CHUNK : CHUNK);
     float z[L][VEC];
+    if (n == CHUNK) {
+        typedef T vec __attribute__((ext_vector_type(VEC)));
+        vec v[L];
 #pragma unroll
-    for (int j = 0; j < L; ++j) {
-        const int64_t i = c * CHUNK + (j * WAVE + lane) * VEC;
-        if (i + VEC <= a.vocab) {
-            typedef T vec __attribute__((ext_vector_type(VEC)));
-            const vec v = *reinterpret_cast<const vec*>(p + i);
+        for (int j = 0; j < L; ++j) v[j] = *reinterpret_cast<const vec*>(p + (j * WAVE + lane) * VEC);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) z[j][e] = float(v[e]);
-        } else {
+        for (int j = 0; j < L; ++j)
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) z[j][e] = i + e < a.vocab ? float(p[i + e]) : -INFINITY;
-        }
+            for (int e = 0; e < VEC; ++e) z[j][e] = float(v[j][e]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < L; ++j)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const int i = (j * WAVE + lane) * VEC + e;
+                z[j][e] = float(p[i < n ? i : n - 1]);
+                if (i >= n) z[j][e] = -INFINITY;
+            }
     }
     const Settings s = settings_of(a, r);
     float top = -INFINITY;
-    float* gr = groups + r * nchunk * (CHUNK / GROUP) + c * (CHUNK / GROUP);
+    float* gr = ws.groups + id * (CHUNK / GROUP);
 #pragma unroll
     for (int j = 0; j < L; ++j) {
-        float m = -INFINITY;
+        float m = z[j][0];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            z[j][e] = clean(z[j][e]);
-            m = fmaxf(m, z[j][e]);
-        }
+        for (int e = 1; e < VEC; ++e) m = fmaxf(m, z[j][e]);
         top = fmaxf(top, m);
 #pragma unroll
         for (int o = 1; o < G; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, WAVE));
-        if (lane % G == 0) gr[(j * WAVE + lane) / G] = m;
+        if (lane % G == 0) gr[(j * WAVE + lane) / G] = m > -INFINITY ? m : -INFINITY;
     }
-    top = wave_max(top);
+    top = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, wave_max(top))));
     uint32_t first = 0xffffffffu;
 #pragma unroll
     for (int j = L - 1; j >= 0; --j)
@@ -778,7 +922,7 @@ __global__ __launch_bounds__(256) void sample_stats(SampleArgs a, Chunk* chunks,
     }
     double sum = 0.0;
     if (s.need_sum() && top > -INFINITY) {
-        const Weigh w{double(top), s.inv_t};
+        const Weigh w(top, s.inv_t);
 #pragma unroll
         for (int j = 0; j < L; ++j)
 #pragma unroll
@@ -786,119 +930,133 @@ __global__ __launch_bounds__(256) void sample_stats(SampleArgs a, Chunk* chunks,
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, WAVE);
     }
-    if (lane == 0) chunks[id] = Chunk{top, first, sum};
+    if (lane == 0) ws.chunks[id] = Chunk{top, first, sum};
 }
-
-// Long rows whose kept tokens do not fit a list, between the kernels.
-struct Pending {
-    uint64_t cut;       // the first item that goes
-    uint32_t kmax;
-    uint32_t step;      // 0: done; 1: the cut is to be found; 2: the draw
-    uint32_t arrived[2];
-};
-struct Workspace {
-    Chunk* chunks;      // [rows][nchunk]
-    float* groups;      // [rows][nchunk * CHUNK / GROUP]
-    Pending* pending;   // [rows]
-    uint64_t* hist;     // [rows][BINS]
-    uint64_t* segs;     // [rows][nchunk * CHUNK / SEG]
-    int64_t nchunk;
-    Workspace from(int64_t r) const {
-        Workspace w = *this;
-        w.chunks += r * nchunk, w.groups += r * nchunk * (CHUNK / GROUP), w.pending += r;
-        w.hist += r * BINS, w.segs += r * nchunk * (CHUNK / SEG);
-        return w;
-    }
-};
-
-constexpr int PART = 16 * NT;  // logits of a workgroup of the wide kernels
 
 template <typename T>
 __global__ __launch_bounds__(NT) void sample_long(SampleArgs a, Workspace ws) {
     __shared__ Shared sm;
-    const int64_t r = blockIdx.x, nchunk = ws.nchunk;
-    const int tid = int(threadIdx.x);
+    const int64_t r = blockIdx.x;
+    const int tid = int(threadIdx.x), nchunk = int(ws.nchunk);  // (nchunk <= NT)
+    const Chunk mine = tid < nchunk ? ws.chunks[r * nchunk + tid] : Chunk{-INFINITY, 0xffffffffu, 0.0};
     const Settings s = settings_of(a, r);
     const float u = a.u[r];
-    const Chunk* chunks = ws.chunks + r * nchunk;
     const float* groups = ws.groups + r * nchunk * (CHUNK / GROUP);
     const Row<T> row(static_cast<const T*>(a.logits) + r * a.ld, a.vocab);
-    if (tid == 0) sm.kmax = 0, sm.kfirst = 0xffffffffu, ws.pending[r].step = 0;
-    __syncthreads();
-    const Chunk mine = tid < nchunk ? chunks[tid] : Chunk{-INFINITY, 0xffffffffu, 0.0};  // (nchunk <= NT)
+    if (tid == 0) sm.kmax = 0, sm.kfirst = 0xffffffffu, ws.pending[r].step = DONE;
     const float wmax = wave_max(mine.max);
-    if (tid % WAVE == 0) atomicMax(&sm.kmax, key_of(wmax));
     __syncthreads();
-    const uint32_t kmax = sm.kmax;
-    const float top = value_of(kmax);
-    Result out{a.tokens + r, a.logprob ? a.logprob + r : nullptr, {double(top), s.inv_t}};
+    if (tid % WAVE == 0 && wmax > -INFINITY) atomicMax(&sm.kmax, key_of(wmax));
+    __syncthreads();
+    const uint32_t kmax = __builtin_amdgcn_readfirstlane(sm.kmax);
+    const float top = kmax ? value_of(kmax) : -INFINITY;
+    const Result out(a, r, top, s);
     if (kmax == 0) {
-        if (tid == 0) nothing_left(out);
+        if (tid == 0) out.certain(-1);
         return;
     }
     if (s.greedy) {
         if (mine.max == top) atomicMin(&sm.kfirst, mine.first);
         __syncthreads();
-        if (tid == 0) out.certain(sm.kfirst);
+        if (tid == 0) out.certain(int(sm.kfirst));
         return;
     }
-    uint64_t own = 0, total = 0;
+    uint64_t total = 0;
     if (s.need_sum()) {
         // (a chunk has a mass where one of its logits has)
         const double x = out.w(mine.max);
-        if (Weigh::fixed(x)) own = uint64_t(rint(mine.sum * x * ONE));
+        const uint64_t own = Weigh::fixed(x) ? uint64_t(rint(mine.sum * x * ONE)) : 0;
         total = block_sum(own, sm);
-    }
-    if (s.k == 0 && s.p >= 1.0f && s.least == 0.0) {
-        sm.hist[tid] = own;
-        const uint64_t target = goal(u, total);
-        pick<false>(sm.hist, NT, target, sm);
-        const int64_t c = sm.bin;
-        const uint64_t left = target - sm.before;
-        // the chunk's segments, then the segment
-        const Row<T> part(row.p + c * CHUNK, a.vocab - c * CHUNK < CHUNK ? a.vocab - c * CHUNK : CHUNK);
-        auto mass = [&](float z, uint32_t) { return out.w.mass(z); };
-        __syncthreads();
-        part.sums(sm.item, mass);
-        pick<false>(sm.item, part.segments(), left, sm);
-        // (the chunk's sum and its logits' masses differ by their rounding:
-        // past the end is the last logit with a mass)
-        int seg = int(sm.bin);
-        uint64_t target2 = left > sm.before ? left - sm.before : 1;
-        if (sm.total < left) {
-            while (seg > 0 && sm.item[seg] == 0) --seg;
-            target2 = sm.item[seg];
+        if (s.p >= 1.0f) {  // no filter: the chunk, its segment, the logit
+            sm.hist[tid] = own;
+            const uint64_t target = goal(u, total);
+            pick<false>(sm.hist, NT, target, sm);
+            const int c = int(sm.bin);
+            const uint64_t left = target - sm.before;
+            const Row<T> part(row.p + c * CHUNK, row.n - c * CHUNK < CHUNK ? row.n - c * CHUNK : CHUNK);
+            auto mass = [&](float z, int) { return out.w.mass(z); };
+            __syncthreads();
+            part.sums(sm.item, mass);
+            pick<false>(sm.item, part.segments(), left, sm);
+            // (the chunk's sum and its logits' masses differ by their
+            // rounding: past the end is the last logit with a mass)
+            int seg = int(sm.bin);
+            uint64_t rest = left > sm.before ? left - sm.before : 1;
+            if (sm.total < left) {
+                while (seg > 0 && sm.item[seg] == 0) --seg;
+                rest = sm.item[seg];
+            }
+            draw_in(row, c * CHUNK + seg * SEG, rest, total, out, mass);
+            return;
         }
-        draw_in(row.p, a.vocab, c * CHUNK + int64_t(seg) * SEG, SEG, target2, total, out, mass);
-        return;
     }
     const Scale sc(top, s.t);
-    const int n = make_list(s, sc, sm, total, row, groups, out.w);
+    const int n = make_list(s, sc, sm, total, row, groups, mine.max, nchunk, out.w);
     if (n >= 0) {
-        finish_list(n, s, u, total, sm, out);
+        finish_list(n, s, u, total, sc, sm, out);
         return;
     }
-    if (s.k) {
-        finish_row(row, s, u, sc, sm, out);
-        return;
+    if (!s.k && s.p < 1.0f)
+        for (int i = tid; i < BINS; i += NT) ws.hist[r * BINS + i] = 0;
+    if (tid == 0)
+        ws.pending[r] = Pending{Cut(), top, s.k ? TO_FINISH : s.p < 1.0f ? TO_CUT : TO_DRAW, {0, 0}, {0, 0}};
+}
+
+// The logits' masses that the filters keep.
+struct Kept {
+    Cut cut;
+    double least;
+    const Weigh& w;
+    __device__ uint64_t operator()(float z, int i) const {
+        if (!cut.keeps(z, i)) return 0;
+        const double x = w(z);
+        return x >= least ? Weigh::fixed(x) : 0;
     }
-    for (int i = tid; i < BINS; i += NT) ws.hist[r * BINS + i] = 0;
-    if (tid == 0) ws.pending[r] = Pending{1, kmax, s.p < 1.0f ? 1u : 2u, {0, 0}};
+};
+
+// The exact cuts and the draw over a whole row.
+template <typename T>
+__global__ __launch_bounds__(NT) void sample_row(SampleArgs a, Workspace ws) {
+    const int64_t r = blockIdx.x;
+    if (ws.pending[r].step != TO_FINISH) return;
+    __shared__ Shared sm;
+    const int tid = int(threadIdx.x);
+    const float top = ws.pending[r].max;
+    const Settings s = settings_of(a, r);
+    const Row<T> row(static_cast<const T*>(a.logits) + r * a.ld, a.vocab);
+    const Result out(a, r, top, s);
+    const Scale sc(top, s.t);
+    auto items = [&](auto&& f) {
+        row.turns([&](const float* z, int i) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                if (z[c] > -INFINITY) f(z[c], i + c);
+        });
+    };
+    const Kept kept{cuts(items, s, sc, 0, sm, sm.item, CAP, out.w), s.least, out.w};
+    row.sums(sm.item, kept);
+    __syncthreads();
+    const int ns = row.segments();
+    uint64_t own = 0;
+    for (int i = tid; i < ns; i += NT) own += sm.item[i];
+    const uint64_t total = block_sum(own, sm), target = goal(a.u[r], total);
+    pick<false>(sm.item, ns, target, sm);
+    draw_in(row, int(sm.bin) * SEG, target - sm.before, total, out, kept);
 }
 
 // Whether this workgroup is the last of its row's to arrive; what the others
 // wrote before is then visible to it.  (One thread fences for all, ordered
 // with them by the barriers: a fence writes back and invalidates the L2, and
 // one by every wave took 300 us of a 16.8 million logits' pass.)
-__device__ inline bool last_of(uint32_t* arrived, Shared& sm) {
+__device__ inline bool last_of(uint32_t* arrived, Common& sm) {
     __syncthreads();
     if (threadIdx.x == 0) {
         __threadfence();
-        sm.count = int(atomicAdd(arrived, 1u));
+        sm.count = atomicAdd(arrived, 1u);
         __threadfence();
     }
     __syncthreads();
-    const bool last = sm.count == int(gridDim.x) - 1;
+    const bool last = sm.count == gridDim.x - 1;
     __syncthreads();
     return last;
 }
@@ -907,30 +1065,32 @@ __device__ inline uint64_t load_shared(const uint64_t* p) {  // written by other
 }
 
 // The logits of this workgroup's part of a row.
-__device__ inline int64_t part_size(int64_t n) {
-    const int64_t left = n - int64_t(blockIdx.x) * PART;
-    return left < PART ? left : PART;
+template <typename T>
+__device__ inline Row<T> part_of(const Row<T>& row) {
+    const int first = int(blockIdx.x) * PART;
+    return Row<T>(row.p + first, row.n - first < PART ? row.n - first : PART);
 }
 
-// The masses of pending rows by bins; the last workgroup of a row finds
+// The masses of rows TO_CUT by bins; the last workgroup of a row finds
 // top_p's cut.
 template <typename T>
 __global__ __launch_bounds__(NT) void sample_bins(SampleArgs a, Workspace ws) {
     const int64_t r = blockIdx.y;
     Pending& pd = ws.pending[r];
-    if (pd.step != 1) return;
+    if (pd.step != TO_CUT) return;
     __shared__ Shared sm;
     const int tid = int(threadIdx.x);
     const Settings s = settings_of(a, r);
     const Row<T> row(static_cast<const T*>(a.logits) + r * a.ld, a.vocab);
-    const float top = value_of(pd.kmax);
-    const Weigh w{double(top), s.inv_t};
-    const Scale sc(top, s.t);
+    const Weigh w(pd.max, s.inv_t);
+    const Scale sc(pd.max, s.t);
     clear(sm.hist, BINS);
-    const Row<T> part(row.p + int64_t(blockIdx.x) * PART, part_size(row.n));
-    part.each([&](float z, uint32_t) {
-        const uint64_t m = w.mass(z);
-        if (m) add(&sm.hist[sc.bin(z)], m);
+    part_of(row).turns([&](const float* z, int) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const uint64_t m = w.mass(z[c]);
+            if (m) add(&sm.hist[sc.bin(z[c])], m);
+        }
     });
     __syncthreads();
     uint64_t* hist = ws.hist + r * BINS;
@@ -943,37 +1103,37 @@ __global__ __launch_bounds__(NT) void sample_bins(SampleArgs a, Workspace ws) {
         own += sm.hist[i];
     }
     const uint64_t total = block_sum(own, sm);
-    const uint64_t cut = cut_by_bins(row, sc, sm, share_of(s.p, total), [&](float z) { return w.mass(z); });
-    if (tid == 0) pd.cut = cut, pd.step = 2;
+    auto items = [&](auto&& f) {
+        row.turns([&](const float* z, int i) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                if (z[c] > -INFINITY) f(z[c], i + c);
+        });
+    };
+    const Cut cut = cut_by_bins(items, sc, sm, sm.item, CAP, share_of(s.p, total), true, w);
+    if (tid == 0) pd.cut = cut, pd.step = TO_DRAW;
 }
 
-// The kept masses of pending rows by segments; the last workgroup of a row
+// The kept masses of rows TO_DRAW by segments; the last workgroup of a row
 // draws.
 template <typename T>
 __global__ __launch_bounds__(NT) void sample_draw(SampleArgs a, Workspace ws) {
     const int64_t r = blockIdx.y;
     Pending& pd = ws.pending[r];
-    if (pd.step != 2) return;
-    __shared__ Shared sm;
+    if (pd.step != TO_DRAW) return;
+    __shared__ DrawShared sm;
     const int tid = int(threadIdx.x);
     const Settings s = settings_of(a, r);
-    const T* p = static_cast<const T*>(a.logits) + r * a.ld;
-    const Result out{a.tokens + r, a.logprob ? a.logprob + r : nullptr, {double(value_of(pd.kmax)), s.inv_t}};
-    const uint64_t cut = pd.cut;
-    auto kept = [&](float z, uint32_t i) -> uint64_t {
-        if (item_of(z, i) < cut) return 0;
-        const double x = out.w(z);
-        return x >= s.least ? Weigh::fixed(x) : 0;
-    };
-    const int64_t first = int64_t(blockIdx.x) * PART, ns = ws.nchunk * (CHUNK / SEG);
-    uint64_t* segs = ws.segs + r * ns;
-    const Row<T> part(p + first, part_size(a.vocab));
-    // (the segments of a part end with the row, the row's with its chunks)
-    part.sums(sm.item, [&](float z, uint32_t i) { return kept(z, uint32_t(first) + i); });
+    const Row<T> row(static_cast<const T*>(a.logits) + r * a.ld, a.vocab);
+    const Result out(a, r, pd.max, s);
+    const Kept kept{pd.cut, s.least, out.w};
+    const int first = int(blockIdx.x) * PART, ns = row.segments();
+    uint64_t* segs = ws.segs + r * ws.nchunk * (CHUNK / SEG);
+    const Row<T> part = part_of(row);
+    part.sums(sm.item, [&](float z, int i) { return kept(z, first + i); });
     __syncthreads();
-    for (int i = tid; i < PART / SEG && first / SEG + i < ns; i += NT)
-        __hip_atomic_store(segs + first / SEG + i, i < part.segments() ? sm.item[i] : 0, __ATOMIC_RELAXED,
-                           __HIP_MEMORY_SCOPE_AGENT);
+    if (tid < part.segments())
+        __hip_atomic_store(segs + first / SEG + tid, sm.item[tid], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     if (!last_of(&pd.arrived[1], sm)) return;
     uint64_t own = 0;
     for (int i = tid; i < ns; i += NT) {
@@ -981,8 +1141,8 @@ __global__ __launch_bounds__(NT) void sample_draw(SampleArgs a, Workspace ws) {
         own += sm.item[i];
     }
     const uint64_t total = block_sum(own, sm), target = goal(a.u[r], total);
-    pick<false>(sm.item, int(ns), target, sm);
-    draw_in(p, a.vocab, int64_t(sm.bin) * SEG, SEG, target - sm.before, total, out, kept);
+    pick<false>(sm.item, ns, target, sm);
+    draw_in(row, int(sm.bin) * SEG, target - sm.before, total, out, kept);
 }
 
 void check(const SampleArgs& a) {
@@ -1004,44 +1164,49 @@ SampleArgs rows_from(SampleArgs a, int64_t r) {
     return a;
 }
 
-int64_t chunks_of(int64_t vocab) { return (vocab + CHUNK - 1) / CHUNK; }
+int64_t chunks_of(int64_t vocab) { return vocab <= SHORT ? 0 : (vocab + CHUNK - 1) / CHUNK; }
 
 template <typename T>
 void launch(hipStream_t s, const SampleArgs& a, void* workspace) {
     const dim3 grid{unsigned(a.rows)}, block{NT};
+    Workspace ws{};
+    ws.nchunk = chunks_of(a.vocab);
+    const int64_t n = a.rows * ws.nchunk;
+    if (a.vocab > CAP) ws.pending = static_cast<Pending*>(workspace);  // (others always fit the list)
+    ws.chunks = reinterpret_cast<Chunk*>(ws.pending + a.rows);
+    ws.groups = reinterpret_cast<float*>(ws.chunks + n);
+    ws.hist = reinterpret_cast<uint64_t*>(ws.groups + n * (CHUNK / GROUP));
+    ws.segs = ws.hist + a.rows * BINS;
     if (a.vocab <= SHORT) {
-        sample_short<T><<<grid, block, 0, s>>>(a);
-    } else {
-        const int64_t nchunk = chunks_of(a.vocab);
-        Workspace ws;
-        ws.nchunk = nchunk;
-        ws.chunks = static_cast<Chunk*>(workspace);
-        ws.hist = reinterpret_cast<uint64_t*>(ws.chunks + a.rows * nchunk);
-        ws.segs = ws.hist + a.rows * BINS;
-        ws.pending = reinterpret_cast<Pending*>(ws.segs + a.rows * nchunk * (CHUNK / SEG));
-        ws.groups = reinterpret_cast<float*>(ws.pending + a.rows);
-        const dim3 wide{unsigned((a.rows * nchunk + 3) / 4)};
-        constexpr int VEC = 16 / int(sizeof(T));
-        if (reinterpret_cast<uintptr_t>(a.logits) % 16 == 0 && a.ld % VEC == 0)
-            sample_stats<T, VEC><<<wide, dim3(256), 0, s>>>(a, ws.chunks, ws.groups, nchunk);
-        else
-            sample_stats<T, 1><<<wide, dim3(256), 0, s>>>(a, ws.chunks, ws.groups, nchunk);
+        sample_short<T><<<grid, block, 0, s>>>(a, ws);
         OMG_HIP(hipGetLastError());
-        sample_long<T><<<grid, block, 0, s>>>(a, ws);
-        if (a.top_p || a.min_p) {
+        if (a.vocab > CAP && (a.top_k || a.top_p || a.min_p)) {
+            sample_row<T><<<grid, block, 0, s>>>(a, ws);
             OMG_HIP(hipGetLastError());
-            for (int64_t r = 0; r < a.rows; r += 65535) {  // (a grid's second size)
-                const dim3 parts{unsigned((a.vocab + PART - 1) / PART), unsigned(std::min<int64_t>(65535, a.rows - r))};
-                const SampleArgs b = rows_from<T>(a, r);
-                const Workspace wr = ws.from(r);
-                if (a.top_p) sample_bins<T><<<parts, block, 0, s>>>(b, wr);
-                OMG_HIP(hipGetLastError());
-                sample_draw<T><<<parts, block, 0, s>>>(b, wr);
-                OMG_HIP(hipGetLastError());
-            }
         }
+        return;
     }
+    const dim3 wide{unsigned((n + 3) / 4)};
+    constexpr int VEC = 16 / int(sizeof(T));
+    if (reinterpret_cast<uintptr_t>(a.logits) % 16 == 0 && a.ld % VEC == 0)
+        sample_stats<T, VEC><<<wide, dim3(256), 0, s>>>(a, ws);
+    else
+        sample_stats<T, 1><<<wide, dim3(256), 0, s>>>(a, ws);
     OMG_HIP(hipGetLastError());
+    sample_long<T><<<grid, block, 0, s>>>(a, ws);
+    OMG_HIP(hipGetLastError());
+    if (a.top_k) {
+        sample_row<T><<<grid, block, 0, s>>>(a, ws);
+        OMG_HIP(hipGetLastError());
+    }
+    if (!a.top_p && !a.min_p) return;
+    for (int64_t r = 0; r < a.rows; r += 65535) {  // (a grid's second size)
+        const dim3 parts{unsigned((a.vocab + PART - 1) / PART), unsigned(std::min<int64_t>(65535, a.rows - r))};
+        if (a.top_p) sample_bins<T><<<parts, block, 0, s>>>(rows_from<T>(a, r), ws.from(r));
+        OMG_HIP(hipGetLastError());
+        sample_draw<T><<<parts, block, 0, s>>>(rows_from<T>(a, r), ws.from(r));
+        OMG_HIP(hipGetLastError());
+    }
 }
 
 }  // namespace
@@ -1050,10 +1215,11 @@ int64_t sample_workspace(int64_t rows, int64_t vocab) {
     SampleArgs a{};
     a.rows = rows, a.vocab = vocab;
     check(a);
-    static_assert(sizeof(Pending) % 8 == 0 && sizeof(Chunk) % 16 == 0, "the workspace's arrays are aligned");
-    return vocab <= SHORT ? 0
-                          : rows * (chunks_of(vocab) * int64_t(sizeof(Chunk) + CHUNK / SEG * 8 + CHUNK / GROUP * 4) +
-                                    BINS * 8 + int64_t(sizeof(Pending)));
+    static_assert(sizeof(Pending) % 16 == 0 && sizeof(Chunk) % 16 == 0, "the workspace's arrays are aligned");
+    if (vocab <= CAP) return 0;
+    const int64_t n = chunks_of(vocab);
+    return rows * (int64_t(sizeof(Pending)) + n * int64_t(sizeof(Chunk) + CHUNK / SEG * 8 + CHUNK / GROUP * 4) +
+                   (n ? BINS * 8 : 0));
 }
 
 void launch_sample(hipStream_t s, const SampleArgs& a, void* workspace, size_t bytes) {
