@@ -53,6 +53,7 @@ constexpr int BINS = 2048;
 constexpr int PAIRS = NT / 4;     // items compared pair by pair: four threads each
 constexpr int SEG = 256;          // consecutive logits a wave takes at once
 constexpr int PART = 16 * NT;     // logits of a workgroup of the wide kernels
+constexpr int EDGE = 2048;        // logits of one bin that they set apart
 constexpr int IDX_BITS = 20;      // vocab <= 2^20
 constexpr uint32_t IDX_MASK = (1u << IDX_BITS) - 1;
 constexpr double ONE = 4398046511104.0;  // 2^42
@@ -194,6 +195,8 @@ struct Shared : Common {
 };
 struct DrawShared : Common {
     uint64_t item[(1 << IDX_BITS) / SEG];  // the masses of the row's segments
+    uint64_t hist[BINS];
+    uint64_t edge[EDGE];
 };
 __device__ inline int wave_id() { return __builtin_amdgcn_readfirstlane(int(threadIdx.x) / WAVE); }
 
@@ -415,8 +418,8 @@ __device__ inline void draw_in(const Row<T>& row, int first, uint64_t target, ui
 // first reaches `target` (>= 1); 0 if it never does, or an item below all
 // that do.  items(f) calls f(z, i) for the thread's items; masses: an item's
 // share is its mass, else one.
-template <typename S>
-__device__ uint64_t find_cut(S&& items, Shared& sm, uint64_t target, bool masses, const Weigh& w) {
+template <typename S, typename M>
+__device__ uint64_t find_cut(S&& items, M& sm, uint64_t target, bool masses, const Weigh& w) {
     uint64_t prefix = 0, before = 0;
     int shift = 52;
 #pragma unroll 1
@@ -438,43 +441,20 @@ __device__ uint64_t find_cut(S&& items, Shared& sm, uint64_t target, bool masses
     return prefix << shift;
 }
 
-// The cut at which the running share reaches `target`, the shares' sums by
-// bins in sm.hist: the items of the bin where it does are collected, in
-// room[0 .. most), and compared pair by pair.
-template <typename S>
-__device__ Cut cut_by_bins(S&& items, const Scale& sc, Shared& sm, uint64_t* room, int most, uint64_t target,
-                           bool masses, const Weigh& w) {
+// The cut within one bin: room[0 .. n) are its items, `left` the share that
+// is taken from them (reached among them).  They are compared pair by pair;
+// half-precision logits are equal by the hundred, and where they are many
+// the digits decide.
+template <typename M>
+__device__ Cut cut_in_bin(const uint64_t* room, int n, M& sm, uint64_t left, bool masses, const Weigh& w) {
     const int tid = int(threadIdx.x);
-    pick<false>(sm.hist, BINS, target, sm);
-    const int bin = int(sm.bin);
-    const uint64_t left = target - sm.before;
-    if (sm.total < target) return Cut();
     __syncthreads();
-    if (tid == 0) sm.count = 0, sm.found = 0;
-    __syncthreads();
-    const float low = bin < BINS - 1 ? sc.under(bin) : -INFINITY;  // (the last holds all further ones)
-    items([&](float z, int i) {
-        if (z >= low && sc.bin(z) == bin) {
-            const uint32_t at = atomicAdd(&sm.count, 1u);
-            if (int(at) < most) room[at] = item_of(z, i);
-        }
-    });
-    __syncthreads();
-    const int n = int(sm.count);
     if (n > PAIRS) {
-        // Half-precision logits are equal by the hundred: the digits decide,
-        // over the room or, past it, over all items.
-        const bool fits = n <= most;
         auto some = [&](auto&& f) {
-            if (fits) {
 #pragma unroll 1
-                for (int i = tid; i < n; i += NT) f(item_value(room[i]), item_index(room[i]));
-            } else {
-                items(f);
-            }
+            for (int i = tid; i < n; i += NT) f(item_value(room[i]), item_index(room[i]));
         };
-        const uint64_t edge = find_cut(some, sm, fits ? left : target, masses, w);
-        if (!fits) return Cut::at(edge);
+        const uint64_t edge = find_cut(some, sm, left, masses, w);
         // (the edge may lie below the bin: the last item of the bin above it)
         if (tid == 0) sm.found = ~uint64_t(0);
         __syncthreads();
@@ -484,6 +464,8 @@ __device__ Cut cut_by_bins(S&& items, const Scale& sc, Shared& sm, uint64_t* roo
         __syncthreads();
         return Cut::at(sm.found);
     }
+    if (tid == 0) sm.found = 0;
+    __syncthreads();
     const int e = tid / 4, lane4 = tid % 4;
     if (e < n) {
         const uint64_t mine = room[e];
@@ -498,6 +480,32 @@ __device__ Cut cut_by_bins(S&& items, const Scale& sc, Shared& sm, uint64_t* roo
     }
     __syncthreads();
     return Cut::at(sm.found);
+}
+
+// The cut at which the running share reaches `target`, the shares' sums by
+// bins in sm.hist: the items of the bin where it does are collected, in
+// room[0 .. most); past the room the digits decide over all items.
+template <typename S>
+__device__ Cut cut_by_bins(S&& items, const Scale& sc, Shared& sm, uint64_t* room, int most, uint64_t target,
+                           bool masses, const Weigh& w) {
+    pick<false>(sm.hist, BINS, target, sm);
+    const int bin = int(sm.bin);
+    const uint64_t left = target - sm.before;
+    if (sm.total < target) return Cut();
+    __syncthreads();
+    if (threadIdx.x == 0) sm.count = 0;
+    __syncthreads();
+    const float low = bin < BINS - 1 ? sc.under(bin) : -INFINITY;  // (the last holds all further ones)
+    items([&](float z, int i) {
+        if (z >= low && sc.bin(z) == bin) {
+            const uint32_t at = atomicAdd(&sm.count, 1u);
+            if (int(at) < most) room[at] = item_of(z, i);
+        }
+    });
+    __syncthreads();
+    const int n = int(sm.count);
+    if (n > most) return Cut::at(find_cut(items, sm, target, masses, w));
+    return cut_in_bin(room, n, sm, left, masses, w);
 }
 
 // The cuts of top_k and top_p over items, whose shares are summed by bins
@@ -711,7 +719,7 @@ __device__ int make_list(const Settings& s, const Scale& sc, Shared& sm, uint64_
     const bool by_p = s.k == 0 && s.least == 0.0;
     const int ngroup = (row.n + GROUP - 1) / GROUP;
     // top_p alone: a threshold with a little more mass above it by estimate,
-    // then with more; at last the whole row, if it fits.
+    // then with more.
     const uint64_t want = by_p ? share_of(s.p, row_mass) : 0;
 #pragma unroll 1
     for (int guess = w.infinite ? 2 : 0;; ++guess) {
@@ -749,10 +757,7 @@ __device__ int make_list(const Settings& s, const Scale& sc, Shared& sm, uint64_
                 const uint64_t rest = row_mass > want ? row_mass - want : 0;
                 last = guess_bin(k < ngroup ? ngroup / 4 : ngroup, want + (guess == 0 ? rest / 4 : rest / 4 * 3), sc,
                                  sm, w);
-                if (sm.found > CAP * 7 / 8) {
-                    if (row.n > CAP) return -1;
-                    last = BINS - 1;
-                }
+                if (sm.found > PAIRS) return -1;  // (the wide kernels are no slower)
             }
         } else {
             // z >= max + T log(min_p), and a bin to spare
@@ -775,12 +780,14 @@ __device__ int make_list(const Settings& s, const Scale& sc, Shared& sm, uint64_
 // Rows whose kept tokens do not fit a list, between the kernels.
 enum Step : uint32_t { DONE = 0, TO_CUT, TO_DRAW, TO_FINISH };
 struct Pending {
-    Cut cut;
+    uint64_t left;       // the mass that top_p takes from bin `bin`
     float max;
     uint32_t step;
+    int bin;             // bins before it stay whole
     uint32_t arrived[2];
-    uint32_t pad[2];
+    uint32_t edges;      // logits of the bin
 };
+__device__ inline Pending to_finish(float max) { return Pending{0, max, TO_FINISH, 0, {0, 0}, 0}; }
 // What sample_stats leaves of a long row's 2,048 logits.
 struct Chunk {
     float max;
@@ -791,13 +798,14 @@ struct Workspace {
     Pending* pending;   // [rows]
     Chunk* chunks;      // [rows][nchunk] (this and what follows: long rows)
     float* groups;      // [rows][nchunk * CHUNK / GROUP]
-    uint64_t* hist;     // [rows][BINS]
+    uint64_t* hist;     // [rows][nparts][BINS]
     uint64_t* segs;     // [rows][nchunk * CHUNK / SEG]
-    int64_t nchunk;
+    uint64_t* edge;     // [rows][EDGE]
+    int64_t nchunk, nparts;
     Workspace from(int64_t r) const {
         Workspace w = *this;
         w.pending += r, w.chunks += r * nchunk, w.groups += r * nchunk * (CHUNK / GROUP);
-        w.hist += r * BINS, w.segs += r * nchunk * (CHUNK / SEG);
+        w.hist += r * nparts * BINS, w.segs += r * nchunk * (CHUNK / SEG), w.edge += r * EDGE;
         return w;
     }
 };
@@ -814,7 +822,7 @@ __global__ __launch_bounds__(NT) void sample_short(SampleArgs a, Workspace ws) {
     const float u = a.u[r];
     if (tid == 0) {
         sm.kmax = 0, sm.kfirst = 0xffffffffu;
-        if (ws.pending) ws.pending[r].step = DONE;
+        ws.pending[r].step = DONE;
     }
     float zmax = -INFINITY;
     uint32_t first = 0xffffffffu;
@@ -845,6 +853,10 @@ __global__ __launch_bounds__(NT) void sample_short(SampleArgs a, Workspace ws) {
         if (tid == 0) out.certain(int(sm.kfirst));
         return;
     }
+    if (s.p < 1.0f && s.k == 0 && s.least == 0.0) {  // its masses by bins settle it in the fewest passes
+        if (tid == 0) ws.pending[r] = to_finish(top);
+        return;
+    }
     auto mass = [&](float z, int) { return out.w.mass(z); };
     uint64_t total = 0;
     if (s.need_sum()) {
@@ -863,7 +875,7 @@ __global__ __launch_bounds__(NT) void sample_short(SampleArgs a, Workspace ws) {
     if (n >= 0)
         finish_list(n, s, u, total, sc, sm, out);
     else if (tid == 0)
-        ws.pending[r] = Pending{Cut(), top, TO_FINISH, {0, 0}, {0, 0}};
+        ws.pending[r] = to_finish(top);
 }
 
 template <typename T, int VEC>
@@ -996,23 +1008,9 @@ __global__ __launch_bounds__(NT) void sample_long(SampleArgs a, Workspace ws) {
         finish_list(n, s, u, total, sc, sm, out);
         return;
     }
-    if (!s.k && s.p < 1.0f)
-        for (int i = tid; i < BINS; i += NT) ws.hist[r * BINS + i] = 0;
     if (tid == 0)
-        ws.pending[r] = Pending{Cut(), top, s.k ? TO_FINISH : s.p < 1.0f ? TO_CUT : TO_DRAW, {0, 0}, {0, 0}};
+        ws.pending[r] = s.k ? to_finish(top) : Pending{0, top, s.p < 1.0f ? TO_CUT : TO_DRAW, BINS, {0, 0}, 0};
 }
-
-// The logits' masses that the filters keep.
-struct Kept {
-    Cut cut;
-    double least;
-    const Weigh& w;
-    __device__ uint64_t operator()(float z, int i) const {
-        if (!cut.keeps(z, i)) return 0;
-        const double x = w(z);
-        return x >= least ? Weigh::fixed(x) : 0;
-    }
-};
 
 // The exact cuts and the draw over a whole row.
 template <typename T>
@@ -1033,7 +1031,12 @@ __global__ __launch_bounds__(NT) void sample_row(SampleArgs a, Workspace ws) {
                 if (z[c] > -INFINITY) f(z[c], i + c);
         });
     };
-    const Kept kept{cuts(items, s, sc, 0, sm, sm.item, CAP, out.w), s.least, out.w};
+    const Cut cut = cuts(items, s, sc, 0, sm, sm.item, CAP, out.w);
+    auto kept = [&](float z, int i) -> uint64_t {
+        if (!cut.keeps(z, i)) return 0;
+        const double x = out.w(z);
+        return x >= s.least ? Weigh::fixed(x) : 0;
+    };
     row.sums(sm.item, kept);
     __syncthreads();
     const int ns = row.segments();
@@ -1093,53 +1096,93 @@ __global__ __launch_bounds__(NT) void sample_bins(SampleArgs a, Workspace ws) {
         }
     });
     __syncthreads();
-    uint64_t* hist = ws.hist + r * BINS;
+    uint64_t* hist = ws.hist + r * ws.nparts * BINS;
     for (int i = tid; i < BINS; i += NT)
-        if (sm.hist[i]) add(hist + i, sm.hist[i]);
+        __hip_atomic_store(hist + blockIdx.x * BINS + i, sm.hist[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     if (!last_of(&pd.arrived[0], sm)) return;
     uint64_t own = 0;
     for (int i = tid; i < BINS; i += NT) {
-        sm.hist[i] = load_shared(hist + i);
-        own += sm.hist[i];
+        uint64_t v = 0;
+#pragma unroll 4
+        for (int k = 0; k < int(ws.nparts); ++k) v += load_shared(hist + k * BINS + i);
+        sm.hist[i] = v;
+        own += v;
     }
-    const uint64_t total = block_sum(own, sm);
-    auto items = [&](auto&& f) {
-        row.turns([&](const float* z, int i) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-                if (z[c] > -INFINITY) f(z[c], i + c);
-        });
-    };
-    const Cut cut = cut_by_bins(items, sc, sm, sm.item, CAP, share_of(s.p, total), true, w);
-    if (tid == 0) pd.cut = cut, pd.step = TO_DRAW;
+    const uint64_t target = share_of(s.p, block_sum(own, sm));
+    pick<false>(sm.hist, BINS, target, sm);
+    if (tid == 0) pd.bin = int(sm.bin), pd.left = target - sm.before, pd.step = TO_DRAW;
 }
 
-// The kept masses of rows TO_DRAW by segments; the last workgroup of a row
-// draws.
+// The kept masses of rows TO_DRAW by segments, the logits of the bin that
+// top_p cuts set apart; the last workgroup of a row cuts and draws.
 template <typename T>
-__global__ __launch_bounds__(NT) void sample_draw(SampleArgs a, Workspace ws) {
+__global__ __launch_bounds__(NT, 8) void sample_draw(SampleArgs a, Workspace ws) {
     const int64_t r = blockIdx.y;
     Pending& pd = ws.pending[r];
     if (pd.step != TO_DRAW) return;
     __shared__ DrawShared sm;
-    const int tid = int(threadIdx.x);
+    const int tid = int(threadIdx.x), bin = pd.bin;
     const Settings s = settings_of(a, r);
     const Row<T> row(static_cast<const T*>(a.logits) + r * a.ld, a.vocab);
     const Result out(a, r, pd.max, s);
-    const Kept kept{pd.cut, s.least, out.w};
+    const Scale sc(pd.max, s.t);
     const int first = int(blockIdx.x) * PART, ns = row.segments();
     uint64_t* segs = ws.segs + r * ws.nchunk * (CHUNK / SEG);
+    uint64_t* edge = ws.edge + r * EDGE;
     const Row<T> part = part_of(row);
-    part.sums(sm.item, [&](float z, int i) { return kept(z, first + i); });
+    // (a logit in a bin before stays, if min_p lets it)
+    auto before = [&](float z, int) -> uint64_t {
+        if (sc.bin(z) >= bin) return 0;
+        const double x = out.w(z);
+        return x >= s.least ? Weigh::fixed(x) : 0;
+    };
+    part.sums(sm.item, [&](float z, int i) {
+        if (sc.bin(z) == bin && z > -INFINITY) {
+            const uint32_t at = atomicAdd(&pd.edges, 1u);
+            if (at < EDGE) __hip_atomic_store(edge + at, item_of(z, first + i), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        return before(z, i);
+    });
     __syncthreads();
     if (tid < part.segments())
         __hip_atomic_store(segs + first / SEG + tid, sm.item[tid], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     if (!last_of(&pd.arrived[1], sm)) return;
-    uint64_t own = 0;
-    for (int i = tid; i < ns; i += NT) {
-        sm.item[i] = load_shared(segs + i);
-        own += sm.item[i];
+    if (tid == 0) sm.kfirst = __hip_atomic_load(&pd.edges, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    for (int i = tid; i < ns; i += NT) sm.item[i] = load_shared(segs + i);
+    __syncthreads();
+    const int n = int(sm.kfirst);
+    Cut cut;
+    if (n > 0 && n <= EDGE) {
+        for (int i = tid; i < n; i += NT) sm.edge[i] = load_shared(edge + i);
+        cut = cut_in_bin(sm.edge, n, sm, pd.left, true, out.w);
+    } else if (n > EDGE) {
+        auto items = [&](auto&& f) {
+            row.turns([&](const float* z, int i) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    if (z[c] > -INFINITY && sc.bin(z[c]) == bin) f(z[c], i + c);
+            });
+        };
+        cut = Cut::at(find_cut(items, sm, pd.left, true, out.w));
     }
+    // (an edge that is no item may lie below the bin: both conditions hold)
+    auto kept = [&](float z, int i) -> uint64_t {
+        if (sc.bin(z) > bin || !cut.keeps(z, i)) return 0;
+        const double x = out.w(z);
+        return x >= s.least ? Weigh::fixed(x) : 0;
+    };
+    if (n <= EDGE) {
+        for (int i = tid; i < n; i += NT) {
+            const uint64_t m = kept(item_value(sm.edge[i]), item_index(sm.edge[i]));
+            if (m) add(&sm.item[item_index(sm.edge[i]) / SEG], m);
+        }
+    } else {
+        __syncthreads();
+        row.sums(sm.item, kept);
+    }
+    __syncthreads();
+    uint64_t own = 0;
+    for (int i = tid; i < ns; i += NT) own += sm.item[i];
     const uint64_t total = block_sum(own, sm), target = goal(a.u[r], total);
     pick<false>(sm.item, ns, target, sm);
     draw_in(row, int(sm.bin) * SEG, target - sm.before, total, out, kept);
@@ -1166,21 +1209,25 @@ SampleArgs rows_from(SampleArgs a, int64_t r) {
 
 int64_t chunks_of(int64_t vocab) { return vocab <= SHORT ? 0 : (vocab + CHUNK - 1) / CHUNK; }
 
+int64_t parts_of(int64_t vocab) { return (vocab + PART - 1) / PART; }
+
 template <typename T>
 void launch(hipStream_t s, const SampleArgs& a, void* workspace) {
     const dim3 grid{unsigned(a.rows)}, block{NT};
     Workspace ws{};
     ws.nchunk = chunks_of(a.vocab);
     const int64_t n = a.rows * ws.nchunk;
-    if (a.vocab > CAP) ws.pending = static_cast<Pending*>(workspace);  // (others always fit the list)
+    ws.pending = static_cast<Pending*>(workspace);
     ws.chunks = reinterpret_cast<Chunk*>(ws.pending + a.rows);
     ws.groups = reinterpret_cast<float*>(ws.chunks + n);
+    ws.nparts = parts_of(a.vocab);
     ws.hist = reinterpret_cast<uint64_t*>(ws.groups + n * (CHUNK / GROUP));
-    ws.segs = ws.hist + a.rows * BINS;
+    ws.segs = ws.hist + a.rows * ws.nparts * BINS;
+    ws.edge = ws.segs + n * (CHUNK / SEG);
     if (a.vocab <= SHORT) {
         sample_short<T><<<grid, block, 0, s>>>(a, ws);
         OMG_HIP(hipGetLastError());
-        if (a.vocab > CAP && (a.top_k || a.top_p || a.min_p)) {
+        if (a.top_p || (a.vocab > CAP && (a.top_k || a.min_p))) {
             sample_row<T><<<grid, block, 0, s>>>(a, ws);
             OMG_HIP(hipGetLastError());
         }
@@ -1201,7 +1248,7 @@ void launch(hipStream_t s, const SampleArgs& a, void* workspace) {
     }
     if (!a.top_p && !a.min_p) return;
     for (int64_t r = 0; r < a.rows; r += 65535) {  // (a grid's second size)
-        const dim3 parts{unsigned((a.vocab + PART - 1) / PART), unsigned(std::min<int64_t>(65535, a.rows - r))};
+        const dim3 parts{unsigned(ws.nparts), unsigned(std::min<int64_t>(65535, a.rows - r))};
         if (a.top_p) sample_bins<T><<<parts, block, 0, s>>>(rows_from<T>(a, r), ws.from(r));
         OMG_HIP(hipGetLastError());
         sample_draw<T><<<parts, block, 0, s>>>(rows_from<T>(a, r), ws.from(r));
@@ -1216,10 +1263,11 @@ int64_t sample_workspace(int64_t rows, int64_t vocab) {
     a.rows = rows, a.vocab = vocab;
     check(a);
     static_assert(sizeof(Pending) % 16 == 0 && sizeof(Chunk) % 16 == 0, "the workspace's arrays are aligned");
-    if (vocab <= CAP) return 0;
     const int64_t n = chunks_of(vocab);
-    return rows * (int64_t(sizeof(Pending)) + n * int64_t(sizeof(Chunk) + CHUNK / SEG * 8 + CHUNK / GROUP * 4) +
-                   (n ? BINS * 8 : 0));
+    return rows * int64_t(sizeof(Pending)) +
+           (n ? rows * (n * int64_t(sizeof(Chunk) + CHUNK / SEG * 8 + CHUNK / GROUP * 4) + parts_of(vocab) * BINS * 8 +
+                        EDGE * 8)
+              : 0);
 }
 
 void launch_sample(hipStream_t s, const SampleArgs& a, void* workspace, size_t bytes) {
