@@ -92,15 +92,6 @@ __device__ inline floatx4 mfma16k16(bf16x4 a, bf16x4 b, floatx4 c) {
                                                      0, 0, 0);
 }
 
-// V rows r .. r + 3 of this lane's 16-lane group, one column a lane: lane i
-// of the group gives the address of row i / 4, columns 4 (i % 4) .. + 3 and
-// gets column i of the four rows.
-template <typename T>
-__device__ inline short4v read_tr(const T* p) {
-    typedef __attribute__((address_space(3))) short4v* ptr;
-    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(p));
-}
-
 template <typename T, int D, int TILE>
 struct Core {
     static constexpr int RW = TILE == WAVES_32 ? 32 : 16;      // rows of a wave
@@ -119,10 +110,6 @@ struct Core {
 
     static __device__ int swz_k(int row) { return CH >= 16 ? row & 15 : row & 7; }
     static __device__ int swz_v(int row) { return CH >= 16 ? (row & 7) << 1 : (row & 3) << 1; }
-    // The tile's key of score r of block j.
-    static __device__ int key_of(int lane, int j, int r) {
-        return RW == 32 ? 8 * (r / 4) + 4 * (lane / 32) + r % 4 : 16 * j + 4 * (lane / 16) + r;
-    }
     static __device__ float row_max(float v) {
         if constexpr (RW == 32) {
             const uint32_t u = __builtin_bit_cast(uint32_t, v);
@@ -156,33 +143,64 @@ struct Core {
         l = 0.0f;
     }
 
-    // One tile whose first key is k0; the lane's query sees the keys lo ..
-    // hi - 1 that are not in `bad` (a bit per key of the tile).
-    __device__ void tile(const T* K, const T* V, int lane, int k0, bool full, int lo, int hi, uint32_t bad, float c) {
+    // The lane's addresses in a tile, in bytes: of its K operands' first chunk
+    // (the chunk of step st XORed in: its bits are apart from the row's) and
+    // of its V reads.  They are hidden from the compiler in each tile, which
+    // would keep all their XORs in registers otherwise: 24 of 256, and no
+    // room left to read operands ahead.
+    static __device__ uint32_t k_base(int lane) {
+        const int row = lane % RW;
+        return uint32_t(row * D * 2 + ((lane / RW) ^ swz_k(row)) * 16);
+    }
+    static __device__ uint32_t v_base(int lane) {
+        const int i16 = lane % 16, g16 = lane / 16;
+        const int row = (RW == 32 ? 4 * (g16 / 2) : 4 * g16) + i16 / 4;
+        const int ch = (RW == 32 ? 2 * (g16 % 2) : 0) + (i16 % 4) / 2;
+        return uint32_t(row * D * 2 + (ch ^ swz_v(row)) * 16 + (i16 % 2) * 8);
+    }
+    // V rows r .. r + 3 of the lane's 16-lane group, one column a lane: lane i
+    // of the group gives the address of row i / 4, columns 4 (i % 4) .. + 3
+    // and gets column i of the four rows.
+    static __device__ short4v read_tr(uint32_t at, int offset) {
+        typedef __attribute__((address_space(3))) short4v* ptr;
+        return __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(uintptr_t)(at + offset));
+    }
+    static __device__ frag read_k(uint32_t at, int offset) {
+        typedef __attribute__((address_space(3))) frag* ptr;
+        return *(ptr)(uintptr_t)(at + offset);
+    }
+
+    // One tile at LDS address `at` (K, then V) whose first key is k0; the
+    // lane's query sees the keys lo .. hi - 1 that are not in `bad` (a bit
+    // per key of the tile).
+    __device__ void tile(uint32_t at, int lane, int k0, bool full, int lo, int hi, uint32_t bad, float c) {
         acc s[NB];
 #pragma unroll
         for (int j = 0; j < NB; ++j)
 #pragma unroll
             for (int r = 0; r < SR; ++r) s[j][r] = 0.0f;
-        const int kr = lane % RW;
+        uint32_t ka = at + k_base(lane), va = at + KT * D * 2 + v_base(lane);
+        asm volatile("" : "+v"(ka), "+v"(va));
 #pragma unroll
         for (int st = 0; st < NS; ++st)
 #pragma unroll
             for (int j = 0; j < NB; ++j) {
-                const int row = j * RW + kr, ch = (st * (KS / 8) + lane / RW) ^ swz_k(row);
-                const frag kf = *reinterpret_cast<const frag*>(K + row * D + ch * 8);
+                const frag kf = read_k(ka ^ uint32_t(st * (KS / 8) * 16), j * RW * D * 2);
                 if constexpr (RW == 32)
                     s[j] = mfma32(kf, q[st], s[j]);
                 else
                     s[j] = mfma16(kf, q[st], s[j]);
             }
         if (!full) {
+            // (the lane's keys: a constant of (j, r) past k0 + 4 * its group)
+            const int first = k0 + 4 * (lane / RW), from = lo - first, to = hi - first;
+            const uint32_t out = bad >> (4 * (lane / RW));
 #pragma unroll
             for (int j = 0; j < NB; ++j)
 #pragma unroll
                 for (int r = 0; r < SR; ++r) {
-                    const int kk = key_of(lane, j, r), key = k0 + kk;
-                    const bool see = key >= lo && key < hi && !(bad >> kk & 1u);
+                    const int kk = RW == 32 ? 8 * (r / 4) + r % 4 : 16 * j + r;
+                    const bool see = kk >= from && kk < to && !(out & (1u << kk));
                     s[j][r] = see ? s[j][r] : -INFINITY;
                 }
         }
@@ -215,41 +233,38 @@ struct Core {
                 sum += p;
             }
         l += sum;
-        const int i16 = lane % 16, g16 = lane / 16;
+        union V8 {
+            short4v h[2];
+            frag f;
+        };
         if constexpr (RW == 32) {
             // (two 16-key steps; the lane's keys of step j: 16 j + 4 h + 0 .. 3 and + 8)
+            frag pf[2];
 #pragma unroll
-            for (int j = 0; j < KT / 16; ++j) {
-                frag pf;
+            for (int j = 0; j < 2; ++j)
 #pragma unroll
-                for (int r = 0; r < 8; ++r) pf[r] = T(s[0][8 * j + r]);
-                const int r0 = 16 * j + 4 * (g16 / 2) + i16 / 4;
+                for (int r = 0; r < 8; ++r) pf[j][r] = T(s[0][8 * j + r]);
 #pragma unroll
-                for (int i = 0; i < NC; ++i) {
-                    const int ch = 4 * i + 2 * (g16 % 2) + (i16 % 4) / 2, e = 4 * (i16 % 2);
-                    union {
-                        short4v h[2];
-                        frag f;
-                    } v;
-                    v.h[0] = read_tr(V + r0 * D + (ch ^ swz_v(r0)) * 8 + e);
-                    v.h[1] = read_tr(V + (r0 + 8) * D + (ch ^ swz_v(r0 + 8)) * 8 + e);
-                    o[i] = mfma32(v.f, pf, o[i]);
+            for (int i = 0; i < NC; ++i) {
+                const uint32_t a = va ^ uint32_t(i * 64);
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    V8 v;
+                    v.h[0] = read_tr(a, (16 * j) * D * 2);
+                    v.h[1] = read_tr(a, (16 * j + 8) * D * 2);
+                    o[i] = mfma32(v.f, pf[j], o[i]);
                 }
             }
         } else if constexpr (KT == 32) {
             frag pf;
 #pragma unroll
             for (int r = 0; r < 8; ++r) pf[r] = T(s[r / 4][r % 4]);
-            const int r0 = 4 * g16 + i16 / 4;
 #pragma unroll
             for (int i = 0; i < NC; ++i) {
-                const int ch = 2 * i + (i16 % 4) / 2, e = 4 * (i16 % 2);
-                union {
-                    short4v h[2];
-                    frag f;
-                } v;
-                v.h[0] = read_tr(V + r0 * D + (ch ^ swz_v(r0)) * 8 + e);
-                v.h[1] = read_tr(V + (r0 + 16) * D + (ch ^ swz_v(r0 + 16)) * 8 + e);
+                const uint32_t a = va ^ uint32_t(i * 32);
+                V8 v;
+                v.h[0] = read_tr(a, 0);
+                v.h[1] = read_tr(a, 16 * D * 2);
                 o[i] = mfma16(v.f, pf, o[i]);
             }
         } else {
@@ -257,13 +272,9 @@ struct Core {
             frag4 pf;
 #pragma unroll
             for (int r = 0; r < 4; ++r) pf[r] = T(s[0][r]);
-            const int r0 = 4 * g16 + i16 / 4;
 #pragma unroll
-            for (int i = 0; i < NC; ++i) {
-                const int ch = 2 * i + (i16 % 4) / 2, e = 4 * (i16 % 2);
-                const short4v v = read_tr(V + r0 * D + (ch ^ swz_v(r0)) * 8 + e);
-                o[i] = mfma16k16(__builtin_bit_cast(frag4, v), pf, o[i]);
-            }
+            for (int i = 0; i < NC; ++i)
+                o[i] = mfma16k16(__builtin_bit_cast(frag4, read_tr(va ^ uint32_t(i * 32), 0)), pf, o[i]);
         }
     }
     // The lane's four consecutive head dims of output quad (i, rr).
@@ -315,12 +326,17 @@ struct Stream {
     static constexpr int INS = TILE_ELEMS * 2 / 1024 / (KEYS ? 1 : NW);  // 1 KiB loads per wave for K, and for V
     static_assert(INS >= 1, "a wave loads at least 1 KiB of a tile");
 
+    static constexpr int NBUF = KEYS || D == 512 ? 1 : 2;  // (2 workgroups a CU either way)
+
     const Args& a;
     int g, wave, lane;
-    T* smem;  // KEYS: [wave][K, V], else [2 buffers][K, V]
+    T* smem;  // KEYS: [wave][K, V], else [NBUF][K, V]
 
-    __device__ T* buf(int which) const { return smem + int64_t(KEYS ? wave : which) * 2 * TILE_ELEMS; }
+    __device__ T* buf(int which) const { return smem + (KEYS ? wave : NBUF > 1 ? which : 0) * 2 * TILE_ELEMS; }
 
+    // One 1 KiB piece holds RPI rows; the lane's byte offsets in the first
+    // piece, from which the others' follow (their rows' bits are apart).
+    static constexpr int RPI = 512 / D;
     __device__ void issue(int k0, int klim, T* dst, int p0, int p1) const {
         // A wave's rows lie in one 16-row half of the tile, so in one page.
         const int hf = !KEYS && wave >= NW / 2 ? 1 : 0;
@@ -328,21 +344,27 @@ struct Stream {
         const bool ok = unsigned(p) < unsigned(a.kv.npages);
         int rows = klim - kk;
         rows = rows < 0 ? 0 : rows > 16 ? 16 : rows;
-        const int bytes = ok ? rows * D * 2 : 0;
-        const int64_t off = (ok ? p : 0) * a.kv.page_stride + (int64_t(g) * a.kv.page + (kk & (a.kv.page - 1))) * D;
-        const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(
-            const_cast<T*>(static_cast<const T*>(a.kv.k) + off), (short)0, bytes, 0x00020000);
-        const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(
-            const_cast<T*>(static_cast<const T*>(a.kv.v) + off), (short)0, bytes, 0x00020000);
+        const int bytes = uni(ok ? rows * D * 2 : 0);
+        const int64_t off = 2 * ((ok ? p : 0) * a.kv.page_stride + (int64_t(g) * a.kv.page + (kk & (a.kv.page - 1))) * D);
+        const __amdgpu_buffer_rsrc_t rk = rsrc(a.kv.k, off, bytes), rv = rsrc(a.kv.v, off, bytes);
+        const int row = (KEYS ? 0 : wave * INS * RPI) + lane / C::CH, pc = lane % C::CH;
+        uint32_t ko = uint32_t((row & 15) * D * 2 + (pc ^ C::swz_k(row)) * 16);
+        uint32_t vo = uint32_t((row & 15) * D * 2 + (pc ^ C::swz_v(row)) * 16);
+        asm volatile("" : "+v"(ko), "+v"(vo));
+        T* to = dst + (KEYS ? 0 : wave * INS) * 512;
 #pragma unroll
         for (int i = 0; i < INS; ++i) {
-            const int piece = (KEYS ? 0 : wave * INS) + i;
-            const int slot = piece * WAVE + lane, row = slot / C::CH, pc = slot % C::CH;
-            const uint32_t ko = uint32_t(((row & 15) * D + (pc ^ C::swz_k(row)) * 8) * 2);
-            const uint32_t vo = uint32_t(((row & 15) * D + (pc ^ C::swz_v(row)) * 8) * 2);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds_ptr)(dst + piece * 512), 16, ko, 0, 0, 0);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds_ptr)(dst + TILE_ELEMS + piece * 512), 16, vo, 0, 0, 0);
+            const int r = i * RPI;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds_ptr)(to + i * 512), 16, ko ^ uint32_t(C::swz_k(r) * 16),
+                                                     r * D * 2, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds_ptr)(to + TILE_ELEMS + i * 512), 16,
+                                                     vo ^ uint32_t(C::swz_v(r) * 16), r * D * 2, 0, 0);
         }
+    }
+    static __device__ __amdgpu_buffer_rsrc_t rsrc(const void* base, int64_t off, int bytes) {
+        const uint64_t p = reinterpret_cast<uint64_t>(base) + uint64_t(off);
+        const uint64_t u = uint64_t(uint32_t(uni(int(uint32_t(p >> 32))))) << 32 | uint32_t(uni(int(uint32_t(p))));
+        return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(u), (short)0, bytes, 0x00020000);
     }
 
     // Keys kb .. ke - 1 (kb a multiple of 32; rows from klim on do not
@@ -362,11 +384,13 @@ struct Stream {
         int pn = fetch(k0);
         if constexpr (!KEYS) __syncthreads();  // the buffers may still be read for the segment before
         int p0 = __builtin_amdgcn_readlane(pn, 0), p1 = __builtin_amdgcn_readlane(pn, 1);
-        if constexpr (!KEYS) issue(k0, klim, buf(0), p0, p1);
+        if constexpr (NBUF > 1) {
+            issue(k0, klim, buf(0), p0, p1);
+            if (k0 + step < ke) pn = fetch(k0 + step);
+        }
         int which = 0;
-        if (!KEYS && k0 + step < ke) pn = fetch(k0 + step);
         for (; k0 < ke; k0 += step, which ^= 1) {
-            if constexpr (KEYS) {
+            if constexpr (NBUF == 1) {
                 issue(k0, klim, buf(0), p0, p1);
                 if (k0 + step < ke) pn = fetch(k0 + step);
             }
@@ -375,16 +399,18 @@ struct Stream {
             uint32_t bad = unsigned(p0) < unsigned(a.kv.npages) ? 0u : 0xffffu;
             if (KT == 32 && unsigned(p1) >= unsigned(a.kv.npages)) bad |= 0xffff0000u;
             p0 = __builtin_amdgcn_readlane(pn, 0), p1 = __builtin_amdgcn_readlane(pn, 1);
-            if (!KEYS && k0 + step < ke) {
+            if (NBUF > 1 && k0 + step < ke) {
                 issue(k0 + step, klim, buf(which ^ 1), p0, p1);
                 if (k0 + 2 * step < ke) pn = fetch(k0 + 2 * step);
             }
             if (__ballot(valid && lo < k0 + KT && hi > k0)) {
                 const bool full = bad == 0 && __all(!valid || (lo <= k0 && hi >= k0 + KT));
-                const T* K = buf(which);
-                core.tile(K, K + TILE_ELEMS, lane, k0, full, lo, hi, bad, a.c);
+                core.tile(uint32_t(uintptr_t((lds_ptr)buf(which))), lane, k0, full, lo, hi, bad, a.c);
             }
-            if constexpr (KEYS) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            if constexpr (NBUF == 1) {
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                if constexpr (!KEYS) __syncthreads();
+            }
         }
     }
 };
@@ -458,12 +484,12 @@ __device__ inline void emit_keys(const Args& a, Core<T, D, WAVES_KEYS>& core, co
 }
 
 template <typename T, int D, int TILE>
-__global__ __launch_bounds__(NW * 64, D == 512 ? 1 : 2) void attention_shared_kernel(Args a) {
-    extern __shared__ __attribute__((aligned(16))) unsigned char smem_raw[];
+__global__ __launch_bounds__(NW * 64, TILE == WAVES_KEYS && D == 512 ? 1 : 2) void attention_shared_kernel(Args a) {
+    extern __shared__ __attribute__((aligned(1024))) unsigned char smem_raw[];  // (whole rows: addresses are XORed)
     T* smem = reinterpret_cast<T*>(smem_raw);
     const int tid = int(threadIdx.x), lane = tid % WAVE;
     const int wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
-    const int G = a.kv.kv_heads, H = a.x.heads, hpg = a.hpg, P = int(a.b.prefix_len), w = a.x.window;
+    const int G = a.kv.kv_heads, hpg = a.hpg, P = int(a.b.prefix_len), w = a.x.window;
     const int cap = int(a.max_len);
 
     // The sequence of token `tok`, known to lie in [s0, s1].
@@ -521,12 +547,13 @@ __global__ __launch_bounds__(NW * 64, D == 512 ? 1 : 2) void attention_shared_ke
             const int lo = w > 0 ? imax(0, P + r.own - w + 1) : 0;
             if (w > 0) {
                 // the first key that any of the workgroup's rows sees
-                __shared__ int first;
+                int& first = *reinterpret_cast<int*>(smem_raw);  // (no tile has arrived yet)
                 if (tid == 0) first = INT_MAX;
                 __syncthreads();
                 if (r.valid) atomicMin(&first, lo);
                 __syncthreads();
                 kb = imax(kb, first == INT_MAX ? ke : first / 32 * 32);
+                __syncthreads();
             }
             if (kb < ke) st.run(core, a.b.prefix_table, (P - 1) >> a.page_shift, kb, ke, P, r.valid, lo, P);
         }
@@ -630,7 +657,6 @@ __global__ __launch_bounds__(256) void attention_join_kernel(Args a) {
             l += wl * ml.y;
         }
         const int n = slots - i0 < WAVE ? slots - i0 : WAVE;
-#pragma unroll 4
         for (int i = 0; i < n; ++i) {
             const float f = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wl), i));
             if (f == 0.0f) continue;  // (its O was not written)
@@ -701,7 +727,8 @@ template <typename T, int D>
 void launch_d(hipStream_t s, const Args& a, unsigned blocks) {
     // tiles: 2 buffers x 32 keys, or 4 waves x 16 keys, of K and V; the
     // waves' join: 4 x 16 rows of f32 and their statistics
-    constexpr unsigned lds = 4 * 32 * D * 2 + 2 * NW * 16 * 4;
+    constexpr unsigned lds_rows = 4 * 32 * D * 2 / (D == 512 ? 2 : 1), lds_keys = NW * 16 * D * 4 + 2 * NW * 16 * 4;
+    const unsigned lds = a.p.fused ? lds_rows : lds_keys > lds_rows ? lds_keys : lds_rows;
     auto go = [&](auto kernel) {
         OMG_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
                                     int(lds)));
