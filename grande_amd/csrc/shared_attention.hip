@@ -191,6 +191,12 @@ struct Core {
                 else
                     s[j] = mfma16(kf, q[st], s[j]);
             }
+        pipeline<NS * NB, 1, 1>();
+        // The first V operands go out ahead of the softmax, which hides them.
+        frag vf[VA];
+#pragma unroll
+        for (int i = 0; i < VA; ++i) vf[i] = read_v(va, i);
+        __builtin_amdgcn_sched_barrier(0);
         if (!full) {
             // (the lane's keys: a constant of (j, r) past k0 + 4 * its group)
             const int first = k0 + 4 * (lane / RW), from = lo - first, to = hi - first;
@@ -233,48 +239,62 @@ struct Core {
                 sum += p;
             }
         l += sum;
-        union V8 {
+        // P^T operands: the lane's scores of each MFMA step over the keys.
+        frag pf[VS];
+#pragma unroll
+        for (int j = 0; j < VS; ++j)
+#pragma unroll
+            for (int r = 0; r < (KT == 16 ? 4 : 8); ++r)
+                pf[j][r] = T(RW == 32 ? s[0][8 * j + r] : s[r / 4][r % 4]);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < NC * VS; ++i) {
+            const frag v = vf[i % VA];
+            if (i + VA < NC * VS) vf[i % VA] = read_v(va, i + VA);
+            if constexpr (RW == 32) {
+                o[i / VS] = mfma32(v, pf[i % VS], o[i / VS]);
+            } else if constexpr (KT == 32) {
+                o[i] = mfma16(v, pf[0], o[i]);
+            } else {
+                typedef T frag4 __attribute__((ext_vector_type(4)));
+                const frag4 a = {v[0], v[1], v[2], v[3]}, b = {pf[0][0], pf[0][1], pf[0][2], pf[0][3]};
+                o[i] = mfma16k16(a, b, o[i]);
+            }
+        }
+        pipeline<NC * VS, KT == 16 ? 1 : 2, 0>();
+    }
+    // V^T operand i: head dims i / VS, keys of step i % VS.
+    static constexpr int VS = RW == 32 ? 2 : 1;      // MFMA steps over the keys
+    static constexpr int VA = 4;                     // operands read ahead
+    static __device__ frag read_v(uint32_t va, int i) {
+        union {
             short4v h[2];
             frag f;
-        };
+        } v;
         if constexpr (RW == 32) {
-            // (two 16-key steps; the lane's keys of step j: 16 j + 4 h + 0 .. 3 and + 8)
-            frag pf[2];
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-                for (int r = 0; r < 8; ++r) pf[j][r] = T(s[0][8 * j + r]);
-#pragma unroll
-            for (int i = 0; i < NC; ++i) {
-                const uint32_t a = va ^ uint32_t(i * 64);
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    V8 v;
-                    v.h[0] = read_tr(a, (16 * j) * D * 2);
-                    v.h[1] = read_tr(a, (16 * j + 8) * D * 2);
-                    o[i] = mfma32(v.f, pf[j], o[i]);
-                }
-            }
-        } else if constexpr (KT == 32) {
-            frag pf;
-#pragma unroll
-            for (int r = 0; r < 8; ++r) pf[r] = T(s[r / 4][r % 4]);
-#pragma unroll
-            for (int i = 0; i < NC; ++i) {
-                const uint32_t a = va ^ uint32_t(i * 32);
-                V8 v;
-                v.h[0] = read_tr(a, 0);
-                v.h[1] = read_tr(a, 16 * D * 2);
-                o[i] = mfma16(v.f, pf, o[i]);
-            }
+            const uint32_t a = va ^ uint32_t(i / 2 * 64);
+            v.h[0] = read_tr(a, 16 * (i % 2) * D * 2);
+            v.h[1] = read_tr(a, (16 * (i % 2) + 8) * D * 2);
         } else {
-            typedef T frag4 __attribute__((ext_vector_type(4)));
-            frag4 pf;
+            const uint32_t a = va ^ uint32_t(i * 32);
+            v.h[0] = read_tr(a, 0);
+            if constexpr (KT == 32)
+                v.h[1] = read_tr(a, 16 * D * 2);
+            else
+                v.h[1] = v.h[0];
+        }
+        return v.f;
+    }
+    // The order of a run of N MFMAs, each on an operand of READS LDS reads:
+    // VA operands' reads go first where FIRST, then one operand's after each
+    // MFMA.  (Left alone, the compiler reads one operand and waits for it.)
+    template <int N, int READS, int FIRST>
+    static __device__ void pipeline() {
+        if constexpr (FIRST) __builtin_amdgcn_sched_group_barrier(0x100, VA * READS, 0);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) pf[r] = T(s[0][r]);
-#pragma unroll
-            for (int i = 0; i < NC; ++i)
-                o[i] = mfma16k16(__builtin_bit_cast(frag4, read_tr(va ^ uint32_t(i * 32), 0)), pf, o[i]);
+        for (int i = 0; i < N; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+            if (i + VA < N) __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
         }
     }
     // The lane's four consecutive head dims of output quad (i, rr).
