@@ -15,11 +15,13 @@
 // Few tiles split the keys over work items; attention_join joins these.
 //
 // Tiles (MFMA shape = rows of a wave x keys):
-//   WAVES_ROWS 32: 4 waves x 32 rows, 32-key K and V tiles shared in LDS,
-//                  two buffers, the next tile's loads in flight;
-//   WAVES_ROWS 16: 4 waves x 16 rows, the same (head_dim 512, few rows);
-//   WAVES_KEYS:    16 rows, each wave takes every fourth 16-key tile into
-//                  LDS of its own; the waves join through LDS at the end.
+//   WAVES_32:   4 waves x 32 rows, 32-key K and V tiles shared in LDS, two
+//               buffers, the next tile's loads in flight (four buffers, and
+//               with them one workgroup a CU: 62 us where two take 42);
+//   WAVES_16:   4 waves x 16 rows, the same (few rows; head_dim 512, whose
+//               tiles are 16 keys long);
+//   WAVES_KEYS: 16 rows, each wave takes every fourth 16-key tile into LDS
+//               of its own; the waves join through LDS at the end.
 // Both products leave the query in the lane: S^T = K Q^T with the lane's
 // query as column, then O^T += V^T P^T, whose P^T operand is the lane's own
 // scores; V^T comes from row-major V by LDS transposing reads of 4 keys.
@@ -94,8 +96,8 @@ __device__ inline floatx4 mfma16k16(bf16x4 a, bf16x4 b, floatx4 c) {
 
 template <typename T, int D, int TILE>
 struct Core {
-    static constexpr int RW = TILE == WAVES_32 ? 32 : 16;      // rows of a wave
-    static constexpr int KT = TILE == WAVES_KEYS ? 16 : 32;    // keys of a tile
+    static constexpr int RW = TILE == WAVES_32 ? 32 : 16;                    // rows of a wave
+    static constexpr int KT = TILE == WAVES_KEYS || D == 512 ? 16 : 32;      // keys of a tile
     static constexpr int KS = RW == 32 ? 16 : 32;              // head dims per MFMA of K Q^T
     static constexpr int NS = D / KS, NC = D / RW;
     static constexpr int NB = KT / RW < 1 ? 1 : KT / RW;       // score blocks
@@ -333,6 +335,10 @@ struct Sink {
 
 // A value that is the same in every lane, in a scalar register.
 __device__ inline int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ inline uint64_t uni_ptr(const void* p) {
+    const uint64_t v = reinterpret_cast<uint64_t>(p);
+    return uint64_t(uint32_t(uni(int(uint32_t(v >> 32))))) << 32 | uint32_t(uni(int(uint32_t(v))));
+}
 
 constexpr int NW = 4;
 
@@ -346,20 +352,20 @@ struct Stream {
     static constexpr int INS = TILE_ELEMS * 2 / 1024 / (KEYS ? 1 : NW);  // 1 KiB loads per wave for K, and for V
     static_assert(INS >= 1, "a wave loads at least 1 KiB of a tile");
 
-    static constexpr int NBUF = KEYS || D == 512 ? 1 : 2;  // (2 workgroups a CU either way)
+    static constexpr int NBUF = KEYS ? 1 : 2;
 
     const Args& a;
     int g, wave, lane;
     T* smem;  // KEYS: [wave][K, V], else [NBUF][K, V]
 
-    __device__ T* buf(int which) const { return smem + (KEYS ? wave : NBUF > 1 ? which : 0) * 2 * TILE_ELEMS; }
+    __device__ T* buf(int which) const { return smem + (KEYS ? wave : which) * 2 * TILE_ELEMS; }
 
     // One 1 KiB piece holds RPI rows; the lane's byte offsets in the first
     // piece, from which the others' follow (their rows' bits are apart).
     static constexpr int RPI = 512 / D;
     __device__ void issue(int k0, int klim, T* dst, int p0, int p1) const {
         // A wave's rows lie in one 16-row half of the tile, so in one page.
-        const int hf = !KEYS && wave >= NW / 2 ? 1 : 0;
+        const int hf = !KEYS && KT == 32 && wave >= NW / 2 ? 1 : 0;
         const int p = hf ? p1 : p0, kk = k0 + 16 * hf;
         const bool ok = unsigned(p) < unsigned(a.kv.npages);
         int rows = klim - kk;
@@ -382,9 +388,8 @@ struct Stream {
         }
     }
     static __device__ __amdgpu_buffer_rsrc_t rsrc(const void* base, int64_t off, int bytes) {
-        const uint64_t p = reinterpret_cast<uint64_t>(base) + uint64_t(off);
-        const uint64_t u = uint64_t(uint32_t(uni(int(uint32_t(p >> 32))))) << 32 | uint32_t(uni(int(uint32_t(p))));
-        return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(u), (short)0, bytes, 0x00020000);
+        return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(uni_ptr(static_cast<const char*>(base) + off)),
+                                                 (short)0, bytes, 0x00020000);
     }
 
     // Keys kb .. ke - 1 (kb a multiple of 32; rows from klim on do not
@@ -396,42 +401,53 @@ struct Stream {
         const int step = KEYS ? NW * KT : KT;
         int k0 = kb + (KEYS ? wave * KT : 0);
         const int shift = a.page_shift;
-        auto fetch = [&](int k) {
-            int i = (k + 16 * (lane & 1)) >> shift;
+        auto fetch = [&](int k) {  // lane 0: the page of key k, lane 1: of key k + 16
+            const int i = (k + 16 * (lane & 1)) >> shift;
             return table[i > plast ? plast : i];
         };
         if (k0 >= ke) return;  // (no barrier below where waves differ in k0)
-        int pn = fetch(k0);
-        if constexpr (!KEYS) __syncthreads();  // the buffers may still be read for the segment before
-        int p0 = __builtin_amdgcn_readlane(pn, 0), p1 = __builtin_amdgcn_readlane(pn, 1);
-        if constexpr (NBUF > 1) {
-            issue(k0, klim, buf(0), p0, p1);
-            if (k0 + step < ke) pn = fetch(k0 + step);
-        }
-        int which = 0;
-        for (; k0 < ke; k0 += step, which ^= 1) {
-            if constexpr (NBUF == 1) {
-                issue(k0, klim, buf(0), p0, p1);
+        if constexpr (KEYS) {
+            for (int pn = fetch(k0); k0 < ke; k0 += step) {
+                const int p = __builtin_amdgcn_readlane(pn, 0);
                 if (k0 + step < ke) pn = fetch(k0 + step);
-            }
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-            if constexpr (!KEYS) __syncthreads();
-            uint32_t bad = unsigned(p0) < unsigned(a.kv.npages) ? 0u : 0xffffu;
-            if (KT == 32 && unsigned(p1) >= unsigned(a.kv.npages)) bad |= 0xffff0000u;
-            p0 = __builtin_amdgcn_readlane(pn, 0), p1 = __builtin_amdgcn_readlane(pn, 1);
-            if (NBUF > 1 && k0 + step < ke) {
-                issue(k0 + step, klim, buf(which ^ 1), p0, p1);
-                if (k0 + 2 * step < ke) pn = fetch(k0 + 2 * step);
-            }
-            if (__ballot(valid && lo < k0 + KT && hi > k0)) {
-                const bool full = bad == 0 && __all(!valid || (lo <= k0 && hi >= k0 + KT));
-                core.tile(uint32_t(uintptr_t((lds_ptr)buf(which))), lane, k0, full, lo, hi, bad, a.c);
-            }
-            if constexpr (NBUF == 1) {
+                issue(k0, klim, buf(0), p, p);
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                use(core, buf(0), k0, valid, lo, hi, bad_keys(p, p));
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                if constexpr (!KEYS) __syncthreads();
+            }
+        } else {
+            // The next tile is under way during a tile; its page is asked for
+            // before the loads of the tile before it.  (Through the scalar
+            // cache every LDS wait would wait for the page too.)
+            int pn = fetch(kb), which = 0;
+            __syncthreads();  // the buffers may still be read for the segment before
+            int p0 = __builtin_amdgcn_readlane(pn, 0), p1 = __builtin_amdgcn_readlane(pn, 1);
+            pn = fetch(kb + KT);
+            issue(kb, klim, buf(0), p0, p1);
+            for (; k0 < ke; k0 += KT, which ^= 1) {
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                // Every wave's part of the tile has landed, and every wave is
+                // done with the other buffer, which is loaded next.
+                __syncthreads();
+                const uint32_t bad = bad_keys(p0, KT == 32 ? p1 : p0);
+                if (k0 + KT < ke) {
+                    p0 = __builtin_amdgcn_readlane(pn, 0), p1 = __builtin_amdgcn_readlane(pn, 1);
+                    pn = fetch(k0 + 2 * KT);
+                    issue(k0 + KT, klim, buf(which ^ 1), p0, p1);
+                }
+                use(core, buf(which), k0, valid, lo, hi, bad);
             }
         }
+    }
+    // The keys of a tile on pages outside the pool.
+    __device__ uint32_t bad_keys(int p0, int p1) const {
+        const uint32_t n = uint32_t(a.kv.npages);
+        return (unsigned(p0) < n ? 0u : 0xffffu) | (unsigned(p1) < n ? 0u : 0xffff0000u);
+    }
+    __device__ void use(C& core, const T* tile, int k0, bool valid, int lo, int hi, uint32_t bad) const {
+        if (!__ballot(valid && lo < k0 + KT && hi > k0)) return;
+        const bool full = bad == 0 && __all(!valid || (lo <= k0 && hi >= k0 + KT));
+        core.tile(uint32_t(uintptr_t((lds_ptr)tile)), lane, k0, full, lo, hi, bad, a.c);
     }
 };
 
@@ -504,7 +520,7 @@ __device__ inline void emit_keys(const Args& a, Core<T, D, WAVES_KEYS>& core, co
 }
 
 template <typename T, int D, int TILE>
-__global__ __launch_bounds__(NW * 64, TILE == WAVES_KEYS && D == 512 ? 1 : 2) void attention_shared_kernel(Args a) {
+__global__ __launch_bounds__(NW * 64, TILE == WAVES_KEYS && D == 512 ? 1 : D == 128 ? 3 : 2) void attention_shared_kernel(Args a) {
     extern __shared__ __attribute__((aligned(1024))) unsigned char smem_raw[];  // (whole rows: addresses are XORed)
     T* smem = reinterpret_cast<T*>(smem_raw);
     const int tid = int(threadIdx.x), lane = tid % WAVE;
@@ -677,12 +693,24 @@ __global__ __launch_bounds__(256) void attention_join_kernel(Args a) {
             l += wl * ml.y;
         }
         const int n = slots - i0 < WAVE ? slots - i0 : WAVE;
-        for (int i = 0; i < n; ++i) {
-            const float f = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wl), i));
-            if (f == 0.0f) continue;  // (its O was not written)
-            const float* o = a.part_o + (int64_t(i0 + i) * rows + row) * D + lane * E;
+        // (eight slots' loads under way; what a slot without a share holds
+        // was not written)
+#pragma unroll 1
+        for (int i = 0; i < n; i += 8) {
+            float x[8][E];
 #pragma unroll
-            for (int e = 0; e < E; ++e) v[e] += f * o[e];
+            for (int k = 0; k < 8; ++k) {
+                const int at = i + k < n ? i + k : 0;
+                const float* o = a.part_o + (int64_t(i0 + at) * rows + row) * D + lane * E;
+#pragma unroll
+                for (int e = 0; e < E; ++e) x[k][e] = o[e];
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float f = i + k < n ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wl), i + k)) : 0.0f;
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[e] += f == 0.0f ? 0.0f : f * x[k][e];
+            }
         }
     }
     l = wave_sum(l);
@@ -700,16 +728,18 @@ int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 Plan plan(const PagedKv& kv, const PagedBatch& b, int heads) {
     Plan p{};
     const int64_t hpg = heads / kv.kv_heads, rows = b.t * hpg, max_len = b.max_pages * kv.page, P = b.prefix_len;
-    const int64_t target = kv.head_dim == 512 ? 256 : 512;
     p.fused = rows >= 32 * b.nseq;
     if (!p.fused && rows <= 16)
         p.tile = WAVES_KEYS;
+    else if (rows <= 64 || kv.head_dim == 512)
+        p.tile = WAVES_16;
     else
-        p.tile = rows <= 64 || kv.head_dim == 512 ? WAVES_16 : WAVES_32;
+        p.tile = WAVES_32;
     const int64_t M = p.tile == WAVES_KEYS ? 16 : p.tile == WAVES_16 ? 64 : 128;
     p.ntile = int((rows + M - 1) / M);
     const int64_t base = p.ntile * int64_t(kv.kv_heads);
-    auto splits = [&](int64_t keys, int64_t items, int64_t least, int& n, int& chunk) {
+    const int64_t target = 512;
+    auto splits = [&](int64_t keys, int64_t items, int64_t target, int64_t least, int& n, int& chunk) {
         int64_t k = std::min(std::max<int64_t>(1, target / std::max<int64_t>(1, items)), (keys + least - 1) / least);
         k = std::max<int64_t>(1, std::min<int64_t>(k, 64));
         chunk = int(up((keys + k - 1) / k, 32));
@@ -719,15 +749,15 @@ Plan plan(const PagedKv& kv, const PagedBatch& b, int heads) {
     if (p.fused) {
         p.whole = base * 2 >= target;
         if (!p.whole) {
-            if (P > 0) splits(P, base, 256, p.np, p.chunk_p);
-            splits(max_len, base, 256, p.os, p.chunk_o);
+            if (P > 0) splits(P, base, target, 128, p.np, p.chunk_p);
+            splits(max_len, base, target, 256, p.os, p.chunk_o);
         }
         return p;
     }
-    if (P > 0) splits(P, base, 256, p.np, p.chunk_p);
+    if (P > 0) splits(P, base, target, 64, p.np, p.chunk_p);
     const int64_t per = (hpg + 15) / 16;
     p.own_tiles = b.start ? rows / 16 + b.nseq : b.nseq * per;
-    splits(max_len, p.own_tiles * kv.kv_heads, 256, p.os, p.chunk_o);
+    splits(max_len, p.own_tiles * kv.kv_heads, 1024, 512, p.os, p.chunk_o);
     return p;
 }
 
@@ -745,26 +775,31 @@ int64_t part_bytes(const Plan& p, const PagedKv& kv, const PagedBatch& b, int he
 
 template <typename T, int D>
 void launch_d(hipStream_t s, const Args& a, unsigned blocks) {
-    // tiles: 2 buffers x 32 keys, or 4 waves x 16 keys, of K and V; the
-    // waves' join: 4 x 16 rows of f32 and their statistics
-    constexpr unsigned lds_rows = 4 * 32 * D * 2 / (D == 512 ? 2 : 1), lds_keys = NW * 16 * D * 4 + 2 * NW * 16 * 4;
-    const unsigned lds = a.p.fused ? lds_rows : lds_keys > lds_rows ? lds_keys : lds_rows;
+    // tiles: 2 buffers of 32 keys (head_dim 512: 16), or 4 waves x 16 keys,
+    // of K and V; the waves' join: 4 x 16 rows of f32 and their
+    // statistics
+    constexpr unsigned lds_rows = 2 * (D == 512 ? 16 : 32) * D * 4;
+    constexpr unsigned lds_keys = NW * 16 * D * 4 + 2 * NW * 16 * 4;
+    const unsigned lds = a.p.fused ? lds_rows : std::max(lds_keys, lds_rows);
     auto go = [&](auto kernel) {
         OMG_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
                                     int(lds)));
         kernel<<<dim3(blocks), dim3(NW * 64), lds, s>>>(a);
     };
+    auto joined = [&] {
+        OMG_HIP(hipGetLastError());
+        if (!a.part_o) return;
+        attention_join_kernel<T, D><<<dim3(unsigned((a.b.t * a.x.heads + 3) / 4)), dim3(256), 0, s>>>(a);
+        OMG_HIP(hipGetLastError());
+    };
     if (a.p.tile == WAVES_KEYS)
         go(attention_shared_kernel<T, D, WAVES_KEYS>);
     else if (a.p.tile == WAVES_16)
         go(attention_shared_kernel<T, D, WAVES_16>);
-    else if constexpr (D < 512)
+    else if constexpr (D < 512) {
         go(attention_shared_kernel<T, D, WAVES_32>);
-    OMG_HIP(hipGetLastError());
-    if (a.part_o) {
-        attention_join_kernel<T, D><<<dim3(unsigned((a.b.t * a.x.heads + 3) / 4)), dim3(256), 0, s>>>(a);
-        OMG_HIP(hipGetLastError());
     }
+    joined();
 }
 
 template <typename T>
