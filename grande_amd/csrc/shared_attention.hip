@@ -667,17 +667,18 @@ __global__ __launch_bounds__(NW * 64, TILE == WAVES_KEYS && D == 512 ? 1 : D == 
     emit_keys<T, D>(a, core, r, lane, wave, a.p.np + split, reinterpret_cast<float*>(smem_raw));
 }
 
-// out = sum_i w_i O_i / sum_i w_i l_i, w_i = 2^(c m_i - max): one wave per
-// (token, head), D / 64 values a lane.
-template <typename T, int D>
+// out = sum_i w_i O_i / sum_i w_i l_i, w_i = 2^(c m_i - max): W waves per
+// (token, head), each for every W-th slot, D / 64 values a lane.
+template <typename T, int D, int W>
 __global__ __launch_bounds__(256) void attention_join_kernel(Args a) {
     constexpr int E = D / WAVE;
-    const int lane = int(threadIdx.x) % WAVE;
+    __shared__ float sums[W > 1 ? W : 1][D];
+    const int lane = int(threadIdx.x) % WAVE, wave = uni(int(threadIdx.x) / WAVE), mine = wave % W;
     const int64_t rows = a.b.t * a.x.heads;
-    const int64_t row = int64_t(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(int(threadIdx.x) / WAVE);
+    const int64_t row = int64_t(blockIdx.x) * (4 / W) + wave / W;
     if (row >= rows) return;
     const int64_t tok = row / a.x.heads, head = row - tok * a.x.heads;
-    if (token_row(a.b, tok, lane).seq < 0) return;
+    if (token_row(a.b, tok, lane).seq < 0) return;  // (W > 1: the whole workgroup)
     const int slots = int(a.p.slots());
     float cm = -INFINITY;
     for (int i = lane; i < slots; i += WAVE) cm = fmaxf(cm, a.part_ml[i * rows + row].x);
@@ -696,24 +697,36 @@ __global__ __launch_bounds__(256) void attention_join_kernel(Args a) {
         // (eight slots' loads under way; what a slot without a share holds
         // was not written)
 #pragma unroll 1
-        for (int i = 0; i < n; i += 8) {
+        for (int i = mine; i < n; i += 8 * W) {
             float x[8][E];
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                const int at = i + k < n ? i + k : 0;
+                const int at = i + k * W < n ? i + k * W : 0;
                 const float* o = a.part_o + (int64_t(i0 + at) * rows + row) * D + lane * E;
 #pragma unroll
                 for (int e = 0; e < E; ++e) x[k][e] = o[e];
             }
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                const float f = i + k < n ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wl), i + k)) : 0.0f;
+                const float f = i + k * W < n ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wl), i + k * W)) : 0.0f;
 #pragma unroll
                 for (int e = 0; e < E; ++e) v[e] += f == 0.0f ? 0.0f : f * x[k][e];
             }
         }
     }
     l = wave_sum(l);
+    if constexpr (W > 1) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) sums[wave][lane * E + e] = v[e];
+        __syncthreads();
+        if (wave) return;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            v[e] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < W; ++k) v[e] += sums[k][lane * E + e];
+        }
+    }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     T* out = static_cast<T*>(a.x.out) + tok * a.x.ldo + head * D + lane * E;
 #pragma unroll
@@ -738,26 +751,34 @@ Plan plan(const PagedKv& kv, const PagedBatch& b, int heads) {
     const int64_t M = p.tile == WAVES_KEYS ? 16 : p.tile == WAVES_16 ? 64 : 128;
     p.ntile = int((rows + M - 1) / M);
     const int64_t base = p.ntile * int64_t(kv.kv_heads);
-    const int64_t target = 512;
-    auto splits = [&](int64_t keys, int64_t items, int64_t target, int64_t least, int& n, int& chunk) {
-        int64_t k = std::min(std::max<int64_t>(1, target / std::max<int64_t>(1, items)), (keys + least - 1) / least);
-        k = std::max<int64_t>(1, std::min<int64_t>(k, 64));
+    // Two workgroups on each of 256 CUs (head_dim 64: four) take up the launch
+    // at once; a few items more wait for a second round (504 items of 512-wide
+    // heads 57 us, 567 78 us).
+    const int64_t SLOTS = kv.head_dim == 64 ? 1024 : 512;
+    auto splits = [&](int64_t keys, int64_t k, int64_t least, int& n, int& chunk) {
+        k = std::max<int64_t>(1, std::min<int64_t>({k, (keys + least - 1) / least, 64}));
         chunk = int(up((keys + k - 1) / k, 32));
         n = int((keys + chunk - 1) / chunk);
     };
     p.os = 1, p.chunk_o = int(std::min<int64_t>(up(max_len, 32), INT_MAX / 2));
     if (p.fused) {
-        p.whole = base * 2 >= target;
+        p.whole = base * 2 >= SLOTS;
         if (!p.whole) {
-            if (P > 0) splits(P, base, target, 128, p.np, p.chunk_p);
-            splits(max_len, base, target, 256, p.os, p.chunk_o);
+            const int64_t all = SLOTS / base;  // shared out by the keys' numbers
+            const int64_t own = std::max<int64_t>(1, all * max_len / (P + max_len));
+            splits(max_len, P > 0 ? own : all, 128, p.os, p.chunk_o);
+            if (P > 0) splits(P, all - p.os, 128, p.np, p.chunk_p);
         }
         return p;
     }
-    if (P > 0) splits(P, base, target, 64, p.np, p.chunk_p);
+    // A prefix split writes and reads 8 bytes a row and head dim, and reads
+    // 4 a key of its own: beyond 2 keys for 3 rows splits cost more than
+    // they fill (208 x 2 rows on 8,000 keys: 12 / 16 / 20 / 32 splits 45 / 43
+    // / 46 / 55 us), unless CUs stay empty.
+    if (P > 0) splits(P, std::min(SLOTS / base, std::max(SLOTS / 2 / base, 2 * P / (3 * rows))), 64, p.np, p.chunk_p);
     const int64_t per = (hpg + 15) / 16;
     p.own_tiles = b.start ? rows / 16 + b.nseq : b.nseq * per;
-    splits(max_len, p.own_tiles * kv.kv_heads, 1024, 512, p.os, p.chunk_o);
+    splits(max_len, SLOTS / (p.own_tiles * kv.kv_heads), 128, p.os, p.chunk_o);
     return p;
 }
 
@@ -789,7 +810,11 @@ void launch_d(hipStream_t s, const Args& a, unsigned blocks) {
     auto joined = [&] {
         OMG_HIP(hipGetLastError());
         if (!a.part_o) return;
-        attention_join_kernel<T, D><<<dim3(unsigned((a.b.t * a.x.heads + 3) / 4)), dim3(256), 0, s>>>(a);
+        const int64_t rows = a.b.t * a.x.heads;
+        if (a.p.slots() > 8)
+            attention_join_kernel<T, D, 4><<<dim3(unsigned(rows)), dim3(256), 0, s>>>(a);
+        else
+            attention_join_kernel<T, D, 1><<<dim3(unsigned((rows + 3) / 4)), dim3(256), 0, s>>>(a);
         OMG_HIP(hipGetLastError());
     };
     if (a.p.tile == WAVES_KEYS)
