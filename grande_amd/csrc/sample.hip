@@ -193,6 +193,9 @@ struct Shared : Common {
     uint64_t hist[BINS];
     uint64_t edge[PAIRS]; // items of one bin
 };
+struct BinsShared : Common {
+    uint64_t hist[BINS];
+};
 struct DrawShared : Common {
     uint64_t item[(1 << IDX_BITS) / SEG];  // the masses of the row's segments
     uint64_t hist[BINS];
@@ -1048,20 +1051,23 @@ __global__ __launch_bounds__(NT) void sample_row(SampleArgs a, Workspace ws) {
 }
 
 // Whether this workgroup is the last of its row's to arrive; what the others
-// wrote before is then visible to it.  (One thread fences for all, ordered
-// with them by the barriers: a fence writes back and invalidates the L2, and
-// one by every wave took 300 us of a 16.8 million logits' pass.)
+// left for it, by store_shared, is then there for load_shared.  These go past
+// the L2s, which are one an XCD: the stores are done when they are waited
+// for, and no fence, which would write back and invalidate an L2, is needed
+// (one a workgroup took 50 us of a pass over 16.8 million logits, one a wave
+// 300).
 __device__ inline bool last_of(uint32_t* arrived, Common& sm) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    if (threadIdx.x == 0) {
-        __threadfence();
-        sm.count = atomicAdd(arrived, 1u);
-        __threadfence();
-    }
+    if (threadIdx.x == 0)
+        sm.count = __hip_atomic_fetch_add(arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __syncthreads();
     const bool last = sm.count == gridDim.x - 1;
     __syncthreads();
     return last;
+}
+__device__ inline void store_shared(uint64_t* p, uint64_t v) {
+    __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 __device__ inline uint64_t load_shared(const uint64_t* p) {  // written by other workgroups of this launch
     return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -1077,11 +1083,11 @@ __device__ inline Row<T> part_of(const Row<T>& row) {
 // The masses of rows TO_CUT by bins; the last workgroup of a row finds
 // top_p's cut.
 template <typename T>
-__global__ __launch_bounds__(NT) void sample_bins(SampleArgs a, Workspace ws) {
+__global__ __launch_bounds__(NT, 8) void sample_bins(SampleArgs a, Workspace ws) {
     const int64_t r = blockIdx.y;
     Pending& pd = ws.pending[r];
     if (pd.step != TO_CUT) return;
-    __shared__ Shared sm;
+    __shared__ BinsShared sm;
     const int tid = int(threadIdx.x);
     const Settings s = settings_of(a, r);
     const Row<T> row(static_cast<const T*>(a.logits) + r * a.ld, a.vocab);
@@ -1098,7 +1104,7 @@ __global__ __launch_bounds__(NT) void sample_bins(SampleArgs a, Workspace ws) {
     __syncthreads();
     uint64_t* hist = ws.hist + r * ws.nparts * BINS;
     for (int i = tid; i < BINS; i += NT)
-        __hip_atomic_store(hist + blockIdx.x * BINS + i, sm.hist[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        store_shared(hist + blockIdx.x * BINS + i, sm.hist[i]);
     if (!last_of(&pd.arrived[0], sm)) return;
     uint64_t own = 0;
     for (int i = tid; i < BINS; i += NT) {
@@ -1136,16 +1142,23 @@ __global__ __launch_bounds__(NT, 8) void sample_draw(SampleArgs a, Workspace ws)
         const double x = out.w(z);
         return x >= s.least ? Weigh::fixed(x) : 0;
     };
+    if (tid == 0) sm.count = 0;
+    __syncthreads();
     part.sums(sm.item, [&](float z, int i) {
         if (sc.bin(z) == bin && z > -INFINITY) {
-            const uint32_t at = atomicAdd(&pd.edges, 1u);
-            if (at < EDGE) __hip_atomic_store(edge + at, item_of(z, first + i), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            const uint32_t at = atomicAdd(&sm.count, 1u);
+            if (at < EDGE) sm.edge[at] = item_of(z, first + i);
         }
         return before(z, i);
     });
     __syncthreads();
+    const uint32_t here = sm.count;
+    if (tid == 0 && here) sm.bin = atomicAdd(&pd.edges, here);
+    __syncthreads();
+    for (uint32_t i = tid; i < here && sm.bin + i < EDGE; i += NT)
+        store_shared(edge + sm.bin + i, sm.edge[i]);
     if (tid < part.segments())
-        __hip_atomic_store(segs + first / SEG + tid, sm.item[tid], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        store_shared(segs + first / SEG + tid, sm.item[tid]);
     if (!last_of(&pd.arrived[1], sm)) return;
     if (tid == 0) sm.kfirst = __hip_atomic_load(&pd.edges, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     for (int i = tid; i < ns; i += NT) sm.item[i] = load_shared(segs + i);

@@ -787,6 +787,7 @@ void check(const PagedKv& kv, const PagedBatch& b, int heads) {
     check_batch(b, kv, "attention_shared");
     if (heads <= 0 || heads > 4096 || heads % kv.kv_heads)
         fail(E_INVALID, "attention_shared: heads must be a multiple of kv_heads, at most 4096");
+    if (b.t * heads > INT_MAX / 2) fail(E_INVALID, "attention_shared: t * heads must stay below 2^30");
 }
 
 int64_t part_bytes(const Plan& p, const PagedKv& kv, const PagedBatch& b, int heads) {
@@ -802,9 +803,13 @@ void launch_d(hipStream_t s, const Args& a, unsigned blocks) {
     constexpr unsigned lds_rows = 2 * (D == 512 ? 16 : 32) * D * 4;
     constexpr unsigned lds_keys = NW * 16 * D * 4 + 2 * NW * 16 * 4;
     const unsigned lds = a.p.fused ? lds_rows : std::max(lds_keys, lds_rows);
+    static bool lds_set[3];  // (by tile, once per instantiation)
     auto go = [&](auto kernel) {
-        OMG_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                    int(lds)));
+        if (!lds_set[a.p.tile]) {
+            OMG_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                        hipFuncAttributeMaxDynamicSharedMemorySize, int(std::max(lds_keys, lds_rows))));
+            lds_set[a.p.tile] = true;
+        }
         kernel<<<dim3(blocks), dim3(NW * 64), lds, s>>>(a);
     };
     auto joined = [&] {
