@@ -292,6 +292,14 @@ struct Scale {
         const float x = (max - z) * per;
         return x < float(BINS - 1) ? int(x) : BINS - 1;  // (NaN, infinity - infinity: the last)
     }
+    // The bins that top_p's cut can lie in, of n logits whose mass is at least
+    // `mass` of the largest's: those below the last one returned weigh less
+    // than (1 - p) mass / (2 n) each, together less than what top_p leaves.
+    __device__ int reach(float p, float mass, int n, float t) const {
+        const float nats = logf(2.0f * float(n) / ((1.0f - p) * mass));
+        const float x = nats * t * per + 2.0f;
+        return x < float(BINS - 1) && max < INFINITY ? int(x) : BINS - 1;  // (infinities lie in the last)
+    }
     // A logit below all that lie in bins 0 .. last, however the bins rounded.
     __device__ float under(int last) const {
         const float x = max - float(last + 1) / per * 1.00001f;
@@ -420,13 +428,13 @@ __device__ inline void draw_in(const Row<T>& row, int first, uint64_t target, ui
 // The item at which the running share, over the items from the first on,
 // first reaches `target` (>= 1); 0 if it never does, or an item below all
 // that do.  items(f) calls f(z, i) for the thread's items; masses: an item's
-// share is its mass, else one.
+// share is its mass, else one.  key: of all items, where it is the same.
 template <typename S, typename M>
-__device__ uint64_t find_cut(S&& items, M& sm, uint64_t target, bool masses, const Weigh& w) {
-    uint64_t prefix = 0, before = 0;
-    int shift = 52;
+__device__ uint64_t find_cut(S&& items, M& sm, uint64_t target, bool masses, const Weigh& w, uint32_t key = 0) {
+    uint64_t prefix = key, before = 0;
+    int shift = key ? IDX_BITS : 52;
 #pragma unroll 1
-    for (int level = 0; level < 5; ++level) {
+    for (int level = key ? 3 : 0; level < 5; ++level) {
         const int bits = level < 2 ? 11 : 10;
         shift -= bits;
         clear(sm.hist, 1 << bits);
@@ -457,7 +465,16 @@ __device__ Cut cut_in_bin(const uint64_t* room, int n, M& sm, uint64_t left, boo
 #pragma unroll 1
             for (int i = tid; i < n; i += NT) f(item_value(room[i]), item_index(room[i]));
         };
-        const uint64_t edge = find_cut(some, sm, left, masses, w);
+        if (tid == 0) sm.kmax = 0, sm.kfirst = ~0u;
+        __syncthreads();
+        uint32_t most = 0, least = ~0u;
+        for (int i = tid; i < n; i += NT) {
+            const uint32_t k = uint32_t(room[i] >> IDX_BITS);
+            most = most > k ? most : k, least = least < k ? least : k;
+        }
+        if (most) atomicMax(&sm.kmax, most), atomicMin(&sm.kfirst, least);
+        __syncthreads();
+        const uint64_t edge = find_cut(some, sm, left, masses, w, sm.kmax == sm.kfirst ? sm.kmax : 0);
         // (the edge may lie below the bin: the last item of the bin above it)
         if (tid == 0) sm.found = ~uint64_t(0);
         __syncthreads();
@@ -511,11 +528,11 @@ __device__ Cut cut_by_bins(S&& items, const Scale& sc, Shared& sm, uint64_t* roo
     return cut_in_bin(room, n, sm, left, masses, w);
 }
 
-// The cuts of top_k and top_p over items, whose shares are summed by bins
+// The cuts of top_k and top_p over n items, whose shares are summed by bins
 // first; row_mass: the mass that top_p is a share of where it is known (0:
 // it is summed here).
 template <typename S>
-__device__ Cut cuts(S&& items, const Settings& s, const Scale& sc, uint64_t row_mass, Shared& sm, uint64_t* room,
+__device__ Cut cuts(S&& items, int n, const Settings& s, const Scale& sc, uint64_t row_mass, Shared& sm, uint64_t* room,
                     int most, const Weigh& w) {
     Cut cut;
 #pragma unroll 1
@@ -523,11 +540,15 @@ __device__ Cut cuts(S&& items, const Settings& s, const Scale& sc, uint64_t row_
         const bool masses = step == 1;
         clear(sm.hist, BINS);
         uint64_t own = 0;
+        // (atomics of many lanes on few bins cost more than exp: only what
+        // the cut can reach is summed by bins)
+        const int reach = masses && s.p > 0.0f ? sc.reach(s.p, 1.0f, n, s.t) : BINS - 1;
         items([&](float z, int i) {
             if (!cut.keeps(z, i)) return;
             const uint64_t v = masses ? w.mass(z) : 1;
             own += v;
-            if (v) add(&sm.hist[sc.bin(z)], v);
+            const int b = sc.bin(z);
+            if (v && b <= reach) add(&sm.hist[b], v);
         });
         uint64_t target = uint64_t(s.k);
         if (masses) {
@@ -586,7 +607,7 @@ __device__ void finish_list(int n, const Settings& s, float u, uint64_t row_mass
 #pragma unroll 1
         for (int i = tid; i < n; i += NT) f(item_value(sm.item[i]), item_index(sm.item[i]));
     };
-    const Cut cut = cuts(items, s, sc, row_mass, sm, sm.edge, PAIRS, w);
+    const Cut cut = cuts(items, n, s, sc, row_mass, sm, sm.edge, PAIRS, w);
     // the kept masses, then the draw: the digits of the index, 10 and 10 bits
     uint64_t own = 0;
 #pragma unroll 1
@@ -736,6 +757,12 @@ __device__ int make_list(const Settings& s, const Scale& sc, Shared& sm, uint64_
             clear(sm.hist, BINS);
             if (2 * k <= nchunk && s.k) {
                 if (chunk > -INFINITY) add(&sm.hist[sc.bin(chunk)], 1);
+            } else if (s.k && 2 * k > ngroup && row.n <= SHORT) {
+                row.turns([&](const float* z, int) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+                        if (z[c] > -INFINITY) add(&sm.hist[sc.bin(z[c])], 1);
+                });
             } else {
                 const bool fours = 2 * k <= ngroup / 4;
 #pragma unroll 2
@@ -783,7 +810,7 @@ __device__ int make_list(const Settings& s, const Scale& sc, Shared& sm, uint64_
 // Rows whose kept tokens do not fit a list, between the kernels.
 enum Step : uint32_t { DONE = 0, TO_CUT, TO_DRAW, TO_FINISH };
 struct Pending {
-    uint64_t left;       // the mass that top_p takes from bin `bin`
+    uint64_t left;       // TO_CUT: the row's mass; TO_DRAW: what top_p takes from bin `bin`
     float max;
     uint32_t step;
     int bin;             // bins before it stay whole
@@ -1012,7 +1039,7 @@ __global__ __launch_bounds__(NT) void sample_long(SampleArgs a, Workspace ws) {
         return;
     }
     if (tid == 0)
-        ws.pending[r] = s.k ? to_finish(top) : Pending{0, top, s.p < 1.0f ? TO_CUT : TO_DRAW, BINS, {0, 0}, 0};
+        ws.pending[r] = s.k ? to_finish(top) : Pending{total, top, s.p < 1.0f ? TO_CUT : TO_DRAW, BINS, {0, 0}, 0};
 }
 
 // The exact cuts and the draw over a whole row.
@@ -1034,7 +1061,7 @@ __global__ __launch_bounds__(NT) void sample_row(SampleArgs a, Workspace ws) {
                 if (z[c] > -INFINITY) f(z[c], i + c);
         });
     };
-    const Cut cut = cuts(items, s, sc, 0, sm, sm.item, CAP, out.w);
+    const Cut cut = cuts(items, row.n, s, sc, 0, sm, sm.item, CAP, out.w);
     auto kept = [&](float z, int i) -> uint64_t {
         if (!cut.keeps(z, i)) return 0;
         const double x = out.w(z);
@@ -1093,28 +1120,32 @@ __global__ __launch_bounds__(NT, 8) void sample_bins(SampleArgs a, Workspace ws)
     const Row<T> row(static_cast<const T*>(a.logits) + r * a.ld, a.vocab);
     const Weigh w(pd.max, s.inv_t);
     const Scale sc(pd.max, s.t);
+    const uint64_t total = pd.left;
+    const int reach = s.p > 0.0f ? sc.reach(s.p, float(double(total) / ONE), row.n, s.t) : BINS - 1;
     clear(sm.hist, BINS);
     part_of(row).turns([&](const float* z, int) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
+            const int b = sc.bin(z[c]);
+            if (b > reach) continue;
             const uint64_t m = w.mass(z[c]);
-            if (m) add(&sm.hist[sc.bin(z[c])], m);
+            if (m) add(&sm.hist[b], m);
         }
     });
     __syncthreads();
     uint64_t* hist = ws.hist + r * ws.nparts * BINS;
-    for (int i = tid; i < BINS; i += NT)
-        store_shared(hist + blockIdx.x * BINS + i, sm.hist[i]);
+    for (int i = tid; i <= reach; i += NT) store_shared(hist + blockIdx.x * BINS + i, sm.hist[i]);
     if (!last_of(&pd.arrived[0], sm)) return;
-    uint64_t own = 0;
+#pragma unroll
     for (int i = tid; i < BINS; i += NT) {
         uint64_t v = 0;
-#pragma unroll 4
-        for (int k = 0; k < int(ws.nparts); ++k) v += load_shared(hist + k * BINS + i);
+        if (i <= reach) {
+#pragma unroll 8
+            for (int k = 0; k < int(ws.nparts); ++k) v += load_shared(hist + k * BINS + i);
+        }
         sm.hist[i] = v;
-        own += v;
     }
-    const uint64_t target = share_of(s.p, block_sum(own, sm));
+    const uint64_t target = share_of(s.p, total);
     pick<false>(sm.hist, BINS, target, sm);
     if (tid == 0) pd.bin = int(sm.bin), pd.left = target - sm.before, pd.step = TO_DRAW;
 }
