@@ -186,7 +186,7 @@ void check_batch(const PagedBatch& b, const PagedKv& kv, const char* who) {
         fail(E_INVALID, w + ": nseq must be 1 to 2^20 and t 1 to 2^24");
     if (!b.lens || !b.table) fail(E_INVALID, w + ": null lens or table");
     if (!b.start && b.t != b.nseq) fail(E_INVALID, w + ": without start every sequence has one token (t = nseq)");
-    if (b.max_pages <= 0 || b.max_pages * kv.page > 0x7fffffff || b.table_ld < b.max_pages)
+    if (b.max_pages <= 0 || b.max_pages > 0x3fffffff / kv.page || b.table_ld < b.max_pages)
         fail(E_INVALID, w + ": max_pages out of range or past table_ld");
     if (b.prefix_len < 0 || b.prefix_len > 0x3fffffff) fail(E_INVALID, w + ": prefix_len out of range");
     if (b.prefix_len > 0 && !b.prefix_table) fail(E_INVALID, w + ": null prefix_table");

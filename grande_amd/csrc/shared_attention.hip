@@ -33,6 +33,7 @@
 // r (K: the 16 rows of an operand read on distinct banks) and with 2 r (V:
 // the 4 rows x 32 bytes of a transposing read).
 #include <algorithm>
+#include <atomic>
 #include <climits>
 #include <string>
 
@@ -461,14 +462,92 @@ struct Row {
     int head, seq, own;  // own: its row in the sequence's cache rows
 };
 
+// The keys of a work item: prefix rows [pb, pe), own rows [ob, oe).
+struct Keys {
+    int g, pb, pe, ob, oe;
+};
+
+// In a tile a key that a query does not see has p = 0, which leaves nothing
+// of its values unless these are infinite or NaN.  Sums that are not finite
+// are therefore taken again from the keys their row sees and no others, one
+// by one: `rows` holds a bit per lane whose row it is (with maximum cm, sum
+// l); a wave writes the quads of head dims it has (quarter < 0: all).
+template <typename T, int D>
+__device__ void seen_alone(const Args& a, const Keys& in, const Row& r, uint64_t rows, float cm, float l, int lane,
+                           int64_t slot, int quarter) {
+    constexpr int NQ = D / 4, E = (NQ + WAVE - 1) / WAVE;
+    typedef T vec4 __attribute__((ext_vector_type(4)));
+    const int P = int(a.b.prefix_len), w = a.x.window;
+#pragma unroll 1
+    for (; rows; rows &= rows - 1) {
+        const int i = __builtin_ctzll(rows);
+        const auto of = [&](int v) { return __builtin_amdgcn_readlane(v, i); };
+        const auto off = [&](float v) { return __builtin_bit_cast(float, of(__builtin_bit_cast(int, v))); };
+        const int64_t tok = of(int(r.tok));
+        const int head = of(r.head), seq = of(r.seq), own = of(r.own);
+        const float row_cm = off(cm), ref = row_cm == -INFINITY ? 0.0f : row_cm;
+        float4 q[E], o[E];
+        const auto load = [&](const void* p, int64_t at, float4* x) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                vec4 v{};
+                if (lane + e * WAVE < NQ) v = reinterpret_cast<const vec4*>(static_cast<const T*>(p) + at)[lane + e * WAVE];
+                x[e] = make_float4(float(v[0]), float(v[1]), float(v[2]), float(v[3]));
+            }
+        };
+        load(a.x.q, tok * a.x.ldq + int64_t(head) * D, q);
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        const auto keys = [&](const int32_t* table, int plast, int from, int to) {
+#pragma unroll 1
+            for (int k = from; k < to; ++k) {
+                const int64_t page = table[imin(k >> a.page_shift, plast)];
+                if (page < 0 || page >= a.kv.npages) continue;
+                const int64_t at = page * a.kv.page_stride + (int64_t(in.g) * a.kv.page + (k & (a.kv.page - 1))) * D;
+                float4 x[E];
+                load(a.kv.k, at, x);
+                float s = 0.0f;
+#pragma unroll
+                for (int e = 0; e < E; ++e) s += x[e].x * q[e].x + x[e].y * q[e].y + x[e].z * q[e].z + x[e].w * q[e].w;
+                const float p = __builtin_amdgcn_exp2f(fmaf(wave_sum(s), a.c, -ref));
+                load(a.kv.v, at, x);
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    o[e].x += p * x[e].x, o[e].y += p * x[e].y, o[e].z += p * x[e].z, o[e].w += p * x[e].w;
+            }
+        };
+        keys(a.b.prefix_table, (P - 1) >> a.page_shift, imax(in.pb, w > 0 ? P + own - w + 1 : 0), in.pe);
+        keys(a.b.table + seq * a.b.table_ld, int(a.b.max_pages) - 1, imax(in.ob, w > 0 ? own - w + 1 : 0),
+             imin(in.oe, own + 1));
+        const Sink<T> out{a, tok * a.x.heads + head, tok * a.x.ldo + int64_t(head) * D, slot};
+        const float sum = off(l);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int c4 = lane + e * WAVE;
+            if (c4 < NQ && (quarter < 0 || c4 % 16 / 4 == quarter)) out.template quad<D>(4 * c4, o[e], sum);
+        }
+    }
+}
+
 // The results of a wave's rows (not KEYS).
 template <typename T, int D, int TILE>
-__device__ inline void emit(const Args& a, Core<T, D, TILE>& core, const Row& r, int lane, int64_t slot) {
+__device__ inline void emit(const Args& a, Core<T, D, TILE>& core, const Keys& in, const Row& r, int lane,
+                            int64_t slot) {
     typedef Core<T, D, TILE> C;
-    const float l = C::row_sum(core.l);
-    if (!r.valid) return;
+    const float l = C::row_sum(core.l), cm = core.m == -INFINITY ? -INFINITY : core.m * a.c;
     const Sink<T> out{a, r.tok * a.x.heads + r.head, r.tok * a.x.ldo + int64_t(r.head) * D, slot};
-    if (lane < C::RW) out.stats(core.m == -INFINITY ? -INFINITY : core.m * a.c, l);
+    if (r.valid && lane < C::RW) out.stats(cm, l);
+    float z[4] = {};  // (NaN where a sum is not finite)
+#pragma unroll
+    for (int i = 0; i < C::NC; ++i)
+#pragma unroll
+        for (int e = 0; e < C::SR; ++e) z[e % 4] = fmaf(core.o[i][e], 0.0f, z[e % 4]);
+    uint64_t bad = __ballot(r.valid && !(z[0] + z[1] + z[2] + z[3] == 0.0f));
+    bad |= bad >> 32;
+    if constexpr (C::RW == 16) bad |= bad >> 16;
+    bad &= (uint64_t(1) << C::RW) - 1;
+    if (bad) seen_alone<T, D>(a, in, r, bad, cm, l, lane, slot, -1);
+    if (!r.valid || (bad >> (lane % C::RW) & 1)) return;
 #pragma unroll
     for (int i = 0; i < C::NC; ++i)
 #pragma unroll
@@ -481,8 +560,8 @@ __device__ inline void emit(const Args& a, Core<T, D, TILE>& core, const Row& r,
 
 // The four waves' results for the same 16 rows, joined through LDS.
 template <typename T, int D>
-__device__ inline void emit_keys(const Args& a, Core<T, D, WAVES_KEYS>& core, const Row& r, int lane, int wave,
-                                 int64_t slot, float* smem) {
+__device__ inline void emit_keys(const Args& a, Core<T, D, WAVES_KEYS>& core, const Keys& in, const Row& r, int lane,
+                                 int wave, int64_t slot, float* smem) {
     typedef Core<T, D, WAVES_KEYS> C;
     const float l = C::row_sum(core.l);
     __syncthreads();  // every wave is done with its tiles
@@ -505,18 +584,27 @@ __device__ inline void emit_keys(const Args& a, Core<T, D, WAVES_KEYS>& core, co
         w[k] = x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x - cm);
         sum += w[k] * ml[64 + k * 16 + lane % 16];
     }
-    if (!r.valid) return;
     const Sink<T> out{a, r.tok * a.x.heads + r.head, r.tok * a.x.ldo + int64_t(r.head) * D, slot};
-    if (wave == 0 && lane < 16) out.stats(cm, sum);
-    for (int c4 = wave * 4 + lane / 16; c4 < D / 4; c4 += NW * 4) {
-        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (r.valid && wave == 0 && lane < 16) out.stats(cm, sum);
+    float4 v[D / 64];  // quads wave * 4 + lane / 16 + 16 i
+    float z = 0.0f;
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) {
+        v[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
         for (int k = 0; k < NW; ++k) {
-            const float4 x = *reinterpret_cast<const float4*>(smem + k * 16 * D + (c4 * 16 + lane % 16) * 4);
-            v.x += w[k] * x.x, v.y += w[k] * x.y, v.z += w[k] * x.z, v.w += w[k] * x.w;
+            const float4 x = *reinterpret_cast<const float4*>(smem + k * 16 * D + ((wave * 4 + lane / 16 + 16 * i) * 16 + lane % 16) * 4);
+            v[i].x += w[k] * x.x, v[i].y += w[k] * x.y, v[i].z += w[k] * x.z, v[i].w += w[k] * x.w;
         }
-        out.template quad<D>(4 * c4, v, sum);
+        z += fmaf(v[i].x, 0.0f, v[i].y * 0.0f) + fmaf(v[i].z, 0.0f, v[i].w * 0.0f);
     }
+    uint64_t bad = __ballot(r.valid && !(z == 0.0f));
+    bad |= bad >> 32;
+    bad = (bad | bad >> 16) & 0xffff;
+    if (bad) seen_alone<T, D>(a, in, r, bad, cm, sum, lane, slot, wave);
+    if (!r.valid || (bad >> (lane % 16) & 1)) return;
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) out.template quad<D>(4 * (wave * 4 + lane / 16 + 16 * i), v[i], sum);
 }
 
 template <typename T, int D, int TILE>
@@ -613,10 +701,15 @@ __global__ __launch_bounds__(NW * 64, TILE == WAVES_KEYS && D == 512 ? 1 : D == 
                        hi);
             }
         }
+        Keys in{g, 0, 0, 0, 0};
+        if (a.p.whole || split < a.p.np)
+            in.pb = a.p.whole ? 0 : split * a.p.chunk_p, in.pe = a.p.whole ? P : imin(P, in.pb + a.p.chunk_p);
+        if (a.p.fused && (a.p.whole || split >= a.p.np))
+            in.ob = a.p.whole ? 0 : (split - a.p.np) * a.p.chunk_o, in.oe = a.p.whole ? cap : imin(cap, in.ob + a.p.chunk_o);
         if constexpr (TILE == WAVES_KEYS)
-            emit_keys<T, D>(a, core, r, lane, wave, split, reinterpret_cast<float*>(smem_raw));
+            emit_keys<T, D>(a, core, in, r, lane, wave, split, reinterpret_cast<float*>(smem_raw));
         else
-            emit<T, D, TILE>(a, core, r, lane, split);
+            emit<T, D, TILE>(a, core, in, r, lane, split);
         return;
     }
 
@@ -664,7 +757,8 @@ __global__ __launch_bounds__(NW * 64, TILE == WAVES_KEYS && D == 512 ? 1 : D == 
     if (kb < ke)
         st.run(core, a.b.table + s * a.b.table_ld, int(a.b.max_pages) - 1, kb, ke, imin(len, cap), r.valid,
                w > 0 ? imax(0, r.own - w + 1) : 0, imin(r.own + 1, cap));
-    emit_keys<T, D>(a, core, r, lane, wave, a.p.np + split, reinterpret_cast<float*>(smem_raw));
+    const Keys in{g, 0, 0, split * a.p.chunk_o, imin(cap, (split + 1) * a.p.chunk_o)};
+    emit_keys<T, D>(a, core, in, r, lane, wave, a.p.np + split, reinterpret_cast<float*>(smem_raw));
 }
 
 // out = sum_i w_i O_i / sum_i w_i l_i, w_i = 2^(c m_i - max): W waves per
@@ -803,12 +897,15 @@ void launch_d(hipStream_t s, const Args& a, unsigned blocks) {
     constexpr unsigned lds_rows = 2 * (D == 512 ? 16 : 32) * D * 4;
     constexpr unsigned lds_keys = NW * 16 * D * 4 + 2 * NW * 16 * 4;
     const unsigned lds = a.p.fused ? lds_rows : std::max(lds_keys, lds_rows);
-    static bool lds_set[3];  // (by tile, once per instantiation)
+    static std::atomic<uint64_t> lds_set[3];  // by tile: the devices, once per instantiation
+    int device = 0;
+    OMG_HIP(hipGetDevice(&device));
     auto go = [&](auto kernel) {
-        if (!lds_set[a.p.tile]) {
+        const uint64_t bit = uint64_t(1) << (device & 63);
+        if (device > 63 || !(lds_set[a.p.tile].load(std::memory_order_relaxed) & bit)) {
             OMG_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                         hipFuncAttributeMaxDynamicSharedMemorySize, int(std::max(lds_keys, lds_rows))));
-            lds_set[a.p.tile] = true;
+            lds_set[a.p.tile].fetch_or(bit, std::memory_order_relaxed);
         }
         kernel<<<dim3(blocks), dim3(NW * 64), lds, s>>>(a);
     };

@@ -339,7 +339,8 @@ typedef struct {
  * sequence s has the token rows [start[s], start[s + 1]) (start NULL: row s,
  * then t = nseq) and, these included, lens[s] rows of its own in the cache;
  * row i is row i % page of page table[s * table_ld + i / page], for
- * i / page < max_pages.  Its new tokens are the last of its rows.  All
+ * i / page < max_pages (max_pages * page and prefix_len below 2^30, nseq up
+ * to 2^20, t up to 2^24).  Its new tokens are the last of its rows.  All
  * sequences follow a shared prefix of prefix_len rows on the pages
  * prefix_table[i / page] (prefix_len 0: none): row i of a sequence has the
  * position prefix_len + i.
@@ -398,11 +399,10 @@ int omg_dev_kv_append(const omg_paged_kv *kv, const omg_paged_batch *b, const om
  * out (row stride ldo) has the cache's type, lse [t][heads] f32 (may be
  * NULL); a token that sees no key gets zeros and -infinity.  The prefix's
  * keys and values are read once for a tile of query rows, whatever
- * sequences these belong to.  What stands in cache rows that nobody sees
- * does not matter, unless another query of the call sees it: a value that
- * is infinite or NaN there may reach queries that do not see its row.
- * scale positive; q and out 16-byte aligned, ldq and ldo multiples of 8.
- * f32 sums; the softmax's probabilities are rounded to the cache's type for
+ * sequences these belong to.  What stands in cache rows that a token does
+ * not see, infinities and NaN among it, does not reach the token.
+ * scale positive; q and out 16-byte aligned and apart, ldq and ldo multiples
+ * of 8.  f32 sums; the softmax's probabilities are rounded to the cache's type for
  * their product with the values.
  *
  * workspace: omg_dev_attention_shared_workspace bytes (a function of the

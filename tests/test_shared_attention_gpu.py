@@ -213,6 +213,40 @@ def test_what_unseen_rows_hold_does_not_matter(hd, new):
     c.run().check()
 
 
+@pytest.mark.parametrize("window", [0, 25])
+@pytest.mark.parametrize("new,before", [([1] * 7, 0), ([33, 40, 36, 47, 50], 0), ([3, 1, 2, 4, 1], 0), ([1] * 3, 900),
+                                        ([40, 60, 35], 700)])
+@pytest.mark.parametrize("hd", [64, 128, 256, 512])
+def test_nan_reaches_the_queries_that_see_its_row_and_no_others(hd, new, before, window):
+    """One sequence's values NaN in a row that some of its queries see, then
+    keys; the rest of its queries and the other sequences are as without it."""
+    rng = np.random.default_rng(30)
+    c = Call(rng, new, before + np.array([0, 17, 30, 15, 40, 31, 47])[:len(new)], 77, 4, 2, hd, page=32, dtype="bf16",
+             window=window)
+    clean = c.run().out.clone(), c.lse.clone()
+    c.check("clean")
+    s = 1
+    n, length = new[s], int(c.pool.lens_host[s])
+    row = length - max(1, n // 2)  # the last half of its queries see it
+    own = length - n + np.arange(n)
+    sees = (own >= row) & ((own < row + window) if window else True)
+    if before or n == 1:  # a row of the first tile, behind the window where there is one
+        row = max(0, length - n - 1 - (30 if window else 0))
+        sees = np.full(n, True) if not window else (own < row + window)
+    at = int(np.sum(new[:s])) + np.flatnonzero(sees)
+    for raw in (c.pool.v, c.pool.k):
+        old = raw.clone()
+        raw[int(c.pool.table_host[s, row // 32]), :, row % 32] = float("nan")
+        c.out.fill_(5.0)
+        c.lse.fill_(5.0)
+        c.run()
+        torch.cuda.synchronize()
+        assert bool(torch.isnan(c.out[at, :4 * hd]).all())
+        c.out[at], c.lse[at] = clean[0][at], clean[1][at]
+        raw.copy_(old)
+        c.check("NaN in a row")
+
+
 def test_pages_outside_the_pool_are_not_seen():
     rng = np.random.default_rng(31)
     for new in ([1] * 4, [35, 40, 50, 33], [3, 4, 1, 2]):
