@@ -6,6 +6,8 @@
 
 namespace omg {
 
+constexpr int64_t MAX_BLOCKS = 1 << 24;  // of 256 threads: a launch holds less than 2^32 threads
+
 // Host checks of the descriptions, shared by the calls that take them (paged.hip).
 bool aligned16(const void* p);
 int log2_of(int64_t n);  // the least s with 2^s >= n

@@ -1,5 +1,5 @@
-// The paged K/V cache: appending rows to it and attention over it for
-// sequences that share a prefix.
+// The paged K/V cache: appending rows to it, and the checks that its callers
+// share.
 #include <string>
 
 #include "common.h"
@@ -69,10 +69,12 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
         }
     }
     // The pairs' (cos, sin) of the lane's elements and its sign in the pair:
-    // y' = y cos + sign * partner * sin; cos 1 and sin 0 outside the pairs.
+    // y' = y cos + sign * partner * sin; outside the pairs elements stay as
+    // they are (whole lanes: rope_dims is a multiple of 16).
     float cs[8], sn[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) cs[i] = 1.0f, sn[i] = 0.0f;
+    bool rotated = false;
     const int half = a.src.rope_dims / 2;
     int hop = 0;  // lanes to the partner (half layouts)
     if (a.src.rope) {
@@ -81,6 +83,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
         const float* rt = a.src.rope + pos * a.src.rope_dims;
         if (a.src.rope_layout == 1) {
             if (c0 < a.src.rope_dims) {
+                rotated = true;
                 float r[8];
                 load8(rt + c0, r);
 #pragma unroll
@@ -95,6 +98,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
             const bool second = c0 >= apart;
             const int i0 = second ? c0 - apart : c0;  // the lane's first pair
             if (i0 < half) {
+                rotated = true;
                 float r[16];
                 load8(rt + 2 * i0, r);
                 load8(rt + 2 * i0 + 8, r + 8);
@@ -136,13 +140,16 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
                 for (int i = 0; i < 8; ++i) x[u][i] = x[u][i] * inv * g[i];
             }
         }
-        float y[8];
+        float y[8];  // (an infinite partner times sin 0 would be NaN; choosing y itself: 35 -> 42 us)
         if (a.src.rope_layout == 1) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = x[u][i] * cs[i] + x[u][i ^ 1] * sn[i];
+            for (int i = 0; i < 8; ++i) y[i] = x[u][i] * cs[i] + (rotated ? x[u][i ^ 1] : 0.0f) * sn[i];
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = x[u][i] * cs[i] + __shfl(x[u][i], lane + hop, WAVE) * sn[i];
+            for (int i = 0; i < 8; ++i) {
+                const float other = __shfl(x[u][i], lane + hop, WAVE);
+                y[i] = x[u][i] * cs[i] + (rotated ? other : 0.0f) * sn[i];
+            }
         }
         if (slot >= slots) continue;
         if (is_q) {
@@ -201,7 +208,9 @@ void append_hd(hipStream_t s, AppendArgs a) {
     const int sets = (slots + W - 1) / W;
     const auto blocks = [&](int u) {
         a.items = (sets + u - 1) / u;
-        return unsigned((a.b.t * a.items + 3) / 4);
+        const int64_t n = (a.b.t * a.items + 3) / 4;
+        if (n >= MAX_BLOCKS) fail(E_CAPACITY, "kv_append: too many rows for one call");
+        return unsigned(n);
     };
     if (sets < 4 || a.b.t * sets <= 8192) {
         const unsigned n = blocks(1);

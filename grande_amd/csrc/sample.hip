@@ -485,17 +485,15 @@ __device__ Cut cut_in_bin(const uint64_t* room, int n, M& sm, uint64_t left, boo
         return Cut::at(sm.found);
     }
     if (tid == 0) sm.found = 0;
+    if (tid < n) sm.hist[tid] = masses ? w.mass(item_value(room[tid])) : 1;
     __syncthreads();
     const int e = tid / 4, lane4 = tid % 4;
     if (e < n) {
-        const uint64_t mine = room[e];
+        const uint64_t mine = room[e], own = sm.hist[e];
         uint64_t run = 0;
-        for (int j = lane4; j < n; j += 4) {
-            const uint64_t it = room[j];
-            if (it >= mine) run += masses ? w.mass(item_value(it)) : 1;
-        }
+#pragma unroll 4
+        for (int j = lane4; j < n; j += 4) run += room[j] >= mine ? sm.hist[j] : 0;
         run = quad_sum_u64(run);
-        const uint64_t own = masses ? w.mass(item_value(mine)) : 1;
         if (lane4 == 0 && own && run >= left && run - own < left) sm.found = mine;
     }
     __syncthreads();
@@ -807,7 +805,35 @@ __device__ int make_list(const Settings& s, const Scale& sc, Shared& sm, uint64_
     }
 }
 
-// Rows whose kept tokens do not fit a list, between the kernels.
+// The exact cuts and the draw over a whole row whose kept tokens do not fit a
+// list.
+template <typename T>
+__device__ void finish_row(const Row<T>& row, const Settings& s, float u, const Scale& sc, Shared& sm,
+                           const Result& out) {
+    auto items = [&](auto&& f) {
+        row.turns([&](const float* z, int i) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                if (z[c] > -INFINITY) f(z[c], i + c);
+        });
+    };
+    const Cut cut = cuts(items, row.n, s, sc, 0, sm, sm.item, CAP, out.w);
+    auto kept = [&](float z, int i) -> uint64_t {
+        if (!cut.keeps(z, i)) return 0;
+        const double x = out.w(z);
+        return x >= s.least ? Weigh::fixed(x) : 0;
+    };
+    row.sums(sm.item, kept);
+    __syncthreads();
+    const int ns = row.segments();
+    uint64_t own = 0;
+    for (int i = threadIdx.x; i < ns; i += NT) own += sm.item[i];
+    const uint64_t total = block_sum(own, sm), target = goal(u, total);
+    pick<false>(sm.item, ns, target, sm);
+    draw_in(row, int(sm.bin) * SEG, target - sm.before, total, out, kept);
+}
+
+// Long rows whose kept tokens do not fit a list, between the kernels.
 enum Step : uint32_t { DONE = 0, TO_CUT, TO_DRAW, TO_FINISH };
 struct Pending {
     uint64_t left;       // TO_CUT: the row's mass; TO_DRAW: what top_p takes from bin `bin`
@@ -817,7 +843,6 @@ struct Pending {
     uint32_t arrived[2];
     uint32_t edges;      // logits of the bin
 };
-__device__ inline Pending to_finish(float max) { return Pending{0, max, TO_FINISH, 0, {0, 0}, 0}; }
 // What sample_stats leaves of a long row's 2,048 logits.
 struct Chunk {
     float max;
@@ -842,7 +867,7 @@ struct Workspace {
 
 // Rows of at most SHORT logits: one workgroup a row.
 template <typename T>
-__global__ __launch_bounds__(NT) void sample_short(SampleArgs a, Workspace ws) {
+__global__ __launch_bounds__(NT) void sample_short(SampleArgs a) {
     __shared__ Shared sm;
     __shared__ __attribute__((aligned(16))) float groups[SHORT / GROUP];
     const int64_t r = blockIdx.x;
@@ -850,10 +875,7 @@ __global__ __launch_bounds__(NT) void sample_short(SampleArgs a, Workspace ws) {
     const Row<T> row(static_cast<const T*>(a.logits) + r * a.ld, a.vocab);
     const Settings s = settings_of(a, r);
     const float u = a.u[r];
-    if (tid == 0) {
-        sm.kmax = 0, sm.kfirst = 0xffffffffu;
-        ws.pending[r].step = DONE;
-    }
+    if (tid == 0) sm.kmax = 0, sm.kfirst = 0xffffffffu;
     float zmax = -INFINITY;
     uint32_t first = 0xffffffffu;
     row.turns([&](const float* z, int i) {
@@ -883,29 +905,26 @@ __global__ __launch_bounds__(NT) void sample_short(SampleArgs a, Workspace ws) {
         if (tid == 0) out.certain(int(sm.kfirst));
         return;
     }
-    if (s.p < 1.0f && s.k == 0 && s.least == 0.0) {  // its masses by bins settle it in the fewest passes
-        if (tid == 0) ws.pending[r] = to_finish(top);
-        return;
-    }
     auto mass = [&](float z, int) { return out.w.mass(z); };
-    uint64_t total = 0;
-    if (s.need_sum()) {
-        row.sums(sm.item, mass);
-        __syncthreads();
-        total = block_sum(tid < row.segments() ? sm.item[tid] : 0, sm);
-        if (s.p >= 1.0f) {  // no filter
-            const uint64_t target = goal(u, total);
-            pick<false>(sm.item, row.segments(), target, sm);
-            draw_in(row, int(sm.bin) * SEG, target - sm.before, total, out, mass);
-            return;
-        }
-    }
     const Scale sc(top, s.t);
-    const int n = make_list(s, sc, sm, total, row, groups, -INFINITY, 0, out.w);
-    if (n >= 0)
-        finish_list(n, s, u, total, sc, sm, out);
-    else if (tid == 0)
-        ws.pending[r] = to_finish(top);
+    int n = -1;
+    if (s.p >= 1.0f || s.k > 0 || s.least > 0.0) {  // (top_p alone: its masses by bins settle it in the fewest passes)
+        uint64_t total = 0;
+        if (s.need_sum()) {
+            row.sums(sm.item, mass);
+            __syncthreads();
+            total = block_sum(tid < row.segments() ? sm.item[tid] : 0, sm);
+            if (s.p >= 1.0f) {  // no filter
+                const uint64_t target = goal(u, total);
+                pick<false>(sm.item, row.segments(), target, sm);
+                draw_in(row, int(sm.bin) * SEG, target - sm.before, total, out, mass);
+                return;
+            }
+        }
+        n = make_list(s, sc, sm, total, row, groups, -INFINITY, 0, out.w);
+        if (n >= 0) finish_list(n, s, u, total, sc, sm, out);
+    }
+    if (n < 0) finish_row(row, s, u, sc, sm, out);
 }
 
 template <typename T, int VEC>
@@ -1039,42 +1058,20 @@ __global__ __launch_bounds__(NT) void sample_long(SampleArgs a, Workspace ws) {
         return;
     }
     if (tid == 0)
-        ws.pending[r] = s.k ? to_finish(top) : Pending{total, top, s.p < 1.0f ? TO_CUT : TO_DRAW, BINS, {0, 0}, 0};
+        ws.pending[r] = Pending{total, top, s.k ? TO_FINISH : s.p < 1.0f ? TO_CUT : TO_DRAW, BINS, {0, 0}, 0};
 }
 
-// The exact cuts and the draw over a whole row.
+// Long rows TO_FINISH (in sample_long their pass's registers slowed the lists
+// of the others: 256 rows of 128,257 132 -> 135 us).
 template <typename T>
 __global__ __launch_bounds__(NT) void sample_row(SampleArgs a, Workspace ws) {
     const int64_t r = blockIdx.x;
-    if (ws.pending[r].step != TO_FINISH) return;
+    const Pending& pd = ws.pending[r];
+    if (pd.step != TO_FINISH) return;
     __shared__ Shared sm;
-    const int tid = int(threadIdx.x);
-    const float top = ws.pending[r].max;
     const Settings s = settings_of(a, r);
     const Row<T> row(static_cast<const T*>(a.logits) + r * a.ld, a.vocab);
-    const Result out(a, r, top, s);
-    const Scale sc(top, s.t);
-    auto items = [&](auto&& f) {
-        row.turns([&](const float* z, int i) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-                if (z[c] > -INFINITY) f(z[c], i + c);
-        });
-    };
-    const Cut cut = cuts(items, row.n, s, sc, 0, sm, sm.item, CAP, out.w);
-    auto kept = [&](float z, int i) -> uint64_t {
-        if (!cut.keeps(z, i)) return 0;
-        const double x = out.w(z);
-        return x >= s.least ? Weigh::fixed(x) : 0;
-    };
-    row.sums(sm.item, kept);
-    __syncthreads();
-    const int ns = row.segments();
-    uint64_t own = 0;
-    for (int i = tid; i < ns; i += NT) own += sm.item[i];
-    const uint64_t total = block_sum(own, sm), target = goal(a.u[r], total);
-    pick<false>(sm.item, ns, target, sm);
-    draw_in(row, int(sm.bin) * SEG, target - sm.before, total, out, kept);
+    finish_row(row, s, a.u[r], Scale(pd.max, s.t), sm, Result(a, r, pd.max, s));
 }
 
 // Whether this workgroup is the last of its row's to arrive; what the others
@@ -1235,7 +1232,7 @@ __global__ __launch_bounds__(NT, 8) void sample_draw(SampleArgs a, Workspace ws)
 void check(const SampleArgs& a) {
     if (a.dtype != ELEM_F32 && a.dtype != ELEM_F16 && a.dtype != ELEM_BF16)
         fail(E_INVALID, "sample: logits must be f32, f16 or bf16");
-    if (a.rows <= 0 || a.rows > (1 << 24)) fail(E_INVALID, "sample: rows must be 1 to 2^24");
+    if (a.rows <= 0 || a.rows > (1 << 21)) fail(E_INVALID, "sample: rows must be 1 to 2^21");
     if (a.vocab <= 0 || a.vocab > (1 << IDX_BITS)) fail(E_INVALID, "sample: vocab must be 1 to 2^20");
 }
 
@@ -1258,25 +1255,22 @@ int64_t parts_of(int64_t vocab) { return (vocab + PART - 1) / PART; }
 template <typename T>
 void launch(hipStream_t s, const SampleArgs& a, void* workspace) {
     const dim3 grid{unsigned(a.rows)}, block{NT};
+    if (a.vocab <= SHORT) {
+        sample_short<T><<<grid, block, 0, s>>>(a);
+        OMG_HIP(hipGetLastError());
+        return;
+    }
     Workspace ws{};
     ws.nchunk = chunks_of(a.vocab);
+    ws.nparts = parts_of(a.vocab);
     const int64_t n = a.rows * ws.nchunk;
     ws.pending = static_cast<Pending*>(workspace);
     ws.chunks = reinterpret_cast<Chunk*>(ws.pending + a.rows);
     ws.groups = reinterpret_cast<float*>(ws.chunks + n);
-    ws.nparts = parts_of(a.vocab);
     ws.hist = reinterpret_cast<uint64_t*>(ws.groups + n * (CHUNK / GROUP));
     ws.segs = ws.hist + a.rows * ws.nparts * BINS;
     ws.edge = ws.segs + n * (CHUNK / SEG);
-    if (a.vocab <= SHORT) {
-        sample_short<T><<<grid, block, 0, s>>>(a, ws);
-        OMG_HIP(hipGetLastError());
-        if (a.top_p || (a.vocab > CAP && (a.top_k || a.min_p))) {
-            sample_row<T><<<grid, block, 0, s>>>(a, ws);
-            OMG_HIP(hipGetLastError());
-        }
-        return;
-    }
+    if ((n + 3) / 4 >= MAX_BLOCKS) fail(E_CAPACITY, "sample: too many logits for one call");
     const dim3 wide{unsigned((n + 3) / 4)};
     constexpr int VEC = 16 / int(sizeof(T));
     if (reinterpret_cast<uintptr_t>(a.logits) % 16 == 0 && a.ld % VEC == 0)
@@ -1308,10 +1302,9 @@ int64_t sample_workspace(int64_t rows, int64_t vocab) {
     check(a);
     static_assert(sizeof(Pending) % 16 == 0 && sizeof(Chunk) % 16 == 0, "the workspace's arrays are aligned");
     const int64_t n = chunks_of(vocab);
-    return rows * int64_t(sizeof(Pending)) +
-           (n ? rows * (n * int64_t(sizeof(Chunk) + CHUNK / SEG * 8 + CHUNK / GROUP * 4) + parts_of(vocab) * BINS * 8 +
-                        EDGE * 8)
-              : 0);
+    if (n == 0) return 0;
+    return rows * (int64_t(sizeof(Pending)) + n * int64_t(sizeof(Chunk) + CHUNK / SEG * 8 + CHUNK / GROUP * 4) +
+                   parts_of(vocab) * BINS * 8 + EDGE * 8);
 }
 
 void launch_sample(hipStream_t s, const SampleArgs& a, void* workspace, size_t bytes) {

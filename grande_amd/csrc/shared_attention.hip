@@ -72,7 +72,6 @@ struct Args {
 
 typedef __attribute__((address_space(3))) void* lds_ptr;
 typedef short short4v __attribute__((ext_vector_type(4)));
-typedef short short8v __attribute__((ext_vector_type(8)));
 
 __device__ inline floatx16 mfma32(half8 a, half8 b, floatx16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
@@ -881,7 +880,7 @@ void check(const PagedKv& kv, const PagedBatch& b, int heads) {
     check_batch(b, kv, "attention_shared");
     if (heads <= 0 || heads > 4096 || heads % kv.kv_heads)
         fail(E_INVALID, "attention_shared: heads must be a multiple of kv_heads, at most 4096");
-    if (b.t * heads > INT_MAX / 2) fail(E_INVALID, "attention_shared: t * heads must stay below 2^30");
+    if (b.t * heads >= (1 << 26)) fail(E_INVALID, "attention_shared: t * heads must stay below 2^26");
 }
 
 int64_t part_bytes(const Plan& p, const PagedKv& kv, const PagedBatch& b, int heads) {
@@ -974,7 +973,7 @@ void launch_attention_shared(hipStream_t s, const PagedKv& kv, const PagedBatch&
     const int64_t nsplit = a.p.whole ? 1 : a.p.np + (a.p.fused ? a.p.os : 0);
     a.prefix_blocks = up(int64_t(a.p.ntile) * kv.kv_heads * nsplit, 8);
     const int64_t blocks = a.prefix_blocks + (a.p.fused ? 0 : a.p.own_tiles * kv.kv_heads * a.p.os);
-    if (blocks > INT_MAX) fail(E_CAPACITY, "attention_shared: too many work items");
+    if (blocks >= MAX_BLOCKS) fail(E_CAPACITY, "attention_shared: too many work items");
     kv.dtype == ELEM_F16 ? launch_t<half_t>(s, a, unsigned(blocks)) : launch_t<bf16_t>(s, a, unsigned(blocks));
 }
 

@@ -392,7 +392,7 @@ int omg_dev_kv_append(const omg_paged_kv *kv, const omg_paged_batch *b, const om
                       int64_t ldq, void *stream);
 
 /* Attention of the batch's token rows (`heads` query heads, heads a multiple
- * of kv_heads; row i, head h at q + i * ldq + h * head_dim) over the cache:
+ * of kv_heads, t * heads below 2^26; row i, head h at q + i * ldq + h * head_dim) over the cache:
  * a token sees the whole shared prefix and its sequence's own rows up to its
  * own, of these (window > 0) the ones less than `window` positions back.
  *   out = softmax(scale * q . k) v, lse = log(sum exp(scale * q . k))
@@ -434,8 +434,9 @@ int omg_dev_attention_shared(const omg_paged_kv *kv, const omg_paged_batch *b, i
  * to 2^-42 (the whole mass of a row of more than 32,768 tokens: sums of w in
  * 64 bits), so a token under 2^-43 of the largest is not drawn, and the same
  * call gives the same tokens.
- * vocab up to 2^20.  workspace: omg_dev_sample_workspace bytes (negative: an
- * OMG_E_* status), 16-byte aligned, this call's own until it has run. */
+ * vocab up to 2^20, rows to 2^21.  workspace: omg_dev_sample_workspace bytes (negative: an
+ * OMG_E_* status; 0 for rows of up to 32,768 tokens), 16-byte aligned, this
+ * call's own until it has run. */
 int64_t omg_dev_sample_workspace(int64_t rows, int64_t vocab);
 typedef struct {
     int dtype;

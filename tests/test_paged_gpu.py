@@ -126,6 +126,37 @@ def test_no_rotation_copies_values_of_the_same_type():
     run_append(rng, [40, 1], [0, 3], 2, 2, 64, 16, "bf16", "bf16", 0, 0, False)
 
 
+@pytest.mark.parametrize("layout", [g.ROPE_HALF, g.ROPE_INTERLEAVED, g.ROPE_HEAD_HALF])
+@pytest.mark.parametrize("dims", [0, 32])
+def test_infinities_outside_the_rotation_stay(dims, layout):
+    """Elements that no pair holds keep their bits (infinities, NaN beside
+    them) and do not reach the rotated ones."""
+    rng = np.random.default_rng(12)
+    pool = Pool(rng, [5, 9], 0, 2, 128, 16, "f16")
+    x = torch.from_numpy(rng.standard_normal((2, 6, 128)).astype(np.float32)).half().cuda()
+    pairs = {g.ROPE_HALF: range(dims), g.ROPE_INTERLEAVED: range(dims),
+             g.ROPE_HEAD_HALF: [*range(dims // 2), *range(64, 64 + dims // 2)]}[layout]
+    out = torch.ones(128, dtype=torch.bool)
+    out[list(pairs)] = False
+    junk = torch.tensor([float("inf"), -float("inf"), float("nan"), 2.0], dtype=torch.float16).repeat(32).cuda()
+    y = torch.where(out.cuda(), junk, x)
+    table = rope_table(16, dims).cuda() if dims else None
+    q = [torch.zeros(2, 2, 128, dtype=torch.float16, device="cuda") for _ in range(2)]
+    for src, to in zip((x, y), q):
+        at = src.data_ptr()
+        pool.kv().append(pool.batch(2), g.KvSource(g.ELEM_F16, 2, at, at + 512, at + 1024, 768,
+                                                   rope=table.data_ptr() if dims else None, rope_rows=16 if dims else 0,
+                                                   rope_dims=dims, rope_layout=layout), to.data_ptr(), 256)
+    torch.cuda.synchronize()
+    assert torch.equal(q[0][..., ~out], q[1][..., ~out])
+    row = torch.stack([pool.k[int(pool.table_host[s, 0]), :, n - 1] for s, n in enumerate([5, 9])])
+    for got in (q[1], row):
+        bits = got[..., out].contiguous().view(torch.int16)
+        exp = y[:, :2, out].contiguous().view(torch.int16)
+        nan = torch.isnan(y[:, :2, out])
+        assert torch.equal(bits[~nan], exp[~nan]) and bool(torch.isnan(got[..., out][nan]).all())
+
+
 def test_rows_outside_the_pool_and_the_table_are_left_out():
     """A page id outside the pool, a row past max_pages and a length too
     short for the tokens: nothing is written for them, the others arrive."""

@@ -124,3 +124,17 @@ def test_sample_workspace_is_refused_or_sized():
     for rows, vocab in ((0, 10), (3, 0), (3, (1 << 20) + 1)):
         with pytest.raises(g.OmgError):
             g.sample_workspace(rows, vocab)
+
+
+def test_calls_past_a_launchs_size_are_refused():
+    big = dict(tokens=1 << 24, start_ptr=P)
+    with pytest.raises(g.OmgError, match="too many rows"):
+        kv().append(batch(**big), source(heads=4096, ld=4096 * 64, ldkv=4096 * 64), P, 4096 * 64)
+    with pytest.raises(g.OmgError, match="t \\* heads"):
+        attend(b=batch(**big))
+    with pytest.raises(g.OmgError, match="too many work items"):
+        attend(kv(kv_heads=16), batch(nseq=1 << 20, tokens=1 << 20, start_ptr=P), heads=32, ldq=2048, ldo=2048)
+    with pytest.raises(g.OmgError, match="rows must"):
+        g.sample_workspace((1 << 21) + 1, 100)
+    with pytest.raises(g.OmgError, match="too many logits"):
+        g.sample(P, g.ELEM_F16, 1 << 21, 1 << 20, 1 << 20, P, P, workspace=P, workspace_bytes=1 << 60)
