@@ -193,12 +193,24 @@ struct Shared : Common {
     uint64_t hist[BINS];
     uint64_t edge[PAIRS]; // items of one bin
 };
+// The wide kernels' lists of logits that pass a threshold, one a wave.
+struct Passed {
+    float z[NWAVE][5 * WAVE];
+    uint16_t at[NWAVE][5 * WAVE];  // in the part
+};
 struct BinsShared : Common {
     uint64_t hist[BINS];
+    Passed list;
 };
 struct DrawShared : Common {
-    uint64_t item[(1 << IDX_BITS) / SEG];  // the masses of the row's segments
-    uint64_t hist[BINS];
+    union {
+        struct {
+            uint64_t item[(1 << IDX_BITS) / SEG];  // the masses of the row's segments
+            uint64_t hist[BINS];
+        };
+        Passed list;
+    };
+    uint64_t seg[PART / SEG];  // of this part's
     uint64_t edge[EDGE];
 };
 __device__ inline int wave_id() { return __builtin_amdgcn_readfirstlane(int(threadIdx.x) / WAVE); }
@@ -299,6 +311,11 @@ struct Scale {
         const float nats = logf(2.0f * float(n) / ((1.0f - p) * mass));
         const float x = nats * t * per + 2.0f;
         return x < float(BINS - 1) && max < INFINITY ? int(x) : BINS - 1;  // (infinities lie in the last)
+    }
+    // The bins that min_p can keep, and one to spare.
+    __device__ int reach_min(double least, float t) const {
+        const float far = float(-log(least) * double(t)) * per + 1.0f;
+        return far < float(BINS - 2) ? int(far) + 1 : BINS - 1;
     }
     // A logit below all that lie in bins 0 .. last, however the bins rounded.
     __device__ float under(int last) const {
@@ -428,13 +445,13 @@ __device__ inline void draw_in(const Row<T>& row, int first, uint64_t target, ui
 // The item at which the running share, over the items from the first on,
 // first reaches `target` (>= 1); 0 if it never does, or an item below all
 // that do.  items(f) calls f(z, i) for the thread's items; masses: an item's
-// share is its mass, else one.  key: of all items, where it is the same.
+// share is its mass, else one.
 template <typename S, typename M>
-__device__ uint64_t find_cut(S&& items, M& sm, uint64_t target, bool masses, const Weigh& w, uint32_t key = 0) {
-    uint64_t prefix = key, before = 0;
-    int shift = key ? IDX_BITS : 52;
+__device__ uint64_t find_cut(S&& items, M& sm, uint64_t target, bool masses, const Weigh& w) {
+    uint64_t prefix = 0, before = 0;
+    int shift = 52;
 #pragma unroll 1
-    for (int level = key ? 3 : 0; level < 5; ++level) {
+    for (int level = 0; level < 5; ++level) {
         const int bits = level < 2 ? 11 : 10;
         shift -= bits;
         clear(sm.hist, 1 << bits);
@@ -453,46 +470,63 @@ __device__ uint64_t find_cut(S&& items, M& sm, uint64_t target, bool masses, con
 }
 
 // The cut within one bin: room[0 .. n) are its items, `left` the share that
-// is taken from them (reached among them).  They are compared pair by pair;
-// half-precision logits are equal by the hundred, and where they are many
-// the digits decide.
+// is taken from them (reached among them).  Up to PAIRS items are compared
+// pair by pair; of more, digits from the first that differs on leave as few.
 template <typename M>
 __device__ Cut cut_in_bin(const uint64_t* room, int n, M& sm, uint64_t left, bool masses, const Weigh& w) {
     const int tid = int(threadIdx.x);
+    uint64_t* mass = sm.hist;
+    const auto share = [&](uint64_t it) { return masses ? w.mass(item_value(it)) : 1; };
     __syncthreads();
     if (n > PAIRS) {
-        auto some = [&](auto&& f) {
-#pragma unroll 1
-            for (int i = tid; i < n; i += NT) f(item_value(room[i]), item_index(room[i]));
-        };
-        if (tid == 0) sm.kmax = 0, sm.kfirst = ~0u;
+        if (tid == 0) sm.found = 0, sm.total = ~uint64_t(0);
         __syncthreads();
-        uint32_t most = 0, least = ~0u;
+        uint64_t most = 0, least = ~uint64_t(0);
         for (int i = tid; i < n; i += NT) {
-            const uint32_t k = uint32_t(room[i] >> IDX_BITS);
-            most = most > k ? most : k, least = least < k ? least : k;
+            const uint64_t it = room[i];
+            most = most > it ? most : it, least = least < it ? least : it;
         }
-        if (most) atomicMax(&sm.kmax, most), atomicMin(&sm.kfirst, least);
+        if (most) {
+            atomicMax(reinterpret_cast<unsigned long long*>(&sm.found), static_cast<unsigned long long>(most));
+            atomicMin(reinterpret_cast<unsigned long long*>(&sm.total), static_cast<unsigned long long>(least));
+        }
         __syncthreads();
-        const uint64_t edge = find_cut(some, sm, left, masses, w, sm.kmax == sm.kfirst ? sm.kmax : 0);
-        // (the edge may lie below the bin: the last item of the bin above it)
-        if (tid == 0) sm.found = ~uint64_t(0);
-        __syncthreads();
-        for (int i = tid; i < n; i += NT)
-            if (room[i] >= edge)
-                atomicMin(reinterpret_cast<unsigned long long*>(&sm.found), static_cast<unsigned long long>(room[i]));
-        __syncthreads();
-        return Cut::at(sm.found);
+        int shift = 64 - __builtin_clzll(sm.found ^ sm.total);  // (items differ)
+        uint64_t prefix = sm.found >> shift;
+        uint64_t* few = sm.hist + BINS / 2;
+        int count;
+        do {
+            const int bits = shift < 11 ? shift : 11;
+            shift -= bits;
+            clear(sm.hist, BINS);
+            if (tid == 0) sm.count = 0;
+            for (int i = tid; i < n; i += NT) {
+                const uint64_t it = room[i], v = it >> (shift + bits) == prefix ? share(it) : 0;
+                if (v) add(&sm.hist[it >> shift & ((1u << bits) - 1)], v);
+            }
+            pick<true>(sm.hist, 1 << bits, left, sm);
+            prefix = prefix << bits | sm.bin;
+            left -= sm.before;
+            for (int i = tid; i < n; i += NT) {
+                const uint64_t it = room[i];
+                if (it >> shift != prefix) continue;
+                const uint32_t at = atomicAdd(&sm.count, 1u);
+                if (at < PAIRS) few[at] = it;
+            }
+            __syncthreads();
+            count = int(sm.count);
+        } while (count > PAIRS);
+        room = few, n = count;
     }
     if (tid == 0) sm.found = 0;
-    if (tid < n) sm.hist[tid] = masses ? w.mass(item_value(room[tid])) : 1;
+    if (tid < n) mass[tid] = share(room[tid]);
     __syncthreads();
     const int e = tid / 4, lane4 = tid % 4;
     if (e < n) {
-        const uint64_t mine = room[e], own = sm.hist[e];
+        const uint64_t mine = room[e], own = mass[e];
         uint64_t run = 0;
 #pragma unroll 4
-        for (int j = lane4; j < n; j += 4) run += room[j] >= mine ? sm.hist[j] : 0;
+        for (int j = lane4; j < n; j += 4) run += room[j] >= mine ? mass[j] : 0;
         run = quad_sum_u64(run);
         if (lane4 == 0 && own && run >= left && run - own < left) sm.found = mine;
     }
@@ -788,9 +822,7 @@ __device__ int make_list(const Settings& s, const Scale& sc, Shared& sm, uint64_
                 if (sm.found > PAIRS) return -1;  // (the wide kernels are no slower)
             }
         } else {
-            // z >= max + T log(min_p), and a bin to spare
-            const float far = float(-log(s.least) * double(s.t)) * sc.per + 1.0f;
-            last = far < float(BINS - 2) ? int(far) + 1 : BINS - 1;
+            last = sc.reach_min(s.least, s.t);
         }
         if (last == BINS - 1) last = sc.whole ? BINS - 2 : -1;  // (all that have a mass)
         const bool all = last < 0;
@@ -1104,6 +1136,40 @@ __device__ inline Row<T> part_of(const Row<T>& row) {
     return Row<T>(row.p + first, row.n - first < PART ? row.n - first : PART);
 }
 
+// f(z, i, on) for the part's logits from bin `last`'s end up, 64 a wave at a
+// time (on: the lane has one).  Few of a row's logits reach a cut, and some
+// lane of a wave has one nearly always: without the lists each took the time
+// of all, 8.5 us of exp for 16 a thread.
+template <typename T, typename F>
+__device__ inline void passing(const Row<T>& part, const Scale& sc, int last, Passed& list, F&& f) {
+    const float low = last < BINS - 1 ? fmaxf(sc.under(last), -3.4028235e38f) : -3.4028235e38f;
+    float* lz = list.z[wave_id()];
+    uint16_t* at = list.at[wave_id()];
+    const int lane = int(threadIdx.x) % WAVE;
+    int have = 0;
+    const auto batch = [&](int from, bool on) {
+        asm volatile("" ::: "memory");  // (a wave's LDS accesses are in order)
+        f(on ? lz[from + lane] : -INFINITY, on ? int(at[from + lane]) : 0, on);
+        asm volatile("" ::: "memory");
+    };
+    part.turns([&](const float* z, int i) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const bool pass = z[c] >= low;
+            const uint64_t all = __ballot(pass);
+            if (!all) continue;
+            if (pass) {
+                const int to = have + int(__builtin_amdgcn_mbcnt_hi(uint32_t(all >> 32),
+                                                                   __builtin_amdgcn_mbcnt_lo(uint32_t(all), 0)));
+                lz[to] = z[c], at[to] = uint16_t(i + c);
+            }
+            have += __popcll(all);
+        }
+        for (; have >= WAVE; have -= WAVE) batch(have - WAVE, true);
+    });
+    if (have) batch(0, lane < have);
+}
+
 // The masses of rows TO_CUT by bins; the last workgroup of a row finds
 // top_p's cut.
 template <typename T>
@@ -1120,14 +1186,10 @@ __global__ __launch_bounds__(NT, 8) void sample_bins(SampleArgs a, Workspace ws)
     const uint64_t total = pd.left;
     const int reach = s.p > 0.0f ? sc.reach(s.p, float(double(total) / ONE), row.n, s.t) : BINS - 1;
     clear(sm.hist, BINS);
-    part_of(row).turns([&](const float* z, int) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            const int b = sc.bin(z[c]);
-            if (b > reach) continue;
-            const uint64_t m = w.mass(z[c]);
-            if (m) add(&sm.hist[b], m);
-        }
+    passing(part_of(row), sc, reach, sm.list, [&](float z, int, bool on) {
+        const int b = sc.bin(z);
+        const uint64_t m = on && b <= reach ? w.mass(z) : 0;
+        if (m) add(&sm.hist[b], m);
     });
     __syncthreads();
     uint64_t* hist = ws.hist + r * ws.nparts * BINS;
@@ -1164,20 +1226,29 @@ __global__ __launch_bounds__(NT, 8) void sample_draw(SampleArgs a, Workspace ws)
     uint64_t* segs = ws.segs + r * ws.nchunk * (CHUNK / SEG);
     uint64_t* edge = ws.edge + r * EDGE;
     const Row<T> part = part_of(row);
-    // (a logit in a bin before stays, if min_p lets it)
-    auto before = [&](float z, int) -> uint64_t {
-        if (sc.bin(z) >= bin) return 0;
-        const double x = out.w(z);
-        return x >= s.least ? Weigh::fixed(x) : 0;
-    };
     if (tid == 0) sm.count = 0;
+    if (tid < PART / SEG) sm.seg[tid] = 0;
     __syncthreads();
-    part.sums(sm.item, [&](float z, int i) {
-        if (sc.bin(z) == bin && z > -INFINITY) {
+    // (a logit in a bin before stays, if min_p lets it)
+    const int last = s.least > 0.0 ? sc.reach_min(s.least, s.t) : BINS;
+    passing(part, sc, bin < last ? bin : last, sm.list, [&](float z, int i, bool on) {
+        const int b = on ? sc.bin(z) : BINS;
+        if (b == bin && on) {
             const uint32_t at = atomicAdd(&sm.count, 1u);
             if (at < EDGE) sm.edge[at] = item_of(z, first + i);
         }
-        return before(z, i);
+        uint64_t m = 0;
+        if (b < bin) {
+            const double x = out.w(z);
+            m = x >= s.least ? Weigh::fixed(x) : 0;
+        }
+        const int seg = i / SEG, one = __builtin_amdgcn_readfirstlane(seg);
+        if (__all(seg == one)) {
+            m = wave_scan_u64(m);
+            if (tid % WAVE == WAVE - 1 && m) add(&sm.seg[one], m);
+        } else if (m) {
+            add(&sm.seg[seg], m);
+        }
     });
     __syncthreads();
     const uint32_t here = sm.count;
@@ -1186,7 +1257,7 @@ __global__ __launch_bounds__(NT, 8) void sample_draw(SampleArgs a, Workspace ws)
     for (uint32_t i = tid; i < here && sm.bin + i < EDGE; i += NT)
         store_shared(edge + sm.bin + i, sm.edge[i]);
     if (tid < part.segments())
-        store_shared(segs + first / SEG + tid, sm.item[tid]);
+        store_shared(segs + first / SEG + tid, sm.seg[tid]);
     if (!last_of(&pd.arrived[1], sm)) return;
     if (tid == 0) sm.kfirst = __hip_atomic_load(&pd.edges, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     for (int i = tid; i < ns; i += NT) sm.item[i] = load_shared(segs + i);
