@@ -45,7 +45,7 @@ namespace {
 
 constexpr int NT = 1024;          // threads of a row's workgroup
 constexpr int NWAVE = NT / WAVE;
-constexpr int CHUNK = 2048;       // logits of a wave of sample_stats
+constexpr int CHUNK = 1024;       // logits of a wave of sample_stats
 constexpr int GROUP = 16;         // logits of a group maximum
 constexpr int SHORT = 32 * NT;    // logits of a row that one workgroup takes alone
 constexpr int CAP = 8192;         // items of the list
@@ -104,20 +104,17 @@ struct Weigh {
         constexpr double c2 = L * L / 2, c3 = c2 * L / 3, c4 = c3 * L / 4, c5 = c4 * L / 5, c6 = c5 * L / 6,
                          c7 = c6 * L / 7, c8 = c7 * L / 8, c9 = c8 * L / 9, c10 = c9 * L / 10, c11 = c10 * L / 11;
         double p = c11;
-        p = fma(p, f, c10);
-        p = fma(p, f, c9);
-        p = fma(p, f, c8);
-        p = fma(p, f, c7);
-        p = fma(p, f, c6);
-        p = fma(p, f, c5);
-        p = fma(p, f, c4);
-        p = fma(p, f, c3);
-        p = fma(p, f, c2);
-        p = fma(p, f, L);
-        p = fma(p, f, 1.0);
+        step(p, f, c10), step(p, f, c9), step(p, f, c8), step(p, f, c7), step(p, f, c6), step(p, f, c5);
+        step(p, f, c4), step(p, f, c3), step(p, f, c2), step(p, f, L), step(p, f, 1.0);
         const uint64_t b = __builtin_bit_cast(uint64_t, p);
         const uint32_t n = uint32_t(__builtin_bit_cast(uint64_t, shifted));  // (its low bits: n)
         return __builtin_bit_cast(double, uint64_t(uint32_t(b >> 32) + (n << 20)) << 32 | uint32_t(b));
+    }
+    // p = p f + c, c in scalar registers (the compiler's form, which adds onto
+    // its third operand, first moves each c into vector registers: 22 of 59
+    // instructions a logit).
+    static __device__ void step(double& p, double f, double c) {
+        asm("v_fma_f64 %0, %0, %1, %2" : "+v"(p) : "v"(f), "s"(c));
     }
     __device__ uint64_t mass(float z) const { return fixed((*this)(z)); }
     // (2^52 + v rounds v to a whole number in its low bits)
