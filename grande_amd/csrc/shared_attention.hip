@@ -29,9 +29,9 @@
 // K and V tiles come by buffer loads to LDS, 16 bytes a lane, from a
 // resource that ends with the last valid row of the page (rows behind it
 // and pages outside the pool arrive as zeros, so that nothing they hold
-// meets a probability of zero).  The 16-byte chunks of row r are XORed with
-// r (K: the 16 rows of an operand read on distinct banks) and with 2 r (V:
-// the 4 rows x 32 bytes of a transposing read).
+// meets a probability of zero).  The 16-byte chunks of a row are XORed with
+// bits of its number, so that half a wave's reads fall on distinct banks: K's
+// 16 rows x 16 bytes, V's 4 rows x 64 bytes or 8 x 32.
 #include <algorithm>
 #include <atomic>
 #include <climits>
@@ -110,8 +110,12 @@ struct Core {
     acc o[NC];
     float m, l;  // running maximum of the raw scores; the lane's share of sum p
 
-    static __device__ int swz_k(int row) { return CH >= 16 ? row & 15 : row & 7; }
-    static __device__ int swz_v(int row) { return CH >= 16 ? (row & 7) << 1 : (row & 3) << 1; }
+    // The chunks of row r are XORed with these (sums of r's bits, so that an
+    // address follows from others): 256 bytes are one turn over the banks.
+    static __device__ int swz_k(int row) { return CH >= 16 ? row & 15 : row >> 1 & 7; }
+    static __device__ int swz_v(int row) {
+        return CH < 16 ? (row & 3) << 1 : RW == 32 ? (row & 3) << 2 : (row & 7) << 1;
+    }
     static __device__ float row_max(float v) {
         if constexpr (RW == 32) {
             const uint32_t u = __builtin_bit_cast(uint32_t, v);
@@ -457,8 +461,8 @@ __device__ inline int imax(int a, int b) { return a > b ? a : b; }
 // A lane's query row.
 struct Row {
     bool valid;
-    int64_t tok;
-    int head, seq, own;  // own: its row in the sequence's cache rows
+    int at;        // tok * heads + head (one register: the tiles need all others)
+    int seq, own;  // own: its row in the sequence's cache rows
 };
 
 // The keys of a work item: prefix rows [pb, pe), own rows [ob, oe).
@@ -482,8 +486,9 @@ __device__ void seen_alone(const Args& a, const Keys& in, const Row& r, uint64_t
         const int i = __builtin_ctzll(rows);
         const auto of = [&](int v) { return __builtin_amdgcn_readlane(v, i); };
         const auto off = [&](float v) { return __builtin_bit_cast(float, of(__builtin_bit_cast(int, v))); };
-        const int64_t tok = of(int(r.tok));
-        const int head = of(r.head), seq = of(r.seq), own = of(r.own);
+        const int at = of(r.at), seq = of(r.seq), own = of(r.own);
+        const int64_t tok = at / a.x.heads;
+        const int head = at % a.x.heads;
         const float row_cm = off(cm), ref = row_cm == -INFINITY ? 0.0f : row_cm;
         float4 q[E], o[E];
         const auto load = [&](const void* p, int64_t at, float4* x) {
@@ -502,14 +507,14 @@ __device__ void seen_alone(const Args& a, const Keys& in, const Row& r, uint64_t
             for (int k = from; k < to; ++k) {
                 const int64_t page = table[imin(k >> a.page_shift, plast)];
                 if (page < 0 || page >= a.kv.npages) continue;
-                const int64_t at = page * a.kv.page_stride + (int64_t(in.g) * a.kv.page + (k & (a.kv.page - 1))) * D;
+                const int64_t key = page * a.kv.page_stride + (int64_t(in.g) * a.kv.page + (k & (a.kv.page - 1))) * D;
                 float4 x[E];
-                load(a.kv.k, at, x);
+                load(a.kv.k, key, x);
                 float s = 0.0f;
 #pragma unroll
                 for (int e = 0; e < E; ++e) s += x[e].x * q[e].x + x[e].y * q[e].y + x[e].z * q[e].z + x[e].w * q[e].w;
                 const float p = __builtin_amdgcn_exp2f(fmaf(wave_sum(s), a.c, -ref));
-                load(a.kv.v, at, x);
+                load(a.kv.v, key, x);
 #pragma unroll
                 for (int e = 0; e < E; ++e)
                     o[e].x += p * x[e].x, o[e].y += p * x[e].y, o[e].z += p * x[e].z, o[e].w += p * x[e].w;
@@ -518,7 +523,7 @@ __device__ void seen_alone(const Args& a, const Keys& in, const Row& r, uint64_t
         keys(a.b.prefix_table, (P - 1) >> a.page_shift, imax(in.pb, w > 0 ? P + own - w + 1 : 0), in.pe);
         keys(a.b.table + seq * a.b.table_ld, int(a.b.max_pages) - 1, imax(in.ob, w > 0 ? own - w + 1 : 0),
              imin(in.oe, own + 1));
-        const Sink<T> out{a, tok * a.x.heads + head, tok * a.x.ldo + int64_t(head) * D, slot};
+        const Sink<T> out{a, at, tok * a.x.ldo + int64_t(head) * D, slot};
         const float sum = off(l);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
@@ -534,7 +539,7 @@ __device__ inline void emit(const Args& a, Core<T, D, TILE>& core, const Keys& i
                             int64_t slot) {
     typedef Core<T, D, TILE> C;
     const float l = C::row_sum(core.l), cm = core.m == -INFINITY ? -INFINITY : core.m * a.c;
-    const Sink<T> out{a, r.tok * a.x.heads + r.head, r.tok * a.x.ldo + int64_t(r.head) * D, slot};
+    const Sink<T> out{a, r.at, r.at / a.x.heads * a.x.ldo + int64_t(r.at % a.x.heads) * D, slot};
     if (r.valid && lane < C::RW) out.stats(cm, l);
     float z[4] = {};  // (NaN where a sum is not finite)
 #pragma unroll
@@ -583,7 +588,7 @@ __device__ inline void emit_keys(const Args& a, Core<T, D, WAVES_KEYS>& core, co
         w[k] = x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x - cm);
         sum += w[k] * ml[64 + k * 16 + lane % 16];
     }
-    const Sink<T> out{a, r.tok * a.x.heads + r.head, r.tok * a.x.ldo + int64_t(r.head) * D, slot};
+    const Sink<T> out{a, r.at, r.at / a.x.heads * a.x.ldo + int64_t(r.at % a.x.heads) * D, slot};
     if (r.valid && wave == 0 && lane < 16) out.stats(cm, sum);
     float4 v[D / 64];  // quads wave * 4 + lane / 16 + 16 i
     float z = 0.0f;
@@ -626,18 +631,18 @@ __global__ __launch_bounds__(NW * 64, TILE == WAVES_KEYS && D == 512 ? 1 : D == 
         }
         return s0;
     };
-    auto place = [&](Row& r, int64_t s0, int64_t s1) {
+    auto place = [&](Row& r, int64_t tok, int64_t s0, int64_t s1) {
         r.seq = 0, r.own = 0;
         if (!r.valid) return;
         if (a.b.start) {
-            const int64_t s = seq_in(r.tok, s0, s1);
-            r.valid = s < a.b.nseq && r.tok >= a.b.start[0];
+            const int64_t s = seq_in(tok, s0, s1);
+            r.valid = s < a.b.nseq && tok >= a.b.start[0];
             if (!r.valid) return;
             r.seq = int(s);
-            r.own = a.b.lens[s] - int(a.b.start[s + 1] - r.tok);
+            r.own = a.b.lens[s] - int(a.b.start[s + 1] - tok);
         } else {
-            r.seq = int(r.tok);
-            r.own = a.b.lens[r.tok] - 1;
+            r.seq = int(tok);
+            r.own = a.b.lens[tok] - 1;
         }
     };
 
@@ -654,16 +659,18 @@ __global__ __launch_bounds__(NW * 64, TILE == WAVES_KEYS && D == 512 ? 1 : D == 
         const int split = uni(int(item / a.p.ntile % nsplit)), g = uni(int(item / a.p.ntile / nsplit));
         const int64_t rows = a.b.t * hpg, row0 = int64_t(tile) * M;
         const int64_t R = row0 + (TILE == WAVES_KEYS ? 0 : wave * C::RW) + lane % C::RW;
-        Row r{R < rows, R / hpg, int(g * hpg + R % hpg), 0, 0};
+        const int64_t tok = R / hpg;
+        const int head = int(g * hpg + R % hpg);
+        Row r{R < rows, int(tok * a.x.heads + head), 0, 0};
         const int64_t tok0 = row0 / hpg, tok1 = ((row0 + M < rows ? row0 + M : rows) - 1) / hpg;
         int64_t s0 = tok0, s1 = tok1;
         if (a.b.start) {
             s0 = count_le(a.b.start, a.b.nseq, tok0, lane);
             s1 = count_le(a.b.start, a.b.nseq, tok1, lane);
         }
-        place(r, s0, s1);
+        place(r, tok, s0, s1);
         C core;
-        core.init(r.valid ? static_cast<const T*>(a.x.q) + r.tok * a.x.ldq + int64_t(r.head) * D : nullptr, lane);
+        core.init(r.valid ? static_cast<const T*>(a.x.q) + tok * a.x.ldq + int64_t(head) * D : nullptr, lane);
         const Stream<T, D, TILE> st{a, g, wave, lane, smem};
         if (a.p.whole || split < a.p.np) {
             int kb = a.p.whole ? 0 : split * a.p.chunk_p, ke = a.p.whole ? P : imin(P, kb + a.p.chunk_p);
@@ -741,12 +748,13 @@ __global__ __launch_bounds__(NW * 64, TILE == WAVES_KEYS && D == 512 ? 1 : D == 
     }
     if (tile < 0 || tile * 16 >= (b1 - b0) * hpg) return;
     const int64_t R = tile * 16 + lane % 16;
-    Row r{R < (b1 - b0) * hpg, b0 + R / hpg, int(g * hpg + R % hpg), int(s), 0};
-    r.valid = r.valid && r.tok >= 0 && r.tok < a.b.t;
+    const int64_t tok = b0 + R / hpg;
+    const int head = int(g * hpg + R % hpg);
+    Row r{R < (b1 - b0) * hpg && tok >= 0 && tok < a.b.t, int(tok * a.x.heads + head), int(s), 0};
     const int len = a.b.lens[s];
-    r.own = len - int(b1 - r.tok);
+    r.own = len - int(b1 - tok);
     C core;
-    core.init(r.valid ? static_cast<const T*>(a.x.q) + r.tok * a.x.ldq + int64_t(r.head) * D : nullptr, lane);
+    core.init(r.valid ? static_cast<const T*>(a.x.q) + tok * a.x.ldq + int64_t(head) * D : nullptr, lane);
     // the keys that the tile's first and last tokens see
     const int64_t last = (tile * 16 + 15 < (b1 - b0) * hpg ? tile * 16 + 15 : (b1 - b0) * hpg - 1) / hpg;
     const int ra = len - int(b1 - b0 - tile * 16 / hpg), rb = len - int(b1 - b0 - last);
