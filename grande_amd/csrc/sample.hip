@@ -10,10 +10,10 @@
 //
 // Rows of up to 32,768 logits take one workgroup each (sample_short), which
 // reads them once from memory and again from its L2.  Longer rows are read
-// once by the whole chip (sample_stats: per 2,048 logits the maximum, its
+// once by the whole chip (sample_stats: per 1,024 logits the maximum, its
 // index and, where the row's filters need it, the sum of exp; per 16 the
-// maximum), then one workgroup a row finishes (sample_long).  Both look for a
-// threshold that few logits pass but all that can be kept do, from the
+// maximum), then one workgroup a row looks at these (sample_long).  Both look
+// for a threshold that few logits pass but all that can be kept do, from the
 // maxima of groups of 16: the k-th largest of these maxima has k logits at or
 // above it; min_p's threshold is its own; for top_p alone a guess is taken
 // and proved by the mass above it.  The logits above it are gathered into a
@@ -22,8 +22,8 @@
 // Where the kept tokens do not fit the list, the row's masses are summed by
 // bins of their distance from the maximum, which leaves one bin's logits to
 // order exactly, and the kept masses by segments in index order: by one
-// workgroup a row (sample_row), or, where a long row's top_p or min_p keeps
-// them, by the whole chip (sample_bins, sample_draw).
+// workgroup a row (finish_row: short rows, and top_k of long ones), or by the
+// whole chip (sample_bins, sample_draw: top_p and min_p of long rows).
 //
 // What bounds the kernels of one workgroup a row is its CU: 64 lanes a cycle
 // (150 lane instructions a nanosecond) and a microsecond for every trip to
@@ -32,6 +32,13 @@
 // pass, and their loops are rolled: a row of 25,000 held in registers, 32 a
 // thread, took 14.5 us for its maximum and 14 for a pass of exp, waiting for
 // instructions; this form takes 5.
+//
+// Measured: one row of 25,000 15.4 us (f32; top_k 40, top_p 0.95: seven steps
+// that wait for one another); 208 of them, each with its own filters, 56 us
+// (the rows whose kept tokens fit no list); 64 rows of 262,144 (bf16, top_p)
+// 104 us: stats 25 (37 vector instructions a logit, most of them exp's),
+// long 20, bins 26, draw 37 (the last rows' cuts, one workgroup each); 256
+// rows of 128,257 (f32, mixed filters) 111 us, of which stats 33 (3.9 TB/s).
 #include <algorithm>
 #include <string>
 
