@@ -1,6 +1,6 @@
 // Attention over a prefix that all sequences of a batch share and over each
 // sequence's own rows, both on pages of a K/V pool:
-//   out = sum_j p_j v_j / sum_j p_j,  p_j = 2^(c (s_j - m)),  s_j = q . k_j,
+//   out = sum_j p_j v_j / sum_j p_j,  p_j = 2^(c (s_j - m) + LIFT),  s_j = q . k_j,
 // c = scale log2(e), m a running maximum of s, over the keys j that the
 // query sees.  Partial results over ranges of keys are joined by
 // (m, l = sum p, O = sum p v): O and l times 2^(c (m - max m)).
@@ -61,6 +61,14 @@ namespace {
 
 enum Tile { WAVES_KEYS = 0, WAVES_16 = 1, WAVES_32 = 2 };
 
+// The running maximum may lag by LAG binary orders in p, and all p stand LIFT
+// orders higher: the largest lie in 2^7 .. 2^15, so that f16 holds p with all
+// its bits down to 2^-21 of the largest, and those below to 2^-32 of it
+// (without: 60,000 keys of 2^-20.5 each 4 % off).  A smaller lag takes the
+// outputs' products with 2^(c (m - m')) more often: 4 orders 530 us for the
+// questions below, 8 480.
+constexpr float LAG = 8.0f, LIFT = 7.0f;
+
 struct Plan {
     int tile;       // Tile of the prefix / fused items
     bool fused;     // own keys in the prefix items' tiles
@@ -81,7 +89,7 @@ struct Args {
     int64_t prefix_blocks;     // (a multiple of 8)
     float c;                   // scale log2(e)
     float* part_o;             // [slots][t * heads][head_dim], null: results go out
-    float2* part_ml;           // [slots][t * heads] (c m, l)
+    float2* part_ml;           // [slots][t * heads] (c m - LIFT, l)
 };
 
 typedef __attribute__((address_space(3))) void* lds_ptr;
@@ -236,9 +244,8 @@ struct Core {
 #pragma unroll
             for (int r = 0; r < SR; ++r) mt = fmaxf(mt, s[j][r]);
         mt = row_max(mt);
-        // The maximum moves where a row's scores pass it by more than 2^8 in
-        // p: p and l stay far from f16's and f32's ends either way.
-        if (__any((mt - m) * c > 8.0f || (m == -INFINITY && mt > m))) {
+        // The maximum moves where a row's scores pass it by more than LAG.
+        if (__any((mt - m) * c > LAG || (m == -INFINITY && mt > m))) {
             const float mn = fmaxf(m, mt);
             const float al = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * c);
             m = mn;
@@ -248,7 +255,7 @@ struct Core {
 #pragma unroll
                 for (int r = 0; r < SR; ++r) o[i][r] *= al;
         }
-        const float mc = m == -INFINITY ? 0.0f : m * c;
+        const float mc = m == -INFINITY ? 0.0f : m * c - LIFT;
         float sum = 0.0f;
 #pragma unroll
         for (int j = 0; j < NB; ++j)
@@ -552,7 +559,7 @@ template <typename T, int D, int TILE>
 __device__ inline void emit(const Args& a, Core<T, D, TILE>& core, const Keys& in, const Row& r, int lane,
                             int64_t slot) {
     typedef Core<T, D, TILE> C;
-    const float l = C::row_sum(core.l), cm = core.m == -INFINITY ? -INFINITY : core.m * a.c;
+    const float l = C::row_sum(core.l), cm = core.m == -INFINITY ? -INFINITY : core.m * a.c - LIFT;
     const Sink<T> out{a, r.at, r.at / a.x.heads * a.x.ldo + int64_t(r.at % a.x.heads) * D, slot};
     if (r.valid && lane < C::RW) out.stats(cm, l);
     float z[4] = {};  // (NaN where a sum is not finite)
@@ -589,7 +596,7 @@ __device__ inline void emit_keys(const Args& a, Core<T, D, WAVES_KEYS>& core, co
     for (int i = 0; i < C::NC; ++i)
         *reinterpret_cast<floatx4*>(mine + ((i * 4 + lane / 16) * 16 + lane % 16) * 4) = core.o[i];
     if (lane < 16) {
-        ml[wave * 16 + lane] = core.m == -INFINITY ? -INFINITY : core.m * a.c;
+        ml[wave * 16 + lane] = core.m == -INFINITY ? -INFINITY : core.m * a.c - LIFT;
         ml[64 + wave * 16 + lane] = l;
     }
     __syncthreads();

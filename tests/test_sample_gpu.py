@@ -241,3 +241,29 @@ def test_captured_draws_replay_on_new_logits(vocab):
         go()
         torch.cuda.synchronize()
         assert tok.tolist() == [plain(zh[r], uh[r], p=0.9)[0] for r in range(7)]
+
+
+def test_more_rows_than_a_grids_second_size():
+    """Rows past 65,535 of a long vocabulary, filters of their own: the same tokens as in a call of their own."""
+    rows, vocab, tail = 66_000, 32_769, 600
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    z = torch.empty(rows, vocab, dtype=torch.bfloat16, device="cuda").normal_(0.0, 2.2, generator=gen)
+    u = torch.rand(rows, device="cuda", generator=gen)
+    p = torch.tensor([0.95, 0.5, 1.0], device="cuda").repeat(rows // 3)
+    mp = torch.tensor([0.0, 1e-3, 0.02, 0.0], device="cuda").repeat(rows // 4)
+    got = []
+    for first in (0, rows - tail):
+        n = rows - first
+        tok = torch.full((n,), -7, dtype=torch.int32, device="cuda")
+        lp = torch.zeros(n, device="cuda")
+        ws = torch.empty(g.sample_workspace(n, vocab), dtype=torch.uint8, device="cuda")
+        g.sample(z[first:].data_ptr(), g.ELEM_BF16, n, vocab, vocab, u[first:].data_ptr(), tok.data_ptr(), lp.data_ptr(),
+                 top_p=p[first:].data_ptr(), min_p=mp[first:].data_ptr(), workspace=ws.data_ptr(),
+                 workspace_bytes=ws.numel(), stream=torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+        assert bool((tok >= 0).all())
+        got.append((tok[-tail:].clone(), lp[-tail:].clone()))
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+    r = rows - 2
+    t, l = plain(z[r].double().cpu().numpy(), float(u[r]), 1.0, 0, float(p[r]), float(mp[r]))
+    assert int(got[0][0][-2]) == t

@@ -346,6 +346,28 @@ def test_large_scores_and_infinite_ones():
     Call(rng, [40] * 4, [20] * 4, 500, 4, 1, 64, qscale=60.0, dtype="bf16").run().check()
 
 
+@pytest.mark.parametrize("new", [[1, 1, 1], [40, 33, 50], [2, 1, 3]])
+def test_many_small_probabilities_beside_a_large_one(new):
+    """60,000 shared keys whose probabilities are 2^-20.5 of one own key's: 4 % of the sum, all of the output."""
+    rng = np.random.default_rng(47)
+    c = Call(rng, new, [20] * 3, 60_000, 2, 1, 64, page=64)
+    c.q.fill_(1.0)
+    c.pool.k.zero_()
+    c.pool.v.fill_(1.0)
+    for s in range(3):
+        page = int(c.pool.table_host[s, 0])
+        c.pool.k[page, 0, 0] = 14.25 * 8 / 64  # (its score is 14.25: e^-14.25 = 2^-20.6)
+        c.pool.v[page, 0, 0] = 0.0
+    c.run().check()
+
+
+@pytest.mark.parametrize("new", [[0, 5, 0, 0, 7, 1, 0], [0, 50, 0, 130, 0], [0, 0, 1]])
+def test_sequences_without_new_tokens(new):
+    rng = np.random.default_rng(49)
+    c = Call(rng, new, rng.integers(0, 90, len(new)), 100, 8, 2, 128, single=False)
+    c.run().check()
+
+
 def test_refuses_a_short_workspace():
     c = Call(np.random.default_rng(45), [1] * 4, [5] * 4, 3000, 4, 1, 256)
     assert c.ws.numel() > 0
