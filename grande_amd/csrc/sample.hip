@@ -64,6 +64,7 @@ constexpr int EDGE = 2048;        // logits of one bin that they set apart
 constexpr int IDX_BITS = 20;      // vocab <= 2^20
 constexpr uint32_t IDX_MASK = (1u << IDX_BITS) - 1;
 constexpr double ONE = 4398046511104.0;  // 2^42
+constexpr float LOWEST = -3.4028235e38f;
 
 // Order-preserving bits of a logit that is not masked (above -infinity); -0
 // is the 0 it equals.
@@ -191,16 +192,19 @@ struct Common {
     uint64_t before, in_bin, total, found;
     uint32_t bin, kmax, kfirst, count;
 };
-struct Shared : Common {
-    uint64_t item[CAP];   // the list; without one, the masses of the row's segments
-    uint64_t mass[CAP];   // kept masses; before, the numbers of the groups to read
-    uint64_t hist[BINS];
-    uint64_t edge[PAIRS]; // items of one bin
-};
-// The wide kernels' lists of logits that pass a threshold, one a wave.
+// Lists of logits that pass a threshold, one a wave.
 struct Passed {
     float z[NWAVE][5 * WAVE];
-    uint16_t at[NWAVE][5 * WAVE];  // in the part
+    int at[NWAVE][5 * WAVE];
+};
+struct Shared : Common {
+    uint64_t item[CAP];   // the list; without one, the masses of the row's segments
+    union {
+        uint64_t mass[CAP];   // kept masses; before, the numbers of the groups to read
+        Passed list;
+    };
+    uint64_t hist[BINS];
+    uint64_t edge[PAIRS]; // items of one bin
 };
 struct BinsShared : Common {
     uint64_t hist[BINS];
@@ -326,6 +330,8 @@ struct Scale {
         const float x = max - float(last + 1) / per * 1.00001f;
         return x - fabsf(x) * 1e-6f - 1e-37f;
     }
+    // The same, finite; the lowest logit where the last bin is among them.
+    __device__ float low(int last) const { return last < BINS - 1 ? fmaxf(under(last), LOWEST) : LOWEST; }
 };
 
 // A row of logits: raw, masked ones as they stand (NaN, -infinity).
@@ -831,13 +837,57 @@ __device__ int make_list(const Settings& s, const Scale& sc, Shared& sm, uint64_
         if (last == BINS - 1) last = sc.whole ? BINS - 2 : -1;  // (all that have a mass)
         const bool all = last < 0;
         if (all && row.n > CAP) return -1;
-        const int n = gather(row, groups, all ? -3.4028235e38f : sc.under(last), sm);
+        const int n = gather(row, groups, all ? LOWEST : sc.under(last), sm);
         if (n <= CAP && (all || !by_p)) return n;
         if (n > CAP) return -1;
         uint64_t own = 0;
 #pragma unroll 1
         for (int i = threadIdx.x; i < n; i += NT) own += w.mass(item_value(sm.item[i]));
         if (block_sum(own, sm) >= want) return n;
+    }
+}
+
+// f(z, i, on) for a row's logits from `low` up (finite), 64 a wave at a time
+// (on: the lane has one).  Few of a row's logits reach a cut, and some lane of
+// a wave has one nearly always: without the lists each took the time of all,
+// 8.5 us of exp for 16 a thread.
+template <typename T, typename F>
+__device__ inline void passing(const Row<T>& row, float low, Passed& list, F&& f) {
+    float* lz = list.z[wave_id()];
+    int* at = list.at[wave_id()];
+    const int lane = int(threadIdx.x) % WAVE;
+    int have = 0;
+    const auto batch = [&](int from, bool on) {
+        asm volatile("" ::: "memory");  // (a wave's LDS accesses are in order)
+        f(on ? lz[from + lane] : -INFINITY, on ? at[from + lane] : 0, on);
+        asm volatile("" ::: "memory");
+    };
+    row.turns([&](const float* z, int i) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const bool pass = z[c] >= low;
+            const uint64_t all = __ballot(pass);
+            if (!all) continue;
+            if (pass) {
+                const int to = have + int(__builtin_amdgcn_mbcnt_hi(uint32_t(all >> 32),
+                                                                   __builtin_amdgcn_mbcnt_lo(uint32_t(all), 0)));
+                lz[to] = z[c], at[to] = i + c;
+            }
+            have += __popcll(all);
+        }
+        for (; have >= WAVE; have -= WAVE) batch(have - WAVE, true);
+    });
+    if (have) batch(0, lane < have);
+}
+
+// A wave's masses m of logits i into the sums of their segments.
+__device__ inline void add_segment(uint64_t* sums, int i, uint64_t m) {
+    const int seg = i / SEG, one = __builtin_amdgcn_readfirstlane(seg);
+    if (__all(seg == one)) {
+        m = wave_scan_u64(m);
+        if (threadIdx.x % WAVE == WAVE - 1 && m) add(&sums[one], m);
+    } else if (m) {
+        add(&sums[seg], m);
     }
 }
 
@@ -859,9 +909,11 @@ __device__ void finish_row(const Row<T>& row, const Settings& s, float u, const 
         const double x = out.w(z);
         return x >= s.least ? Weigh::fixed(x) : 0;
     };
-    row.sums(sm.item, kept);
-    __syncthreads();
     const int ns = row.segments();
+    __syncthreads();
+    clear(sm.item, ns);
+    passing(row, fmaxf(cut.z, LOWEST), sm.list, [&](float z, int i, bool on) { add_segment(sm.item, i, on ? kept(z, i) : 0); });
+    __syncthreads();
     uint64_t own = 0;
     for (int i = threadIdx.x; i < ns; i += NT) own += sm.item[i];
     const uint64_t total = block_sum(own, sm), target = goal(u, total);
@@ -1140,40 +1192,6 @@ __device__ inline Row<T> part_of(const Row<T>& row) {
     return Row<T>(row.p + first, row.n - first < PART ? row.n - first : PART);
 }
 
-// f(z, i, on) for the part's logits from bin `last`'s end up, 64 a wave at a
-// time (on: the lane has one).  Few of a row's logits reach a cut, and some
-// lane of a wave has one nearly always: without the lists each took the time
-// of all, 8.5 us of exp for 16 a thread.
-template <typename T, typename F>
-__device__ inline void passing(const Row<T>& part, const Scale& sc, int last, Passed& list, F&& f) {
-    const float low = last < BINS - 1 ? fmaxf(sc.under(last), -3.4028235e38f) : -3.4028235e38f;
-    float* lz = list.z[wave_id()];
-    uint16_t* at = list.at[wave_id()];
-    const int lane = int(threadIdx.x) % WAVE;
-    int have = 0;
-    const auto batch = [&](int from, bool on) {
-        asm volatile("" ::: "memory");  // (a wave's LDS accesses are in order)
-        f(on ? lz[from + lane] : -INFINITY, on ? int(at[from + lane]) : 0, on);
-        asm volatile("" ::: "memory");
-    };
-    part.turns([&](const float* z, int i) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            const bool pass = z[c] >= low;
-            const uint64_t all = __ballot(pass);
-            if (!all) continue;
-            if (pass) {
-                const int to = have + int(__builtin_amdgcn_mbcnt_hi(uint32_t(all >> 32),
-                                                                   __builtin_amdgcn_mbcnt_lo(uint32_t(all), 0)));
-                lz[to] = z[c], at[to] = uint16_t(i + c);
-            }
-            have += __popcll(all);
-        }
-        for (; have >= WAVE; have -= WAVE) batch(have - WAVE, true);
-    });
-    if (have) batch(0, lane < have);
-}
-
 // The masses of rows TO_CUT by bins; the last workgroup of a row finds
 // top_p's cut.
 template <typename T>
@@ -1190,7 +1208,7 @@ __global__ __launch_bounds__(NT, 8) void sample_bins(SampleArgs a, Workspace ws)
     const uint64_t total = pd.left;
     const int reach = s.p > 0.0f ? sc.reach(s.p, float(double(total) / ONE), row.n, s.t) : BINS - 1;
     clear(sm.hist, BINS);
-    passing(part_of(row), sc, reach, sm.list, [&](float z, int, bool on) {
+    passing(part_of(row), sc.low(reach), sm.list, [&](float z, int, bool on) {
         const int b = sc.bin(z);
         const uint64_t m = on && b <= reach ? w.mass(z) : 0;
         if (m) add(&sm.hist[b], m);
@@ -1235,7 +1253,7 @@ __global__ __launch_bounds__(NT, 8) void sample_draw(SampleArgs a, Workspace ws)
     __syncthreads();
     // (a logit in a bin before stays, if min_p lets it)
     const int last = s.least > 0.0 ? sc.reach_min(s.least, s.t) : BINS;
-    passing(part, sc, bin < last ? bin : last, sm.list, [&](float z, int i, bool on) {
+    passing(part, sc.low(bin < last ? bin : last), sm.list, [&](float z, int i, bool on) {
         const int b = on ? sc.bin(z) : BINS;
         if (b == bin && on) {
             const uint32_t at = atomicAdd(&sm.count, 1u);
@@ -1246,13 +1264,7 @@ __global__ __launch_bounds__(NT, 8) void sample_draw(SampleArgs a, Workspace ws)
             const double x = out.w(z);
             m = x >= s.least ? Weigh::fixed(x) : 0;
         }
-        const int seg = i / SEG, one = __builtin_amdgcn_readfirstlane(seg);
-        if (__all(seg == one)) {
-            m = wave_scan_u64(m);
-            if (tid % WAVE == WAVE - 1 && m) add(&sm.seg[one], m);
-        } else if (m) {
-            add(&sm.seg[seg], m);
-        }
+        add_segment(sm.seg, i, m);
     });
     __syncthreads();
     const uint32_t here = sm.count;
