@@ -34,11 +34,11 @@
 // instructions; this form takes 5.
 //
 // Measured: one row of 25,000 15.4 us (f32; top_k 40, top_p 0.95: seven steps
-// that wait for one another); 208 of them, each with its own filters, 56 us
+// that wait for one another); 208 of them, each with its own filters, 52 us
 // (the rows whose kept tokens fit no list); 64 rows of 262,144 (bf16, top_p)
-// 104 us: stats 25 (37 vector instructions a logit, most of them exp's),
-// long 20, bins 26, draw 37 (the last rows' cuts, one workgroup each); 256
-// rows of 128,257 (f32, mixed filters) 111 us, of which stats 33 (3.9 TB/s).
+// 104 us: stats 24 (37 vector instructions a logit, most of them exp's),
+// long 20, bins 26, draw 39 (the last rows' cuts, one workgroup each); 256
+// rows of 128,257 (f32, mixed filters) 107 us, of which stats 33 (3.9 TB/s).
 #include <algorithm>
 #include <string>
 

@@ -34,8 +34,8 @@
 // 16 rows x 16 bytes, V's 4 rows x 64 bytes or 8 x 32 (counted: none meet).
 //
 // Measured, and what bounds it:
-//   questions, 6,300 tokens x 8 heads of 256 on 8,000 keys (f16): 451-480 us,
-//     860-920 TFLOP/s of the 1,190 that a product of 8,192^3 reaches.  392
+//   questions, 6,300 tokens x 8 heads of 256 on 8,000 keys (f16): 460-490 us,
+//     850-900 TFLOP/s of the 1,190 that a product of 8,192^3 reaches.  392
 //     tiles on 512 places; MFMAs take 45 % of the busy CUs' cycles, other
 //     vector instructions 32 %, LDS 22 %: a tile is one chain of dependent
 //     steps with two waves a SIMD to fill it, registers allow no third.
