@@ -204,7 +204,7 @@ def test_queries_in_place():
     cs = rope_table(8, 256).cuda()
     outs = []
     for dst in (torch.zeros_like(x), x):
-        src = g.KvSource(g.ELEM_BF16, 4, x.data_ptr(), x.data_ptr() + 2048, x.data_ptr() + 3072, 2048,
+        src = g.KvSource(g.ELEM_BF16, 4, x.data_ptr(), x.data_ptr() + 2048, x.data_ptr() + 2048 + 1024, 2048,
                          rope=cs.data_ptr(), rope_rows=8, rope_dims=256)
         pool.kv().append(pool.batch(40), src, dst.data_ptr(), 2048)
         torch.cuda.synchronize()
