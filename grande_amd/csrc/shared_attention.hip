@@ -493,9 +493,10 @@ struct Keys {
 
 // In a tile a key that a query does not see has p = 0, which leaves nothing
 // of its values unless these are infinite or NaN.  Sums that are not finite
-// are therefore taken again from the keys their row sees and no others, one
-// by one: `rows` holds a bit per lane whose row it is (with maximum cm, sum
-// l); a wave writes the quads of head dims it has (quarter < 0: all).
+// are therefore taken again from the keys their row sees and no others:
+// `rows` holds a bit per lane whose row it is (with maximum cm, sum l); a wave
+// writes the quads of head dims it has (quarter < 0: all).  A row whose scores
+// hold a NaN has it in l, and in its outputs as they are.
 template <typename T, int D>
 __device__ void seen_alone(const Args& a, const Keys& in, const Row& r, uint64_t rows, float cm, float l, int lane,
                            int64_t slot, int quarter) {
@@ -523,22 +524,46 @@ __device__ void seen_alone(const Args& a, const Keys& in, const Row& r, uint64_t
         load(a.x.q, tok * a.x.ldq + int64_t(head) * D, q);
 #pragma unroll
         for (int e = 0; e < E; ++e) o[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        bool lost = false;  // every element is NaN, and stays so
         const auto keys = [&](const int32_t* table, int plast, int from, int to) {
+            constexpr int U = 4;  // keys under way together
 #pragma unroll 1
-            for (int k = from; k < to; ++k) {
-                const int64_t page = table[imin(k >> a.page_shift, plast)];
-                if (page < 0 || page >= a.kv.npages) continue;
-                const int64_t key = page * a.kv.page_stride + (int64_t(in.g) * a.kv.page + (k & (a.kv.page - 1))) * D;
-                float4 x[E];
-                load(a.kv.k, key, x);
-                float s = 0.0f;
+            for (int k = from; k < to && !lost; k += U) {
+                int64_t key[U];
+                bool ok[U];
+                float4 x[U][E];
+                float p[U];
 #pragma unroll
-                for (int e = 0; e < E; ++e) s += x[e].x * q[e].x + x[e].y * q[e].y + x[e].z * q[e].z + x[e].w * q[e].w;
-                const float p = __builtin_amdgcn_exp2f(fmaf(wave_sum(s), a.c, -ref));
-                load(a.kv.v, key, x);
+                for (int u = 0; u < U; ++u) {
+                    const int64_t page = table[imin(imin(k + u, to - 1) >> a.page_shift, plast)];
+                    ok[u] = k + u < to && page >= 0 && page < a.kv.npages;
+                    key[u] = ok[u] ? page * a.kv.page_stride + (int64_t(in.g) * a.kv.page + ((k + u) & (a.kv.page - 1))) * D : 0;
+                }
 #pragma unroll
-                for (int e = 0; e < E; ++e)
-                    o[e].x += p * x[e].x, o[e].y += p * x[e].y, o[e].z += p * x[e].z, o[e].w += p * x[e].w;
+                for (int u = 0; u < U; ++u) load(a.kv.k, key[u], x[u]);
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    float s = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < E; ++e)
+                        s += x[u][e].x * q[e].x + x[u][e].y * q[e].y + x[u][e].z * q[e].z + x[u][e].w * q[e].w;
+                    p[u] = __builtin_amdgcn_exp2f(fmaf(wave_sum(s), a.c, -ref));
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) load(a.kv.v, key[u], x[u]);
+                bool nan = true;
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        if (!ok[u]) continue;
+                        o[e].x += p[u] * x[u][e].x, o[e].y += p[u] * x[u][e].y;
+                        o[e].z += p[u] * x[u][e].z, o[e].w += p[u] * x[u][e].w;
+                    }
+                    nan = nan && (lane + e * WAVE >= NQ || (o[e].x != o[e].x && o[e].y != o[e].y && o[e].z != o[e].z &&
+                                                            o[e].w != o[e].w));
+                }
+                lost = __all(nan);
             }
         };
         keys(a.b.prefix_table, (P - 1) >> a.page_shift, imax(in.pb, w > 0 ? P + own - w + 1 : 0), in.pe);
@@ -567,20 +592,21 @@ __device__ inline void emit(const Args& a, Core<T, D, TILE>& core, const Keys& i
     for (int i = 0; i < C::NC; ++i)
 #pragma unroll
         for (int e = 0; e < C::SR; ++e) z[e % 4] = fmaf(core.o[i][e], 0.0f, z[e % 4]);
-    uint64_t bad = __ballot(r.valid && !(z[0] + z[1] + z[2] + z[3] == 0.0f));
+    uint64_t bad = __ballot(r.valid && l == l && !(z[0] + z[1] + z[2] + z[3] == 0.0f));
     bad |= bad >> 32;
     if constexpr (C::RW == 16) bad |= bad >> 16;
     bad &= (uint64_t(1) << C::RW) - 1;
+    if (r.valid && !(bad >> (lane % C::RW) & 1)) {
+#pragma unroll
+        for (int i = 0; i < C::NC; ++i)
+#pragma unroll
+            for (int rr = 0; rr < C::QUADS; ++rr)
+                out.template quad<D>(C::dim_of(lane, i, rr),
+                                     make_float4(core.o[i][4 * rr], core.o[i][4 * rr + 1], core.o[i][4 * rr + 2],
+                                                 core.o[i][4 * rr + 3]),
+                                     l);
+    }
     if (bad) seen_alone<T, D>(a, in, r, bad, cm, l, lane, slot, -1);
-    if (!r.valid || (bad >> (lane % C::RW) & 1)) return;
-#pragma unroll
-    for (int i = 0; i < C::NC; ++i)
-#pragma unroll
-        for (int rr = 0; rr < C::QUADS; ++rr)
-            out.template quad<D>(C::dim_of(lane, i, rr),
-                                 make_float4(core.o[i][4 * rr], core.o[i][4 * rr + 1], core.o[i][4 * rr + 2],
-                                             core.o[i][4 * rr + 3]),
-                                 l);
 }
 
 // The four waves' results for the same 16 rows, joined through LDS.
@@ -623,13 +649,14 @@ __device__ inline void emit_keys(const Args& a, Core<T, D, WAVES_KEYS>& core, co
         }
         z += fmaf(v[i].x, 0.0f, v[i].y * 0.0f) + fmaf(v[i].z, 0.0f, v[i].w * 0.0f);
     }
-    uint64_t bad = __ballot(r.valid && !(z == 0.0f));
+    uint64_t bad = __ballot(r.valid && sum == sum && !(z == 0.0f));
     bad |= bad >> 32;
     bad = (bad | bad >> 16) & 0xffff;
-    if (bad) seen_alone<T, D>(a, in, r, bad, cm, sum, lane, slot, wave);
-    if (!r.valid || (bad >> (lane % 16) & 1)) return;
+    if (r.valid && !(bad >> (lane % 16) & 1)) {
 #pragma unroll
-    for (int i = 0; i < D / 64; ++i) out.template quad<D>(4 * (wave * 4 + lane / 16 + 16 * i), v[i], sum);
+        for (int i = 0; i < D / 64; ++i) out.template quad<D>(4 * (wave * 4 + lane / 16 + 16 * i), v[i], sum);
+    }
+    if (bad) seen_alone<T, D>(a, in, r, bad, cm, sum, lane, slot, wave);
 }
 
 template <typename T, int D, int TILE>

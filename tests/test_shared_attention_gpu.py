@@ -247,6 +247,43 @@ def test_nan_reaches_the_queries_that_see_its_row_and_no_others(hd, new, before,
         c.check("NaN in a row")
 
 
+@pytest.mark.parametrize("new", [[1] * 7, [33, 40, 36, 47, 50], [3, 1, 2, 4, 1]])
+@pytest.mark.parametrize("hd", [64, 256, 512])
+def test_a_query_of_nan_spoils_its_own_row_alone(hd, new):
+    rng = np.random.default_rng(32)
+    c = Call(rng, new, [20] * len(new), 300, 4, 2, hd)
+    clean = c.run().out.clone(), c.lse.clone()
+    c.q[2, hd:2 * hd] = float("nan")  # (token 2, head 1)
+    c.q[2, 3 * hd] = float("inf")     # (head 3: scores of both signs, infinite)
+    c.out.fill_(5.0)
+    c.run()
+    torch.cuda.synchronize()
+    mine = torch.zeros(c.rows, 4, hd, dtype=torch.bool, device="cuda")
+    mine[2, 1], mine[2, 3] = True, True
+    mine = mine.view(c.rows, 4 * hd)
+    assert bool(torch.isnan(c.out[2, hd:2 * hd]).all()) and bool(torch.isnan(c.out[2, 3 * hd:4 * hd]).all())
+    assert torch.equal(c.out[:, :4 * hd][~mine], clean[0][:, :4 * hd][~mine])
+
+
+def test_values_of_infinity_that_a_row_sees():
+    """One key's values infinite of both signs, seen by the second half of a question: infinite there, as without them
+    before."""
+    rng = np.random.default_rng(34)
+    for hd, new in ((128, [64, 40]), (256, [4, 3])):
+        c = Call(rng, new, [10, 10], 40, 4, 2, hd)
+        clean = c.run().out.clone()
+        row = 10 + new[0] // 2
+        sign = torch.where(torch.arange(hd) % 2 == 0, 1.0, -1.0).half().cuda()
+        c.pool.v[int(c.pool.table_host[0, row // 16]), :, row % 16] = sign * float("inf")
+        c.run()
+        torch.cuda.synchronize()
+        at = new[0] // 2
+        assert torch.equal(c.out[at:new[0], :4 * hd], (sign * float("inf")).repeat(4).expand(new[0] - at, -1))
+        got, exp = torch.cat([c.out[:at], c.out[new[0]:]]), torch.cat([clean[:at], clean[new[0]:]])
+        # (one of the two rounds p: 2^-11 of sum p |v|, which is below 6; each output rounds by half a step)
+        assert bool(((got - exp).abs().float() <= 2.0 ** -10 * exp.abs().float() + 6 * 2.0 ** -11).all())
+
+
 def test_pages_outside_the_pool_are_not_seen():
     rng = np.random.default_rng(31)
     for new in ([1] * 4, [35, 40, 50, 33], [3, 4, 1, 2]):
