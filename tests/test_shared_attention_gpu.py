@@ -175,6 +175,33 @@ def test_strides_and_rows_that_no_sequence_has():
     Call(rng, [50, 45], [0, 4], 10, 4, 4, 64, tail=70).run().check()
 
 
+@pytest.mark.parametrize("new", [[1, 1, 1, 1], [40, 35, 50, 33]])
+@pytest.mark.parametrize("hd", [64, 512])
+def test_pages_with_room_between_them(hd, new):
+    """A page stride past the page's rows, NaN between: the same bits."""
+    rng = np.random.default_rng(26)
+    c = Call(rng, new, [20] * 4, 100, 4, 2, hd)
+    near = c.run().out.clone()
+    stride = c.pool.stride + 72
+    wide = [torch.full((c.pool.npages, stride), float("nan"), dtype=torch.float16, device="cuda") for _ in range(2)]
+    for w, raw in zip(wide, (c.pool.k_raw, c.pool.v_raw)):
+        w[:, :c.pool.stride] = raw
+    c.kv = g.PagedKv(wide[0].data_ptr(), wide[1].data_ptr(), c.pool.npages, 2, c.pool.page, hd, g.ELEM_F16, stride)
+    c.out.fill_(5.0)
+    c.run()
+    torch.cuda.synchronize()
+    assert torch.equal(near, c.out)
+
+
+def test_two_sequences_on_the_same_pages():
+    """Forks of one sequence: the same rows under two numbers, other queries."""
+    rng = np.random.default_rng(28)
+    c = Call(rng, [1, 1, 1], [49, 49, 30], 64, 4, 2, 128)
+    c.pool.table[1] = c.pool.table[0]
+    c.pool.table_host[1] = c.pool.table_host[0]
+    c.run().check()
+
+
 @pytest.mark.parametrize("new", [[1, 1, 1, 1], [40, 35, 50, 33], [2, 5, 1, 3]])
 def test_tokens_that_see_nothing(new):
     """No prefix and lengths too short for the tokens: zeros and -infinity."""
