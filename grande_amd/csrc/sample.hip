@@ -191,6 +191,7 @@ struct Common {
     uint64_t part[NWAVE];
     uint64_t before, in_bin, total, found;
     uint32_t bin, kmax, kfirst, count;
+    int row_n;  // the row's logits (as an argument 27 more scalars spilled: one row of 25,000 15.4 -> 17.2 us)
 };
 // Lists of logits that pass a threshold, one a wave.
 struct Passed {
@@ -312,11 +313,16 @@ struct Scale {
         const float x = (max - z) * per;
         return x < float(BINS - 1) ? int(x) : BINS - 1;  // (NaN, infinity - infinity: the last)
     }
-    // The bins that top_p's cut can lie in, of n logits whose mass is at least
-    // `mass` of the largest's: those below the last one returned weigh less
-    // than (1 - p) mass / (2 n) each, together less than what top_p leaves.
+    // The bins that top_p's cut can lie in, of the n logits that p is a share
+    // of, whose mass is at least `mass` of the largest's: those below the last
+    // one returned weigh less than (1 - p) mass / (2 n) each, together less
+    // than half of what top_p leaves.  The other half is for the masses'
+    // rounding, up to 2^-42 a logit in the sums compared: all bins where that
+    // is more.
     __device__ int reach(float p, float mass, int n, float t) const {
-        const float nats = logf(2.0f * float(n) / ((1.0f - p) * mass));
+        const float leaves = (1.0f - p) * mass;
+        if (!(leaves > 5e-13f * float(n))) return BINS - 1;  // (2^-41)
+        const float nats = logf(2.0f * float(n) / leaves);
         const float x = nats * t * per + 2.0f;
         return x < float(BINS - 1) && max < INFINITY ? int(x) : BINS - 1;  // (infinities lie in the last)
     }
@@ -570,9 +576,10 @@ __device__ Cut cut_by_bins(S&& items, const Scale& sc, Shared& sm, uint64_t* roo
     return cut_in_bin(room, n, sm, left, masses, w);
 }
 
-// The cuts of top_k and top_p over n items, whose shares are summed by bins
+// The cuts of top_k and top_p over items whose shares are summed by bins
 // first; row_mass: the mass that top_p is a share of where it is known (0:
-// it is summed here).
+// it is summed here) and top_k is off; n: how many logits that mass is of,
+// the items or a whole row that holds more.
 template <typename S>
 __device__ Cut cuts(S&& items, int n, const Settings& s, const Scale& sc, uint64_t row_mass, Shared& sm, uint64_t* room,
                     int most, const Weigh& w) {
@@ -605,7 +612,7 @@ __device__ Cut cuts(S&& items, int n, const Settings& s, const Scale& sc, uint64
 
 // The exact cuts and the draw over the list's n items (every item that can
 // be kept is there); `row_mass`: the mass that top_p is a share of, unless
-// top_k is on.
+// top_k is on, that of the row's sm.row_n logits.
 __device__ void finish_list(int n, const Settings& s, float u, uint64_t row_mass, const Scale& sc, Shared& sm,
                             const Result& out) {
     const Weigh& w = out.w;
@@ -649,7 +656,7 @@ __device__ void finish_list(int n, const Settings& s, float u, uint64_t row_mass
 #pragma unroll 1
         for (int i = tid; i < n; i += NT) f(item_value(sm.item[i]), item_index(sm.item[i]));
     };
-    const Cut cut = cuts(items, n, s, sc, row_mass, sm, sm.edge, PAIRS, w);
+    const Cut cut = cuts(items, s.k ? n : sm.row_n, s, sc, row_mass, sm, sm.edge, PAIRS, w);
     // the kept masses, then the draw: the digits of the index, 10 and 10 bits
     uint64_t own = 0;
 #pragma unroll 1
@@ -963,7 +970,7 @@ __global__ __launch_bounds__(NT) void sample_short(SampleArgs a) {
     const Row<T> row(static_cast<const T*>(a.logits) + r * a.ld, a.vocab);
     const Settings s = settings_of(a, r);
     const float u = a.u[r];
-    if (tid == 0) sm.kmax = 0, sm.kfirst = 0xffffffffu;
+    if (tid == 0) sm.kmax = 0, sm.kfirst = 0xffffffffu, sm.row_n = row.n;
     float zmax = -INFINITY;
     uint32_t first = 0xffffffffu;
     row.turns([&](const float* z, int i) {
@@ -1092,7 +1099,7 @@ __global__ __launch_bounds__(NT) void sample_long(SampleArgs a, Workspace ws) {
     const float u = a.u[r];
     const float* groups = ws.groups + r * nchunk * (CHUNK / GROUP);
     const Row<T> row(static_cast<const T*>(a.logits) + r * a.ld, a.vocab);
-    if (tid == 0) sm.kmax = 0, sm.kfirst = 0xffffffffu, ws.pending[r].step = DONE;
+    if (tid == 0) sm.kmax = 0, sm.kfirst = 0xffffffffu, sm.row_n = row.n, ws.pending[r].step = DONE;
     const float wmax = wave_max(mine.max);
     __syncthreads();
     if (tid % WAVE == 0 && wmax > -INFINITY) atomicMax(&sm.kmax, key_of(wmax));

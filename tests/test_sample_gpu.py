@@ -267,3 +267,32 @@ def test_more_rows_than_a_grids_second_size():
     r = rows - 2
     t, l = plain(z[r].double().cpu().numpy(), float(u[r]), 1.0, 0, float(p[r]), float(mp[r]))
     assert int(got[0][0][-2]) == t
+
+
+def light_tail(rng, vocab, light, weight, mass, temp, twins=0):
+    """One row: a token of weight 1, `light` tokens of `weight` each (give or take a thousandth; the first 2 `twins`
+    of them side by side in pairs), and the rest, `mass` of them all together, give or take a tenth."""
+    w = mass / (vocab - light - 1) * (1 + 0.1 * (2 * rng.random(vocab) - 1))
+    block = rng.permutation(vocab // 64 - 1)[:light - twins + 1] * 64
+    at = block + 2 * rng.integers(0, 31, len(block))
+    w[at[0]] = 1.0
+    w[np.concatenate([at[1:], at[1:twins + 1] + 1])] = weight * (1 + 1e-3 * (2 * rng.random(light) - 1))
+    return (temp * np.log(w)).astype(np.float32)
+
+
+@pytest.mark.parametrize("vocab,light,weight,mass,twins,temp,p,mp", [
+    (25_000, 350, 1.2e-4, 0.08, 0, 1.0, 0.9, 5e-5),
+    (25_000, 350, 1.2e-4, 0.08, 0, 1.0, 0.9, 0.0),
+    (25_000, 380, 1e-4, 0.08, 0, 1.3, 0.9, 5e-5),
+    (100_000, 1500, 1e-4, 0.78, 0, 1.0, 0.55, 5e-5),
+    (100_000, 1500, 1e-4, 0.78, 0, 0.6, 0.55, 5e-5),
+    (262_144, 4000, 2e-5, 0.23, 0, 1.0, 0.8, 1e-5),
+    (100_000, 300, 1.58e-4, 0.0659, 60, 6.0, 0.9, 0.0),
+    (262_144, 300, 1.58e-4, 0.0659, 60, 6.0, 0.9, 0.0)])
+def test_top_p_cuts_among_light_tokens_beside_a_heavy_rest(vocab, light, weight, mass, twins, temp, p, mp):
+    """The border of top_p lies among tokens lighter than (1 - p) / (2 n) of the largest, n the tokens that min_p (or
+    top_p's own threshold) leaves: what top_p removes is mostly the rest of the row, not these."""
+    rng = np.random.default_rng(light + vocab)
+    z = np.stack([light_tail(rng, vocab, light, weight, mass, temp, twins) for _ in range(6)])
+    below = np.nextafter(np.float32(1), np.float32(0))
+    same(z, [0.1, 0.5, 0.97, 0.99, 0.999, below], temp=temp, p=p, mp=mp or None)
