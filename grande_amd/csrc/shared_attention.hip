@@ -1,9 +1,11 @@
 // Attention over a prefix that all sequences of a batch share and over each
 // sequence's own rows, both on pages of a K/V pool:
-//   out = sum_j p_j v_j / sum_j p_j,  p_j = 2^(c (s_j - m) + LIFT),  s_j = q . k_j,
+//   out = sum_j p_j v_j / sum_j p_j,  p_j = 2^(c (s_j - m) + lift),  s_j = q . k_j,
 // c = scale log2(e), m a running maximum of s, over the keys j that the
-// query sees.  Partial results over ranges of keys are joined by
-// (m, l = sum p, O = sum p v): O and l times 2^(c (m - max m)).
+// query sees.  Partial results over ranges of keys are their means sum p v /
+// sum p and lg = log2 of the ranges' sums of 2^(c s): out is the means' mean
+// with the weights 2^(lg - max lg).  (Sums of bf16 values may pass f32's
+// largest, means do not.)
 //
 // Queries are rows (token, head) of one KV head, so that a tile of rows
 // takes every key and value it reads once for all of them: tiles of the
@@ -61,13 +63,16 @@ namespace {
 
 enum Tile { WAVES_KEYS = 0, WAVES_16 = 1, WAVES_32 = 2 };
 
-// The running maximum may lag by LAG binary orders in p, and all p stand LIFT
-// orders higher: the largest lie in 2^7 .. 2^15, so that f16 holds p with all
-// its bits down to 2^-21 of the largest, and those below to 2^-32 of it
-// (without: 60,000 keys of 2^-20.5 each 4 % off).  A smaller lag takes the
-// outputs' products with 2^(c (m - m')) more often: 4 orders 530 us for the
-// questions below, 8 480.
-constexpr float LAG = 8.0f, LIFT = 7.0f;
+// The running maximum may lag by LAG binary orders in p.  For f16 all p stand
+// 7 orders higher: the largest lie in 2^7 .. 2^15, so that f16 holds p with
+// all its bits down to 2^-21 of the largest, and those below to 2^-32 of it
+// (without: 60,000 keys of 2^-20.5 each 4 % off).  bf16 has f32's exponents,
+// and values that leave its sums no room to be lifted.  A smaller lag takes
+// the outputs' products with 2^(c (m - m')) more often: 4 orders 530 us for
+// the questions above, 8 480.
+constexpr float LAG = 8.0f;
+template <typename T>
+constexpr float lift = std::is_same_v<T, half_t> ? 7.0f : 0.0f;
 
 struct Plan {
     int tile;       // Tile of the prefix / fused items
@@ -89,7 +94,7 @@ struct Args {
     int64_t prefix_blocks;     // (a multiple of 8)
     float c;                   // scale log2(e)
     float* part_o;             // [slots][t * heads][head_dim], null: results go out
-    float2* part_ml;           // [slots][t * heads] (c m - LIFT, l)
+    float* part_lg;            // [slots][t * heads]
 };
 
 typedef __attribute__((address_space(3))) void* lds_ptr;
@@ -255,7 +260,7 @@ struct Core {
 #pragma unroll
                 for (int r = 0; r < SR; ++r) o[i][r] *= al;
         }
-        const float mc = m == -INFINITY ? 0.0f : m * c - LIFT;
+        const float mc = m == -INFINITY ? 0.0f : m * c - lift<T>;
         float sum = 0.0f;
 #pragma unroll
         for (int j = 0; j < NB; ++j)
@@ -331,6 +336,9 @@ struct Core {
     }
 };
 
+// log2 of a row's sum of 2^(c s), from its c m - lift and l.
+__device__ inline float log_sum(float cm, float l) { return l == 0.0f ? -INFINITY : cm + __builtin_amdgcn_logf(l); }
+
 // Where a row's result of slot `slot` goes: the partials, or the output.
 template <typename T>
 struct Sink {
@@ -338,25 +346,24 @@ struct Sink {
     int64_t row;    // tok * heads + head
     int64_t out;    // tok * ldo + head * D
     int64_t slot;
-    __device__ void stats(float cm, float l) const {
+    __device__ void stats(float lg) const {
         if (a.part_o)
-            a.part_ml[slot * a.b.t * a.x.heads + row] = make_float2(cm, l);
+            a.part_lg[slot * a.b.t * a.x.heads + row] = lg;
         else if (a.x.lse)
-            a.x.lse[row] = l == 0.0f ? -INFINITY : (cm + __builtin_amdgcn_logf(l)) * 0.69314718055994531f;
+            a.x.lse[row] = lg * 0.69314718055994531f;
     }
+    // Four elements of the mean (`some`: the row sees a key here).
     template <int D>
-    __device__ void quad(int dim, float4 v, float l) const {
+    __device__ void quad(int dim, float4 v, bool some) const {
         if (a.part_o) {
-            if (l != 0.0f)
-                *reinterpret_cast<float4*>(a.part_o + (slot * a.b.t * a.x.heads + row) * D + dim) = v;
+            if (some) *reinterpret_cast<float4*>(a.part_o + (slot * a.b.t * a.x.heads + row) * D + dim) = v;
         } else {
-            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             typedef T vec4 __attribute__((ext_vector_type(4)));
-            *reinterpret_cast<vec4*>(static_cast<T*>(a.x.out) + out + dim) =
-                vec4{T(v.x * inv), T(v.y * inv), T(v.z * inv), T(v.w * inv)};
+            *reinterpret_cast<vec4*>(static_cast<T*>(a.x.out) + out + dim) = vec4{T(v.x), T(v.y), T(v.z), T(v.w)};
         }
     }
 };
+__device__ inline float4 times(float4 v, float f) { return make_float4(v.x * f, v.y * f, v.z * f, v.w * f); }
 
 // A value that is the same in every lane, in a scalar register.
 __device__ inline int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -492,14 +499,16 @@ struct Keys {
 };
 
 // In a tile a key that a query does not see has p = 0, which leaves nothing
-// of its values unless these are infinite or NaN.  Sums that are not finite
-// are therefore taken again from the keys their row sees and no others:
-// `rows` holds a bit per lane whose row it is (with maximum cm, sum l); a wave
-// writes the quads of head dims it has (quarter < 0: all).  A row whose scores
-// hold a NaN has it in l, and in its outputs as they are.
+// of its values unless these are infinite or NaN, and a sum of finite bf16
+// values may pass f32's largest where their mean does not.  Sums that are not
+// finite are therefore taken again from the keys their row sees and no
+// others, with probabilities that add up to one: `rows` holds a bit per lane
+// whose row it is (with log sum lg); a wave writes the quads of head dims it
+// has (quarter < 0: all).  A row whose scores hold a NaN has it in lg, and in
+// its outputs as they are.
 template <typename T, int D>
-__device__ void seen_alone(const Args& a, const Keys& in, const Row& r, uint64_t rows, float cm, float l, int lane,
-                           int64_t slot, int quarter) {
+__device__ void seen_alone(const Args& a, const Keys& in, const Row& r, uint64_t rows, float lg, int lane, int64_t slot,
+                           int quarter) {
     constexpr int NQ = D / 4, E = (NQ + WAVE - 1) / WAVE;
     typedef T vec4 __attribute__((ext_vector_type(4)));
     const int P = int(a.b.prefix_len), w = a.x.window;
@@ -511,7 +520,7 @@ __device__ void seen_alone(const Args& a, const Keys& in, const Row& r, uint64_t
         const int at = of(r.at), seq = of(r.seq), own = of(r.own);
         const int64_t tok = at / a.x.heads;
         const int head = at % a.x.heads;
-        const float row_cm = off(cm), ref = row_cm == -INFINITY ? 0.0f : row_cm;
+        const float row_lg = off(lg), ref = row_lg == -INFINITY ? 0.0f : row_lg;
         float4 q[E], o[E];
         const auto load = [&](const void* p, int64_t at, float4* x) {
 #pragma unroll
@@ -524,7 +533,8 @@ __device__ void seen_alone(const Args& a, const Keys& in, const Row& r, uint64_t
         load(a.x.q, tok * a.x.ldq + int64_t(head) * D, q);
 #pragma unroll
         for (int e = 0; e < E; ++e) o[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        bool lost = false;  // every element is NaN, and stays so
+        float total = 0.0f;  // of the probabilities: one, but for rounding
+        bool lost = false;   // every element is NaN, and stays so
         const auto keys = [&](const int32_t* table, int plast, int from, int to) {
             constexpr int U = 4;  // keys under way together
 #pragma unroll 1
@@ -548,6 +558,7 @@ __device__ void seen_alone(const Args& a, const Keys& in, const Row& r, uint64_t
                     for (int e = 0; e < E; ++e)
                         s += x[u][e].x * q[e].x + x[u][e].y * q[e].y + x[u][e].z * q[e].z + x[u][e].w * q[e].w;
                     p[u] = __builtin_amdgcn_exp2f(fmaf(wave_sum(s), a.c, -ref));
+                    total += ok[u] ? p[u] : 0.0f;
                 }
 #pragma unroll
                 for (int u = 0; u < U; ++u) load(a.kv.v, key[u], x[u]);
@@ -570,11 +581,12 @@ __device__ void seen_alone(const Args& a, const Keys& in, const Row& r, uint64_t
         keys(a.b.table + seq * a.b.table_ld, int(a.b.max_pages) - 1, imax(in.ob, w > 0 ? own - w + 1 : 0),
              imin(in.oe, own + 1));
         const Sink<T> out{a, at, tok * a.x.ldo + int64_t(head) * D, slot};
-        const float sum = off(l);
+        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             const int c4 = lane + e * WAVE;
-            if (c4 < NQ && (quarter < 0 || c4 % 16 / 4 == quarter)) out.template quad<D>(4 * c4, o[e], sum);
+            if (c4 < NQ && (quarter < 0 || c4 % 16 / 4 == quarter))
+                out.template quad<D>(4 * c4, times(o[e], inv), row_lg != -INFINITY);
         }
     }
 }
@@ -584,9 +596,10 @@ template <typename T, int D, int TILE>
 __device__ inline void emit(const Args& a, Core<T, D, TILE>& core, const Keys& in, const Row& r, int lane,
                             int64_t slot) {
     typedef Core<T, D, TILE> C;
-    const float l = C::row_sum(core.l), cm = core.m == -INFINITY ? -INFINITY : core.m * a.c - LIFT;
+    const float l = C::row_sum(core.l), inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const float lg = log_sum(core.m * a.c - lift<T>, l);
     const Sink<T> out{a, r.at, r.at / a.x.heads * a.x.ldo + int64_t(r.at % a.x.heads) * D, slot};
-    if (r.valid && lane < C::RW) out.stats(cm, l);
+    if (r.valid && lane < C::RW) out.stats(lg);
     float z[4] = {};  // (NaN where a sum is not finite)
 #pragma unroll
     for (int i = 0; i < C::NC; ++i)
@@ -602,11 +615,12 @@ __device__ inline void emit(const Args& a, Core<T, D, TILE>& core, const Keys& i
 #pragma unroll
             for (int rr = 0; rr < C::QUADS; ++rr)
                 out.template quad<D>(C::dim_of(lane, i, rr),
-                                     make_float4(core.o[i][4 * rr], core.o[i][4 * rr + 1], core.o[i][4 * rr + 2],
-                                                 core.o[i][4 * rr + 3]),
-                                     l);
+                                     times(make_float4(core.o[i][4 * rr], core.o[i][4 * rr + 1], core.o[i][4 * rr + 2],
+                                                       core.o[i][4 * rr + 3]),
+                                           inv),
+                                     l != 0.0f);
     }
-    if (bad) seen_alone<T, D>(a, in, r, bad, cm, l, lane, slot, -1);
+    if (bad) seen_alone<T, D>(a, in, r, bad, lg, lane, slot, -1);
 }
 
 // The four waves' results for the same 16 rows, joined through LDS.
@@ -622,7 +636,7 @@ __device__ inline void emit_keys(const Args& a, Core<T, D, WAVES_KEYS>& core, co
     for (int i = 0; i < C::NC; ++i)
         *reinterpret_cast<floatx4*>(mine + ((i * 4 + lane / 16) * 16 + lane % 16) * 4) = core.o[i];
     if (lane < 16) {
-        ml[wave * 16 + lane] = core.m == -INFINITY ? -INFINITY : core.m * a.c - LIFT;
+        ml[wave * 16 + lane] = core.m == -INFINITY ? -INFINITY : core.m * a.c - lift<T>;
         ml[64 + wave * 16 + lane] = l;
     }
     __syncthreads();
@@ -636,7 +650,8 @@ __device__ inline void emit_keys(const Args& a, Core<T, D, WAVES_KEYS>& core, co
         sum += w[k] * ml[64 + k * 16 + lane % 16];
     }
     const Sink<T> out{a, r.at, r.at / a.x.heads * a.x.ldo + int64_t(r.at % a.x.heads) * D, slot};
-    if (r.valid && wave == 0 && lane < 16) out.stats(cm, sum);
+    const float lg = log_sum(cm, sum), inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    if (r.valid && wave == 0 && lane < 16) out.stats(lg);
     float4 v[D / 64];  // quads wave * 4 + lane / 16 + 16 i
     float z = 0.0f;
 #pragma unroll
@@ -654,9 +669,9 @@ __device__ inline void emit_keys(const Args& a, Core<T, D, WAVES_KEYS>& core, co
     bad = (bad | bad >> 16) & 0xffff;
     if (r.valid && !(bad >> (lane % 16) & 1)) {
 #pragma unroll
-        for (int i = 0; i < D / 64; ++i) out.template quad<D>(4 * (wave * 4 + lane / 16 + 16 * i), v[i], sum);
+        for (int i = 0; i < D / 64; ++i) out.template quad<D>(4 * (wave * 4 + lane / 16 + 16 * i), times(v[i], inv), sum != 0.0f);
     }
-    if (bad) seen_alone<T, D>(a, in, r, bad, cm, sum, lane, slot, wave);
+    if (bad) seen_alone<T, D>(a, in, r, bad, lg, lane, slot, wave);
 }
 
 template <typename T, int D, int TILE>
@@ -816,7 +831,7 @@ __global__ __launch_bounds__(NW * 64, TILE == WAVES_KEYS && D == 512 ? 1 : D == 
     emit_keys<T, D>(a, core, in, r, lane, wave, a.p.np + split, reinterpret_cast<float*>(smem_raw));
 }
 
-// out = sum_i w_i O_i / sum_i w_i l_i, w_i = 2^(c m_i - max): W waves per
+// out = sum_i w_i O_i / sum_i w_i, w_i = 2^(lg_i - max lg): W waves per
 // (token, head), each for every W-th slot, D / 64 values a lane.
 template <typename T, int D, int W>
 __global__ __launch_bounds__(256) void attention_join_kernel(Args a) {
@@ -829,19 +844,19 @@ __global__ __launch_bounds__(256) void attention_join_kernel(Args a) {
     const int64_t tok = row / a.x.heads, head = row - tok * a.x.heads;
     if (token_row(a.b, tok, lane).seq < 0) return;  // (W > 1: the whole workgroup)
     const int slots = int(a.p.slots());
-    float cm = -INFINITY;
-    for (int i = lane; i < slots; i += WAVE) cm = fmaxf(cm, a.part_ml[i * rows + row].x);
-    cm = wave_max(cm);
-    float l = 0.0f, v[E];
+    float lg[2], w[2];  // the lane's slots (at most 64 of each kind)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+        lg[j] = lane + j * WAVE < slots ? a.part_lg[(lane + j * WAVE) * rows + row] : -INFINITY;
+    const float most = wave_max(fmaxf(lg[0], lg[1]));
+#pragma unroll
+    for (int j = 0; j < 2; ++j) w[j] = lg[j] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(lg[j] - most);
+    const float l = wave_sum(w[0] + w[1]), inv = l == 0.0f ? 0.0f : 1.0f / l;
+    float v[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) v[e] = 0.0f;
     for (int i0 = 0; i0 < slots; i0 += WAVE) {
-        float wl = 0.0f;
-        if (i0 + lane < slots) {
-            const float2 ml = a.part_ml[(i0 + lane) * rows + row];
-            wl = ml.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(ml.x - cm);
-            l += wl * ml.y;
-        }
+        const float wl = (i0 ? w[1] : w[0]) * inv;
         const int n = slots - i0 < WAVE ? slots - i0 : WAVE;
         // (eight slots' loads under way; what a slot without a share holds
         // was not written)
@@ -863,7 +878,6 @@ __global__ __launch_bounds__(256) void attention_join_kernel(Args a) {
             }
         }
     }
-    l = wave_sum(l);
     if constexpr (W > 1) {
 #pragma unroll
         for (int e = 0; e < E; ++e) sums[wave][lane * E + e] = v[e];
@@ -876,11 +890,10 @@ __global__ __launch_bounds__(256) void attention_join_kernel(Args a) {
             for (int k = 0; k < W; ++k) v[e] += sums[k][lane * E + e];
         }
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     T* out = static_cast<T*>(a.x.out) + tok * a.x.ldo + head * D + lane * E;
 #pragma unroll
-    for (int e = 0; e < E; ++e) out[e] = T(v[e] * inv);
-    if (lane == 0 && a.x.lse) a.x.lse[row] = l == 0.0f ? -INFINITY : (cm + __builtin_amdgcn_logf(l)) * 0.69314718055994531f;
+    for (int e = 0; e < E; ++e) out[e] = T(v[e]);
+    if (lane == 0 && a.x.lse) a.x.lse[row] = log_sum(most, l) * 0.69314718055994531f;
 }
 
 int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
@@ -941,7 +954,7 @@ void check(const PagedKv& kv, const PagedBatch& b, int heads) {
 
 int64_t part_bytes(const Plan& p, const PagedKv& kv, const PagedBatch& b, int heads) {
     const int64_t n = p.slots();
-    return n <= 1 ? 0 : n * b.t * heads * (kv.head_dim * 4 + 8);
+    return n <= 1 ? 0 : n * b.t * heads * (kv.head_dim * 4 + 4);
 }
 
 template <typename T, int D>
@@ -1024,7 +1037,7 @@ void launch_attention_shared(hipStream_t s, const PagedKv& kv, const PagedBatch&
     if (need) {
         if (!workspace || !aligned16(workspace)) fail(E_INVALID, "attention_shared: the workspace must be 16-byte aligned");
         a.part_o = static_cast<float*>(workspace);
-        a.part_ml = reinterpret_cast<float2*>(a.part_o + a.p.slots() * b.t * x.heads * kv.head_dim);
+        a.part_lg = a.part_o + a.p.slots() * b.t * x.heads * kv.head_dim;
     }
     const int64_t nsplit = a.p.whole ? 1 : a.p.np + (a.p.fused ? a.p.os : 0);
     a.prefix_blocks = up(int64_t(a.p.ntile) * kv.kv_heads * nsplit, 8);

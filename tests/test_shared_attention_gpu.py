@@ -438,3 +438,17 @@ def test_refuses_a_short_workspace():
     c.ws = c.ws[:-16]
     with pytest.raises(g.OmgError, match="workspace needs"):
         c.run()
+
+
+BATCHES = [([1] * 7, [20] * 7, 300), ([1] * 70, [90] * 70, 301), ([33, 40, 36, 47, 50], [0, 17, 30, 15, 40], 200),
+           ([3, 1, 2, 4, 1], [9, 0, 200, 4, 31], 77), ([50] * 45, [5] * 45, 70), ([9, 70], [400, 700], 0)]
+
+
+@pytest.mark.parametrize("new,before,prefix", BATCHES)
+@pytest.mark.parametrize("hd", [64, 128, 256, 512])
+def test_values_up_to_the_types_largest(hd, new, before, prefix):
+    """bf16 values of up to 3e38: sums over keys, unlike their mean, lie past f32's largest."""
+    rng = np.random.default_rng(51 + hd)
+    c = Call(rng, new, before, prefix, 16 if len(new) == 45 else 4, 8 if len(new) == 45 else 2, hd, dtype="bf16")
+    c.pool.v_raw.copy_((c.pool.v_raw.float() * 1e38).clamp_(-3e38, 3e38))
+    c.run().check()
