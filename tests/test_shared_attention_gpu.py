@@ -452,3 +452,18 @@ def test_values_up_to_the_types_largest(hd, new, before, prefix):
     c = Call(rng, new, before, prefix, 16 if len(new) == 45 else 4, 8 if len(new) == 45 else 2, hd, dtype="bf16")
     c.pool.v_raw.copy_((c.pool.v_raw.float() * 1e38).clamp_(-3e38, 3e38))
     c.run().check()
+
+
+@pytest.mark.parametrize("new,before,prefix", BATCHES)
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128, 256, 512])
+def test_equal_values_up_to_the_types_largest(hd, dtype, new, before, prefix):
+    """All keys' values alike, the type's largest among them: their mean within the probabilities' rounding, and finite."""
+    rng = np.random.default_rng(53 + hd)
+    c = Call(rng, new, before, prefix, 16 if len(new) == 45 else 4, 8 if len(new) == 45 else 2, hd, dtype=dtype)
+    most = torch.finfo(TYPES[dtype]).max
+    row = torch.randn(hd).to(TYPES[dtype])
+    row[::5], row[1::5] = most, -most
+    c.pool.v.copy_(row.cuda())
+    c.run().check()
+    assert bool(torch.isfinite(c.out).all())
