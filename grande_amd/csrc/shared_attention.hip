@@ -722,9 +722,11 @@ __global__ __launch_bounds__(NW * 64, TILE == WAVES_KEYS && D == 512 ? 1 : D == 
     if (int64_t(blockIdx.x) < a.prefix_blocks) {
         typedef Core<T, D, TILE> C;
         constexpr int M = TILE == WAVES_KEYS ? 16 : NW * C::RW;
+        // (too few rows for WAVES_16 are never fused)
+        const bool fused = TILE != WAVES_KEYS && a.p.fused, whole = TILE != WAVES_KEYS && a.p.whole;
         // Consecutive workgroups go to the 8 XCDs in turn: each XCD takes a
         // run of items, whose tiles share their keys in its L2.
-        const int64_t nsplit = a.p.whole ? 1 : a.p.np + (a.p.fused ? a.p.os : 0);
+        const int64_t nsplit = whole ? 1 : a.p.np + (fused ? a.p.os : 0);
         const int64_t items = int64_t(a.p.ntile) * G * nsplit;
         const int64_t item = (blockIdx.x % 8) * (a.prefix_blocks / 8) + blockIdx.x / 8;
         if (item >= items) return;
@@ -745,8 +747,8 @@ __global__ __launch_bounds__(NW * 64, TILE == WAVES_KEYS && D == 512 ? 1 : D == 
         C core;
         core.init(r.valid ? static_cast<const T*>(a.x.q) + tok * a.x.ldq + int64_t(head) * D : nullptr, lane);
         const Stream<T, D, TILE> st{a, g, wave, lane, smem};
-        if (a.p.whole || split < a.p.np) {
-            int kb = a.p.whole ? 0 : split * a.p.chunk_p, ke = a.p.whole ? P : imin(P, kb + a.p.chunk_p);
+        if (whole || split < a.p.np) {
+            int kb = whole ? 0 : split * a.p.chunk_p, ke = whole ? P : imin(P, kb + a.p.chunk_p);
             const int lo = w > 0 ? imax(0, P + r.own - w + 1) : 0;
             if (w > 0) {
                 // the first key that any of the workgroup's rows sees
@@ -760,9 +762,9 @@ __global__ __launch_bounds__(NW * 64, TILE == WAVES_KEYS && D == 512 ? 1 : D == 
             }
             if (kb < ke) st.run(core, a.b.prefix_table, (P - 1) >> a.page_shift, kb, ke, P, r.valid, lo, P);
         }
-        if (a.p.fused && (a.p.whole || split >= a.p.np)) {
-            const int ob = a.p.whole ? 0 : (split - a.p.np) * a.p.chunk_o;
-            const int oe = a.p.whole ? cap : imin(cap, ob + a.p.chunk_o);
+        if (fused && (whole || split >= a.p.np)) {
+            const int ob = whole ? 0 : (split - a.p.np) * a.p.chunk_o;
+            const int oe = whole ? cap : imin(cap, ob + a.p.chunk_o);
             for (int64_t s = s0; s <= s1 && s < a.b.nseq; ++s) {
                 // the sequence's tokens of this tile and the keys they see
                 const int64_t b0 = a.b.start ? a.b.start[s] : s, b1 = a.b.start ? a.b.start[s + 1] : s + 1;
@@ -781,10 +783,10 @@ __global__ __launch_bounds__(NW * 64, TILE == WAVES_KEYS && D == 512 ? 1 : D == 
             }
         }
         Keys in{g, 0, 0, 0, 0};
-        if (a.p.whole || split < a.p.np)
-            in.pb = a.p.whole ? 0 : split * a.p.chunk_p, in.pe = a.p.whole ? P : imin(P, in.pb + a.p.chunk_p);
-        if (a.p.fused && (a.p.whole || split >= a.p.np))
-            in.ob = a.p.whole ? 0 : (split - a.p.np) * a.p.chunk_o, in.oe = a.p.whole ? cap : imin(cap, in.ob + a.p.chunk_o);
+        if (whole || split < a.p.np)
+            in.pb = whole ? 0 : split * a.p.chunk_p, in.pe = whole ? P : imin(P, in.pb + a.p.chunk_p);
+        if (fused && (whole || split >= a.p.np))
+            in.ob = whole ? 0 : (split - a.p.np) * a.p.chunk_o, in.oe = whole ? cap : imin(cap, in.ob + a.p.chunk_o);
         if constexpr (TILE == WAVES_KEYS)
             emit_keys<T, D>(a, core, in, r, lane, wave, split, reinterpret_cast<float*>(smem_raw));
         else
