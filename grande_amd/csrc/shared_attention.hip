@@ -496,6 +496,13 @@ struct Stream {
 __device__ inline int imin(int a, int b) { return a < b ? a : b; }
 __device__ inline int imax(int a, int b) { return a > b ? a : b; }
 
+// The first key that the window of a query at row `own` behind `prefix` rows
+// leaves (own is below zero where a length is short of its sequence's tokens:
+// sums that saturate, one instruction each).
+__device__ inline int first_seen(int prefix, int own, int window) {
+    return window > 0 ? imax(0, __builtin_elementwise_sub_sat(__builtin_elementwise_add_sat(prefix, own), window - 1)) : 0;
+}
+
 // A lane's query row.
 struct Row {
     bool valid;
@@ -587,8 +594,8 @@ __device__ void seen_alone(const Args& a, const Keys& in, const Row& r, uint64_t
                 lost = __all(nan);
             }
         };
-        keys(a.b.prefix_table, (P - 1) >> a.page_shift, imax(in.pb, w > 0 ? P + own - w + 1 : 0), in.pe);
-        keys(a.b.table + seq * a.b.table_ld, int(a.b.max_pages) - 1, imax(in.ob, w > 0 ? own - w + 1 : 0),
+        keys(a.b.prefix_table, (P - 1) >> a.page_shift, imax(in.pb, first_seen(P, own, w)), in.pe);
+        keys(a.b.table + seq * a.b.table_ld, int(a.b.max_pages) - 1, imax(in.ob, first_seen(0, own, w)),
              imin(in.oe, own + 1));
         const Sink<T> out{a, at, tok * a.x.ldo + int64_t(head) * D, slot};
         const float inv = total == 0.0f ? 0.0f : 1.0f / total;
@@ -749,7 +756,7 @@ __global__ __launch_bounds__(NW * 64, TILE == WAVES_KEYS && D == 512 ? 1 : D == 
         const Stream<T, D, TILE> st{a, g, wave, lane, smem};
         if (whole || split < a.p.np) {
             int kb = whole ? 0 : split * a.p.chunk_p, ke = whole ? P : imin(P, kb + a.p.chunk_p);
-            const int lo = w > 0 ? imax(0, P + r.own - w + 1) : 0;
+            const int lo = first_seen(P, r.own, w);
             if (w > 0) {
                 // the first key that any of the workgroup's rows sees
                 int& first = *reinterpret_cast<int*>(smem_raw);  // (no tile has arrived yet)
@@ -772,11 +779,11 @@ __global__ __launch_bounds__(NW * 64, TILE == WAVES_KEYS && D == 512 ? 1 : D == 
                 if (ta > tb) continue;
                 const int len = a.b.lens[s];
                 const int ra = len - int(b1 - ta), rb = len - int(b1 - tb);
-                const int kb = imax(ob, w > 0 ? imax(0, ra - w + 1) / 32 * 32 : 0);
+                const int kb = imax(ob, first_seen(0, ra, w) / 32 * 32);
                 const int ke = imin(oe, rb + 1);
                 if (kb >= ke) continue;
                 const bool here = r.valid && r.seq == int(s);
-                const int lo = here ? (w > 0 ? imax(0, r.own - w + 1) : 0) : 0;
+                const int lo = here ? first_seen(0, r.own, w) : 0;
                 const int hi = here ? imin(r.own + 1, cap) : 0;
                 st.run(core, a.b.table + s * a.b.table_ld, int(a.b.max_pages) - 1, kb, ke, imin(len, cap), r.valid, lo,
                        hi);
@@ -833,12 +840,12 @@ __global__ __launch_bounds__(NW * 64, TILE == WAVES_KEYS && D == 512 ? 1 : D == 
     // the keys that the tile's first and last tokens see
     const int64_t last = (tile * 16 + 15 < (b1 - b0) * hpg ? tile * 16 + 15 : (b1 - b0) * hpg - 1) / hpg;
     const int ra = len - int(b1 - b0 - tile * 16 / hpg), rb = len - int(b1 - b0 - last);
-    const int kb = imax(split * a.p.chunk_o, w > 0 ? imax(0, ra - w + 1) / 32 * 32 : 0);
+    const int kb = imax(split * a.p.chunk_o, first_seen(0, ra, w) / 32 * 32);
     const int ke = imin(imin(cap, (split + 1) * a.p.chunk_o), rb + 1);
     const Stream<T, D, WAVES_KEYS> st{a, g, wave, lane, smem};
     if (kb < ke)
         st.run(core, a.b.table + s * a.b.table_ld, int(a.b.max_pages) - 1, kb, ke, imin(len, cap), r.valid,
-               w > 0 ? imax(0, r.own - w + 1) : 0, imin(r.own + 1, cap));
+               first_seen(0, r.own, w), imin(r.own + 1, cap));
     const Keys in{g, 0, 0, split * a.p.chunk_o, imin(cap, (split + 1) * a.p.chunk_o)};
     emit_keys<T, D>(a, core, in, r, lane, wave, a.p.np + split, reinterpret_cast<float*>(smem_raw));
 }

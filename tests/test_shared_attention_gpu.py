@@ -467,3 +467,18 @@ def test_equal_values_up_to_the_types_largest(hd, dtype, new, before, prefix):
     c.pool.v.copy_(row.cuda())
     c.run().check()
     assert bool(torch.isfinite(c.out).all())
+
+
+@pytest.mark.parametrize("new", [[1] * 4, [40, 35, 50, 33], [6, 5, 9, 7]])
+def test_the_largest_window_is_no_window(new):
+    """A window of 2^31 - 1, with sequences whose lengths are short of their tokens: positions below zero."""
+    rng = np.random.default_rng(55)
+    c = Call(rng, new, [0, 20, 3, 0], 2, 4, 2, 64)
+    c.pool.lens.copy_(torch.tensor([max(0, new[0] - 6), new[1] + 20, new[2] // 2, 0], dtype=torch.int32))
+    c.run()
+    torch.cuda.synchronize()
+    whole = c.out.clone(), c.lse.clone()
+    c.window = 2 ** 31 - 1
+    c.run()
+    torch.cuda.synchronize()
+    assert torch.equal(whole[0], c.out) and torch.equal(whole[1], c.lse)
