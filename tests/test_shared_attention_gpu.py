@@ -482,3 +482,11 @@ def test_the_largest_window_is_no_window(new):
     c.run()
     torch.cuda.synchronize()
     assert torch.equal(whole[0], c.out) and torch.equal(whole[1], c.lse)
+
+
+@pytest.mark.parametrize("new,heads", [([1], 4), ([1, 1], 2), ([5], 2)])
+def test_the_most_splits_of_prefix_and_own_rows(new, heads):
+    """64 splits each: a join of 128 partial results."""
+    rng = np.random.default_rng(57)
+    Call(rng, new, [9000] * len(new), 5000, heads, 1, 128, page=64).run().check()
+    Call(rng, new, [9000] * len(new), 5000, heads, 1, 128, page=64, window=9700, dtype="bf16").run().check()
