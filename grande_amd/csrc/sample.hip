@@ -38,7 +38,7 @@
 // (the rows whose kept tokens fit no list); 64 rows of 262,144 (bf16, top_p)
 // 104 us: stats 24 (37 vector instructions a logit, most of them exp's),
 // long 20, bins 26, draw 39 (the last rows' cuts, one workgroup each); 256
-// rows of 128,257 (f32, mixed filters) 107 us, of which stats 33 (3.9 TB/s).
+// rows of 128,257 (f32, mixed filters) 111 us, of which stats 33 (3.9 TB/s).
 #include <algorithm>
 #include <string>
 
@@ -938,7 +938,7 @@ struct Pending {
     uint32_t arrived[2];
     uint32_t edges;      // logits of the bin
 };
-// What sample_stats leaves of a long row's 2,048 logits.
+// What sample_stats leaves of CHUNK logits of a long row.
 struct Chunk {
     float max;
     uint32_t first;  // index of the first maximum
@@ -1174,7 +1174,11 @@ __global__ __launch_bounds__(NT) void sample_row(SampleArgs a, Workspace ws) {
 // the L2s, which are one an XCD: the stores are done when they are waited
 // for, and no fence, which would write back and invalidate an L2, is needed
 // (one a workgroup took 50 us of a pass over 16.8 million logits, one a wave
-// 300).
+// 300).  This relies on the hardware and not on the language's memory model,
+// which orders relaxed accesses to different places by fences alone: on gfx950
+// stores and loads of agent scope carry sc1, and a store has left vmcnt when
+// other XCDs can read it.  The barrier has every wave's wait before the one
+// add; the loads follow the add's return, which the second barrier waits for.
 __device__ inline bool last_of(uint32_t* arrived, Common& sm) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();

@@ -36,18 +36,25 @@
 // 16 rows x 16 bytes, V's 4 rows x 64 bytes or 8 x 32 (counted: none meet).
 //
 // Measured, and what bounds it:
-//   questions, 6,300 tokens x 8 heads of 256 on 8,000 keys (f16): 460-490 us,
-//     850-900 TFLOP/s of the 1,190 that a product of 8,192^3 reaches.  392
+//   questions, 6,300 tokens x 8 heads of 256 on 8,000 keys (f16): 460-500 us,
+//     830-900 TFLOP/s of the 1,190 that a product of 8,192^3 reaches.  392
 //     tiles on 512 places; MFMAs take 45 % of the busy CUs' cycles, other
-//     vector instructions 32 %, LDS 22 %: a tile is one chain of dependent
-//     steps with two waves a SIMD to fill it, registers allow no third.
+//     vector instructions 33 %, LDS 22 %: a tile is one chain of dependent
+//     steps with two waves a SIMD to fill it, registers allow no third (256
+//     vector registers, 4 spilled).
 //   64 answers' tokens x 32 heads of 128 on 65,521 shared and 131,000 own
 //     keys (bf16): 153 us, 4.4 TB/s: the bytes.
 //   208 answers' tokens x 8 heads of 256 on 8,000 keys: 38 + 8 us: 256 items
 //     of 16 tiles, the same chain (2.5 us a tile), and 29 MB of partials.
-//   12 answers' tokens x 4 heads of 256 on 2,000 keys: 8.5 + 4.5 us: latency.
+//   12 answers' tokens x 4 heads of 256 on 2,000 keys: 8.5 + 4 us: latency.
 //   questions, 470 tokens x 8 heads of 512 on 2,000 keys (bf16): 43 + 12 us:
 //     61 MB of partials written and read.
+//   208 answers' tokens x 8 heads of 512 on 8,000 keys (f16): 100 us: one
+//     workgroup a CU, by the own items' 128 KiB of LDS.
+//   A window shortens work items and does not lessen them: of the 208 answers'
+//     prefix splits most have nothing to do at a window of 512, 46 -> 32 us;
+//     64 answers on 65,521 keys at 1,024 154 -> 66 us; the 6,300 questions'
+//     tokens, whose items are not split, at 512 480 -> 61 us.
 #include <algorithm>
 #include <atomic>
 #include <climits>
@@ -523,6 +530,10 @@ struct Keys {
 // whose row it is (with log sum lg); a wave writes the quads of head dims it
 // has (quarter < 0: all).  A row whose scores hold a NaN has it in lg, and in
 // its outputs as they are.
+//   A wave takes its rows one after another and a row's keys four at a time,
+// until every element is NaN: 0.3 to 0.4 us a key and row.  One infinite
+// value in a prefix of 8,000 keys, which all rows see: 208 answers' tokens x 8
+// heads of 256 45 us -> 4.4 ms, 6,300 questions' tokens 0.5 -> 111 ms.
 template <typename T, int D>
 __device__ void seen_alone(const Args& a, const Keys& in, const Row& r, uint64_t rows, float lg, int lane, int64_t slot,
                            int quarter) {
@@ -917,8 +928,8 @@ __global__ __launch_bounds__(256) void attention_join_kernel(Args a) {
 
 int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
-// Work items fill the chip's 256 CUs twice (head_dim 512: once, by LDS)
-// where the keys are long enough to be split.
+// Work items fill the places that the chip's 256 CUs are counted to have
+// where the keys are long enough to be split.  (The window is no part of it.)
 Plan plan(const PagedKv& kv, const PagedBatch& b, int heads) {
     Plan p{};
     const int64_t hpg = heads / kv.kv_heads, rows = b.t * hpg, max_len = b.max_pages * kv.page, P = b.prefix_len;
@@ -934,7 +945,8 @@ Plan plan(const PagedKv& kv, const PagedBatch& b, int heads) {
     const int64_t base = p.ntile * int64_t(kv.kv_heads);
     // Two workgroups on each of 256 CUs (head_dim 64: four) take up the launch
     // at once; a few items more wait for a second round (504 items of 512-wide
-    // heads 57 us, 567 78 us).
+    // heads 57 us, 567 78 us).  Launches of 512-wide heads with own items hold
+    // one a CU, by LDS, and are counted alike.
     const int64_t SLOTS = kv.head_dim == 64 ? 1024 : 512;
     auto splits = [&](int64_t keys, int64_t k, int64_t least, int& n, int& chunk) {
         k = std::max<int64_t>(1, std::min<int64_t>({k, (keys + least - 1) / least, 64}));

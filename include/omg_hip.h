@@ -400,10 +400,15 @@ int omg_dev_kv_append(const omg_paged_kv *kv, const omg_paged_batch *b, const om
  * NULL); a token that sees no key gets zeros and -infinity.  The prefix's
  * keys and values are read once for a tile of query rows, whatever
  * sequences these belong to.  What stands in cache rows that a token does
- * not see, infinities and NaN among it, does not reach the token.
+ * not see, infinities and NaN among it, does not reach the token.  (Where a
+ * value is infinite or NaN, or a sum of bf16 values passes f32's largest, the
+ * rows that meet it take all their keys again one by one: right, and some
+ * hundred times slower.)  A window saves the keys outside it; the work is
+ * shared out as without one.
  * scale positive; q and out 16-byte aligned and apart, ldq and ldo multiples
- * of 8.  f32 sums; the softmax's probabilities are rounded to the cache's type for
- * their product with the values.
+ * of 8.  f32 sums; the softmax's probabilities are rounded to the cache's type
+ * for their product with the values, not in their sum: equal values come out
+ * within half a step.  A mean of finite values is finite.
  *
  * workspace: omg_dev_attention_shared_workspace bytes (a function of the
  * shapes alone: nseq, t, max_pages, prefix_len, heads and the cache's;
