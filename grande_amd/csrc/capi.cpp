@@ -706,6 +706,23 @@ int omg_dev_attention_shared(const omg_paged_kv* kv, const omg_paged_batch* b, i
     });
 }
 
+int64_t omg_dev_attention_tree_workspace(const omg_paged_kv* kv, const omg_paged_batch* b, int heads) {
+    int64_t n = 0;
+    const int rc = guard([&] { n = omg::attention_tree_workspace(paged_kv(kv), paged_batch(b), heads); });
+    return rc == OMG_OK ? n : rc;
+}
+
+int omg_dev_attention_tree(const omg_paged_kv* kv, const omg_paged_batch* b, int heads, const void* q, int64_t ldq,
+                           void* out, int64_t ldo, float* lse, float scale, const uint32_t* mask, int64_t mask_ld,
+                           int window, const int32_t* positions, void* workspace, size_t workspace_bytes,
+                           void* stream) {
+    return guard([&] {
+        const omg::SharedAttn x{heads, q, ldq, out, ldo, lse, scale, window};
+        omg::launch_attention_tree(static_cast<hipStream_t>(stream), paged_kv(kv), paged_batch(b), x,
+                                   {mask, mask_ld, positions}, workspace, workspace_bytes);
+    });
+}
+
 int64_t omg_dev_sample_workspace(int64_t rows, int64_t vocab) {
     int64_t n = 0;
     const int rc = guard([&] { n = omg::sample_workspace(rows, vocab); });

@@ -349,6 +349,26 @@ int64_t attention_shared_workspace(const PagedKv& kv, const PagedBatch& b, int h
 void launch_attention_shared(hipStream_t s, const PagedKv& kv, const PagedBatch& b, const SharedAttn& x,
                              void* workspace, size_t bytes);
 
+// The same for drafted tokens (tree_attention.hip): of a sequence's new rows a
+// token sees those whose bits its mask has.
+struct TreeMask {
+    const uint32_t* mask;  // [t][words]
+    int64_t words;
+    const int32_t* positions;  // [t], with a window
+    // Bits of the new rows rel .. rel + 31 of the sequence (rows before the
+    // new ones: set) that token `tok` sees.
+    __device__ uint32_t seen(int64_t tok, int rel) const {
+        const int w = rel >> 5, sh = rel & 31;
+        const uint32_t* m = mask + tok * words;
+        const uint32_t lo = w < 0 ? ~0u : w < words ? m[w] : 0u;
+        const uint32_t hi = w + 1 < 0 ? ~0u : w + 1 < words ? m[w + 1] : 0u;
+        return uint32_t((uint64_t(hi) << 32 | lo) >> sh);
+    }
+};
+int64_t attention_tree_workspace(const PagedKv& kv, const PagedBatch& b, int heads);
+void launch_attention_tree(hipStream_t s, const PagedKv& kv, const PagedBatch& b, const SharedAttn& x,
+                           const TreeMask& tree, void* workspace, size_t bytes);
+
 // ---- sampling (sample.hip) ----
 struct SampleArgs {  // omg_sample_args
     int dtype;

@@ -577,6 +577,21 @@ class PagedKv(L.omg_paged_kv):
         L.check(L.lib().omg_dev_attention_shared(self, batch, heads, q_ptr, ldq, out_ptr, ldo, lse, scale, window,
                                                  workspace, workspace_bytes, stream))
 
+    def attention_tree_workspace(self, batch: PagedBatch, heads: int) -> int:
+        """Bytes of workspace that `attention_tree` needs for batches of these sizes."""
+        return L.size(L.lib().omg_dev_attention_tree_workspace(self, batch, heads))
+
+    def attention_tree(self, batch: PagedBatch, heads: int, q_ptr: int, ldq: int, out_ptr: int, ldo: int, scale: float,
+                       mask_ptr: int, mask_ld: int, *, window: int = 0, positions: int | None = None,
+                       lse: int | None = None, workspace: int | None = None, workspace_bytes: int = 0,
+                       stream: int | None = None) -> None:
+        """omg_dev_attention_tree: as `attention`, for drafted tokens; of its
+        sequence's new rows a token sees those whose bits are set in its
+        mask_ld 32-bit words at mask_ptr.  A window counts back from the
+        tokens' int32 `positions`."""
+        L.check(L.lib().omg_dev_attention_tree(self, batch, heads, q_ptr, ldq, out_ptr, ldo, lse, scale, mask_ptr,
+                                               mask_ld, window, positions, workspace, workspace_bytes, stream))
+
 
 def sample_workspace(rows: int, vocab: int) -> int:
     """Bytes of workspace that `sample` needs."""

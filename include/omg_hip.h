@@ -419,6 +419,22 @@ int omg_dev_attention_shared(const omg_paged_kv *kv, const omg_paged_batch *b, i
                              void *out, int64_t ldo, float *lse, float scale, int window, void *workspace,
                              size_t workspace_bytes, void *stream);
 
+/* The same for drafted tokens: of its sequence's new rows a token sees not
+ * those up to its own but those whose bits are set in its mask, bit j % 32 of
+ * word mask[i * mask_ld + j / 32] for token row i and the j-th new token of
+ * its sequence (the token itself has a bit like any other; new tokens past
+ * the words are not seen).  For a tree the bits are the token's ancestors and
+ * itself.  Its sequence's rows before the new ones and the prefix it sees
+ * whole or, with a window > 0, as far as they lie less than `window`
+ * positions before positions[i] (device int32 [t], the rows that an append
+ * takes from its table; may be NULL without a window); the window leaves the
+ * new rows to the masks.  mask_ld 1 to 2^20. */
+int64_t omg_dev_attention_tree_workspace(const omg_paged_kv *kv, const omg_paged_batch *b, int heads);
+int omg_dev_attention_tree(const omg_paged_kv *kv, const omg_paged_batch *b, int heads, const void *q, int64_t ldq,
+                           void *out, int64_t ldo, float *lse, float scale, const uint32_t *mask, int64_t mask_ld,
+                           int window, const int32_t *positions, void *workspace, size_t workspace_bytes,
+                           void *stream);
+
 /* The next token of each row of logits (row r, token i at logits[r * ld + i];
  * dtype OMG_ELEM_F32, F16 or BF16; any ld from vocab up), drawn with the
  * given random number u[r] in [0, 1).  With z the row, M its maximum and
