@@ -60,6 +60,7 @@
 #include <algorithm>
 #include <atomic>
 #include <climits>
+#include <cmath>
 #include <string>
 
 #include "common.h"
@@ -645,10 +646,11 @@ __device__ void seen_alone(const Args& a, const Keys& in, const Row& r, uint64_t
     }
 }
 
-// The results of a wave's rows (not KEYS).
-template <typename T, int D, int TILE, bool MASKED>
+// The results of a wave's rows (not KEYS).  `place`: called ahead of
+// seen_alone, which needs the rows' sequences.
+template <typename T, int D, int TILE, bool MASKED, typename F>
 __device__ inline void emit(const Args& a, Core<T, D, TILE>& core, const Keys& in, const Row& r, int lane,
-                            int64_t slot) {
+                            int64_t slot, F place) {
     typedef Core<T, D, TILE> C;
     const float l = C::row_sum(core.l), inv = l == 0.0f ? 0.0f : 1.0f / l;
     const float lg = log_sum(core.m * a.c - lift<T>, l);
@@ -674,13 +676,13 @@ __device__ inline void emit(const Args& a, Core<T, D, TILE>& core, const Keys& i
                                            inv),
                                      l != 0.0f);
     }
-    if (bad) seen_alone<T, D, MASKED>(a, in, r, bad, lg, lane, slot, -1);
+    if (bad) place(), seen_alone<T, D, MASKED>(a, in, r, bad, lg, lane, slot, -1);
 }
 
 // The four waves' results for the same 16 rows, joined through LDS.
-template <typename T, int D, bool MASKED>
+template <typename T, int D, bool MASKED, typename F>
 __device__ inline void emit_keys(const Args& a, Core<T, D, WAVES_KEYS>& core, const Keys& in, const Row& r, int lane,
-                                 int wave, int64_t slot, float* smem) {
+                                 int wave, int64_t slot, float* smem, F place) {
     typedef Core<T, D, WAVES_KEYS> C;
     const float l = C::row_sum(core.l);
     __syncthreads();  // every wave is done with its tiles
@@ -725,7 +727,7 @@ __device__ inline void emit_keys(const Args& a, Core<T, D, WAVES_KEYS>& core, co
 #pragma unroll
         for (int i = 0; i < D / 64; ++i) out.template quad<D>(4 * (wave * 4 + lane / 16 + 16 * i), times(v[i], inv), sum != 0.0f);
     }
-    if (bad) seen_alone<T, D, MASKED>(a, in, r, bad, lg, lane, slot, wave);
+    if (bad) place(), seen_alone<T, D, MASKED>(a, in, r, bad, lg, lane, slot, wave);
 }
 
 template <typename T, int D, int TILE, bool MASKED>
@@ -796,11 +798,20 @@ __global__ __launch_bounds__(NW * 64, TILE == WAVES_KEYS && D == 512 ? 1 : D == 
         Row r{R < rows, int(tok * a.x.heads + head), 0, 0};
         const int64_t tok0 = row0 / hpg, tok1 = ((row0 + M < rows ? row0 + M : rows) - 1) / hpg;
         int64_t s0 = tok0, s1 = tok1;
-        if (a.b.start) {
-            s0 = count_le(a.b.start, a.b.nseq, tok0, lane);
-            s1 = count_le(a.b.start, a.b.nseq, tok1, lane);
-        }
-        place(r, tok, s0, s1);
+        // The rows' sequences, which prefix keys without a window do not ask
+        // for (searches: dependent loads ahead of the first tile).
+        auto find = [&] {
+            if (a.b.start) {
+                s0 = count_le(a.b.start, a.b.nseq, tok0, lane);
+                s1 = count_le(a.b.start, a.b.nseq, tok1, lane);
+            }
+            place(r, r.at / a.x.heads, s0, s1);  // (the row's token again: no register holds it until here)
+        };
+        const bool placed = w > 0 || whole || split >= a.p.np;
+        if (placed)
+            find();
+        else if (a.b.start)
+            r.valid = r.valid && tok >= a.b.start[0] && tok < a.b.start[a.b.nseq];
         C core;
         core.init(r.valid ? static_cast<const T*>(a.x.q) + tok * a.x.ldq + int64_t(head) * D : nullptr, lane);
         const Stream<T, D, TILE> st{a, g, wave, lane, smem};
@@ -853,9 +864,10 @@ __global__ __launch_bounds__(NW * 64, TILE == WAVES_KEYS && D == 512 ? 1 : D == 
         if (fused && (whole || split >= a.p.np))
             in.ob = whole ? 0 : (split - a.p.np) * a.p.chunk_o, in.oe = whole ? cap : imin(cap, in.ob + a.p.chunk_o);
         if constexpr (TILE == WAVES_KEYS)
-            emit_keys<T, D, MASKED>(a, core, in, r, lane, wave, split, reinterpret_cast<float*>(smem_raw));
+            emit_keys<T, D, MASKED>(a, core, in, r, lane, wave, split, reinterpret_cast<float*>(smem_raw),
+                                    [&] { if (!placed) find(); });
         else
-            emit<T, D, TILE, MASKED>(a, core, in, r, lane, split);
+            emit<T, D, TILE, MASKED>(a, core, in, r, lane, split, [&] { if (!placed) find(); });
         return;
     }
 
@@ -915,7 +927,7 @@ __global__ __launch_bounds__(NW * 64, TILE == WAVES_KEYS && D == 512 ? 1 : D == 
                first_seen(0, r.own, w), imin(r.own + 1, cap));
     }
     const Keys in{g, 0, 0, split * a.p.chunk_o, imin(cap, (split + 1) * a.p.chunk_o)};
-    emit_keys<T, D, MASKED>(a, core, in, r, lane, wave, a.p.np + split, reinterpret_cast<float*>(smem_raw));
+    emit_keys<T, D, MASKED>(a, core, in, r, lane, wave, a.p.np + split, reinterpret_cast<float*>(smem_raw), [] {});
 }
 
 // out = sum_i w_i O_i / sum_i w_i, w_i = 2^(lg_i - max lg): W waves per
@@ -1107,15 +1119,15 @@ void launch_t(hipStream_t s, const Args& a, unsigned blocks) {
     }
 }
 
-template <bool MASKED>
+template <bool MASKED, typename F>
 void launch_attention(hipStream_t s, const PagedKv& kv, const PagedBatch& b, const SharedAttn& x, const TreeMask& tree,
-                      void* workspace, size_t bytes, const char* who) {
+                      F planned, void* workspace, size_t bytes, const char* who) {
     const std::string name(who);
     check(kv, b, x.heads, who);
     check_rows(kv, x, who);
     Args a{};
     a.kv = kv, a.b = b, a.x = x, a.tree = tree;
-    a.p = plan(kv, b, x.heads);
+    a.p = planned(kv, b, x.heads);
     a.hpg = x.heads / kv.kv_heads;
     a.page_shift = log2_of(kv.page);
     a.max_len = b.max_pages * kv.page;

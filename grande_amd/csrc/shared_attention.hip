@@ -11,7 +11,7 @@ int64_t attention_shared_workspace(const PagedKv& kv, const PagedBatch& b, int h
 
 void launch_attention_shared(hipStream_t s, const PagedKv& kv, const PagedBatch& b, const SharedAttn& x,
                              void* workspace, size_t bytes) {
-    launch_attention<false>(s, kv, b, x, TreeMask{}, workspace, bytes, "attention_shared");
+    launch_attention<false>(s, kv, b, x, TreeMask{}, plan, workspace, bytes, "attention_shared");
 }
 
 }  // namespace omg
