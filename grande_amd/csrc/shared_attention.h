@@ -60,7 +60,6 @@
 #include <algorithm>
 #include <atomic>
 #include <climits>
-#include <cmath>
 #include <string>
 
 #include "common.h"

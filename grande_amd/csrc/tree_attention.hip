@@ -8,53 +8,63 @@ namespace omg {
 
 namespace {
 
-// The splits of least time by a model of the launch: a work item takes so long
-// a tile of keys (a chain of dependent steps: hardly longer with two or three
-// workgroups on the CU) and two tiles' time besides; the places that the chip
-// has take items in rounds; a slot of partial results is written and read.
+// The tile and the splits of least time by a model of the launch: a work item
+// takes so long a tile of keys (a chain of dependent steps: hardly longer with
+// two or three workgroups on the CU) and two tiles' time besides; the places
+// that the chip has take items in rounds; a slot of partial results is written
+// and read.  Measured, for 32 and 16 rows a wave: 1.76 and 0.97 us a tile of
+// 256-wide heads, 1.24 and 0.67 of 128-wide ones.  (One split of the 8,000 keys
+// for 2,100 tokens x 8 heads of 256, 132 items, 459 us, three 189; the best at 16
+// rows a wave 280.  70 tokens x 4 heads on 2,000 keys 17 us at 32 rows, 13 at
+// 16.)
 Plan plan_tree(const PagedKv& kv, const PagedBatch& b, int heads) {
-    Plan p = plan(kv, b, heads);  // the tile shape and whether own keys go into its tiles
+    const Plan from = plan(kv, b, heads);
     const int64_t hpg = heads / kv.kv_heads, rows = b.t * hpg, max_len = b.max_pages * kv.page, P = b.prefix_len;
-    const int64_t M = p.tile == WAVES_KEYS ? 16 : p.tile == WAVES_16 ? 64 : 128;
-    const int64_t base = p.ntile * int64_t(kv.kv_heads);
-    const int D = kv.head_dim, KT = p.tile == WAVES_KEYS || D == 512 ? 16 : 32;
-    const double tile_us = 0.7 + D / 240.0, slot_us = double(b.t) * heads * D * 8 / 4.5e6;
-    const int64_t places = 256 * (D == 64 ? 4 : D == 128 ? 3 : D == 512 && !p.fused ? 1 : 2);
-    auto tiles = [&](int64_t keys) { return double((keys + KT - 1) / KT) / (p.tile == WAVES_KEYS ? NW : 1) + 2; };
+    const int D = kv.head_dim;
+    const double slot_us = double(b.t) * heads * D * 8 / 4.5e6;
     auto chunk = [](int64_t keys, int64_t n) { return up((keys + n - 1) / n, 32); };
-    double best = 1e30;
-    const Plan from = p;
-    if (p.fused) {
-        // A tile runs through the own keys of the sequences it holds.
-        const int64_t held = std::min<int64_t>(b.nseq, M * b.nseq / rows + 2);
-        auto take = [&](Plan q, double items, double most) {
-            const double t = std::max(1.0, std::ceil(items / places)) * most * tile_us +
-                             (q.whole ? 0.0 : 3.0 + slot_us * (q.np + q.os));
-            if (t < best) best = t, p = q;
-        };
+    Plan best = from;
+    double best_us = 1e30;
+    for (const int tile : {int(WAVES_16), int(WAVES_32)}) {
+        if (from.tile == WAVES_KEYS || (tile == WAVES_32 && D == 512)) continue;
         Plan q = from;
+        q.tile = tile;
+        const int64_t M = tile == WAVES_16 ? 64 : 128;
+        q.ntile = int((rows + M - 1) / M);
+        const int64_t base = q.ntile * int64_t(kv.kv_heads);
+        const int KT = D == 512 ? 16 : 32;
+        const double tile_us = (0.7 + D / 240.0) * (tile == WAVES_16 ? 0.55 : 1.0);
+        const int64_t places = 256 * (D == 64 ? 4 : D == 128 ? 3 : D == 512 && !q.fused ? 1 : 2);
+        auto tiles = [&](int64_t keys) { return double((keys + KT - 1) / KT) + 2; };
+        auto take = [&](const Plan& p, double most) {
+            const int64_t nsplit = p.whole ? 1 : p.np + (p.fused ? p.os : 0);
+            const double us = double((base * nsplit + places - 1) / places) * most * tile_us +
+                              (p.slots() > 1 ? 3.0 + slot_us * p.slots() : 0.0);
+            if (us < best_us) best_us = us, best = p;
+        };
+        if (!q.fused) {  // (the own keys' items as they are)
+            if (P == 0) take(q, 0);
+            for (int n = 1; n <= 64 && P > 0; ++n) {
+                q.chunk_p = int(chunk(P, n)), q.np = int((P + q.chunk_p - 1) / q.chunk_p);
+                take(q, tiles(q.chunk_p));
+            }
+            continue;
+        }
+        // A tile runs through the own keys of each sequence that it holds.
+        const int64_t held = std::min<int64_t>(b.nseq, M * b.nseq / rows + 2);
         q.whole = true, q.np = 0, q.chunk_p = 0, q.os = 1, q.chunk_o = int(std::min<int64_t>(up(max_len, 32), INT_MAX / 2));
-        take(q, double(base), tiles(P) + held * tiles(max_len));
+        take(q, tiles(P) + held * tiles(max_len));
         q.whole = false;
-        for (int np = P > 0 ? 1 : 0; np <= (P > 0 ? 64 : 0); ++np) {
-            if (np) q.chunk_p = int(chunk(P, np)), q.np = int((P + q.chunk_p - 1) / q.chunk_p);
+        for (int n = 1; n <= (P > 0 ? 64 : 1); ++n) {
+            if (P > 0) q.chunk_p = int(chunk(P, n)), q.np = int((P + q.chunk_p - 1) / q.chunk_p);
             for (int os = 1; os <= 64; os *= 2) {
                 q.chunk_o = int(std::min<int64_t>(chunk(max_len, os), INT_MAX / 2));
                 q.os = int((max_len + q.chunk_o - 1) / q.chunk_o);
-                take(q, double(base) * (q.np + q.os),
-                     std::max(np ? tiles(q.chunk_p) : 0.0, held * tiles(std::min<int64_t>(q.chunk_o, max_len))));
+                take(q, std::max(P > 0 ? tiles(q.chunk_p) : 0.0, held * tiles(std::min<int64_t>(q.chunk_o, max_len))));
             }
         }
-        return p;
     }
-    for (int np = 1; np <= 64 && P > 0; ++np) {
-        Plan q = from;
-        q.chunk_p = int(chunk(P, np)), q.np = int((P + q.chunk_p - 1) / q.chunk_p);
-        const double items = double(base) * q.np;
-        const double t = std::max(1.0, std::ceil(items / places)) * tiles(q.chunk_p) * tile_us + slot_us * (q.np + q.os);
-        if (t < best) best = t, p = q;
-    }
-    return p;
+    return best;
 }
 
 }  // namespace
