@@ -723,6 +723,25 @@ int omg_dev_attention_tree(const omg_paged_kv* kv, const omg_paged_batch* b, int
     });
 }
 
+int omg_dev_kv_keep(const omg_paged_kv* kv, const omg_paged_batch* b, const int32_t* rows, int64_t rows_ld,
+                    int64_t count, const int32_t* first, int per_head, const int32_t* to_table, int64_t to_ld,
+                    void* stream) {
+    return guard([&] {
+        omg::launch_kv_keep(static_cast<hipStream_t>(stream), paged_kv(kv), paged_batch(b),
+                            {rows, rows_ld, count, first, per_head, to_table, to_ld});
+    });
+}
+
+int omg_dev_kv_evict(const omg_paged_kv* kv, const omg_paged_batch* b, int64_t keep, int64_t recent, float* weights,
+                     int64_t ldw, int32_t* rows, float* kept, int64_t kept_ld, const int32_t* to_table, int64_t to_ld,
+                     void* stream) {
+    return guard([&] {
+        const bool own = !kept || kept == weights;
+        omg::launch_kv_evict(static_cast<hipStream_t>(stream), paged_kv(kv), paged_batch(b),
+                             {keep, recent, weights, ldw, rows, own ? weights : kept, own ? ldw : kept_ld, to_table, to_ld});
+    });
+}
+
 int64_t omg_dev_sample_workspace(int64_t rows, int64_t vocab) {
     int64_t n = 0;
     const int rc = guard([&] { n = omg::sample_workspace(rows, vocab); });

@@ -369,6 +369,29 @@ int64_t attention_tree_workspace(const PagedKv& kv, const PagedBatch& b, int hea
 void launch_attention_tree(hipStream_t s, const PagedKv& kv, const PagedBatch& b, const SharedAttn& x,
                            const TreeMask& tree, void* workspace, size_t bytes);
 
+// ---- rows that stay (keep.hip) ----
+// Row first[s] + j of a sequence becomes its row rows[j].
+struct KeepRows {
+    const int32_t* rows;  // [nseq] or [nseq][kv_heads] lists, rows_ld apart
+    int64_t rows_ld, count;
+    const int32_t* first;  // [nseq] or null: 0
+    int per_head;
+    const int32_t* to_table;  // [nseq][to_ld]; null: in place
+    int64_t to_ld;
+};
+void launch_kv_keep(hipStream_t s, const PagedKv& kv, const PagedBatch& b, const KeepRows& x);
+struct EvictRows {
+    int64_t keep, recent;
+    const float* weights;  // [nseq][kv_heads] lists, ldw apart
+    int64_t ldw;
+    int32_t* rows;  // [nseq][kv_heads][keep]
+    float* kept;    // lists kept_ld apart; the weights' own: in place
+    int64_t kept_ld;
+    const int32_t* to_table;
+    int64_t to_ld;
+};
+void launch_kv_evict(hipStream_t s, const PagedKv& kv, const PagedBatch& b, const EvictRows& x);
+
 // ---- sampling (sample.hip) ----
 struct SampleArgs {  // omg_sample_args
     int dtype;

@@ -592,6 +592,24 @@ class PagedKv(L.omg_paged_kv):
         L.check(L.lib().omg_dev_attention_tree(self, batch, heads, q_ptr, ldq, out_ptr, ldo, lse, scale, mask_ptr,
                                                mask_ld, window, positions, workspace, workspace_bytes, stream))
 
+    def keep(self, batch: PagedBatch, rows_ptr: int, rows_ld: int, count: int, *, first: int | None = None,
+             per_head: bool = False, to_table: int | None = None, to_ld: int = 0, stream: int | None = None) -> None:
+        """omg_dev_kv_keep: row first[s] + j of each sequence becomes its row
+        rows[j], for the `count` entries of its list (one for all KV heads, or
+        `per_head`): in place, or on the pages of to_table [nseq][to_ld]."""
+        L.check(L.lib().omg_dev_kv_keep(self, batch, rows_ptr, rows_ld, count, first, int(per_head), to_table, to_ld,
+                                        stream))
+
+    def evict(self, batch: PagedBatch, keep: int, recent: int, weights_ptr: int, ldw: int, rows_ptr: int, *,
+              kept_weights: int | None = None, kept_ld: int = 0, to_table: int | None = None, to_ld: int = 0,
+              stream: int | None = None) -> None:
+        """omg_dev_kv_evict: of each sequence and KV head the `recent` last
+        rows and the heaviest others stay, `keep` in all; their numbers go to
+        rows [nseq][kv_heads][keep], their weights to kept_weights (None: where
+        they are) and the rows to the pages of to_table (None: their own)."""
+        L.check(L.lib().omg_dev_kv_evict(self, batch, keep, recent, weights_ptr, ldw, rows_ptr, kept_weights, kept_ld,
+                                         to_table, to_ld, stream))
+
 
 def sample_workspace(rows: int, vocab: int) -> int:
     """Bytes of workspace that `sample` needs."""

@@ -435,6 +435,39 @@ int omg_dev_attention_tree(const omg_paged_kv *kv, const omg_paged_batch *b, int
                            int window, const int32_t *positions, void *workspace, size_t workspace_bytes,
                            void *stream);
 
+/* Rows that stay: row first[s] + j of sequence s (first NULL: row j) becomes
+ * what its row rows[j] was, K and V, for j < count; `rows` (int32, device) holds
+ * a list per sequence, rows_ld apart, for all its KV heads, or per_head != 0 a
+ * list per sequence and KV head, list s * kv_heads + h.  So an accepted path of
+ * drafted tokens closes up (first: the rows before the draft), or what an
+ * eviction leaves moves down.
+ *   to_table NULL: in place.  A list's rows ascend, and none stands before its
+ * new place (rows[j] >= first[s] + j; one that does is left out).  Pages with
+ * rows that move belong to one sequence.
+ *   to_table [nseq][to_ld]: the pages of the new rows, none of which any
+ * sequence's list is read from; rows in any order, also twice.
+ * Entries below zero or past the table, and rows on pages outside the pool,
+ * move nothing.  Of the batch nseq, the table and its sizes count; its lengths
+ * stay as they are.  count at most max_pages * page. */
+int omg_dev_kv_keep(const omg_paged_kv *kv, const omg_paged_batch *b, const int32_t *rows, int64_t rows_ld,
+                    int64_t count, const int32_t *first, int per_head, const int32_t *to_table, int64_t to_ld,
+                    void *stream);
+
+/* Eviction by weight: of the n = lens[s] own rows of each sequence and KV head
+ * `keep` stay (all, where n is no more), the `recent` last ones and of the
+ * others those of the largest weights[(s * kv_heads + h) * ldw + i] (ties: the
+ * first rows; NaN lowest), in their order.  rows [nseq][kv_heads][keep]
+ * (int32) gets their numbers, -1 behind the last; kept (lists kept_ld apart;
+ * NULL: the weights themselves) their weights and zeros for the other rows, up
+ * to n or kept_ld; K and V move as omg_dev_kv_keep moves them, in place or to
+ * the pages of to_table (then all that stays moves, also of short sequences).
+ * The caller's lengths become min(n, keep), its new tokens' positions go on
+ * from where they were (omg_kv_source.positions), and a window, which counts
+ * rows, no longer counts positions.  keep at most max_pages * page, ldw at least that. */
+int omg_dev_kv_evict(const omg_paged_kv *kv, const omg_paged_batch *b, int64_t keep, int64_t recent, float *weights,
+                     int64_t ldw, int32_t *rows, float *kept, int64_t kept_ld, const int32_t *to_table, int64_t to_ld,
+                     void *stream);
+
 /* The next token of each row of logits (row r, token i at logits[r * ld + i];
  * dtype OMG_ELEM_F32, F16 or BF16; any ld from vocab up), drawn with the
  * given random number u[r] in [0, 1).  With z the row, M its maximum and

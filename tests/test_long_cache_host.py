@@ -58,3 +58,62 @@ def test_tree_refuses_null_descriptions():
     for args in ((None, batch()), (kv(), None)):
         with pytest.raises(g.OmgError, match="null"):
             L.check(L.lib().omg_dev_attention_tree(*args, 4, P, 256, P, 256, None, 0.125, P, 1, 0, None, P, 1 << 40, None))
+
+
+def keep(k=None, b=None, rows=P, rows_ld=8, count=8, **kw):
+    (k or kv()).keep(b or batch(), rows, rows_ld, count, **kw)
+
+
+@pytest.mark.parametrize("over,why", BAD_KV)
+def test_keep_and_evict_refuse_caches(over, why):
+    with pytest.raises(g.OmgError, match=f"kv_keep.*{why}"):
+        keep(k=kv(**over))
+    with pytest.raises(g.OmgError, match=f"kv_evict.*{why}"):
+        evict(k=kv(**over))
+
+
+@pytest.mark.parametrize("over,why", [x for x in BAD_BATCH if "prefix_len" not in x[0]])
+def test_keep_and_evict_refuse_batches(over, why):
+    with pytest.raises(g.OmgError, match=f"kv_keep.*{why}"):
+        keep(b=batch(**over))
+    with pytest.raises(g.OmgError, match=f"kv_evict.*{why}"):
+        evict(b=batch(**over))
+
+
+@pytest.mark.parametrize("over,why", [
+    (dict(rows=None), "null rows"), (dict(count=0), "count"), (dict(count=65, rows_ld=65), "count"),
+    (dict(rows_ld=7), "rows_ld"), (dict(to_table=P, to_ld=0), "to_ld"), (dict(to_table=P, to_ld=1 << 28), "to_ld")])
+def test_keep_refuses_arguments(over, why):
+    with pytest.raises(g.OmgError, match=f"kv_keep.*{why}"):
+        keep(**over)
+
+
+def evict(k=None, b=None, keep=20, recent=5, weights=P, ldw=64, rows=P, **kw):
+    (k or kv()).evict(b or batch(), keep, recent, weights, ldw, rows, **kw)
+
+
+@pytest.mark.parametrize("over,why", [
+    (dict(weights=None), "null"), (dict(rows=None), "null"), (dict(keep=0), "keep"), (dict(recent=-1), "recent"),
+    (dict(recent=21), "recent"), (dict(keep=65), "sequence's rows"), (dict(ldw=63), "ldw"),
+    (dict(kept_weights=P + 4096, kept_ld=19), "kept_ld"), (dict(to_table=P, to_ld=0), "to_ld"),
+    (dict(to_table=P, to_ld=1 << 28), "to_ld")])
+def test_evict_refuses_arguments(over, why):
+    with pytest.raises(g.OmgError, match=f"kv_evict.*{why}"):
+        evict(**over)
+
+
+def test_keep_and_evict_refuse_null_descriptions_and_too_many_lists():
+    import grande_amd._lib as L
+
+    for args in ((None, batch()), (kv(), None)):
+        with pytest.raises(g.OmgError, match="null"):
+            L.check(L.lib().omg_dev_kv_keep(*args, P, 8, 8, None, 0, None, 0, None))
+        with pytest.raises(g.OmgError, match="null"):
+            L.check(L.lib().omg_dev_kv_evict(*args, 20, 5, P, 64, P, None, 0, None, 0, None))
+    many = batch(nseq=1 << 20, tokens=1 << 20)
+    with pytest.raises(g.OmgError, match="kv_keep: too many lists"):
+        keep(k=kv(kv_heads=64), b=many)
+    with pytest.raises(g.OmgError, match="kv_keep: too many rows"):
+        keep(k=kv(kv_heads=64), b=many, count=64, rows_ld=64, to_table=P, to_ld=4)
+    with pytest.raises(g.OmgError, match="kv_evict: too many lists"):
+        evict(k=kv(kv_heads=64), b=many)
