@@ -106,7 +106,7 @@ __global__ __launch_bounds__(256) void keep_in_place_kernel(KeepArgs a) {
 
 template <int D>
 void launch_apart(hipStream_t s, KeepArgs a) {
-    constexpr int W = 512 / D, U = 4;
+    constexpr int W = 512 / D, U = 2;
     a.groups = int((a.x.count + U * W - 1) / (U * W));
     a.waves = a.b.nseq * a.kv.kv_heads * a.groups;
     const int64_t blocks = (a.waves + 3) / 4;
