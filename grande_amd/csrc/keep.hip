@@ -69,10 +69,13 @@ __global__ __launch_bounds__(256) void keep_apart_kernel(KeepArgs a) {
     }
 }
 
-// In place: entry j of an ascending list has rows[j] >= first + j, so what an
-// entry writes is read by entries up to its own alone.  One wave takes a
-// list's K or V (or a slice of SB bytes of each row) from the first entry on
-// and has read an entry before it writes it or a later one.
+// In place: entry j of an ascending list has rows[j] >= first + j, so the place
+// that an entry writes is read by entries up to its own alone.  One wave takes
+// a list's K or V (or a slice of SB bytes of each row) from the first entry on,
+// in steps of U pieces, and a wave's loads return in order: an entry has its
+// row, and all entries before it theirs, when its place is written.  Loads run
+// ahead of the stores: while a step's rows arrive the next step's pages and the
+// entries of the one after are asked for.
 template <int SB>
 __global__ __launch_bounds__(256) void keep_in_place_kernel(KeepArgs a) {
     constexpr int L = SB / 16, W = WAVE / L, U = 8;
@@ -83,24 +86,60 @@ __global__ __launch_bounds__(256) void keep_in_place_kernel(KeepArgs a) {
     const int64_t half = id / a.slices, list = half / 2, s = list / a.kv.kv_heads, g = list - s * a.kv.kv_heads;
     uint16_t* x = static_cast<uint16_t*>(half % 2 ? a.kv.v : a.kv.k) + slice * (SB / 2) + lane % L * 8;
     const int32_t *rows = a.x.rows + (a.x.per_head ? list : s) * a.x.rows_ld, *table = a.b.table + s * a.b.table_ld;
-    const int64_t first = a.x.first ? a.x.first[s] : 0;
-    for (int64_t j0 = lane / L; j0 - lane / L < a.x.count; j0 += U * W) {
-        int64_t from[U], to[U];
-        chunk_t v[U];
+    const int64_t first = (a.x.first ? a.x.first[s] : 0) + int64_t(lane / L), count = a.x.count - lane / L;
+    const int mask = a.kv.page - 1;
+    struct Step {
+        int row[U], from[U], to[U];  // source rows, pages of the sources and places (below zero: nothing moves)
+    };
+    auto entries = [&](int64_t j0, Step& t) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) t.row[u] = -1;
+        if (j0 >= a.x.count) return;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (j0 + u * W < count) t.row[u] = rows[lane / L + j0 + u * W];
+    };
+    auto pages = [&](int64_t j0, Step& t) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) t.from[u] = t.to[u] = -1;
+        if (j0 >= a.x.count) return;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int64_t j = j0 + u * W, row = j < a.x.count ? rows[j] : -1;
-            from[u] = row > first + j ? row_at(a, table, a.b.max_pages, row, g) : -1;
-            to[u] = from[u] < 0 ? -1 : row_at(a, table, a.b.max_pages, first + j, g);
+            const int64_t r = t.row[u], d = first + j0 + u * W;
+            const bool moves = r > d && d >= 0 && r >> a.page_shift < a.b.max_pages;
+            if (moves) t.from[u] = table[r >> a.page_shift], t.to[u] = table[d >> a.page_shift];
         }
+    };
+    auto place = [&](int p, int64_t row) {
+        return x + p * a.kv.page_stride + (g * a.kv.page + (row & mask)) * a.kv.head_dim;
+    };
+    auto moves = [&](const Step& t, int u) { return uint64_t(t.from[u]) < uint64_t(a.kv.npages) && uint64_t(t.to[u]) < uint64_t(a.kv.npages); };
+    auto load = [&](const Step& t, chunk_t* v) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (to[u] >= 0) v[u] = *reinterpret_cast<const chunk_t*>(x + from[u]);
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (to[u] >= 0) *reinterpret_cast<chunk_t*>(x + to[u]) = v[u];
+            if (moves(t, u)) v[u] = *reinterpret_cast<const chunk_t*>(place(t.from[u], t.row[u]));
+    };
+    Step now, next, then;
+    chunk_t v[U], w[U];
+    entries(0, now);
+    entries(U * W, next);
+    pages(0, now);
+    entries(2 * U * W, then);
+    pages(U * W, next);
+    load(now, v);
+    for (int64_t j0 = 0; j0 < a.x.count; j0 += U * W) {
+        load(next, w);
+        pages(j0 + 2 * U * W, then);
+        Step more;
+        entries(j0 + 3 * U * W, more);
         asm volatile("" ::: "memory");
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (moves(now, u)) *reinterpret_cast<chunk_t*>(place(now.to[u], first + j0 + u * W)) = v[u];
+        asm volatile("" ::: "memory");
+        now = next, next = then, then = more;
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = w[u];
     }
 }
 
