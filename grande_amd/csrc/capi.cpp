@@ -723,6 +723,21 @@ int omg_dev_attention_tree(const omg_paged_kv* kv, const omg_paged_batch* b, int
     });
 }
 
+int64_t omg_dev_attention_weights_workspace(const omg_paged_kv* kv, const omg_paged_batch* b, int heads) {
+    int64_t n = 0;
+    const int rc = guard([&] { n = omg::attention_weights_workspace(paged_kv(kv), paged_batch(b), heads); });
+    return rc == OMG_OK ? n : rc;
+}
+
+int omg_dev_attention_weights(const omg_paged_kv* kv, const omg_paged_batch* b, int heads, const void* q, int64_t ldq,
+                              const float* lse, float scale, int window, float* weights, int64_t ldw, void* workspace,
+                              size_t workspace_bytes, void* stream) {
+    return guard([&] {
+        omg::launch_attention_weights(static_cast<hipStream_t>(stream), paged_kv(kv), paged_batch(b),
+                                      {heads, q, ldq, lse, scale, window, weights, ldw}, workspace, workspace_bytes);
+    });
+}
+
 int omg_dev_kv_keep(const omg_paged_kv* kv, const omg_paged_batch* b, const int32_t* rows, int64_t rows_ld,
                     int64_t count, const int32_t* first, int per_head, const int32_t* to_table, int64_t to_ld,
                     void* stream) {

@@ -369,6 +369,21 @@ int64_t attention_tree_workspace(const PagedKv& kv, const PagedBatch& b, int hea
 void launch_attention_tree(hipStream_t s, const PagedKv& kv, const PagedBatch& b, const SharedAttn& x,
                            const TreeMask& tree, void* workspace, size_t bytes);
 
+// ---- the attention weight of cached rows (weights.hip) ----
+struct AttnWeights {
+    int heads;
+    const void* q;
+    int64_t ldq;
+    const float* lse;  // [t][heads]
+    float scale;
+    int window;
+    float* weights;  // [nseq][kv_heads] lists, ldw apart
+    int64_t ldw;
+};
+int64_t attention_weights_workspace(const PagedKv& kv, const PagedBatch& b, int heads);
+void launch_attention_weights(hipStream_t s, const PagedKv& kv, const PagedBatch& b, const AttnWeights& x,
+                              void* workspace, size_t bytes);
+
 // ---- rows that stay (keep.hip) ----
 // Row first[s] + j of a sequence becomes its row rows[j].
 struct KeepRows {

@@ -1,0 +1,435 @@
+// The attention weight that each cached row gathers:
+//   weights[s][g][i] += sum of exp(scale q . k_i - lse) over the sequence's
+// tokens that see its row i and the query heads of KV head g, lse the log sums
+// that attention left.  No softmax runs here, so every key's sum stands alone:
+// what a row holds reaches its own weight and no other.
+//
+// Keys stay, queries pass by.  A wave holds its keys in registers, as the A
+// operand straight from their pages, and S = K Q^T leaves a key's scores in
+// the same registers whatever query tile comes: probabilities add up there, and
+// the lanes (queries) are summed once at the end, in an order that the sizes
+// fix.  A weight is read and written by one lane of one wave.
+//
+// Few rows a sequence (steps of decoding): weights_few_kernel, 16 keys x 16
+// rows, bound by reading K.  Many (prompts): weights_many_kernel, a wave 32 or
+// 64 keys, query tiles of 32 rows in LDS for its four waves; where keys are few
+// the queries are split and the parts' sums added by weights_join_kernel.
+#include <algorithm>
+#include <atomic>
+#include <string>
+
+#include "common.h"
+#include "kern_common.h"
+#include "paged.h"
+
+namespace omg {
+
+namespace {
+
+typedef __attribute__((address_space(3))) void* lds_ptr;
+
+__device__ inline floatx16 mfma32(half8 a, half8 b, floatx16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ inline floatx16 mfma32(bf16x8 a, bf16x8 b, floatx16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ inline floatx4 mfma16(half8 a, half8 b, floatx4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ inline floatx4 mfma16(bf16x8 a, bf16x8 b, floatx4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+struct Args {
+    PagedKv kv;
+    PagedBatch b;
+    AttnWeights x;
+    int hpg, page_shift;
+    int64_t max_len;
+    int64_t blocks;  // few: key chunks, many: key blocks of a sequence
+    int chunk;       // few: keys of a workgroup
+    int splits;      // many: of a sequence's tokens
+    float* part;     // [splits][nseq * kv_heads][max_len], null: into the weights
+};
+
+// A sequence's tokens, its rows in the cache and the row of its first token.
+struct Seq {
+    int tok, n, len, base;
+};
+__device__ inline Seq sequence(const Args& a, int64_t s) {
+    const int tok = a.b.start ? a.b.start[s] : int(s), n = a.b.start ? a.b.start[s + 1] - tok : 1;
+    const int len = a.b.lens[s] < 0 ? 0 : a.b.lens[s];
+    return {tok, n, len < a.max_len ? len : int(a.max_len), len - n};
+}
+
+// exp(s scale - lse); lse of minus infinity (a token that sees nothing) leaves 0.
+__device__ inline float prob(float s, float scale, float neg_lse) {
+    return __builtin_amdgcn_exp2f(fmaf(s, scale, neg_lse) * 1.4426950408889634f);
+}
+__device__ inline float negated(float lse) { return lse == -INFINITY ? -INFINITY : -lse; }
+
+__device__ inline float sum16(float v) {  // over the 16 lanes of a row, the same bits in each
+    v += dpp_f32<0xb1>(v);
+    v += dpp_f32<0x4e>(v);
+    v += dpp_f32<0x141>(v);
+    v += dpp_f32<0x140>(v);
+    return v;
+}
+
+// The elements of a row's page (null: not in the pool).
+template <typename T>
+__device__ inline const T* key_row(const Args& a, const int32_t* table, int row, int g, int D) {
+    const int i = row >> a.page_shift;
+    if (i >= a.b.max_pages) return nullptr;
+    const int64_t p = table[i];
+    if (p < 0 || p >= a.kv.npages) return nullptr;
+    return static_cast<const T*>(a.kv.k) + p * a.kv.page_stride + (int64_t(g) * a.kv.page + (row & (a.kv.page - 1))) * D;
+}
+
+// Four waves, each every fourth group of U 16-key tiles of the chunk.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void weights_few_kernel(Args a) {
+    typedef typename Vec8<T>::type frag;
+    constexpr int NS = D / 32, U = D >= 512 ? 1 : D >= 256 ? 2 : 4, KEYS = 16 * U;
+    const int lane = int(threadIdx.x) % WAVE, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / WAVE);
+    const int64_t id = blockIdx.x, list = id / a.blocks, s = list / a.kv.kv_heads;
+    const int g = int(list - s * a.kv.kv_heads), from = int(id - list * a.blocks) * a.chunk;
+    const Seq q = sequence(a, s);
+    const int to = from + a.chunk < q.len ? from + a.chunk : q.len;
+    if (from >= to || q.n <= 0) return;
+    const int32_t* table = a.b.table + s * a.b.table_ld;
+    float* out = a.x.weights + list * a.x.ldw;
+    const int rows = q.n * a.hpg, w = a.x.window;
+    // keys that a window hides from the first token are seen by none
+    const int lo = w > 0 && q.base + 1 > w ? q.base + 1 - w : 0;
+
+    frag qf[NS];
+    float nl = -INFINITY;  // the row's negated lse
+    int own = 0;           // the row's token's row in the cache
+    auto load = [&](int r0) {
+        const int r = r0 + lane % 16, tok = r / a.hpg, head = g * a.hpg + r - tok * a.hpg;
+        const int64_t at = q.tok + tok;
+        const bool valid = r < rows && at >= 0 && at < a.b.t;
+        nl = valid ? negated(a.x.lse[at * a.x.heads + head]) : -INFINITY;
+        own = valid ? q.base + tok : -1;
+        const T* p = static_cast<const T*>(a.x.q) + (valid ? at * a.x.ldq + int64_t(head) * D : 0) + 8 * (lane / 16);
+        frag z{};
+#pragma unroll
+        for (int st = 0; st < NS; ++st) qf[st] = valid ? *reinterpret_cast<const frag*>(p + 32 * st) : z;
+    };
+    load(0);
+    for (int k0 = from + wave * KEYS; k0 < to; k0 += 4 * KEYS) {
+        if (k0 + KEYS <= lo) continue;
+        frag kf[U][NS];
+        bool there[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            // (a tile lies in one page, which is whole in the pool)
+            const T* p = k0 + 16 * u < to ? key_row<T>(a, table, k0 + 16 * u, g, D) : nullptr;
+            there[u] = p != nullptr;
+            if (!p) continue;
+            p += int64_t(lane % 16) * D + 8 * (lane / 16);
+#pragma unroll
+            for (int st = 0; st < NS; ++st) kf[u][st] = *reinterpret_cast<const frag*>(p + 32 * st);
+        }
+        float sum[U][4];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sum[u][r] = 0.0f;
+        for (int r0 = 0; r0 < rows; r0 += 16) {
+            if (rows > 16) load(r0);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (!there[u]) continue;
+                floatx4 sc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int st = 0; st < NS; ++st) sc = mfma16(kf[u][st], qf[st], sc);
+                const int first = k0 + 16 * u + 4 * (lane / 16);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const bool see = first + r <= own && (w == 0 || own - (first + r) < w) && nl != -INFINITY;
+                    const float p = prob(sc[r], a.x.scale, nl);
+                    sum[u][r] += see ? p : 0.0f;
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sum[u][r] = sum16(sum[u][r]);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int key = k0 + 16 * u + 4 * (lane / 16) + lane % 16;
+            float mine = sum[u][0];
+#pragma unroll
+            for (int r = 1; r < 4; ++r) mine = lane % 16 == r ? sum[u][r] : mine;
+            if (there[u] && lane % 16 < 4 && key < to) out[key] += mine;
+        }
+    }
+}
+
+// Many rows.
+template <typename T, int D>
+struct Many {
+    static constexpr int NB = D >= 512 ? 1 : 2;  // 32-key blocks of a wave
+    static constexpr int KEYS = 4 * 32 * NB;     // of a workgroup
+    static constexpr int CH = D / 8, RPI = 512 / D > 0 ? 512 / D : 1;
+    static constexpr int INS = 32 * D * 2 / 1024 / 4;  // 1 KiB pieces of a query tile per wave
+    static constexpr int TILE = 32 * D;
+    static __device__ int swz(int row) { return CH >= 16 ? row & 15 : row >> 1 & 7; }
+};
+
+template <typename T, int D>
+__global__ __launch_bounds__(256, 2) void weights_many_kernel(Args a) {
+    typedef typename Vec8<T>::type frag;
+    typedef Many<T, D> M;
+    constexpr int NB = M::NB, NS = D / 16;
+    extern __shared__ __attribute__((aligned(1024))) unsigned char smem_raw[];
+    T* smem = reinterpret_cast<T*>(smem_raw);  // two query tiles
+    const int lane = int(threadIdx.x) % WAVE, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / WAVE);
+    const int G = a.kv.kv_heads, hpg = a.hpg;
+    // (KV heads fastest: the workgroups of one XCD share a few heads' queries)
+    int64_t id = blockIdx.x;
+    const int g = int(id % G);
+    id /= G;
+    const int split = int(id % a.splits);
+    id /= a.splits;
+    const int block = int(id % a.blocks);
+    const int64_t s = id / a.blocks, list = s * G + g;
+    const Seq q = sequence(a, s);
+    const int kb = block * M::KEYS;
+    if (kb >= q.len) return;
+    const int k0 = kb + wave * 32 * NB, w = a.x.window;
+    // The split's tokens, those of them that see a key of the block.
+    const int per = (q.n + a.splits - 1) / a.splits;
+    int ta = split * per, tb = ta + per < q.n ? ta + per : q.n;
+    ta = ta > kb - q.base ? ta : kb - q.base;
+    // (token rows outside the batch's are nobody's)
+    if (q.tok < 0 && ta < -q.tok) ta = -q.tok;
+    if (tb > a.b.t - q.tok) tb = int(a.b.t - q.tok);
+    if (w > 0) {
+        const int64_t end = int64_t(kb) + M::KEYS - 1 + w - q.base;  // own < key + w
+        if (tb > end) tb = int(end < 0 ? 0 : end);
+    }
+    float sum[NB][16];
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sum[j][r] = 0.0f;
+    const int32_t* table = a.b.table + s * a.b.table_ld;
+    if (ta < tb) {
+        frag kf[NB][NS];
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+            const int row = k0 + 32 * j + lane % 32;
+            const T* p = row < q.len ? key_row<T>(a, table, row, g, D) : nullptr;
+            frag z{};
+#pragma unroll
+            for (int st = 0; st < NS; ++st)
+                kf[j][st] = p ? *reinterpret_cast<const frag*>(p + 16 * st + 8 * (lane / 32)) : z;
+        }
+        const int rows = (tb - ta) * hpg, ntile = (rows + 31) / 32;
+        const int64_t tok0 = q.tok + ta;
+        // The queries from the split's first token on; rows behind its last
+        // token's repeat the first one and do not count.
+        const int have = tb - ta;
+        const T* qb = static_cast<const T*>(a.x.q) + tok0 * a.x.ldq + int64_t(g) * hpg * D;
+        const int step_tok = 32 / hpg, step_head = 32 % hpg;
+        // The lane's rows of the wave's pieces, and its own query row.
+        int tok[M::INS], head[M::INS];
+        const int prow = wave * M::INS * M::RPI + (D < 512 ? lane / M::CH : 0);
+#pragma unroll
+        for (int i = 0; i < M::INS; ++i) {
+            const int r = prow + i * M::RPI;
+            tok[i] = r / hpg, head[i] = r - tok[i] * hpg;
+        }
+        int mtok = lane % 32 / hpg, mhead = lane % 32 - mtok * hpg;
+        auto advance = [&](int& t, int& h) {
+            t += step_tok, h += step_head;
+            if (h >= hpg) h -= hpg, ++t;
+        };
+        auto issue = [&](T* dst) {
+#pragma unroll
+            for (int i = 0; i < M::INS; ++i) {
+                const int r = prow + i * M::RPI;
+                const bool ok = tok[i] < have;
+                const T* src = qb + (ok ? int64_t(tok[i]) * a.x.ldq + head[i] * D : 0) + ((lane % M::CH) ^ M::swz(r)) * 8;
+                __builtin_amdgcn_global_load_lds(
+                    reinterpret_cast<__attribute__((address_space(1))) void*>(reinterpret_cast<uintptr_t>(src)),
+                    (lds_ptr)(dst + (wave * M::INS + i) * 512), 16, 0, 0);
+                advance(tok[i], head[i]);
+            }
+        };
+        auto log_sum = [&] {
+            return mtok < have ? negated(a.x.lse[(tok0 + mtok) * a.x.heads + g * hpg + mhead]) : -INFINITY;
+        };
+        issue(smem);
+        float next = log_sum();
+        for (int i = 0; i < ntile; ++i) {
+            const float nl = next;
+            const int own = q.base + ta + mtok;  // the lane's query's row in the cache
+            advance(mtok, mhead);
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            __syncthreads();
+            if (i + 1 < ntile) {
+                issue(smem + (i + 1) % 2 * M::TILE);
+                next = log_sum();
+            }
+            const T* tile = smem + i % 2 * M::TILE;
+            floatx16 sc[NB];
+#pragma unroll
+            for (int j = 0; j < NB; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) sc[j][r] = 0.0f;
+            const int row = lane % 32;
+#pragma unroll
+            for (int st = 0; st < NS; ++st) {
+                const frag qf = *reinterpret_cast<const frag*>(tile + row * D + ((2 * st + lane / 32) ^ M::swz(row)) * 8);
+#pragma unroll
+                for (int j = 0; j < NB; ++j) sc[j] = mfma32(kf[j][st], qf, sc[j]);
+            }
+            // The tile's tokens lie in [t0, t1]: whether all see all the wave's keys.
+            const int t0 = q.base + ta + i * 32 / hpg, t1 = q.base + ta + (i * 32 + 31) / hpg;
+            const bool full = t0 >= k0 + 32 * NB - 1 && (w == 0 || t1 - k0 < w);
+#pragma unroll
+            for (int j = 0; j < NB; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const float p = prob(sc[j][r], a.x.scale, nl);
+                    if (full) {
+                        sum[j][r] += nl == -INFINITY ? 0.0f : p;
+                    } else {
+                        const int key = k0 + 32 * j + 8 * (r / 4) + 4 * (lane / 32) + r % 4;
+                        const bool see = key <= own && (w == 0 || own - key < w) && nl != -INFINITY;
+                        sum[j][r] += see ? p : 0.0f;
+                    }
+                }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+        float mine = 0.0f;  // lane 16 a + r % 16 of a half: element r
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            float v = sum16(sum[j][r]);
+            v += __shfl_xor(v, 16, WAVE);
+            mine = lane % 16 == r ? v : mine;
+        }
+        const int r = lane % 16, key = k0 + 32 * j + 8 * (r / 4) + 4 * (lane / 32) + r % 4;
+        if (lane % 32 >= 16 || key >= q.len || !key_row<T>(a, table, key, g, D)) continue;
+        if (a.part)
+            a.part[(split * a.b.nseq * G + list) * a.max_len + key] = mine;
+        else
+            a.x.weights[list * a.x.ldw + key] += mine;
+    }
+}
+
+// The splits' sums, in their order.
+__global__ __launch_bounds__(256) void weights_join_kernel(Args a) {
+    const int64_t list = blockIdx.y, s = list / a.kv.kv_heads, key = int64_t(blockIdx.x) * 256 + threadIdx.x;
+    const Seq q = sequence(a, s);
+    if (key >= q.len) return;
+    const int64_t p = a.b.table[s * a.b.table_ld + (key >> a.page_shift)];
+    if (p < 0 || p >= a.kv.npages) return;
+    float v = 0.0f;
+    for (int i = 0; i < a.splits; ++i) v += a.part[(i * a.b.nseq * a.kv.kv_heads + list) * a.max_len + key];
+    a.x.weights[list * a.x.ldw + key] += v;
+}
+
+void check(const PagedKv& kv, const PagedBatch& b, int heads) {
+    check_kv(kv, "attention_weights");
+    check_batch(b, kv, "attention_weights");
+    if (heads <= 0 || heads > 4096 || heads % kv.kv_heads)
+        fail(E_INVALID, "attention_weights: heads must be a multiple of kv_heads, at most 4096");
+    if (b.t * heads >= (1 << 26)) fail(E_INVALID, "attention_weights: t * heads must stay below 2^26");
+}
+
+bool few(const PagedKv& kv, const PagedBatch& b, int heads) { return b.t * (heads / kv.kv_heads) <= 32 * b.nseq; }
+
+int many_keys(int head_dim) { return head_dim == 512 ? 128 : 256; }
+
+// Splits of the queries until some two rounds of work items are there.
+int splits(const PagedKv& kv, const PagedBatch& b, int heads) {
+    if (few(kv, b, heads)) return 1;
+    const int64_t max_len = b.max_pages * kv.page, keys = many_keys(kv.head_dim);
+    const int64_t items = b.nseq * kv.kv_heads * ((max_len + keys - 1) / keys);
+    const int64_t rows = (b.t + b.nseq - 1) / b.nseq * (heads / kv.kv_heads);  // of a sequence
+    return int(std::max<int64_t>(1, std::min<int64_t>({1024 / items, rows / 256, 32})));
+}
+
+int64_t part_bytes(const PagedKv& kv, const PagedBatch& b, int heads) {
+    const int64_t n = splits(kv, b, heads);
+    return n == 1 ? 0 : n * b.nseq * kv.kv_heads * b.max_pages * kv.page * 4;
+}
+
+template <typename T, int D>
+void launch_d(hipStream_t s, Args a) {
+    const int64_t lists = a.b.nseq * a.kv.kv_heads;
+    if (few(a.kv, a.b, a.x.heads)) {
+        // Chunks of 256 keys and more, some eight workgroups a CU.
+        a.chunk = 256;
+        while (a.chunk < 4096 && lists * (a.max_len / a.chunk) > 4096) a.chunk *= 2;
+        a.blocks = (a.max_len + a.chunk - 1) / a.chunk;
+        if (lists * a.blocks >= MAX_BLOCKS) fail(E_CAPACITY, "attention_weights: too many work items");
+        weights_few_kernel<T, D><<<dim3(unsigned(lists * a.blocks)), dim3(256), 0, s>>>(a);
+        OMG_HIP(hipGetLastError());
+        return;
+    }
+    a.blocks = (a.max_len + Many<T, D>::KEYS - 1) / Many<T, D>::KEYS;
+    const int64_t n = lists * a.blocks * a.splits;
+    if (n >= MAX_BLOCKS || lists > 65535) fail(E_CAPACITY, "attention_weights: too many work items");
+    constexpr unsigned lds = 2 * Many<T, D>::TILE * 2;
+    weights_many_kernel<T, D><<<dim3(unsigned(n)), dim3(256), lds, s>>>(a);
+    OMG_HIP(hipGetLastError());
+    if (a.splits > 1) {
+        weights_join_kernel<<<dim3(unsigned((a.max_len + 255) / 256), unsigned(lists)), dim3(256), 0, s>>>(a);
+        OMG_HIP(hipGetLastError());
+    }
+}
+
+template <typename T>
+void launch_t(hipStream_t s, const Args& a) {
+    switch (a.kv.head_dim) {
+        case 64: return launch_d<T, 64>(s, a);
+        case 128: return launch_d<T, 128>(s, a);
+        case 256: return launch_d<T, 256>(s, a);
+        default: return launch_d<T, 512>(s, a);
+    }
+}
+
+}  // namespace
+
+int64_t attention_weights_workspace(const PagedKv& kv, const PagedBatch& b, int heads) {
+    check(kv, b, heads);
+    return part_bytes(kv, b, heads);
+}
+
+void launch_attention_weights(hipStream_t s, const PagedKv& kv, const PagedBatch& b, const AttnWeights& x,
+                              void* workspace, size_t bytes) {
+    check(kv, b, x.heads);
+    if (!x.q || !aligned16(x.q)) fail(E_INVALID, "attention_weights: q must be a 16-byte aligned device pointer");
+    if (x.ldq < int64_t(x.heads) * kv.head_dim || x.ldq % 8)
+        fail(E_INVALID, "attention_weights: ldq must hold the heads and be a multiple of 8");
+    if (!x.lse || !x.weights) fail(E_INVALID, "attention_weights: null lse or weights");
+    if (x.ldw < b.max_pages * kv.page) fail(E_INVALID, "attention_weights: ldw must hold a sequence's rows");
+    if (!(x.scale > 0.0f) || x.scale > 1e30f)
+        fail(E_INVALID, "attention_weights: scale must be positive and finite");
+    if (x.window < 0) fail(E_INVALID, "attention_weights: window must not be negative");
+    const int64_t need = part_bytes(kv, b, x.heads);
+    if (int64_t(bytes) < need)
+        fail(E_CAPACITY, "attention_weights: the workspace needs " + std::to_string(need) + " bytes");
+    if (need && (!workspace || !aligned16(workspace)))
+        fail(E_INVALID, "attention_weights: the workspace must be 16-byte aligned");
+    Args a{};
+    a.kv = kv, a.b = b, a.x = x;
+    a.hpg = x.heads / kv.kv_heads;
+    a.page_shift = log2_of(kv.page);
+    a.max_len = b.max_pages * kv.page;
+    a.splits = splits(kv, b, x.heads);
+    a.part = need ? static_cast<float*>(workspace) : nullptr;
+    kv.dtype == ELEM_F16 ? launch_t<half_t>(s, a) : launch_t<bf16_t>(s, a);
+}
+
+}  // namespace omg

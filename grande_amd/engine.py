@@ -592,6 +592,19 @@ class PagedKv(L.omg_paged_kv):
         L.check(L.lib().omg_dev_attention_tree(self, batch, heads, q_ptr, ldq, out_ptr, ldo, lse, scale, mask_ptr,
                                                mask_ld, window, positions, workspace, workspace_bytes, stream))
 
+    def attention_weights_workspace(self, batch: PagedBatch, heads: int) -> int:
+        """Bytes of workspace that `attention_weights` needs for batches of these sizes."""
+        return L.size(L.lib().omg_dev_attention_weights_workspace(self, batch, heads))
+
+    def attention_weights(self, batch: PagedBatch, heads: int, q_ptr: int, ldq: int, lse_ptr: int, scale: float,
+                          weights_ptr: int, ldw: int, *, window: int = 0, workspace: int | None = None,
+                          workspace_bytes: int = 0, stream: int | None = None) -> None:
+        """omg_dev_attention_weights: the probabilities that the step's
+        queries give each own row, from the log sums `attention` left, added
+        to weights [nseq][kv_heads][ldw]."""
+        L.check(L.lib().omg_dev_attention_weights(self, batch, heads, q_ptr, ldq, lse_ptr, scale, window, weights_ptr,
+                                                  ldw, workspace, workspace_bytes, stream))
+
     def keep(self, batch: PagedBatch, rows_ptr: int, rows_ld: int, count: int, *, first: int | None = None,
              per_head: bool = False, to_table: int | None = None, to_ld: int = 0, stream: int | None = None) -> None:
         """omg_dev_kv_keep: row first[s] + j of each sequence becomes its row

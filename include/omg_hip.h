@@ -435,6 +435,21 @@ int omg_dev_attention_tree(const omg_paged_kv *kv, const omg_paged_batch *b, int
                            int window, const int32_t *positions, void *workspace, size_t workspace_bytes,
                            void *stream);
 
+/* The attention weight that the batch's tokens give each own row of their
+ * sequences, added to what it has gathered before:
+ *   weights[(s * kv_heads + h) * ldw + i] += sum exp(scale * q . k_i - lse)
+ * over the tokens of sequence s that see its row i (as omg_dev_attention_shared
+ * lets them, window included) and the query heads of KV head h; lse [t][heads]
+ * is what that call gave (its prefix keys in it; minus infinity: a token that
+ * sees nothing).  f32 sums in an order that the shapes fix.  A row's weight
+ * hears from its own key alone, infinite and NaN ones too; rows from lens[s] on
+ * and on pages outside the pool keep theirs.  ldw at least max_pages * page.
+ * Sizes, scale and workspace as there. */
+int64_t omg_dev_attention_weights_workspace(const omg_paged_kv *kv, const omg_paged_batch *b, int heads);
+int omg_dev_attention_weights(const omg_paged_kv *kv, const omg_paged_batch *b, int heads, const void *q, int64_t ldq,
+                              const float *lse, float scale, int window, float *weights, int64_t ldw, void *workspace,
+                              size_t workspace_bytes, void *stream);
+
 /* Rows that stay: row first[s] + j of sequence s (first NULL: row j) becomes
  * what its row rows[j] was, K and V, for j < count; `rows` (int32, device) holds
  * a list per sequence, rows_ld apart, for all its KV heads, or per_head != 0 a

@@ -117,3 +117,47 @@ def test_keep_and_evict_refuse_null_descriptions_and_too_many_lists():
         keep(k=kv(kv_heads=64), b=many, count=64, rows_ld=64, to_table=P, to_ld=4)
     with pytest.raises(g.OmgError, match="kv_evict: too many lists"):
         evict(k=kv(kv_heads=64), b=many)
+
+
+def weigh(k=None, b=None, heads=4, q=P, ldq=256, lse=P, scale=0.125, weights=P, ldw=64, workspace=P,
+          workspace_bytes=1 << 40, **kw):
+    (k or kv()).attention_weights(b or batch(), heads, q, ldq, lse, scale, weights, ldw, workspace=workspace,
+                                  workspace_bytes=workspace_bytes, **kw)
+
+
+@pytest.mark.parametrize("over,why", BAD_KV)
+def test_weights_refuse_caches(over, why):
+    with pytest.raises(g.OmgError, match=f"attention_weights.*{why}"):
+        weigh(k=kv(**over))
+
+
+@pytest.mark.parametrize("over,why", BAD_BATCH)
+def test_weights_refuse_batches(over, why):
+    with pytest.raises(g.OmgError, match=f"attention_weights.*{why}"):
+        weigh(b=batch(**over))
+
+
+PROMPT = dict(nseq=1, tokens=4000, start_ptr=P, max_pages=300)
+
+
+@pytest.mark.parametrize("over,why", [
+    (dict(heads=3), "heads"), (dict(heads=0), "heads"), (dict(q=None), "q must"), (dict(q=P + 2), "q must"),
+    (dict(ldq=248), "ldq"), (dict(ldq=260), "ldq"), (dict(lse=None), "null"), (dict(weights=None), "null"),
+    (dict(ldw=63), "ldw"), (dict(scale=0.0), "scale"), (dict(scale=NAN), "scale"), (dict(scale=INF), "scale"),
+    (dict(window=-1), "window"), (dict(b=batch(**PROMPT), ldw=4800, workspace_bytes=16), "workspace needs"),
+    (dict(b=batch(**PROMPT), ldw=4800, workspace=None), "workspace must"),
+    (dict(b=batch(**PROMPT), ldw=4800, workspace=P + 8), "workspace must")])
+def test_weights_refuse_arguments(over, why):
+    with pytest.raises(g.OmgError, match=f"attention_weights.*{why}"):
+        weigh(**over)
+
+
+def test_weights_workspace_and_sizes():
+    assert kv().attention_weights_workspace(batch(), 4) == 0
+    assert kv().attention_weights_workspace(batch(**PROMPT), 4) > 0
+    with pytest.raises(g.OmgError, match="attention_weights.*heads"):
+        kv().attention_weights_workspace(batch(), 3)
+    with pytest.raises(g.OmgError, match="t \\* heads"):
+        weigh(b=batch(tokens=1 << 24, start_ptr=P))
+    with pytest.raises(g.OmgError, match="too many work items"):
+        weigh(k=kv(kv_heads=32), b=batch(nseq=1 << 20, tokens=1 << 20), heads=32, ldq=2048)
