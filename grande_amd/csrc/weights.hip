@@ -15,7 +15,7 @@
 // 64 keys, query tiles of 32 rows in LDS for its four waves; where keys are few
 // the queries are split and the parts' sums added by weights_join_kernel.
 #include <algorithm>
-#include <atomic>
+#include <climits>
 #include <string>
 
 #include "common.h"
@@ -178,8 +178,26 @@ struct Many {
     static constexpr int CH = D / 8, RPI = 512 / D > 0 ? 512 / D : 1;
     static constexpr int INS = 32 * D * 2 / 1024 / 4;  // 1 KiB pieces of a query tile per wave
     static constexpr int TILE = 32 * D;
+    static constexpr int BUFS = D >= 512 ? 2 : 4;  // query tiles in LDS
     static __device__ int swz(int row) { return CH >= 16 ? row & 15 : row >> 1 & 7; }
 };
+
+// N pieces of 1 KiB to LDS from the lanes' offsets behind `base`; zeros from
+// `bytes` on.
+template <int N>
+__device__ inline void to_lds(const char* base, int bytes, const uint32_t* off, void* dst) {
+    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), (short)0, bytes, 0x00020000);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr)(static_cast<char*>(dst) + 1024 * i), 16, off[i], 0, 0, 0);
+}
+
+// All but the last N loads have arrived, and LDS reads.
+template <int N>
+__device__ inline void wait_loads() {
+    static_assert(N < 64, "vmcnt holds 6 bits");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+}
 
 template <typename T, int D>
 __global__ __launch_bounds__(256, 2) void weights_many_kernel(Args a) {
@@ -187,7 +205,7 @@ __global__ __launch_bounds__(256, 2) void weights_many_kernel(Args a) {
     typedef Many<T, D> M;
     constexpr int NB = M::NB, NS = D / 16;
     extern __shared__ __attribute__((aligned(1024))) unsigned char smem_raw[];
-    T* smem = reinterpret_cast<T*>(smem_raw);  // two query tiles
+    T* smem = reinterpret_cast<T*>(smem_raw);  // BUFS query tiles
     const int lane = int(threadIdx.x) % WAVE, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / WAVE);
     const int G = a.kv.kv_heads, hpg = a.hpg;
     // (KV heads fastest: the workgroups of one XCD share a few heads' queries)
@@ -230,54 +248,47 @@ __global__ __launch_bounds__(256, 2) void weights_many_kernel(Args a) {
             for (int st = 0; st < NS; ++st)
                 kf[j][st] = p ? *reinterpret_cast<const frag*>(p + 16 * st + 8 * (lane / 32)) : z;
         }
-        const int rows = (tb - ta) * hpg, ntile = (rows + 31) / 32;
+        // A query tile: the heads of TPT tokens, or 32 heads of one, so that a
+        // lane's row is the same token and head past the tile's first in each.
+        const int heads = hpg < 32 ? hpg : 32, TPT = 32 / heads, parts = (hpg + 31) / 32;
+        const int have = tb - ta, ntile = (have + TPT - 1) / TPT * parts;
         const int64_t tok0 = q.tok + ta;
-        // The queries from the split's first token on; rows behind its last
-        // token's repeat the first one and do not count.
-        const int have = tb - ta;
-        const T* qb = static_cast<const T*>(a.x.q) + tok0 * a.x.ldq + int64_t(g) * hpg * D;
-        const int step_tok = 32 / hpg, step_head = 32 % hpg;
-        // The lane's rows of the wave's pieces, and its own query row.
-        int tok[M::INS], head[M::INS];
-        const int prow = wave * M::INS * M::RPI + (D < 512 ? lane / M::CH : 0);
+        const char* qb = reinterpret_cast<const char*>(static_cast<const T*>(a.x.q) + tok0 * a.x.ldq + int64_t(g) * hpg * D);
+        uint32_t off[M::INS];  // of the rows that the lane loads a chunk of; no row: the first
 #pragma unroll
         for (int i = 0; i < M::INS; ++i) {
-            const int r = prow + i * M::RPI;
-            tok[i] = r / hpg, head[i] = r - tok[i] * hpg;
+            const int r = (wave * M::INS + i) * M::RPI + lane / M::CH, t = r / heads;
+            off[i] = (t < TPT ? uint32_t(t * a.x.ldq + (r - t * heads) * D) * 2 : 0u) + ((lane % M::CH) ^ M::swz(r)) * 16;
         }
-        int mtok = lane % 32 / hpg, mhead = lane % 32 - mtok * hpg;
-        auto advance = [&](int& t, int& h) {
-            t += step_tok, h += step_head;
-            if (h >= hpg) h -= hpg, ++t;
-        };
+        const int mt = lane % 32 / heads, mh = lane % 32 - mt * heads;  // the lane's query row
+        int t0 = 0, part = 0;                                           // of the next tile
+        // Rows that are not there arrive as zeros, or as others, and have a
+        // negated log sum of minus infinity.  (A load each way: the waits count.)
         auto issue = [&](T* dst) {
+            const int64_t skip = t0 * a.x.ldq + part * 32 * D;
+            const int64_t left = t0 < have ? 2 * ((have - 1) * a.x.ldq + hpg * D - skip) : 0;
+            to_lds<M::INS>(qb + (t0 < have ? 2 * skip : 0), int(left < INT_MAX ? left : INT_MAX), off, dst + wave * M::INS * 512);
+            const bool ok = t0 + mt < have && mt < TPT && part * 32 + mh < hpg;
+            const float lse = a.x.lse[tok0 * a.x.heads + g * hpg + (ok ? int64_t(t0 + mt) * a.x.heads + part * 32 + mh : 0)];
+            if (++part == parts) part = 0, t0 += TPT;
+            return ok ? negated(lse) : -INFINITY;
+        };
+        // BUFS - 1 tiles are under way; behind the last one the loads go on, to
+        // nothing, so that a wait leaves the same number out.
+        constexpr int AHEAD = M::BUFS - 1;
+        float ahead[AHEAD];
 #pragma unroll
-            for (int i = 0; i < M::INS; ++i) {
-                const int r = prow + i * M::RPI;
-                const bool ok = tok[i] < have;
-                const T* src = qb + (ok ? int64_t(tok[i]) * a.x.ldq + head[i] * D : 0) + ((lane % M::CH) ^ M::swz(r)) * 8;
-                __builtin_amdgcn_global_load_lds(
-                    reinterpret_cast<__attribute__((address_space(1))) void*>(reinterpret_cast<uintptr_t>(src)),
-                    (lds_ptr)(dst + (wave * M::INS + i) * 512), 16, 0, 0);
-                advance(tok[i], head[i]);
-            }
-        };
-        auto log_sum = [&] {
-            return mtok < have ? negated(a.x.lse[(tok0 + mtok) * a.x.heads + g * hpg + mhead]) : -INFINITY;
-        };
-        issue(smem);
-        float next = log_sum();
+        for (int i = 0; i < AHEAD; ++i) ahead[i] = issue(smem + i * M::TILE);
+        int at = 0;
         for (int i = 0; i < ntile; ++i) {
-            const float nl = next;
-            const int own = q.base + ta + mtok;  // the lane's query's row in the cache
-            advance(mtok, mhead);
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            const float nl = ahead[0];
+            wait_loads<(AHEAD - 1) * (M::INS + 1)>();
             __syncthreads();
-            if (i + 1 < ntile) {
-                issue(smem + (i + 1) % 2 * M::TILE);
-                next = log_sum();
-            }
-            const T* tile = smem + i % 2 * M::TILE;
+#pragma unroll
+            for (int k = 0; k + 1 < AHEAD; ++k) ahead[k] = ahead[k + 1];
+            ahead[AHEAD - 1] = issue(smem + (at + AHEAD) % M::BUFS * M::TILE);
+            const T* tile = smem + at * M::TILE;
+            at = (at + 1) % M::BUFS;
             floatx16 sc[NB];
 #pragma unroll
             for (int j = 0; j < NB; ++j)
@@ -290,23 +301,41 @@ __global__ __launch_bounds__(256, 2) void weights_many_kernel(Args a) {
 #pragma unroll
                 for (int j = 0; j < NB; ++j) sc[j] = mfma32(kf[j][st], qf, sc[j]);
             }
-            // The tile's tokens lie in [t0, t1]: whether all see all the wave's keys.
-            const int t0 = q.base + ta + i * 32 / hpg, t1 = q.base + ta + (i * 32 + 31) / hpg;
-            const bool full = t0 >= k0 + 32 * NB - 1 && (w == 0 || t1 - k0 < w);
+            // Operands are read READ steps ahead of their MFMAs.  (Left alone, the
+            // compiler reads one and waits for it.)
+            constexpr int READ = 3;
+            __builtin_amdgcn_sched_group_barrier(0x100, READ, 0);
+#pragma unroll
+            for (int st = 0; st < NS; ++st) {
+                __builtin_amdgcn_sched_group_barrier(0x8, NB, 0);
+                if (st + READ < NS) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            // The tile's tokens have the rows own .. own + TPT - 1 in the cache:
+            // whether all see all the wave's keys.
+            const int own = q.base + ta + i / parts * TPT;
+            const bool full = own >= k0 + 32 * NB - 1 && (w == 0 || own + TPT - 1 - k0 < w) && __all(nl != -INFINITY);
+            if (full) {
+#pragma unroll
+                for (int j = 0; j < NB; ++j)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) sum[j][r] += prob(sc[j][r], a.x.scale, nl);
+                continue;
+            }
+            // the lane's keys past k0 + 4 (lane / 32): constants of (j, r)
+            const int last = own + mt - k0 - 4 * (lane / 32);
+            const int from = w == 0 ? INT_MIN : __builtin_elementwise_sub_sat(last, w);
 #pragma unroll
             for (int j = 0; j < NB; ++j)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
+                    const int key = 32 * j + 8 * (r / 4) + r % 4;
+                    const bool see = key <= last && key > from && nl != -INFINITY;
                     const float p = prob(sc[j][r], a.x.scale, nl);
-                    if (full) {
-                        sum[j][r] += nl == -INFINITY ? 0.0f : p;
-                    } else {
-                        const int key = k0 + 32 * j + 8 * (r / 4) + 4 * (lane / 32) + r % 4;
-                        const bool see = key <= own && (w == 0 || own - key < w) && nl != -INFINITY;
-                        sum[j][r] += see ? p : 0.0f;
-                    }
+                    sum[j][r] += see ? p : 0.0f;
                 }
         }
+        wait_loads<0>();  // (no load may find the LDS another workgroup's)
     }
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
@@ -356,7 +385,7 @@ int splits(const PagedKv& kv, const PagedBatch& b, int heads) {
     const int64_t max_len = b.max_pages * kv.page, keys = many_keys(kv.head_dim);
     const int64_t items = b.nseq * kv.kv_heads * ((max_len + keys - 1) / keys);
     const int64_t rows = (b.t + b.nseq - 1) / b.nseq * (heads / kv.kv_heads);  // of a sequence
-    return int(std::max<int64_t>(1, std::min<int64_t>({1024 / items, rows / 256, 32})));
+    return int(std::max<int64_t>(1, std::min<int64_t>({4096 / items, rows / 256, 32})));
 }
 
 int64_t part_bytes(const PagedKv& kv, const PagedBatch& b, int heads) {
@@ -380,7 +409,8 @@ void launch_d(hipStream_t s, Args a) {
     a.blocks = (a.max_len + Many<T, D>::KEYS - 1) / Many<T, D>::KEYS;
     const int64_t n = lists * a.blocks * a.splits;
     if (n >= MAX_BLOCKS || lists > 65535) fail(E_CAPACITY, "attention_weights: too many work items");
-    constexpr unsigned lds = 2 * Many<T, D>::TILE * 2;
+    constexpr unsigned lds = Many<T, D>::BUFS * Many<T, D>::TILE * 2;
+    static_assert(lds <= 65536, "no attribute asked for");
     weights_many_kernel<T, D><<<dim3(unsigned(n)), dim3(256), lds, s>>>(a);
     OMG_HIP(hipGetLastError());
     if (a.splits > 1) {
@@ -412,6 +442,7 @@ void launch_attention_weights(hipStream_t s, const PagedKv& kv, const PagedBatch
     if (!x.q || !aligned16(x.q)) fail(E_INVALID, "attention_weights: q must be a 16-byte aligned device pointer");
     if (x.ldq < int64_t(x.heads) * kv.head_dim || x.ldq % 8)
         fail(E_INVALID, "attention_weights: ldq must hold the heads and be a multiple of 8");
+    if (x.ldq > (1 << 24)) fail(E_INVALID, "attention_weights: ldq must be at most 2^24");
     if (!x.lse || !x.weights) fail(E_INVALID, "attention_weights: null lse or weights");
     if (x.ldw < b.max_pages * kv.page) fail(E_INVALID, "attention_weights: ldw must hold a sequence's rows");
     if (!(x.scale > 0.0f) || x.scale > 1e30f)

@@ -444,7 +444,7 @@ int omg_dev_attention_tree(const omg_paged_kv *kv, const omg_paged_batch *b, int
  * sees nothing).  f32 sums in an order that the shapes fix.  A row's weight
  * hears from its own key alone, infinite and NaN ones too; rows from lens[s] on
  * and on pages outside the pool keep theirs.  ldw at least max_pages * page.
- * Sizes, scale and workspace as there. */
+ * Sizes, scale and workspace as there; ldq at most 2^24. */
 int64_t omg_dev_attention_weights_workspace(const omg_paged_kv *kv, const omg_paged_batch *b, int heads);
 int omg_dev_attention_weights(const omg_paged_kv *kv, const omg_paged_batch *b, int heads, const void *q, int64_t ldq,
                               const float *lse, float scale, int window, float *weights, int64_t ldw, void *workspace,

@@ -142,7 +142,7 @@ PROMPT = dict(nseq=1, tokens=4000, start_ptr=P, max_pages=300)
 
 @pytest.mark.parametrize("over,why", [
     (dict(heads=3), "heads"), (dict(heads=0), "heads"), (dict(q=None), "q must"), (dict(q=P + 2), "q must"),
-    (dict(ldq=248), "ldq"), (dict(ldq=260), "ldq"), (dict(lse=None), "null"), (dict(weights=None), "null"),
+    (dict(ldq=248), "ldq"), (dict(ldq=260), "ldq"), (dict(ldq=(1 << 24) + 8), "ldq"), (dict(lse=None), "null"), (dict(weights=None), "null"),
     (dict(ldw=63), "ldw"), (dict(scale=0.0), "scale"), (dict(scale=NAN), "scale"), (dict(scale=INF), "scale"),
     (dict(window=-1), "window"), (dict(b=batch(**PROMPT), ldw=4800, workspace_bytes=16), "workspace needs"),
     (dict(b=batch(**PROMPT), ldw=4800, workspace=None), "workspace must"),
