@@ -15,6 +15,7 @@
 // 64 keys, query tiles of 32 rows in LDS for its four waves; where keys are few
 // the queries are split and the parts' sums added by weights_join_kernel.
 #include <algorithm>
+#include <atomic>
 #include <climits>
 #include <string>
 
@@ -206,6 +207,7 @@ __global__ __launch_bounds__(256, 2) void weights_many_kernel(Args a) {
     constexpr int NB = M::NB, NS = D / 16;
     extern __shared__ __attribute__((aligned(1024))) unsigned char smem_raw[];
     T* smem = reinterpret_cast<T*>(smem_raw);  // BUFS query tiles
+    float* log_sums = reinterpret_cast<float*>(smem_raw + M::BUFS * M::TILE * 2);  // [BUFS][4][64]
     const int lane = int(threadIdx.x) % WAVE, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / WAVE);
     const int G = a.kv.kv_heads, hpg = a.hpg;
     // (KV heads fastest: the workgroups of one XCD share a few heads' queries)
@@ -254,11 +256,11 @@ __global__ __launch_bounds__(256, 2) void weights_many_kernel(Args a) {
         const int have = tb - ta, ntile = (have + TPT - 1) / TPT * parts;
         const int64_t tok0 = q.tok + ta;
         const char* qb = reinterpret_cast<const char*>(static_cast<const T*>(a.x.q) + tok0 * a.x.ldq + int64_t(g) * hpg * D);
-        uint32_t off[M::INS];  // of the rows that the lane loads a chunk of; no row: the first
+        uint32_t off[M::INS];  // of the rows that the lane loads a chunk of; no row: past all
 #pragma unroll
         for (int i = 0; i < M::INS; ++i) {
             const int r = (wave * M::INS + i) * M::RPI + lane / M::CH, t = r / heads;
-            off[i] = (t < TPT ? uint32_t(t * a.x.ldq + (r - t * heads) * D) * 2 : 0u) + ((lane % M::CH) ^ M::swz(r)) * 16;
+            off[i] = (t < TPT ? uint32_t(t * a.x.ldq + (r - t * heads) * D) * 2 : 1u << 31) + ((lane % M::CH) ^ M::swz(r)) * 16;
         }
         const int mt = lane % 32 / heads, mh = lane % 32 - mt * heads;  // the lane's query row
         int t0 = 0, part = 0;                                           // of the next tile
@@ -268,72 +270,113 @@ __global__ __launch_bounds__(256, 2) void weights_many_kernel(Args a) {
             const int64_t skip = t0 * a.x.ldq + part * 32 * D;
             const int64_t left = t0 < have ? 2 * ((have - 1) * a.x.ldq + hpg * D - skip) : 0;
             to_lds<M::INS>(qb + (t0 < have ? 2 * skip : 0), int(left < INT_MAX ? left : INT_MAX), off, dst + wave * M::INS * 512);
+            // (log sums into registers would be waited for, and all loads before them, tile by tile)
             const bool ok = t0 + mt < have && mt < TPT && part * 32 + mh < hpg;
-            const float lse = a.x.lse[tok0 * a.x.heads + g * hpg + (ok ? int64_t(t0 + mt) * a.x.heads + part * 32 + mh : 0)];
+            const float* lse = a.x.lse + tok0 * a.x.heads + g * hpg + (ok ? int64_t(t0 + mt) * a.x.heads + part * 32 + mh : 0);
+            __builtin_amdgcn_global_load_lds(
+                reinterpret_cast<__attribute__((address_space(1))) void*>(reinterpret_cast<uintptr_t>(lse)),
+                (lds_ptr)(log_sums + (int(dst - smem) / M::TILE * 4 + wave) * WAVE), 4, 0, 0);
             if (++part == parts) part = 0, t0 += TPT;
-            return ok ? negated(lse) : -INFINITY;
         };
         // BUFS - 1 tiles are under way; behind the last one the loads go on, to
         // nothing, so that a wait leaves the same number out.
         constexpr int AHEAD = M::BUFS - 1;
-        float ahead[AHEAD];
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i) ahead[i] = issue(smem + i * M::TILE);
-        int at = 0;
-        for (int i = 0; i < ntile; ++i) {
-            const float nl = ahead[0];
+        for (int i = 0; i < AHEAD; ++i) issue(smem + i * M::TILE);
+        const bool pad = mt >= TPT;
+        const uint32_t my_row = uint32_t(lane % 32 * D * 2 + ((lane / 32) ^ M::swz(lane % 32)) * 16);
+        typedef __attribute__((address_space(3))) frag* operand;
+        int at = 0, tok = 0, hp = 0;  // of the tile at hand: its buffer, first token and part
+        // The next tile has landed: its LDS address for the lane's row, and the
+        // row's negated log sum.
+        auto arrive = [&](float& nl) {
             wait_loads<(AHEAD - 1) * (M::INS + 1)>();
             __syncthreads();
-#pragma unroll
-            for (int k = 0; k + 1 < AHEAD; ++k) ahead[k] = ahead[k + 1];
-            ahead[AHEAD - 1] = issue(smem + (at + AHEAD) % M::BUFS * M::TILE);
-            const T* tile = smem + at * M::TILE;
+            issue(smem + (at + AHEAD) % M::BUFS * M::TILE);
+            const bool ok = tok + mt < have && !pad && hp * 32 + mh < hpg;
+            nl = ok ? negated(log_sums[(at * 4 + wave) * WAVE + lane]) : -INFINITY;
+            uint32_t row = uint32_t(uintptr_t((lds_ptr)(smem + at * M::TILE))) + my_row;
+            asm volatile("" : "+v"(row));  // (or all steps' addresses are kept in registers)
             at = (at + 1) % M::BUFS;
-            floatx16 sc[NB];
+            return row;
+        };
+        auto next = [&] {
+            if (++hp == parts) hp = 0, tok += TPT;
+        };
+        // Tiles [f0, f1) hold tokens that see all keys of the block.
+        int f0 = q.base + ta >= kb + M::KEYS - 1 ? 0 : (kb + M::KEYS - 1 - q.base - ta + TPT - 1) / TPT * parts, f1 = ntile;
+        if (w > 0) {
+            const int64_t most = int64_t(w) + kb - q.base - ta - TPT;  // the last first token
+            f1 = most < 0 ? 0 : int(most / TPT + 1 < f1 ? (most / TPT + 1) * parts : f1);
+        }
+        if (hpg > 32 && hpg % 32) f0 = ntile;  // (a part's last rows are other heads')
+        f0 = f0 < ntile ? f0 : ntile, f1 = f1 < ntile ? f1 : ntile, f1 = f1 > f0 ? f1 : f0;
+#pragma unroll 1
+        for (int i = 0; i < ntile;) {
+            if (i != f0 || f0 == f1) {
+                // Tiles at the diagonal and the window's end.
+                const int end = i < f0 ? f0 : ntile;
+#pragma unroll 1
+                for (; i < end; ++i, next()) {
+                    float nl;
+                    const uint32_t row = arrive(nl);
+                    // (the lane's keys past k0 + 4 (lane / 32): constants of an element)
+                    const int last = q.base + ta + tok + mt - k0 - 4 * (lane / 32);
+                    const int from = w == 0 ? INT_MIN : __builtin_elementwise_sub_sat(last, w);
 #pragma unroll
-            for (int j = 0; j < NB; ++j)
+                    for (int j = 0; j < NB; ++j) {
+                        floatx16 sc;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) sc[j][r] = 0.0f;
-            const int row = lane % 32;
+                        for (int r = 0; r < 16; ++r) sc[r] = 0.0f;
 #pragma unroll
-            for (int st = 0; st < NS; ++st) {
-                const frag qf = *reinterpret_cast<const frag*>(tile + row * D + ((2 * st + lane / 32) ^ M::swz(row)) * 8);
+                        for (int st = 0; st < NS; ++st) sc = mfma32(kf[j][st], *(operand)(uintptr_t)(row ^ uint32_t(32 * st)), sc);
 #pragma unroll
-                for (int j = 0; j < NB; ++j) sc[j] = mfma32(kf[j][st], qf, sc[j]);
-            }
-            // Operands are read READ steps ahead of their MFMAs.  (Left alone, the
-            // compiler reads one and waits for it.)
-            constexpr int READ = 3;
-            __builtin_amdgcn_sched_group_barrier(0x100, READ, 0);
-#pragma unroll
-            for (int st = 0; st < NS; ++st) {
-                __builtin_amdgcn_sched_group_barrier(0x8, NB, 0);
-                if (st + READ < NS) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-            // The tile's tokens have the rows own .. own + TPT - 1 in the cache:
-            // whether all see all the wave's keys.
-            const int own = q.base + ta + i / parts * TPT;
-            const bool full = own >= k0 + 32 * NB - 1 && (w == 0 || own + TPT - 1 - k0 < w) && __all(nl != -INFINITY);
-            if (full) {
-#pragma unroll
-                for (int j = 0; j < NB; ++j)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) sum[j][r] += prob(sc[j][r], a.x.scale, nl);
+                        for (int r = 0; r < 16; ++r) {
+                            const int key = 32 * j + 8 * (r / 4) + r % 4;
+                            const float p = prob(sc[r], a.x.scale, nl);
+                            sum[j][r] += key <= last && key > from && nl != -INFINITY ? p : 0.0f;
+                        }
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                }
                 continue;
             }
-            // the lane's keys past k0 + 4 (lane / 32): constants of (j, r)
-            const int last = own + mt - k0 - 4 * (lane / 32);
-            const int from = w == 0 ? INT_MIN : __builtin_elementwise_sub_sat(last, w);
+            // The scores of a block wait for the next block's MFMAs, in whose shadow
+            // their exponentials run (one after the other they took 132,000 and
+            // 154,000 of a SIMD's 351,000 cycles).  A step: an MFMA, the operand of
+            // the one READ steps on and a part of the block before, in this order.
+            // (Left alone, the compiler reads one operand and waits for it.)
+            floatx16 was;
+            float was_nl = -INFINITY;
 #pragma unroll
-            for (int j = 0; j < NB; ++j)
+            for (int r = 0; r < 16; ++r) was[r] = 0.0f;
+#pragma unroll 1
+            for (; i < f1; ++i, next()) {
+                float nl;
+                const uint32_t row = arrive(nl);
+                constexpr int READ = 3;
+                frag qf[READ];
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int key = 32 * j + 8 * (r / 4) + r % 4;
-                    const bool see = key <= last && key > from && nl != -INFINITY;
-                    const float p = prob(sc[j][r], a.x.scale, nl);
-                    sum[j][r] += see ? p : 0.0f;
+                for (int k = 0; k < READ; ++k) qf[k] = *(operand)(uintptr_t)(row ^ uint32_t(32 * k));
+#pragma unroll
+                for (int j = 0; j < NB; ++j) {
+                    floatx16 sc;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) sc[r] = 0.0f;
+#pragma unroll
+                    for (int st = 0; st < NS; ++st) {
+                        const int n = j * NS + st;
+                        sc = mfma32(kf[j][st], qf[n % READ], sc);
+                        if (n + READ < NB * NS) qf[n % READ] = *(operand)(uintptr_t)(row ^ uint32_t(32 * ((n + READ) % NS)));
+#pragma unroll
+                        for (int r = st * 16 / NS; r < (st + 1) * 16 / NS; ++r) sum[(j + NB - 1) % NB][r] += prob(was[r], a.x.scale, was_nl);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                    was = sc, was_nl = nl;
                 }
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) sum[NB - 1][r] += prob(was[r], a.x.scale, was_nl);
         }
         wait_loads<0>();  // (no load may find the LDS another workgroup's)
     }
@@ -409,8 +452,16 @@ void launch_d(hipStream_t s, Args a) {
     a.blocks = (a.max_len + Many<T, D>::KEYS - 1) / Many<T, D>::KEYS;
     const int64_t n = lists * a.blocks * a.splits;
     if (n >= MAX_BLOCKS || lists > 65535) fail(E_CAPACITY, "attention_weights: too many work items");
-    constexpr unsigned lds = Many<T, D>::BUFS * Many<T, D>::TILE * 2;
-    static_assert(lds <= 65536, "no attribute asked for");
+    constexpr unsigned lds = Many<T, D>::BUFS * (Many<T, D>::TILE * 2 + 4 * WAVE * 4);
+    static std::atomic<uint64_t> lds_set{0};  // the devices, once per instantiation
+    int device = 0;
+    OMG_HIP(hipGetDevice(&device));
+    const uint64_t bit = uint64_t(1) << (device & 63);
+    if (device > 63 || !(lds_set.load(std::memory_order_relaxed) & bit)) {
+        OMG_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(weights_many_kernel<T, D>),
+                                    hipFuncAttributeMaxDynamicSharedMemorySize, int(lds)));
+        lds_set.fetch_or(bit, std::memory_order_relaxed);
+    }
     weights_many_kernel<T, D><<<dim3(unsigned(n)), dim3(256), lds, s>>>(a);
     OMG_HIP(hipGetLastError());
     if (a.splits > 1) {
