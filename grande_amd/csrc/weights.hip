@@ -193,6 +193,13 @@ __device__ inline void to_lds(const char* base, int bytes, const uint32_t* off, 
         __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr)(static_cast<char*>(dst) + 1024 * i), 16, off[i], 0, 0, 0);
 }
 
+// A value a lane.  (Not by a global load to LDS: behind one the compiler waits
+// for all LDS reads where it needs the oldest.)
+__device__ inline void log_sums_to_lds(const char* base, int bytes, uint32_t off, void* dst) {
+    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), (short)0, bytes, 0x00020000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr)dst, 4, off, 0, 0, 0);
+}
+
 // All but the last N loads have arrived, and LDS reads.
 template <int N>
 __device__ inline void wait_loads() {
@@ -264,6 +271,8 @@ __global__ __launch_bounds__(256, 2) void weights_many_kernel(Args a) {
         }
         const int mt = lane % 32 / heads, mh = lane % 32 - mt * heads;  // the lane's query row
         int t0 = 0, part = 0;                                           // of the next tile
+        const float* lse = a.x.lse + tok0 * a.x.heads + g * hpg;
+        const uint32_t lse_off = uint32_t(mt * a.x.heads + mh) * 4;
         // Rows that are not there arrive as zeros, or as others, and have a
         // negated log sum of minus infinity.  (A load each way: the waits count.)
         auto issue = [&](T* dst) {
@@ -271,11 +280,9 @@ __global__ __launch_bounds__(256, 2) void weights_many_kernel(Args a) {
             const int64_t left = t0 < have ? 2 * ((have - 1) * a.x.ldq + hpg * D - skip) : 0;
             to_lds<M::INS>(qb + (t0 < have ? 2 * skip : 0), int(left < INT_MAX ? left : INT_MAX), off, dst + wave * M::INS * 512);
             // (log sums into registers would be waited for, and all loads before them, tile by tile)
-            const bool ok = t0 + mt < have && mt < TPT && part * 32 + mh < hpg;
-            const float* lse = a.x.lse + tok0 * a.x.heads + g * hpg + (ok ? int64_t(t0 + mt) * a.x.heads + part * 32 + mh : 0);
-            __builtin_amdgcn_global_load_lds(
-                reinterpret_cast<__attribute__((address_space(1))) void*>(reinterpret_cast<uintptr_t>(lse)),
-                (lds_ptr)(log_sums + (int(dst - smem) / M::TILE * 4 + wave) * WAVE), 4, 0, 0);
+            const int64_t past = int64_t(t0) * a.x.heads + part * 32, rest = t0 < have ? 4 * (int64_t(have) * a.x.heads - g * hpg - past) : 0;
+            log_sums_to_lds(reinterpret_cast<const char*>(lse + (t0 < have ? past : 0)), int(rest < INT_MAX ? rest : INT_MAX),
+                            lse_off, log_sums + (int(dst - smem) / M::TILE * 4 + wave) * WAVE);
             if (++part == parts) part = 0, t0 += TPT;
         };
         // BUFS - 1 tiles are under way; behind the last one the loads go on, to
@@ -294,7 +301,8 @@ __global__ __launch_bounds__(256, 2) void weights_many_kernel(Args a) {
             __syncthreads();
             issue(smem + (at + AHEAD) % M::BUFS * M::TILE);
             const bool ok = tok + mt < have && !pad && hp * 32 + mh < hpg;
-            nl = ok ? negated(log_sums[(at * 4 + wave) * WAVE + lane]) : -INFINITY;
+            const float lse = log_sums[(at * 4 + wave) * WAVE + lane];
+            nl = ok ? negated(lse) : -INFINITY;
             uint32_t row = uint32_t(uintptr_t((lds_ptr)(smem + at * M::TILE))) + my_row;
             asm volatile("" : "+v"(row));  // (or all steps' addresses are kept in registers)
             at = (at + 1) % M::BUFS;
@@ -346,6 +354,8 @@ __global__ __launch_bounds__(256, 2) void weights_many_kernel(Args a) {
             // 154,000 of a SIMD's 351,000 cycles).  A step: an MFMA, the operand of
             // the one READ steps on and a part of the block before, in this order.
             // (Left alone, the compiler reads one operand and waits for it.)
+            // (from the third step on: the block's last MFMA is still under way)
+            auto first = [](int st) { return st < 2 ? 0 : (st - 2) * 16 / (NS - 2); };
             floatx16 was;
             float was_nl = -INFINITY;
 #pragma unroll
@@ -369,7 +379,7 @@ __global__ __launch_bounds__(256, 2) void weights_many_kernel(Args a) {
                         sc = mfma32(kf[j][st], qf[n % READ], sc);
                         if (n + READ < NB * NS) qf[n % READ] = *(operand)(uintptr_t)(row ^ uint32_t(32 * ((n + READ) % NS)));
 #pragma unroll
-                        for (int r = st * 16 / NS; r < (st + 1) * 16 / NS; ++r) sum[(j + NB - 1) % NB][r] += prob(was[r], a.x.scale, was_nl);
+                        for (int r = first(st); r < first(st + 1); ++r) sum[(j + NB - 1) % NB][r] += prob(was[r], a.x.scale, was_nl);
                         __builtin_amdgcn_sched_barrier(0);
                     }
                     was = sc, was_nl = nl;
@@ -406,6 +416,7 @@ __global__ __launch_bounds__(256) void weights_join_kernel(Args a) {
     const int64_t p = a.b.table[s * a.b.table_ld + (key >> a.page_shift)];
     if (p < 0 || p >= a.kv.npages) return;
     float v = 0.0f;
+#pragma unroll 8
     for (int i = 0; i < a.splits; ++i) v += a.part[(i * a.b.nseq * a.kv.kv_heads + list) * a.max_len + key];
     a.x.weights[list * a.x.ldw + key] += v;
 }
@@ -422,13 +433,29 @@ bool few(const PagedKv& kv, const PagedBatch& b, int heads) { return b.t * (head
 
 int many_keys(int head_dim) { return head_dim == 512 ? 128 : 256; }
 
-// Splits of the queries until some two rounds of work items are there.
+// The splits of the queries of least time, by the rounds in which the places
+// that the chip has take the items with something to do (keys near a prompt's
+// end have few queries) and an item's tiles, three more for its start and end,
+// for sequences of the mean number of tokens.  (8,000 tokens x 8 heads of 256 on
+// 4 KV heads: 4 / 7 / 14 / 32 splits 244 / 172 / 216 / 220 us; 7 is what this
+// gives.)
 int splits(const PagedKv& kv, const PagedBatch& b, int heads) {
     if (few(kv, b, heads)) return 1;
-    const int64_t max_len = b.max_pages * kv.page, keys = many_keys(kv.head_dim);
-    const int64_t items = b.nseq * kv.kv_heads * ((max_len + keys - 1) / keys);
-    const int64_t rows = (b.t + b.nseq - 1) / b.nseq * (heads / kv.kv_heads);  // of a sequence
-    return int(std::max<int64_t>(1, std::min<int64_t>({4096 / items, rows / 256, 32})));
+    const int64_t max_len = b.max_pages * kv.page, keys = many_keys(kv.head_dim), blocks = (max_len + keys - 1) / keys;
+    const int64_t n = (b.t + b.nseq - 1) / b.nseq, tiles = (n * (heads / kv.kv_heads) + 31) / 32;
+    const int64_t base = max_len - n, places = kv.head_dim == 64 ? 768 : 512;
+    const double tile_us = 0.4 + kv.head_dim * 0.0057;
+    int best = 1;
+    double best_us = 1e30;
+    for (int k = 1; k <= 32 && (k == 1 || tiles >= 8 * k); ++k) {
+        // Split c has tokens up to (c + 1) n / k, which see blocks up to theirs.
+        int64_t items = 0;
+        for (int c = 0; c < k; ++c) items += std::min(blocks, (base + (c + 1) * n / k) / keys + 1);
+        const double rounds = double((items * b.nseq * kv.kv_heads + places - 1) / places);
+        const double us = rounds * (double((tiles + k - 1) / k) + 3) * tile_us + (k > 1 ? 3 + 0.2 * k : 0);
+        if (us < best_us) best_us = us, best = k;
+    }
+    return best;
 }
 
 int64_t part_bytes(const PagedKv& kv, const PagedBatch& b, int heads) {
