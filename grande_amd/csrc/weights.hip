@@ -88,11 +88,13 @@ __device__ inline const T* key_row(const Args& a, const int32_t* table, int row,
     return static_cast<const T*>(a.kv.k) + p * a.kv.page_stride + (int64_t(g) * a.kv.page + (row & (a.kv.page - 1))) * D;
 }
 
-// Four waves, each every fourth group of U 16-key tiles of the chunk.
+// Four waves, each every fourth group of U 16-key tiles of the chunk.  (More
+// waves on a CU keep more loads under way than more tiles in a wave: 128-wide
+// heads with four tiles, 130 registers, 200 us, with one, 58, 170.)
 template <typename T, int D>
 __global__ __launch_bounds__(256) void weights_few_kernel(Args a) {
     typedef typename Vec8<T>::type frag;
-    constexpr int NS = D / 32, U = D >= 512 ? 1 : D >= 256 ? 2 : 4, KEYS = 16 * U;
+    constexpr int NS = D / 32, U = D >= 128 ? 1 : 2, KEYS = 16 * U;
     const int lane = int(threadIdx.x) % WAVE, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / WAVE);
     const int64_t id = blockIdx.x, list = id / a.blocks, s = list / a.kv.kv_heads;
     const int g = int(list - s * a.kv.kv_heads), from = int(id - list * a.blocks) * a.chunk;
@@ -467,9 +469,10 @@ template <typename T, int D>
 void launch_d(hipStream_t s, Args a) {
     const int64_t lists = a.b.nseq * a.kv.kv_heads;
     if (few(a.kv, a.b, a.x.heads)) {
-        // Chunks of 256 keys and more, some eight workgroups a CU.
+        // Chunks of 256 keys and more: 64 workgroups a CU are enough.  (512 lists of
+        // 8,192 rows: 32 / 16 / 8 of them 170 / 174 / 185 us.)
         a.chunk = 256;
-        while (a.chunk < 4096 && lists * (a.max_len / a.chunk) > 4096) a.chunk *= 2;
+        while (a.chunk < 4096 && lists * (a.max_len / a.chunk) > 16384) a.chunk *= 2;
         a.blocks = (a.max_len + a.chunk - 1) / a.chunk;
         if (lists * a.blocks >= MAX_BLOCKS) fail(E_CAPACITY, "attention_weights: too many work items");
         weights_few_kernel<T, D><<<dim3(unsigned(lists * a.blocks)), dim3(256), 0, s>>>(a);
