@@ -158,6 +158,11 @@ _SIGS = {
     "omg_dev_attention_tree_workspace": (C.c_int64, [C.POINTER(omg_paged_kv), C.POINTER(omg_paged_batch), C.c_int]),
     "omg_dev_attention_tree": (C.c_int, [C.POINTER(omg_paged_kv), C.POINTER(omg_paged_batch), C.c_int, _P, C.c_int64,
                                          _P, C.c_int64, _P, C.c_float, _P, C.c_int64, C.c_int, _P, _P, C.c_size_t, _P]),
+    "omg_dev_block_means": (C.c_int, [C.POINTER(omg_paged_kv), C.POINTER(omg_paged_batch), _P, _P]),
+    "omg_dev_attention_blocks_workspace": (C.c_int64, [C.POINTER(omg_paged_kv), C.POINTER(omg_paged_batch), C.c_int,
+                                                       C.c_int64]),
+    "omg_dev_attention_blocks": (C.c_int, [C.POINTER(omg_paged_kv), C.POINTER(omg_paged_batch), C.c_int, _P, C.c_int64,
+                                           _P, C.c_int64, _P, C.c_float, _P, C.c_int64, _P, _P, C.c_size_t, _P]),
     "omg_dev_attention_weights_workspace": (C.c_int64, [C.POINTER(omg_paged_kv), C.POINTER(omg_paged_batch), C.c_int]),
     "omg_dev_attention_weights": (C.c_int, [C.POINTER(omg_paged_kv), C.POINTER(omg_paged_batch), C.c_int, _P, C.c_int64,
                                             _P, C.c_float, C.c_int, _P, C.c_int64, _P, C.c_size_t, _P]),

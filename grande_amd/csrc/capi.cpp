@@ -723,6 +723,28 @@ int omg_dev_attention_tree(const omg_paged_kv* kv, const omg_paged_batch* b, int
     });
 }
 
+int omg_dev_block_means(const omg_paged_kv* kv, const omg_paged_batch* b, float* means, void* stream) {
+    return guard([&] {
+        omg::launch_block_means(static_cast<hipStream_t>(stream), paged_kv(kv), paged_batch(b), means);
+    });
+}
+
+int64_t omg_dev_attention_blocks_workspace(const omg_paged_kv* kv, const omg_paged_batch* b, int heads, int64_t blocks) {
+    int64_t n = 0;
+    const int rc = guard([&] { n = omg::attention_blocks_workspace(paged_kv(kv), paged_batch(b), heads, blocks); });
+    return rc == OMG_OK ? n : rc;
+}
+
+int omg_dev_attention_blocks(const omg_paged_kv* kv, const omg_paged_batch* b, int heads, const void* q, int64_t ldq,
+                             void* out, int64_t ldo, float* lse, float scale, const float* means, int64_t blocks,
+                             int32_t* chosen, void* workspace, size_t workspace_bytes, void* stream) {
+    return guard([&] {
+        const omg::SharedAttn x{heads, q, ldq, out, ldo, lse, scale, 0};
+        omg::launch_attention_blocks(static_cast<hipStream_t>(stream), paged_kv(kv), paged_batch(b), x, means, blocks,
+                                     chosen, workspace, workspace_bytes);
+    });
+}
+
 int64_t omg_dev_attention_weights_workspace(const omg_paged_kv* kv, const omg_paged_batch* b, int heads) {
     int64_t n = 0;
     const int rc = guard([&] { n = omg::attention_weights_workspace(paged_kv(kv), paged_batch(b), heads); });

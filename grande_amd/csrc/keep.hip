@@ -3,6 +3,7 @@
 #include <algorithm>
 #include <string>
 
+#include "choose.h"
 #include "common.h"
 #include "kern_common.h"
 #include "paged.h"
@@ -195,21 +196,9 @@ void check_sequences(const PagedBatch& b, const PagedKv& kv, const char* who) {
 // ------------------------------------------------------------------- evict
 //
 // A workgroup chooses a list's rows: the `recent` last ones and, of those
-// before them, the keep - recent of the largest weights.  Weights become
-// 32-bit keys of the same order.  Passes over 8 bits each, from the top, narrow
-// the key of the last one chosen down (a histogram of 256 bins, 8 copies by
-// lane, so that equal bits seldom meet in one LDS word) until at most FEW rows
-// share the bits found: these are counted against each other.  Then a pass
-// counts per 64 rows what lies over that key and at it, and a last one writes
-// the chosen, of the equal ones the first.
-//
-// One workgroup a list and a chain of barriers: lists of up to 8,192 rows stay
-// in registers, 8 a thread; longer ones are read again from L2 in each pass.
+// before them, the keep - recent of the largest weights (choose.h).
 
-constexpr int EVICT_T = 1024, EVICT_WAVES = EVICT_T / WAVE;
-constexpr int EVICT_CELLS = 1024;  // of 64 rows
-constexpr int EVICT_R = 8;         // rows of a thread in registers
-constexpr int COPIES = 8, FEW = 128;
+constexpr int EVICT_T = 1024;
 
 struct EvictArgs {
     PagedBatch b;
@@ -218,18 +207,11 @@ struct EvictArgs {
     int64_t max_len;
 };
 
-// Ascending with the weight; NaN lowest, the zeros alike.
-__device__ inline uint32_t weight_key(float w) {
-    const uint32_t u = __builtin_bit_cast(uint32_t, w + 0.0f);
-    return w != w ? 0u : u >> 31 ? ~u : u | 0x80000000u;
-}
-
 template <bool HELD>
 __global__ __launch_bounds__(EVICT_T) void evict_kernel(EvictArgs a) {
-    __shared__ uint32_t bins[COPIES * 256];
-    __shared__ uint32_t cells[2 * EVICT_CELLS];
-    __shared__ uint32_t few[FEW], sums[2 * EVICT_WAVES], found[3], nfew;
-    const int tid = int(threadIdx.x), lane = tid % WAVE, wave = tid / WAVE;
+    typedef Choose<EVICT_T, HELD> C;
+    __shared__ typename C::Shared shared;
+    const int tid = int(threadIdx.x);
     const int64_t list = blockIdx.x, s = list / a.kv_heads;
     const float* w = a.x.weights + list * a.x.ldw;
     float* kept = a.x.kept + list * a.x.kept_ld;
@@ -243,155 +225,9 @@ __global__ __launch_bounds__(EVICT_T) void evict_kernel(EvictArgs a) {
         }
         return;
     }
-    const int old = n - recent;
-    float held[EVICT_R];
-    if constexpr (HELD) {
-#pragma unroll
-        for (int u = 0; u < EVICT_R; ++u) held[u] = tid + u * EVICT_T < old ? w[tid + u * EVICT_T] : 0.0f;
-    }
-    // f(key) for each of the thread's rows of the first `old`.
-    auto each = [&](auto f) {
-        if constexpr (HELD) {
-#pragma unroll
-            for (int u = 0; u < EVICT_R; ++u)
-                if (tid + u * EVICT_T < old) f(weight_key(held[u]));
-        } else {
-            for (int i0 = tid; i0 < old; i0 += EVICT_R * EVICT_T) {
-                float x[EVICT_R];
-#pragma unroll
-                for (int u = 0; u < EVICT_R; ++u) x[u] = i0 + u * EVICT_T < old ? w[i0 + u * EVICT_T] : 0.0f;
-#pragma unroll
-                for (int u = 0; u < EVICT_R; ++u)
-                    if (i0 + u * EVICT_T < old) f(weight_key(x[u]));
-            }
-        }
-    };
-    uint32_t left = uint32_t(keep - recent);  // to be chosen of the first `old` rows
-    uint32_t key = 0xffffffffu;                   // ... over this key, and `left` at it
-    if (left) {
-        key = 0;
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            for (int i = tid; i < COPIES * 256; i += EVICT_T) bins[i] = 0;
-            if (tid == 0) nfew = 0;
-            __syncthreads();
-            const uint32_t mask = shift == 24 ? 0u : ~0u << (shift + 8);
-            each([&](uint32_t k) {
-                if ((k & mask) == key) atomicAdd(&bins[lane % COPIES * 256 + (k >> shift & 255)], 1u);
-            });
-            __syncthreads();
-            // A thread a bin: its count and how many lie over it.
-            uint32_t mine = 0, upto = 0;
-            if (tid < 256) {
-#pragma unroll
-                for (int i = 0; i < COPIES; ++i) mine += bins[i * 256 + tid];
-                upto = mine;
-                for (int d = 1; d < WAVE; d *= 2) {
-                    const uint32_t x = __shfl_down(upto, d, WAVE);
-                    if (lane + d < WAVE) upto += x;
-                }
-                if (lane == 0) sums[wave] = upto;
-            }
-            __syncthreads();
-            if (tid < 256) {
-                for (int i = wave + 1; i < 4; ++i) upto += sums[i];
-                if (upto - mine < left && left <= upto) found[0] = uint32_t(tid), found[1] = upto - mine, found[2] = mine;
-            }
-            __syncthreads();
-            key |= found[0] << shift;
-            left -= found[1];
-            if (shift && found[2] <= FEW) {
-                const uint32_t m = found[2], bits = ~0u << shift;
-                each([&](uint32_t k) {
-                    if ((k & bits) == key) few[atomicAdd(&nfew, 1u)] = k;
-                });
-                __syncthreads();
-                if (uint32_t(tid) < m) {
-                    uint32_t over = 0, upto = 0;
-                    for (uint32_t j = 0; j < m; ++j) over += few[j] > few[tid], upto += few[j] >= few[tid];
-                    if (over < left && left <= upto) found[0] = few[tid], found[1] = over;
-                }
-                __syncthreads();
-                key = found[0], left -= found[1];
-                break;
-            }
-        }
-    }
-    // Rows over the key and at it, by cells of 64.
-    uint32_t over = 0, at = 0;  // before this part
-    for (int base = 0; base < old; base += EVICT_CELLS * WAVE) {
-        const int end = old - base < EVICT_CELLS * WAVE ? old - base : EVICT_CELLS * WAVE;
-        const int ncell = (end + WAVE - 1) / WAVE;
-        auto count = [&](int c, int i, float x) {
-            const uint32_t k = weight_key(x);
-            const uint64_t bo = __ballot(i < old && k > key), be = __ballot(i < old && k == key);
-            if (lane == 0) cells[2 * c] = __popcll(bo), cells[2 * c + 1] = __popcll(be);
-        };
-        if constexpr (HELD) {
-#pragma unroll
-            for (int u = 0; u < EVICT_R; ++u)
-                if (u * EVICT_WAVES + wave < ncell) count(u * EVICT_WAVES + wave, tid + u * EVICT_T, held[u]);
-        } else {
-            for (int c = wave; c < ncell; c += EVICT_WAVES) {
-                const int i = base + c * WAVE + lane;
-                count(c, i, i < old ? w[i] : 0.0f);
-            }
-        }
-        __syncthreads();
-        // Each thread a cell: the counts before it.
-        const uint32_t o = tid < ncell ? cells[2 * tid] : 0, e = tid < ncell ? cells[2 * tid + 1] : 0;
-        uint32_t po = o, pe = e;
-        for (int d = 1; d < WAVE; d *= 2) {
-            const uint32_t x = __shfl_up(po, d, WAVE), y = __shfl_up(pe, d, WAVE);
-            if (lane >= d) po += x, pe += y;
-        }
-        if (lane == WAVE - 1) sums[2 * wave] = po, sums[2 * wave + 1] = pe;
-        __syncthreads();
-        uint32_t to = over, te = at;
-        for (int i = 0; i < EVICT_WAVES; ++i) {
-            if (i < wave) po += sums[2 * i], pe += sums[2 * i + 1];
-            to += sums[2 * i], te += sums[2 * i + 1];
-        }
-        if (tid < ncell) cells[2 * tid] = over + po - o, cells[2 * tid + 1] = at + pe - e;
-        __syncthreads();
-        // A chosen row's place is the number of the chosen before it, which no
-        // row of a later part has.  (In place a part is read before any of it
-        // is written.)
-        for (int c0 = 0; c0 < ncell; c0 += EVICT_R * EVICT_WAVES) {
-            float x[EVICT_R];
-            int place[EVICT_R];
-#pragma unroll
-            for (int u = 0; u < EVICT_R; ++u) {
-                const int i = base + (c0 + u * EVICT_WAVES + wave) * WAVE + lane;
-                if constexpr (HELD)
-                    x[u] = held[u];
-                else
-                    x[u] = i < old ? w[i] : 0.0f;
-            }
-#pragma unroll
-            for (int u = 0; u < EVICT_R; ++u) {
-                const int c = c0 + u * EVICT_WAVES + wave;
-                const int i = base + c * WAVE + lane;
-                place[u] = -1;
-                if (c >= ncell) continue;
-                const uint32_t k = weight_key(x[u]);
-                const uint64_t before = (uint64_t(1) << lane) - 1;
-                const uint64_t bo = __ballot(i < old && k > key), be = __ballot(i < old && k == key);
-                const uint32_t no = cells[2 * c] + __popcll(bo & before), ne = cells[2 * c + 1] + __popcll(be & before);
-                if (i < old && (k > key || (k == key && ne < left))) place[u] = no + (ne < left ? ne : left);
-            }
-            if constexpr (!HELD) __syncthreads();
-#pragma unroll
-            for (int u = 0; u < EVICT_R; ++u)
-                if (place[u] >= 0) {
-                    rows[place[u]] = (base + (c0 + u * EVICT_WAVES + wave) * WAVE + lane);
-                    kept[place[u]] = x[u];
-                }
-        }
-        over = to, at = te;
-        __syncthreads();
-    }
+    const int old = n - recent, chosen = keep - recent;
+    C::run(shared, w, old, uint32_t(chosen), [&](int rank, int row, float x) { rows[rank] = row, kept[rank] = x; });
     // The recent rows, and zeros for the rows to come.
-    const int chosen = keep - recent;
     for (int i0 = 0; i0 < recent; i0 += EVICT_T) {
         const int i = i0 + tid;
         const float x = i < recent ? w[old + i] : 0.0f;
@@ -431,7 +267,7 @@ void launch_kv_evict(hipStream_t s, const PagedKv& kv, const PagedBatch& b, cons
     if (b.nseq * kv.kv_heads >= MAX_BLOCKS) fail(E_CAPACITY, "kv_evict: too many lists for one call");
     EvictArgs a{b, x, kv.kv_heads, max_len};
     const dim3 grid(unsigned(b.nseq * kv.kv_heads));
-    if (max_len <= EVICT_R * EVICT_T)
+    if (max_len <= CHOOSE_R * EVICT_T)
         evict_kernel<true><<<grid, dim3(EVICT_T), 0, s>>>(a);
     else
         evict_kernel<false><<<grid, dim3(EVICT_T), 0, s>>>(a);

@@ -369,6 +369,12 @@ int64_t attention_tree_workspace(const PagedKv& kv, const PagedBatch& b, int hea
 void launch_attention_tree(hipStream_t s, const PagedKv& kv, const PagedBatch& b, const SharedAttn& x,
                            const TreeMask& tree, void* workspace, size_t bytes);
 
+// ---- attention over few blocks (block_attention.hip) ----
+void launch_block_means(hipStream_t s, const PagedKv& kv, const PagedBatch& b, float* means);
+int64_t attention_blocks_workspace(const PagedKv& kv, const PagedBatch& b, int heads, int64_t keep);
+void launch_attention_blocks(hipStream_t s, const PagedKv& kv, const PagedBatch& b, const SharedAttn& x,
+                             const float* means, int64_t keep, int32_t* chosen, void* workspace, size_t bytes);
+
 // ---- the attention weight of cached rows (weights.hip) ----
 struct AttnWeights {
     int heads;

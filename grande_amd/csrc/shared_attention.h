@@ -557,18 +557,20 @@ struct Keys {
 // until every element is NaN: 0.3 to 0.4 us a key and row.  One infinite
 // value in a prefix of 8,000 keys, which all rows see: 208 answers' tokens x 8
 // heads of 256 45 us -> 4.4 ms, 6,300 questions' tokens 0.5 -> 111 ms.
-template <typename T, int D, bool MASKED>
-__device__ void seen_alone(const Args& a, const Keys& in, const Row& r, uint64_t rows, float lg, int lane, int64_t slot,
-                           int quarter) {
+//   `walk(lane of a row, keys)` calls keys(from, to, page) for each run of keys
+// that the row sees: key k is row k % page length of page(k), which is outside
+// the pool where the row does not see it.
+template <typename T, int D, typename W>
+__device__ void seen_alone(const Args& a, int g, const Row& r, uint64_t rows, float lg, int lane, int64_t slot,
+                           int quarter, W walk) {
     constexpr int NQ = D / 4, E = (NQ + WAVE - 1) / WAVE;
     typedef T vec4 __attribute__((ext_vector_type(4)));
-    const int P = int(a.b.prefix_len), w = a.x.window;
 #pragma unroll 1
     for (; rows; rows &= rows - 1) {
         const int i = __builtin_ctzll(rows);
         const auto of = [&](int v) { return __builtin_amdgcn_readlane(v, i); };
         const auto off = [&](float v) { return __builtin_bit_cast(float, of(__builtin_bit_cast(int, v))); };
-        const int at = of(r.at), seq = of(r.seq), own = of(r.own);
+        const int at = of(r.at);
         const int64_t tok = at / a.x.heads;
         const int head = at % a.x.heads;
         const float row_lg = off(lg), ref = row_lg == -INFINITY ? 0.0f : row_lg;
@@ -586,7 +588,7 @@ __device__ void seen_alone(const Args& a, const Keys& in, const Row& r, uint64_t
         for (int e = 0; e < E; ++e) o[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         float total = 0.0f;  // of the probabilities: one, but for rounding
         bool lost = false;   // every element is NaN, and stays so
-        const auto keys = [&](const int32_t* table, int plast, int from, int to, int base) {
+        const auto keys = [&](int from, int to, auto page_of) {
             constexpr int U = 4;  // keys under way together
 #pragma unroll 1
             for (int k = from; k < to && !lost; k += U) {
@@ -596,10 +598,9 @@ __device__ void seen_alone(const Args& a, const Keys& in, const Row& r, uint64_t
                 float p[U];
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
-                    const int64_t page = table[imin(imin(k + u, to - 1) >> a.page_shift, plast)];
+                    const int64_t page = page_of(imin(k + u, to - 1));
                     ok[u] = k + u < to && page >= 0 && page < a.kv.npages;
-                    if (MASKED && k + u >= base) ok[u] = ok[u] && (a.tree.seen(tok, k + u - base) & 1);
-                    key[u] = ok[u] ? page * a.kv.page_stride + (int64_t(in.g) * a.kv.page + ((k + u) & (a.kv.page - 1))) * D : 0;
+                    key[u] = ok[u] ? page * a.kv.page_stride + (int64_t(g) * a.kv.page + ((k + u) & (a.kv.page - 1))) * D : 0;
                 }
 #pragma unroll
                 for (int u = 0; u < U; ++u) load(a.kv.k, key[u], x[u]);
@@ -629,11 +630,7 @@ __device__ void seen_alone(const Args& a, const Keys& in, const Row& r, uint64_t
                 lost = __all(nan);
             }
         };
-        keys(a.b.prefix_table, (P - 1) >> a.page_shift, imax(in.pb, first_seen(P, own, w)), in.pe, INT_MAX);
-        const int base = MASKED ? own_base(a, seq) : 0;
-        keys(a.b.table + seq * a.b.table_ld, int(a.b.max_pages) - 1,
-             imax(in.ob, MASKED ? imin(first_seen(0, own, w), imax(base, 0)) : first_seen(0, own, w)),
-             MASKED ? imin(in.oe, a.b.lens[seq]) : imin(in.oe, own + 1), base);
+        walk(i, keys);
         const Sink<T> out{a, at, tok * a.x.ldo + int64_t(head) * D, slot};
         const float inv = total == 0.0f ? 0.0f : 1.0f / total;
 #pragma unroll
@@ -645,11 +642,27 @@ __device__ void seen_alone(const Args& a, const Keys& in, const Row& r, uint64_t
     }
 }
 
-// The results of a wave's rows (not KEYS).  `place`: called ahead of
-// seen_alone, which needs the rows' sequences.
-template <typename T, int D, int TILE, bool MASKED, typename F>
-__device__ inline void emit(const Args& a, Core<T, D, TILE>& core, const Keys& in, const Row& r, int lane,
-                            int64_t slot, F place) {
+// The keys of an item that the row of lane i sees.
+template <bool MASKED, typename F>
+__device__ inline void seen_keys(const Args& a, const Keys& in, const Row& r, int i, F keys) {
+    const auto of = [&](int v) { return __builtin_amdgcn_readlane(v, i); };
+    const int P = int(a.b.prefix_len), w = a.x.window, seq = of(r.seq), own = of(r.own), plast = (P - 1) >> a.page_shift;
+    const int64_t tok = of(r.at) / a.x.heads;
+    keys(imax(in.pb, first_seen(P, own, w)), in.pe,
+         [&](int k) { return int64_t(a.b.prefix_table[imin(k >> a.page_shift, plast)]); });
+    const int base = MASKED ? own_base(a, seq) : 0;
+    const int32_t* table = a.b.table + seq * a.b.table_ld;
+    keys(imax(in.ob, MASKED ? imin(first_seen(0, own, w), imax(base, 0)) : first_seen(0, own, w)),
+         MASKED ? imin(in.oe, a.b.lens[seq]) : imin(in.oe, own + 1), [&](int k) -> int64_t {
+             if (MASKED && k >= base && !(a.tree.seen(tok, k - base) & 1)) return -1;
+             return table[imin(k >> a.page_shift, int(a.b.max_pages) - 1)];
+         });
+}
+
+// The results of a wave's rows (not KEYS).  `alone(rows, lg)` takes those again
+// whose sums are not finite.
+template <typename T, int D, int TILE, typename F>
+__device__ inline void emit(const Args& a, Core<T, D, TILE>& core, const Row& r, int lane, int64_t slot, F alone) {
     typedef Core<T, D, TILE> C;
     const float l = C::row_sum(core.l), inv = l == 0.0f ? 0.0f : 1.0f / l;
     const float lg = log_sum(core.m * a.c - lift<T>, l);
@@ -675,13 +688,13 @@ __device__ inline void emit(const Args& a, Core<T, D, TILE>& core, const Keys& i
                                            inv),
                                      l != 0.0f);
     }
-    if (bad) place(), seen_alone<T, D, MASKED>(a, in, r, bad, lg, lane, slot, -1);
+    if (bad) alone(bad, lg);
 }
 
 // The four waves' results for the same 16 rows, joined through LDS.
-template <typename T, int D, bool MASKED, typename F>
-__device__ inline void emit_keys(const Args& a, Core<T, D, WAVES_KEYS>& core, const Keys& in, const Row& r, int lane,
-                                 int wave, int64_t slot, float* smem, F place) {
+template <typename T, int D, typename F>
+__device__ inline void emit_keys(const Args& a, Core<T, D, WAVES_KEYS>& core, const Row& r, int lane, int wave,
+                                 int64_t slot, float* smem, F alone) {
     typedef Core<T, D, WAVES_KEYS> C;
     const float l = C::row_sum(core.l);
     __syncthreads();  // every wave is done with its tiles
@@ -726,7 +739,7 @@ __device__ inline void emit_keys(const Args& a, Core<T, D, WAVES_KEYS>& core, co
 #pragma unroll
         for (int i = 0; i < D / 64; ++i) out.template quad<D>(4 * (wave * 4 + lane / 16 + 16 * i), times(v[i], inv), sum != 0.0f);
     }
-    if (bad) place(), seen_alone<T, D, MASKED>(a, in, r, bad, lg, lane, slot, wave);
+    if (bad) alone(bad, lg);
 }
 
 template <typename T, int D, int TILE, bool MASKED>
@@ -862,11 +875,15 @@ __global__ __launch_bounds__(NW * 64, TILE == WAVES_KEYS && D == 512 ? 1 : D == 
             in.pb = whole ? 0 : split * a.p.chunk_p, in.pe = whole ? P : imin(P, in.pb + a.p.chunk_p);
         if (fused && (whole || split >= a.p.np))
             in.ob = whole ? 0 : (split - a.p.np) * a.p.chunk_o, in.oe = whole ? cap : imin(cap, in.ob + a.p.chunk_o);
+        auto alone = [&](uint64_t rows, float lg) {
+            if (!placed) find();
+            seen_alone<T, D>(a, g, r, rows, lg, lane, split, TILE == WAVES_KEYS ? wave : -1,
+                             [&](int i, auto keys) { seen_keys<MASKED>(a, in, r, i, keys); });
+        };
         if constexpr (TILE == WAVES_KEYS)
-            emit_keys<T, D, MASKED>(a, core, in, r, lane, wave, split, reinterpret_cast<float*>(smem_raw),
-                                    [&] { if (!placed) find(); });
+            emit_keys<T, D>(a, core, r, lane, wave, split, reinterpret_cast<float*>(smem_raw), alone);
         else
-            emit<T, D, TILE, MASKED>(a, core, in, r, lane, split, [&] { if (!placed) find(); });
+            emit<T, D, TILE>(a, core, r, lane, split, alone);
         return;
     }
 
@@ -926,7 +943,10 @@ __global__ __launch_bounds__(NW * 64, TILE == WAVES_KEYS && D == 512 ? 1 : D == 
                first_seen(0, r.own, w), imin(r.own + 1, cap));
     }
     const Keys in{g, 0, 0, split * a.p.chunk_o, imin(cap, (split + 1) * a.p.chunk_o)};
-    emit_keys<T, D, MASKED>(a, core, in, r, lane, wave, a.p.np + split, reinterpret_cast<float*>(smem_raw), [] {});
+    emit_keys<T, D>(a, core, r, lane, wave, a.p.np + split, reinterpret_cast<float*>(smem_raw), [&](uint64_t rows, float lg) {
+        seen_alone<T, D>(a, g, r, rows, lg, lane, a.p.np + split, wave,
+                         [&](int i, auto keys) { seen_keys<MASKED>(a, in, r, i, keys); });
+    });
 }
 
 // out = sum_i w_i O_i / sum_i w_i, w_i = 2^(lg_i - max lg): W waves per
@@ -998,7 +1018,7 @@ int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
 // Work items fill the places that the chip's 256 CUs are counted to have
 // where the keys are long enough to be split.  (The window is no part of it.)
-Plan plan(const PagedKv& kv, const PagedBatch& b, int heads) {
+[[maybe_unused]] Plan plan(const PagedKv& kv, const PagedBatch& b, int heads) {
     Plan p{};
     const int64_t hpg = heads / kv.kv_heads, rows = b.t * hpg, max_len = b.max_pages * kv.page, P = b.prefix_len;
     p.fused = rows >= 32 * b.nseq;
@@ -1063,7 +1083,7 @@ void check_rows(const PagedKv& kv, const SharedAttn& x, const char* who) {
     if (x.window < 0) fail(E_INVALID, w + ": window must not be negative");
 }
 
-int64_t part_bytes(const Plan& p, const PagedKv& kv, const PagedBatch& b, int heads) {
+[[maybe_unused]] int64_t part_bytes(const Plan& p, const PagedKv& kv, const PagedBatch& b, int heads) {
     const int64_t n = p.slots();
     return n <= 1 ? 0 : n * b.t * heads * (kv.head_dim * 4 + 4);
 }

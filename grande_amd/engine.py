@@ -592,6 +592,25 @@ class PagedKv(L.omg_paged_kv):
         L.check(L.lib().omg_dev_attention_tree(self, batch, heads, q_ptr, ldq, out_ptr, ldo, lse, scale, mask_ptr,
                                                mask_ld, window, positions, workspace, workspace_bytes, stream))
 
+    def block_means(self, batch: PagedBatch, means_ptr: int, stream: int | None = None) -> None:
+        """omg_dev_block_means: the mean keys of the pages that the step's new
+        rows are on, into means [npages][kv_heads][head_dim] (f32)."""
+        L.check(L.lib().omg_dev_block_means(self, batch, means_ptr, stream))
+
+    def attention_blocks_workspace(self, batch: PagedBatch, heads: int, blocks: int) -> int:
+        """Bytes of workspace that `attention_blocks` needs for batches of these sizes."""
+        return L.size(L.lib().omg_dev_attention_blocks_workspace(self, batch, heads, blocks))
+
+    def attention_blocks(self, batch: PagedBatch, heads: int, q_ptr: int, ldq: int, out_ptr: int, ldo: int,
+                         scale: float, means_ptr: int, blocks: int, *, lse: int | None = None,
+                         chosen: int | None = None, workspace: int | None = None, workspace_bytes: int = 0,
+                         stream: int | None = None) -> None:
+        """omg_dev_attention_blocks: each token's queries over its own page
+        and the blocks - 1 pages before it (the prefix's first) whose means
+        score highest; their numbers go to chosen [t][kv_heads][blocks]."""
+        L.check(L.lib().omg_dev_attention_blocks(self, batch, heads, q_ptr, ldq, out_ptr, ldo, lse, scale, means_ptr,
+                                                 blocks, chosen, workspace, workspace_bytes, stream))
+
     def attention_weights_workspace(self, batch: PagedBatch, heads: int) -> int:
         """Bytes of workspace that `attention_weights` needs for batches of these sizes."""
         return L.size(L.lib().omg_dev_attention_weights_workspace(self, batch, heads))

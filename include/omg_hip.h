@@ -435,6 +435,29 @@ int omg_dev_attention_tree(const omg_paged_kv *kv, const omg_paged_batch *b, int
                            int window, const int32_t *positions, void *workspace, size_t workspace_bytes,
                            void *stream);
 
+/* Attention over few blocks, a block being a page of the cache.  means
+ * [npages][kv_heads][head_dim] (f32, 16-byte aligned) are the mean keys of the
+ * pages; omg_dev_block_means sets those of the pages that the batch's new rows
+ * are on, over the rows up to lens[s] (64-bit sums, one rounding), and leaves
+ * the others: one call behind each append keeps them, the prefix's by the call
+ * that made it as a sequence of its own.
+ *
+ * A token's blocks are numbered through the prefix's pages, then its sequence's
+ * own ones; score = sum over a KV head's query heads of q . mean (64-bit sums,
+ * rounded to f32).  For each token and KV head the block of the token's own
+ * row and, of those before it, the blocks - 1 of the highest score are chosen
+ * (ties: the first ones; NaN lowest; all, where there are no more), and
+ *   out, lse = omg_dev_attention_shared's over their rows
+ * up to the token's own.  chosen [t][kv_heads][blocks] (int32, may be NULL)
+ * gets the numbers, ascending, -1 behind the last.  A page outside the pool has
+ * the score 0 and no rows.  There is no window.  blocks 1 to 4096; alignments,
+ * strides, sizes, scale, numbers and workspace as there. */
+int omg_dev_block_means(const omg_paged_kv *kv, const omg_paged_batch *b, float *means, void *stream);
+int64_t omg_dev_attention_blocks_workspace(const omg_paged_kv *kv, const omg_paged_batch *b, int heads, int64_t blocks);
+int omg_dev_attention_blocks(const omg_paged_kv *kv, const omg_paged_batch *b, int heads, const void *q, int64_t ldq,
+                             void *out, int64_t ldo, float *lse, float scale, const float *means, int64_t blocks,
+                             int32_t *chosen, void *workspace, size_t workspace_bytes, void *stream);
+
 /* The attention weight that the batch's tokens give each own row of their
  * sequences, added to what it has gathered before:
  *   weights[(s * kv_heads + h) * ldw + i] += sum exp(scale * q . k_i - lse)

@@ -161,3 +161,61 @@ def test_weights_workspace_and_sizes():
         weigh(b=batch(tokens=1 << 24, start_ptr=P))
     with pytest.raises(g.OmgError, match="too many work items"):
         weigh(k=kv(kv_heads=32), b=batch(nseq=1 << 20, tokens=1 << 20), heads=32, ldq=2048)
+
+
+def blocks(k=None, b=None, heads=4, q=P, ldq=256, out=P, ldo=256, scale=0.125, means=P, blocks=4, workspace=P,
+           workspace_bytes=1 << 40, **kw):
+    (k or kv()).attention_blocks(b or batch(), heads, q, ldq, out, ldo, scale, means, blocks, workspace=workspace,
+                                 workspace_bytes=workspace_bytes, **kw)
+
+
+@pytest.mark.parametrize("over,why", BAD_KV)
+def test_blocks_refuse_caches(over, why):
+    with pytest.raises(g.OmgError, match=f"attention_blocks.*{why}"):
+        blocks(k=kv(**over))
+    with pytest.raises(g.OmgError, match=f"block_means.*{why}"):
+        kv(**over).block_means(batch(), P)
+
+
+@pytest.mark.parametrize("over,why", BAD_BATCH)
+def test_blocks_refuse_batches(over, why):
+    with pytest.raises(g.OmgError, match=f"attention_blocks.*{why}"):
+        blocks(b=batch(**over))
+    with pytest.raises(g.OmgError, match=f"block_means.*{why}"):
+        kv().block_means(batch(**over), P)
+
+
+@pytest.mark.parametrize("over,why", ROWS + [
+    (dict(means=None), "means"), (dict(means=P + 8), "means"), (dict(blocks=0), "blocks must"), (dict(blocks=4097), "blocks must"),
+    (dict(workspace_bytes=16), "workspace needs"), (dict(workspace=None), "workspace must"),
+    (dict(workspace=P + 8), "workspace must")])
+def test_blocks_refuse_arguments(over, why):
+    with pytest.raises(g.OmgError, match=f"attention_blocks.*{why}"):
+        blocks(**over)
+
+
+def test_blocks_workspace_and_sizes():
+    assert kv().attention_blocks_workspace(batch(), 4, 2) > 0
+    for heads, n in ((3, 2), (4, 0), (4, 4097)):
+        with pytest.raises(g.OmgError, match="attention_blocks"):
+            kv().attention_blocks_workspace(batch(), heads, n)
+    for means in (None, P + 4):
+        with pytest.raises(g.OmgError, match="block_means: means"):
+            kv().block_means(batch(), means)
+    with pytest.raises(g.OmgError, match="too many rows"):
+        kv(kv_heads=64).block_means(batch(nseq=1 << 20, tokens=1 << 20), P)
+    with pytest.raises(g.OmgError, match="t \\* heads"):
+        blocks(b=batch(tokens=1 << 24, start_ptr=P))
+    with pytest.raises(g.OmgError, match="too many work items"):
+        blocks(k=kv(kv_heads=32), b=batch(nseq=1 << 20, tokens=1 << 20), heads=32, ldq=2048, ldo=2048, workspace_bytes=1 << 60)
+
+
+def test_blocks_and_weights_refuse_null_descriptions():
+    import grande_amd._lib as L
+
+    for args in ((None, batch()), (kv(), None)):
+        for call in (lambda: L.lib().omg_dev_block_means(*args, P, None),
+                     lambda: L.lib().omg_dev_attention_blocks(*args, 4, P, 256, P, 256, None, 0.125, P, 4, None, P, 1 << 40, None),
+                     lambda: L.lib().omg_dev_attention_weights(*args, 4, P, 256, P, 0.125, 0, P, 64, P, 1 << 40, None)):
+            with pytest.raises(g.OmgError, match="null"):
+                L.check(call())
