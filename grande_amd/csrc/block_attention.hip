@@ -164,11 +164,14 @@ __global__ __launch_bounds__(256) void block_scores_kernel(BlockArgs x) {
             double sum[8] = {};
             if (t0 + tok >= 0 && t0 + tok < t1) {
                 const T* q = static_cast<const T*>(a.x.q) + (t0 + tok) * a.x.ldq + int64_t(g) * a.hpg * D + quarter * Q + c + d;
-                for (int h = 0; h < a.hpg; ++h) {
-                    float v[8];
-                    load8(q + int64_t(h) * D, v);
+                for (int h0 = 0; h0 < a.hpg; h0 += 4) {
+                    float v[4][8];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) sum[e] += double(v[e]);
+                    for (int h = 0; h < 4; ++h) load8(q + int64_t(h0 + h < a.hpg ? h0 + h : h0) * D, v[h]);
+#pragma unroll
+                    for (int h = 0; h < 4; ++h)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) sum[e] += h0 + h < a.hpg ? double(v[h][e]) : 0.0;
                 }
             }
 #pragma unroll
@@ -234,9 +237,11 @@ __global__ __launch_bounds__(CHOOSE_T) void block_choose_kernel(BlockArgs x) {
 // --------------------------------------------------------------- attention
 
 // 16 query rows of a token and KV head over up to 64 entries of its list: each
-// wave every fourth 16-key tile.  All rows see the same keys.
+// wave every fourth 16-key tile.  All rows see the same keys.  (512 lists of 64 x
+// 64 rows, 128-wide: 82 us, 1.1 GB through L2 and 270 MB from HBM; a second tile
+// a wave under way 85.)
 template <typename T, int D>
-__global__ __launch_bounds__(NW * 64, D == 512 ? 1 : D == 128 ? 3 : 2) void attention_blocks_kernel(BlockArgs x) {
+__global__ __launch_bounds__(NW * 64, D == 512 ? 1 : D == 64 ? 4 : 2) void attention_blocks_kernel(BlockArgs x) {
     typedef Core<T, D, WAVES_KEYS> C;
     extern __shared__ __attribute__((aligned(1024))) unsigned char smem_raw[];
     const Args& a = x.a;
@@ -304,14 +309,16 @@ void check_blocks(const PagedKv& kv, const PagedBatch& b, int heads, int64_t kee
     if (keep <= 0 || keep > 4096) fail(E_INVALID, "attention_blocks: blocks must be 1 to 4096");
 }
 
-// Entries are split over work items until these fill the chip's places (three
-// workgroups a CU at most), at least two at a time and at most a lane each.
+// Entries are split over work items until these fill the chip's places (by
+// LDS), at least two at a time and at most a lane each.  (Lists of one token
+// each that start together stay together, and what one reads the next finds in
+// L2: 512 lists as 1,024 items 116 us, as 512 82.)
 BlockPlan plan_blocks(const PagedKv& kv, const PagedBatch& b, int heads, int64_t keep) {
     BlockPlan p{};
     p.np = (b.prefix_len + kv.page - 1) / kv.page;
     p.blocks = p.np + b.max_pages;
     const int64_t hpg = heads / kv.kv_heads, items = b.t * kv.kv_heads * ((hpg + 15) / 16);
-    const int64_t places = 256 * (kv.head_dim == 512 ? 1 : kv.head_dim == 256 ? 2 : 3);
+    const int64_t places = 256 * (kv.head_dim == 64 ? 4 : kv.head_dim == 512 ? 1 : 2);
     const int64_t least = (keep + 63) / 64, most = std::min<int64_t>(64, (keep + 1) / 2);
     const int64_t want = std::max(least, std::min(most, places / items));
     p.chunk = int((keep + want - 1) / want);
