@@ -178,24 +178,32 @@ __global__ __launch_bounds__(256) void block_scores_kernel(BlockArgs x) {
             for (int e = 0; e < 8; ++e) qs[(d + e) * WAVE + quarter * 16 + tok] = sum[e];
         }
         __syncthreads();
-#pragma unroll 4
-        for (int d = 0; d < DC; d += 4) {
-            float4 m = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (there) m = *reinterpret_cast<const float4*>(mean + c + d);
-            const double* q = qs + d * WAVE + lane;
-            acc = __builtin_amdgcn_mfma_f64_16x16x4f64(double(m.x), q[0], acc, 0, 0, 0);
-            acc = __builtin_amdgcn_mfma_f64_16x16x4f64(double(m.y), q[WAVE], acc, 0, 0, 0);
-            acc = __builtin_amdgcn_mfma_f64_16x16x4f64(double(m.z), q[2 * WAVE], acc, 0, 0, 0);
-            acc = __builtin_amdgcn_mfma_f64_16x16x4f64(double(m.w), q[3 * WAVE], acc, 0, 0, 0);
+        // (a page that is not there: the first page's means, and no score from them)
+#pragma unroll 1
+        for (int d0 = 0; d0 < DC; d0 += 32) {
+            constexpr int N = DC < 32 ? DC : 32;
+            float4 m[N / 4];
+#pragma unroll
+            for (int d = 0; d < N; d += 4) m[d / 4] = *reinterpret_cast<const float4*>(mean + c + d0 + d);
+#pragma unroll
+            for (int d = 0; d < N; d += 4) {
+                const double* q = qs + (d0 + d) * WAVE + lane;
+                acc = __builtin_amdgcn_mfma_f64_16x16x4f64(double(m[d / 4].x), q[0], acc, 0, 0, 0);
+                acc = __builtin_amdgcn_mfma_f64_16x16x4f64(double(m[d / 4].y), q[WAVE], acc, 0, 0, 0);
+                acc = __builtin_amdgcn_mfma_f64_16x16x4f64(double(m[d / 4].z), q[2 * WAVE], acc, 0, 0, 0);
+                acc = __builtin_amdgcn_mfma_f64_16x16x4f64(double(m[d / 4].w), q[3 * WAVE], acc, 0, 0, 0);
+            }
         }
     }
     // The lane has blocks 4 r + lane / 16 of the wave's, token lane % 16.
+    const uint64_t gone = __ballot(!there) & 0xffff;
     const int64_t tok = t0 + lane % 16;
     if (tok < 0 || tok >= t1) return;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
         const int64_t b = b0 + wave * 16 + 4 * r + lane / 16;
-        if (b < nblocks) x.scores[(tok * G + g) * x.blocks_ld + first + b] = float(acc[r]);
+        if (b < nblocks)
+            x.scores[(tok * G + g) * x.blocks_ld + first + b] = gone >> (4 * r + lane / 16) & 1 ? 0.0f : float(acc[r]);
     }
 }
 

@@ -471,7 +471,7 @@ void launch_d(hipStream_t s, Args a) {
     if (few(a.kv, a.b, a.x.heads)) {
         // Chunks of 256 keys and more: 64 workgroups a CU are enough.  (512 lists of
         // 8,192 rows: 32 / 16 / 8 of them 170 / 174 / 185 us.)
-        a.chunk = 256;
+        a.chunk = 4 * (D >= 128 ? 16 : 32);
         while (a.chunk < 4096 && lists * (a.max_len / a.chunk) > 16384) a.chunk *= 2;
         a.blocks = (a.max_len + a.chunk - 1) / a.chunk;
         if (lists * a.blocks >= MAX_BLOCKS) fail(E_CAPACITY, "attention_weights: too many work items");

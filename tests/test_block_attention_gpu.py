@@ -62,8 +62,6 @@ class BlockCall(Call):
         bad = (ids < 0) | (ids >= self.pool.npages)
         q = self.q[at].double().cpu()[:self.heads * self.hd].view(self.kv_heads, G, self.hd)[h].sum(0)
         score = np.where(bad[:last], 0.0, (means[np.where(bad, 0, ids)[:last], h] @ q).numpy()).astype(np.float32)
-        if bad[:last].any() and bool(torch.isnan(q).any()):
-            score[bad[:last]] = np.nan
         key = np.where(np.isnan(score), -np.inf, score)
         take = np.lexsort((np.arange(last), np.isnan(score), -key))[:self.blocks - 1]
         return np.append(np.sort(take), last), ids
