@@ -11,9 +11,22 @@
 // fix.  A weight is read and written by one lane of one wave.
 //
 // Few rows a sequence (steps of decoding): weights_few_kernel, 16 keys x 16
-// rows, bound by reading K.  Many (prompts): weights_many_kernel, a wave 32 or
-// 64 keys, query tiles of 32 rows in LDS for its four waves; where keys are few
-// the queries are split and the parts' sums added by weights_join_kernel.
+// rows, bound by reading K.  Many (prompts): weights_many_kernel, a wave 64 keys
+// (512-wide heads: 32), query tiles of 32 rows in LDS for its four waves; where
+// keys are few the queries are split and the parts' sums added by
+// weights_join_kernel.
+//
+// Measured, and what bounds it:
+//   64 sequences of 6,100 rows x 8 KV heads of 128 (bf16), one token each: 170 us,
+//     4.9 TB/s: the keys' bytes.
+//   12 sequences of 2,000 rows x 1 KV head of 256 (f16): 5.8 us: latency.
+//   a prompt of 8,000 tokens x 8 heads of 256 on 4 KV heads (f16): 165 us, 795
+//     TFLOP/s of the 1,190 that a product of 8,192^3 reaches: the products (at
+//     this operand data the chip lowers its clock; the same MFMAs with nothing
+//     else take 130 us), and 15 % of the places idle, since prompts' last keys
+//     have few queries.  16 x 16 x 32 products draw less than 32 x 32 x 16 (from
+//     registers alone 2,050 and 1,700 TFLOP/s on random data): 174 -> 165 us, at
+//     128-wide heads 160 -> 132.
 #include <algorithm>
 #include <atomic>
 #include <climits>
@@ -29,12 +42,6 @@ namespace {
 
 typedef __attribute__((address_space(3))) void* lds_ptr;
 
-__device__ inline floatx16 mfma32(half8 a, half8 b, floatx16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
-}
-__device__ inline floatx16 mfma32(bf16x8 a, bf16x8 b, floatx16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
-}
 __device__ inline floatx4 mfma16(half8 a, half8 b, floatx4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
@@ -176,8 +183,8 @@ __global__ __launch_bounds__(256) void weights_few_kernel(Args a) {
 // Many rows.
 template <typename T, int D>
 struct Many {
-    static constexpr int NB = D >= 512 ? 1 : 2;  // 32-key blocks of a wave
-    static constexpr int KEYS = 4 * 32 * NB;     // of a workgroup
+    static constexpr int NB = D >= 512 ? 2 : 4;  // 16-key blocks of a wave
+    static constexpr int KEYS = 4 * 16 * NB;     // of a workgroup
     static constexpr int CH = D / 8, RPI = 512 / D > 0 ? 512 / D : 1;
     static constexpr int INS = 32 * D * 2 / 1024 / 4;  // 1 KiB pieces of a query tile per wave
     static constexpr int TILE = 32 * D;
@@ -213,7 +220,7 @@ template <typename T, int D>
 __global__ __launch_bounds__(256, 2) void weights_many_kernel(Args a) {
     typedef typename Vec8<T>::type frag;
     typedef Many<T, D> M;
-    constexpr int NB = M::NB, NS = D / 16;
+    constexpr int NB = M::NB, NS = D / 32, E = 4 * NB;  // blocks; steps of a product; scores of a lane
     extern __shared__ __attribute__((aligned(1024))) unsigned char smem_raw[];
     T* smem = reinterpret_cast<T*>(smem_raw);  // BUFS query tiles
     float* log_sums = reinterpret_cast<float*>(smem_raw + M::BUFS * M::TILE * 2);  // [BUFS][4][64]
@@ -230,7 +237,7 @@ __global__ __launch_bounds__(256, 2) void weights_many_kernel(Args a) {
     const Seq q = sequence(a, s);
     const int kb = block * M::KEYS;
     if (kb >= q.len) return;
-    const int k0 = kb + wave * 32 * NB, w = a.x.window;
+    const int k0 = kb + wave * 16 * NB, w = a.x.window;
     // The split's tokens, those of them that see a key of the block.
     const int per = (q.n + a.splits - 1) / a.splits;
     int ta = split * per, tb = ta + per < q.n ? ta + per : q.n;
@@ -242,22 +249,20 @@ __global__ __launch_bounds__(256, 2) void weights_many_kernel(Args a) {
         const int64_t end = int64_t(kb) + M::KEYS - 1 + w - q.base;  // own < key + w
         if (tb > end) tb = int(end < 0 ? 0 : end);
     }
-    float sum[NB][16];
+    float sum[E];  // of key 16 (e / 4) + 4 (lane / 16) + e % 4 of the wave's
 #pragma unroll
-    for (int j = 0; j < NB; ++j)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) sum[j][r] = 0.0f;
+    for (int e = 0; e < E; ++e) sum[e] = 0.0f;
     const int32_t* table = a.b.table + s * a.b.table_ld;
     if (ta < tb) {
         frag kf[NB][NS];
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
-            const int row = k0 + 32 * j + lane % 32;
+            const int row = k0 + 16 * j + lane % 16;
             const T* p = row < q.len ? key_row<T>(a, table, row, g, D) : nullptr;
             frag z{};
 #pragma unroll
             for (int st = 0; st < NS; ++st)
-                kf[j][st] = p ? *reinterpret_cast<const frag*>(p + 16 * st + 8 * (lane / 32)) : z;
+                kf[j][st] = p ? *reinterpret_cast<const frag*>(p + 32 * st + 8 * (lane / 16)) : z;
         }
         // A query tile: the heads of TPT tokens, or 32 heads of one, so that a
         // lane's row is the same token and head past the tile's first in each.
@@ -271,7 +276,7 @@ __global__ __launch_bounds__(256, 2) void weights_many_kernel(Args a) {
             const int r = (wave * M::INS + i) * M::RPI + lane / M::CH, t = r / heads;
             off[i] = (t < TPT ? uint32_t(t * a.x.ldq + (r - t * heads) * D) * 2 : 1u << 31) + ((lane % M::CH) ^ M::swz(r)) * 16;
         }
-        const int mt = lane % 32 / heads, mh = lane % 32 - mt * heads;  // the lane's query row
+        const int mt = lane % 32 / heads, mh = lane % 32 - mt * heads;  // of the row whose log sum it loads
         int t0 = 0, part = 0;                                           // of the next tile
         const float* lse = a.x.lse + tok0 * a.x.heads + g * hpg;
         const uint32_t lse_off = uint32_t(mt * a.x.heads + mh) * 4;
@@ -292,23 +297,31 @@ __global__ __launch_bounds__(256, 2) void weights_many_kernel(Args a) {
         constexpr int AHEAD = M::BUFS - 1;
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) issue(smem + i * M::TILE);
-        const bool pad = mt >= TPT;
-        const uint32_t my_row = uint32_t(lane % 32 * D * 2 + ((lane / 32) ^ M::swz(lane % 32)) * 16);
+        // The lane's query rows are lane % 16 of the tile's two halves.
+        const int ht[2] = {lane % 16 / heads, (16 + lane % 16) / heads};
+        const int hh[2] = {lane % 16 - ht[0] * heads, 16 + lane % 16 - ht[1] * heads};
+        const uint32_t my_row = uint32_t(lane % 16 * D * 2 + ((lane / 16) ^ M::swz(lane % 16)) * 16);
         typedef __attribute__((address_space(3))) frag* operand;
         int at = 0, tok = 0, hp = 0;  // of the tile at hand: its buffer, first token and part
-        // The next tile has landed: its LDS address for the lane's row, and the
-        // row's negated log sum.
-        auto arrive = [&](float& nl) {
+        // The next tile has landed: the LDS address of the lane's first row, and
+        // the rows' negated log sums.
+        auto arrive = [&](float* nl) {
             wait_loads<(AHEAD - 1) * (M::INS + 1)>();
             __syncthreads();
             issue(smem + (at + AHEAD) % M::BUFS * M::TILE);
-            const bool ok = tok + mt < have && !pad && hp * 32 + mh < hpg;
-            const float lse = log_sums[(at * 4 + wave) * WAVE + lane];
-            nl = ok ? negated(lse) : -INFINITY;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float lse = log_sums[(at * 4 + wave) * WAVE + 16 * h + lane % 16];
+                nl[h] = tok + ht[h] < have && ht[h] < TPT && hp * 32 + hh[h] < hpg ? negated(lse) : -INFINITY;
+            }
             uint32_t row = uint32_t(uintptr_t((lds_ptr)(smem + at * M::TILE))) + my_row;
             asm volatile("" : "+v"(row));  // (or all steps' addresses are kept in registers)
             at = (at + 1) % M::BUFS;
             return row;
+        };
+        // The operand of step n of a tile: of rows 16 (n / NS), dims 32 (n % NS).
+        auto read = [&](uint32_t row, int n) {
+            return *(operand)(uintptr_t)((row ^ uint32_t(64 * (n % NS))) + uint32_t(n / NS * 16 * D * 2));
         };
         auto next = [&] {
             if (++hp == parts) hp = 0, tok += TPT;
@@ -328,86 +341,89 @@ __global__ __launch_bounds__(256, 2) void weights_many_kernel(Args a) {
                 const int end = i < f0 ? f0 : ntile;
 #pragma unroll 1
                 for (; i < end; ++i, next()) {
-                    float nl;
+                    float nl[2];
                     const uint32_t row = arrive(nl);
-                    // (the lane's keys past k0 + 4 (lane / 32): constants of an element)
-                    const int last = q.base + ta + tok + mt - k0 - 4 * (lane / 32);
-                    const int from = w == 0 ? INT_MIN : __builtin_elementwise_sub_sat(last, w);
 #pragma unroll
-                    for (int j = 0; j < NB; ++j) {
-                        floatx16 sc;
+                    for (int h = 0; h < 2; ++h) {
+                        floatx4 sc[NB];
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) sc[r] = 0.0f;
+                        for (int j = 0; j < NB; ++j) sc[j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                        for (int st = 0; st < NS; ++st) sc = mfma32(kf[j][st], *(operand)(uintptr_t)(row ^ uint32_t(32 * st)), sc);
+                        for (int st = 0; st < NS; ++st) {
+                            const frag qf = read(row, h * NS + st);
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            const int key = 32 * j + 8 * (r / 4) + r % 4;
-                            const float p = prob(sc[r], a.x.scale, nl);
-                            sum[j][r] += key <= last && key > from && nl != -INFINITY ? p : 0.0f;
+                            for (int j = 0; j < NB; ++j) sc[j] = mfma16(kf[j][st], qf, sc[j]);
+                        }
+                        // (the lane's keys past k0 + 4 (lane / 16): constants of an element)
+                        const int last = q.base + ta + tok + ht[h] - k0 - 4 * (lane / 16);
+                        const int from = w == 0 ? INT_MIN : __builtin_elementwise_sub_sat(last, w);
+#pragma unroll
+                        for (int e = 0; e < E; ++e) {
+                            const int key = 16 * (e / 4) + e % 4;
+                            const float p = prob(sc[e / 4][e % 4], a.x.scale, nl[h]);
+                            sum[e] += key <= last && key > from && nl[h] != -INFINITY ? p : 0.0f;
                         }
                         __builtin_amdgcn_sched_barrier(0);
                     }
                 }
                 continue;
             }
-            // The scores of a block wait for the next block's MFMAs, in whose shadow
-            // their exponentials run (one after the other they took 132,000 and
-            // 154,000 of a SIMD's 351,000 cycles).  A step: an MFMA, the operand of
-            // the one READ steps on and a part of the block before, in this order.
-            // (Left alone, the compiler reads one operand and waits for it.)
-            // (from the third step on: the block's last MFMA is still under way)
-            auto first = [](int st) { return st < 2 ? 0 : (st - 2) * 16 / (NS - 2); };
-            floatx16 was;
+            // The scores of half a tile wait for the next half's MFMAs, in whose
+            // shadow their exponentials run.  A step: the MFMAs of one operand, the
+            // operand of the step READ on and a part of the half before, in this
+            // order.  (Left alone, the compiler reads one operand and waits for it.)
+            // From the third step on: the last half's MFMAs are still under way.
+            constexpr int LATE = NS > 2 ? 2 : 1, READ = 4;
+            auto first = [](int st) { return st < LATE ? 0 : (st - LATE) * E / (NS - LATE); };
+            floatx4 was[NB];
             float was_nl = -INFINITY;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) was[r] = 0.0f;
+            for (int j = 0; j < NB; ++j) was[j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 1
             for (; i < f1; ++i, next()) {
-                float nl;
+                float nl[2];
                 const uint32_t row = arrive(nl);
-                constexpr int READ = 3;
                 frag qf[READ];
 #pragma unroll
-                for (int k = 0; k < READ; ++k) qf[k] = *(operand)(uintptr_t)(row ^ uint32_t(32 * k));
+                for (int k = 0; k < READ; ++k) qf[k] = read(row, k);
 #pragma unroll
-                for (int j = 0; j < NB; ++j) {
-                    floatx16 sc;
+                for (int h = 0; h < 2; ++h) {
+                    floatx4 sc[NB];
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) sc[r] = 0.0f;
+                    for (int j = 0; j < NB; ++j) sc[j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                     for (int st = 0; st < NS; ++st) {
-                        const int n = j * NS + st;
-                        sc = mfma32(kf[j][st], qf[n % READ], sc);
-                        if (n + READ < NB * NS) qf[n % READ] = *(operand)(uintptr_t)(row ^ uint32_t(32 * ((n + READ) % NS)));
+                        const int n = h * NS + st;
 #pragma unroll
-                        for (int r = first(st); r < first(st + 1); ++r) sum[(j + NB - 1) % NB][r] += prob(was[r], a.x.scale, was_nl);
+                        for (int j = 0; j < NB; ++j) sc[j] = mfma16(kf[j][st], qf[n % READ], sc[j]);
+                        if (n + READ < 2 * NS) qf[n % READ] = read(row, n + READ);
+#pragma unroll
+                        for (int e = first(st); e < first(st + 1); ++e) sum[e] += prob(was[e / 4][e % 4], a.x.scale, was_nl);
                         __builtin_amdgcn_sched_barrier(0);
                     }
-                    was = sc, was_nl = nl;
+#pragma unroll
+                    for (int j = 0; j < NB; ++j) was[j] = sc[j];
+                    was_nl = nl[h];
                 }
             }
 #pragma unroll
-            for (int r = 0; r < 16; ++r) sum[NB - 1][r] += prob(was[r], a.x.scale, was_nl);
+            for (int e = 0; e < E; ++e) sum[e] += prob(was[e / 4][e % 4], a.x.scale, was_nl);
         }
         wait_loads<0>();  // (no load may find the LDS another workgroup's)
     }
+    // Lane 16 g + e has the sum of element e of the group.
+    float mine = 0.0f;
 #pragma unroll
-    for (int j = 0; j < NB; ++j) {
-        float mine = 0.0f;  // lane 16 a + r % 16 of a half: element r
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            float v = sum16(sum[j][r]);
-            v += __shfl_xor(v, 16, WAVE);
-            mine = lane % 16 == r ? v : mine;
-        }
-        const int r = lane % 16, key = k0 + 32 * j + 8 * (r / 4) + 4 * (lane / 32) + r % 4;
-        if (lane % 32 >= 16 || key >= q.len || !key_row<T>(a, table, key, g, D)) continue;
-        if (a.part)
-            a.part[(split * a.b.nseq * G + list) * a.max_len + key] = mine;
-        else
-            a.x.weights[list * a.x.ldw + key] += mine;
+    for (int e = 0; e < E; ++e) {
+        const float v = sum16(sum[e]);
+        mine = lane % 16 == e ? v : mine;
     }
+    const int e = lane % 16, key = k0 + 16 * (e / 4) + 4 * (lane / 16) + e % 4;
+    if (e >= E || key >= q.len || !key_row<T>(a, table, key, g, D)) return;
+    if (a.part)
+        a.part[(split * a.b.nseq * G + list) * a.max_len + key] = mine;
+    else
+        a.x.weights[list * a.x.ldw + key] += mine;
 }
 
 // The splits' sums, in their order.
@@ -439,13 +455,13 @@ int many_keys(int head_dim) { return head_dim == 512 ? 128 : 256; }
 // that the chip has take the items with something to do (keys near a prompt's
 // end have few queries) and an item's tiles, three more for its start and end,
 // for sequences of the mean number of tokens.  (8,000 tokens x 8 heads of 256 on
-// 4 KV heads: 4 / 7 / 14 / 32 splits 244 / 172 / 216 / 220 us; 7 is what this
-// gives.)
+// 4 KV heads: 4 / 7 / 14 / 32 splits 244 / 172 / 216 / 220 us when it was 172; 7
+// is what this gives.)
 int splits(const PagedKv& kv, const PagedBatch& b, int heads) {
     if (few(kv, b, heads)) return 1;
     const int64_t max_len = b.max_pages * kv.page, keys = many_keys(kv.head_dim), blocks = (max_len + keys - 1) / keys;
     const int64_t n = (b.t + b.nseq - 1) / b.nseq, tiles = (n * (heads / kv.kv_heads) + 31) / 32;
-    const int64_t base = max_len - n, places = kv.head_dim == 64 ? 768 : 512;
+    const int64_t base = max_len - n, places = kv.head_dim == 64 ? 1024 : kv.head_dim == 128 ? 768 : 512;
     const double tile_us = 0.4 + kv.head_dim * 0.0057;
     int best = 1;
     double best_us = 1e30;
