@@ -16,6 +16,9 @@
 // decoding) the own keys have work items of their own, in the same launch.
 // Few tiles split the keys over work items; attention_join joins these.
 //
+// MASKED (tree_attention.hip): of its sequence's new rows a token sees those
+// that its mask has bits for; the lengths' order says nothing about these.
+//
 // Tiles (MFMA shape = rows of a wave x keys):
 //   WAVES_32:   4 waves x 32 rows, 32-key K and V tiles shared in LDS, two
 //               buffers, the next tile's loads in flight (four buffers, and
