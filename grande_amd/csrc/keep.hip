@@ -70,8 +70,8 @@ __global__ __launch_bounds__(256) void keep_apart_kernel(KeepArgs a) {
     }
 }
 
-// In place: entry j of an ascending list has rows[j] >= first + j, so the place
-// that an entry writes is read by entries up to its own alone.  One wave takes
+// In place: an entry that moves has rows[j] >= first + j, so the place that an
+// entry writes is read by entries up to its own alone.  One wave takes
 // a list's K or V (or a slice of SB bytes of each row) from the first entry on,
 // in steps of U pieces, and a wave's loads return in order: an entry has its
 // row, and all entries before it theirs, when its place is written.  Loads run
@@ -264,7 +264,7 @@ void launch_kv_evict(hipStream_t s, const PagedKv& kv, const PagedBatch& b, cons
     if (x.kept == x.weights && x.kept_ld != x.ldw) fail(E_INVALID, "kv_evict: kept_ld must be ldw in place");
     if (x.to_table && (x.to_ld <= 0 || x.to_ld > 0x3fffffff / kv.page))
         fail(E_INVALID, "kv_evict: to_ld out of range");
-    if (b.nseq * kv.kv_heads >= MAX_BLOCKS) fail(E_CAPACITY, "kv_evict: too many lists for one call");
+    if (b.nseq * kv.kv_heads >= MAX_BLOCKS / (EVICT_T / 256)) fail(E_CAPACITY, "kv_evict: too many lists for one call");
     EvictArgs a{b, x, kv.kv_heads, max_len};
     const dim3 grid(unsigned(b.nseq * kv.kv_heads));
     if (max_len <= CHOOSE_R * EVICT_T)

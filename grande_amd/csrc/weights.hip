@@ -497,7 +497,7 @@ void launch_d(hipStream_t s, Args a) {
     }
     a.blocks = (a.max_len + Many<T, D>::KEYS - 1) / Many<T, D>::KEYS;
     const int64_t n = lists * a.blocks * a.splits;
-    if (n >= MAX_BLOCKS || lists > 65535) fail(E_CAPACITY, "attention_weights: too many work items");
+    if (n >= MAX_BLOCKS || (a.splits > 1 && lists > 65535)) fail(E_CAPACITY, "attention_weights: too many work items");
     constexpr unsigned lds = Many<T, D>::BUFS * (Many<T, D>::TILE * 2 + 4 * WAVE * 4);
     static std::atomic<uint64_t> lds_set{0};  // the devices, once per instantiation
     int device = 0;

@@ -479,9 +479,9 @@ int omg_dev_attention_weights(const omg_paged_kv *kv, const omg_paged_batch *b, 
  * list per sequence and KV head, list s * kv_heads + h.  So an accepted path of
  * drafted tokens closes up (first: the rows before the draft), or what an
  * eviction leaves moves down.
- *   to_table NULL: in place.  A list's rows ascend, and none stands before its
- * new place (rows[j] >= first[s] + j; one that does is left out).  Pages with
- * rows that move belong to one sequence.
+ *   to_table NULL: in place.  No row stands before its new place (rows[j] >=
+ * first[s] + j, as in every list that ascends; one that does is left out).
+ * Pages with rows that move belong to one sequence.
  *   to_table [nseq][to_ld]: the pages of the new rows, none of which any
  * sequence's list is read from; rows in any order, also twice.
  * Entries below zero or past the table, and rows on pages outside the pool,
@@ -491,7 +491,8 @@ int omg_dev_kv_keep(const omg_paged_kv *kv, const omg_paged_batch *b, const int3
                     int64_t count, const int32_t *first, int per_head, const int32_t *to_table, int64_t to_ld,
                     void *stream);
 
-/* Eviction by weight: of the n = lens[s] own rows of each sequence and KV head
+/* Eviction by weight: of the n = lens[s] own rows (as far as the table reaches)
+ * of each sequence and KV head
  * `keep` stay (all, where n is no more), the `recent` last ones and of the
  * others those of the largest weights[(s * kv_heads + h) * ldw + i] (ties: the
  * first rows; NaN lowest), in their order.  rows [nseq][kv_heads][keep]

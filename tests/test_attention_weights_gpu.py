@@ -264,6 +264,30 @@ def test_pool_past_32_bit_offsets():
         del big
 
 
+def test_more_lists_than_a_grids_second_dimension():
+    """8,300 sequences of 33 tokens x 8 heads: each list's weights add up to its tokens."""
+    nseq, n, heads, hd, page = 8300, 33, 8, 64, 16
+    pages = -(-n // page)
+    k, v = (torch.randn(nseq * pages, heads, page, hd, device="cuda").half() for _ in range(2))
+    kv = g.PagedKv(k.data_ptr(), v.data_ptr(), nseq * pages, heads, page, hd, g.ELEM_F16)
+    table = torch.arange(nseq * pages, dtype=torch.int32, device="cuda")
+    lens = torch.full((nseq,), n, dtype=torch.int32, device="cuda")
+    start = torch.arange(nseq + 1, dtype=torch.int32, device="cuda") * n
+    b = g.PagedBatch(nseq, nseq * n, lens.data_ptr(), table.data_ptr(), pages, start.data_ptr())
+    q = torch.randn(nseq * n, heads * hd, device="cuda").half()
+    out, lse = torch.empty_like(q), torch.empty(nseq * n, heads, device="cuda")
+    ws = torch.empty(max(16, kv.attention_workspace(b, heads)), dtype=torch.uint8, device="cuda")
+    kv.attention(b, heads, q.data_ptr(), heads * hd, out.data_ptr(), heads * hd, hd ** -0.5, lse=lse.data_ptr(),
+                 workspace=ws.data_ptr(), workspace_bytes=ws.numel())
+    w = torch.zeros(nseq, heads, pages * page, device="cuda")
+    assert kv.attention_weights_workspace(b, heads) == 0
+    kv.attention_weights(b, heads, q.data_ptr(), heads * hd, lse.data_ptr(), hd ** -0.5, w.data_ptr(), pages * page)
+    torch.cuda.synchronize()
+    assert bool((w[:, :, n:] == 0).all())
+    # (log sums off by 1e-6 + 2^-19 of scores' sums below 64, 33 additions)
+    assert bool(((w.double().sum(-1) - n).abs() <= n * (2e-4 + 33 * 2.0 ** -22)).all())
+
+
 def test_weights_of_attentions_own_log_sums_add_up_to_the_tokens():
     """Without a prefix each token gives its rows a weight of one in all, for each of its heads."""
     rng = np.random.default_rng(21)

@@ -110,6 +110,21 @@ def test_in_place_rows_run_over_their_own_lists():
             c.check(exp, f"{len(lists)} rows")
 
 
+@pytest.mark.parametrize("nseq,kv_heads,hd", [(1, 1, 256), (3, 2, 128), (300, 2, 64)])
+def test_in_place_in_any_order(nseq, kv_heads, hd):
+    """Lists that do not ascend, rows twice among them, none before its place."""
+    rng = np.random.default_rng(4 + hd)
+    n = 1200 if nseq < 10 else 150
+    c = Rows(rng, [n] * nseq, kv_heads, hd, page=32)
+    first = rng.integers(0, 20, nseq)
+    count = n - 25
+    lists = np.stack([[[int(rng.integers(first[s] + j, n)) for j in range(count)] for _ in range(kv_heads)] for s in range(nseq)])
+    exp = c.expect(lists, first)
+    rows, f = i32(lists.reshape(-1, count)), i32(first)
+    c.kv.keep(c.batch, rows.data_ptr(), count, count, per_head=True, first=f.data_ptr())
+    c.check(exp)
+
+
 def test_to_other_pages_in_any_order_and_twice():
     rng = np.random.default_rng(5)
     c = Rows(rng, [50, 70], 2, 128, to=4)
