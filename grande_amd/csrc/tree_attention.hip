@@ -23,6 +23,7 @@ Plan plan_tree(const PagedKv& kv, const PagedBatch& b, int heads) {
     const int D = kv.head_dim;
     const double slot_us = double(b.t) * heads * D * 8 / 4.5e6;
     auto chunk = [](int64_t keys, int64_t n) { return up((keys + n - 1) / n, 32); };
+    static constexpr int splits[] = {1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 14, 16, 20, 24, 32, 48, 64};
     Plan best = from;
     double best_us = 1e30;
     for (const int tile : {int(WAVES_16), int(WAVES_32)}) {
@@ -44,7 +45,8 @@ Plan plan_tree(const PagedKv& kv, const PagedBatch& b, int heads) {
         };
         if (!q.fused) {  // (the own keys' items as they are)
             if (P == 0) take(q, 0);
-            for (int n = 1; n <= 64 && P > 0; ++n) {
+            for (const int n : splits) {
+                if (P == 0) break;
                 q.chunk_p = int(chunk(P, n)), q.np = int((P + q.chunk_p - 1) / q.chunk_p);
                 take(q, tiles(q.chunk_p));
             }
@@ -55,9 +57,10 @@ Plan plan_tree(const PagedKv& kv, const PagedBatch& b, int heads) {
         q.whole = true, q.np = 0, q.chunk_p = 0, q.os = 1, q.chunk_o = int(std::min<int64_t>(up(max_len, 32), INT_MAX / 2));
         take(q, tiles(P) + held * tiles(max_len));
         q.whole = false;
-        for (int n = 1; n <= (P > 0 ? 64 : 1); ++n) {
+        for (const int n : splits) {
+            if (P == 0 && n > 1) break;
             if (P > 0) q.chunk_p = int(chunk(P, n)), q.np = int((P + q.chunk_p - 1) / q.chunk_p);
-            for (int os = 1; os <= 64; os *= 2) {
+            for (int os = 1; os <= 64; os *= 4) {
                 q.chunk_o = int(std::min<int64_t>(chunk(max_len, os), INT_MAX / 2));
                 q.os = int((max_len + q.chunk_o - 1) / q.chunk_o);
                 take(q, std::max(P > 0 ? tiles(q.chunk_p) : 0.0, held * tiles(std::min<int64_t>(q.chunk_o, max_len))));

@@ -465,7 +465,8 @@ int splits(const PagedKv& kv, const PagedBatch& b, int heads) {
     const double tile_us = 0.4 + kv.head_dim * 0.0057;
     int best = 1;
     double best_us = 1e30;
-    for (int k = 1; k <= 32 && (k == 1 || tiles >= 8 * k); ++k) {
+    for (const int k : {1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 14, 16, 20, 24, 32}) {
+        if (k > 1 && tiles < 8 * k) break;
         // Split c has tokens up to (c + 1) n / k, which see blocks up to theirs.
         int64_t items = 0;
         for (int c = 0; c < k; ++c) items += std::min(blocks, (base + (c + 1) * n / k) / keys + 1);
