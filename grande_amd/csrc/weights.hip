@@ -20,8 +20,9 @@
 //   64 sequences of 6,100 rows x 8 KV heads of 128 (bf16), one token each: 170 us,
 //     4.9 TB/s: the keys' bytes.
 //   12 sequences of 2,000 rows x 1 KV head of 256 (f16): 5.8 us: latency.
-//   a prompt of 8,000 tokens x 8 heads of 256 on 4 KV heads (f16): 165 us, 795
-//     TFLOP/s of the 1,190 that a product of 8,192^3 reaches: the products (at
+//   a prompt of 8,000 tokens x 8 heads of 256 on 4 KV heads (f16): 164 us
+//     alone, 152 in a row, 800 to 860 TFLOP/s of the 1,154 that a product of 8,192^3
+//     reaches: the products (at
 //     this operand data the chip lowers its clock; the same MFMAs with nothing
 //     else take 130 us), and 15 % of the places idle, since prompts' last keys
 //     have few queries.  16 x 16 x 32 products draw less than 32 x 32 x 16 (from
