@@ -33,29 +33,17 @@ __device__ inline int64_t row_at(const KeepArgs& a, const int32_t* table, int64_
     return p * a.kv.page_stride + (g * a.kv.page + (row & (a.kv.page - 1))) * a.kv.head_dim;
 }
 
-// To other pages: no row is read and written, so every wave moves rows of its
-// own, U pieces of 1 KiB (512 / D rows each) of K and of V at once.  Bound by the
-// bytes: 64 x 8 lists of 1,000 rows of 128 105 us, 5.0 TB/s, what a large copy
-// reaches; 4,095 rows each 455 us, 4.7 TB/s.  (U = 2: with 1 too few loads are under
-// way, with 4 fewer waves fit a CU, 124 us, with 8 217; non-temporal 106.)
-template <int D, int U>
-__global__ __launch_bounds__(256) void keep_apart_kernel(KeepArgs a) {
-    constexpr int L = D / 8, W = WAVE / L;  // lanes of a row, rows of a piece
-    const int lane = int(threadIdx.x) % WAVE;
-    const int64_t id = int64_t(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(int(threadIdx.x) / WAVE);
-    if (id >= a.waves) return;
-    const int64_t list = id / a.groups, s = list / a.kv.kv_heads, g = list - s * a.kv.kv_heads;
-    const int64_t j0 = (id - list * a.groups) * (U * W) + lane / L;
-    const int32_t* rows = a.x.rows + (a.x.per_head ? list : s) * a.x.rows_ld;
-    const int64_t first = a.x.first ? a.x.first[s] : 0;
-    const int c = lane % L * 8;
+// Rows j0, j0 + W, .. (U of them, below `end`) of sequence s and KV head g, from
+// its rows row(j) to its rows first + j on other pages: 8 head dims at c of each.
+template <int U, typename F>
+__device__ inline void move_apart(const KeepArgs& a, int64_t s, int64_t g, int64_t first, int64_t j0, int64_t end, int W, int c, F row) {
     int64_t from[U], to[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const int64_t j = j0 + u * W;
         from[u] = to[u] = -1;
-        if (j >= a.x.count) continue;
-        from[u] = row_at(a, a.b.table + s * a.b.table_ld, a.b.max_pages, rows[j], g);
+        if (j >= end) continue;
+        from[u] = row_at(a, a.b.table + s * a.b.table_ld, a.b.max_pages, row(j), g);
         to[u] = row_at(a, a.x.to_table + s * a.x.to_ld, a.x.to_ld, first + j, g);
     }
     chunk_t k[U], v[U];
@@ -71,6 +59,23 @@ __global__ __launch_bounds__(256) void keep_apart_kernel(KeepArgs a) {
         *reinterpret_cast<chunk_t*>(static_cast<uint16_t*>(a.kv.k) + to[u] + c) = k[u];
         *reinterpret_cast<chunk_t*>(static_cast<uint16_t*>(a.kv.v) + to[u] + c) = v[u];
     }
+}
+
+// To other pages: no row is read and written, so every wave moves rows of its
+// own, U pieces of 1 KiB (512 / D rows each) of K and of V at once.  Bound by the
+// bytes: 64 x 8 lists of 1,000 rows of 128 105 us, 5.0 TB/s, what a large copy
+// reaches; 4,095 rows each 455 us, 4.7 TB/s.  (U = 2: with 1 too few loads are under
+// way, with 4 fewer waves fit a CU, 124 us, with 8 217; non-temporal 106.)
+template <int D, int U>
+__global__ __launch_bounds__(256) void keep_apart_kernel(KeepArgs a) {
+    constexpr int L = D / 8, W = WAVE / L;  // lanes of a row, rows of a piece
+    const int lane = int(threadIdx.x) % WAVE;
+    const int64_t id = int64_t(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(int(threadIdx.x) / WAVE);
+    if (id >= a.waves) return;
+    const int64_t list = id / a.groups, s = list / a.kv.kv_heads, g = list - s * a.kv.kv_heads;
+    const int32_t* rows = a.x.rows + (a.x.per_head ? list : s) * a.x.rows_ld;
+    move_apart<U>(a, s, g, a.x.first ? a.x.first[s] : 0, (id - list * a.groups) * (U * W) + lane / L, a.x.count, W, lane % L * 8,
+                  [&](int64_t j) { return rows[j]; });
 }
 
 // In place: an entry that moves has rows[j] >= first + j, so the place that an
@@ -203,47 +208,94 @@ void check_sequences(const PagedBatch& b, const PagedKv& kv, const char* who) {
 //
 // A workgroup chooses a list's rows: the `recent` last ones and, of those
 // before them, the keep - recent of the largest weights (choose.h).  Bound by the
-// choice's chain of barriers: 12 lists of 2,300 weights 9.6 us; 512 lists of 6,100
-// 28 us (their 12.5 MB alone 2.5 us).
+// choice's chain of barriers: 12 lists of 2,300 weights 9 us; 512 lists of 6,100
+// 28 us (their 12.5 MB alone 2.5 us).  (512 threads where they hold the list: its
+// barriers are shorter, 1,024 take 1.4 us more; past that 1,024, and past these
+// the list is read in every pass: 8,000 values by 512 threads 6 us more.)
+//
+// MOVE: each of a list's `groups` workgroups makes the same choice, which costs
+// nothing where they fill places that would be empty, and moves the rows of its
+// slice of the places to other pages; the first writes the lists.  (12 lists of
+// 2,300 cut to 1,024 rows of 256 12 us, in two launches 15.3; 32 of 4,000 cut to
+// 2,000 rows of 128 21 and 22; at 64 the same, at 128 74 and 68, since so few waves
+// move rows at less than the rate of a launch of their own.)
 
-constexpr int EVICT_T = 1024;
+constexpr int EVICT_MOVES = 32;  // lists
 
 struct EvictArgs {
-    PagedBatch b;
+    KeepArgs move;  // (with its pool, batch and places)
     EvictRows x;
-    int kv_heads;
     int64_t max_len;
+    int groups, per;  // MOVE: of a list, and the rows of each
 };
 
-template <bool HELD>
-__global__ __launch_bounds__(EVICT_T) void evict_kernel(EvictArgs a) {
-    typedef Choose<EVICT_T, HELD> C;
+template <int T, bool HELD, bool MOVE>
+__global__ __launch_bounds__(T) void evict_kernel(EvictArgs a) {
+    typedef Choose<T, HELD> C;
     __shared__ typename C::Shared shared;
+    extern __shared__ int32_t slice[];  // the rows that the workgroup moves
     const int tid = int(threadIdx.x);
-    const int64_t list = blockIdx.x, s = list / a.kv_heads;
+    const int64_t list = MOVE ? blockIdx.x / a.groups : blockIdx.x, s = list / a.move.kv.kv_heads;
     const float* w = a.x.weights + list * a.x.ldw;
     float* kept = a.x.kept + list * a.x.kept_ld;
     int32_t* rows = a.x.rows + list * a.x.keep;
-    const int len = a.b.lens[s], n = len < 0 ? 0 : len < a.max_len ? len : int(a.max_len);
+    const int len = a.move.b.lens[s], n = len < 0 ? 0 : len < a.max_len ? len : int(a.max_len);
     const int keep = int(a.x.keep), recent = int(a.x.recent);
+    const int part = MOVE ? int(blockIdx.x % a.groups) : 0, from = part * a.per, to = from + a.per < keep ? from + a.per : keep;
+    auto place = [&](int rank, int row) {
+        if (part == 0) rows[rank] = row;
+        if (MOVE && rank >= from && rank < to) slice[rank - from] = row;
+    };
     if (n <= keep) {
-        for (int i = tid; i < keep; i += EVICT_T) {
-            rows[i] = i < n ? i : -1;
-            if (i < n && kept != w) kept[i] = w[i];
+        for (int i = tid; i < keep; i += T) {
+            place(i, i < n ? i : -1);
+            if (part == 0 && i < n && kept != w) kept[i] = w[i];
         }
-        return;
-    }
-    const int old = n - recent, chosen = keep - recent;
-    C::run(shared, w, old, uint32_t(chosen), [&](int rank, int row, float x) { rows[rank] = row, kept[rank] = x; });
-    // The recent rows, and zeros for the rows to come.
-    for (int i0 = 0; i0 < recent; i0 += EVICT_T) {
-        const int i = i0 + tid;
-        const float x = i < recent ? w[old + i] : 0.0f;
+    } else {
+        const int old = n - recent, chosen = keep - recent;
+        C::run(shared, w, old, uint32_t(chosen), [&](int rank, int row, float x) {
+            place(rank, row);
+            if (part == 0) kept[rank] = x;
+        });
+        // The recent rows, and zeros for the rows to come.
+        for (int i0 = 0; i0 < recent; i0 += T) {
+            const int i = i0 + tid;
+            const float x = i < recent ? w[old + i] : 0.0f;
+            if (!MOVE) __syncthreads();
+            if (i < recent) place(chosen + i, old + i);
+            if (i < recent && part == 0) kept[chosen + i] = x;
+        }
         __syncthreads();
-        if (i < recent) rows[chosen + i] = old + i, kept[chosen + i] = x;
+        if (part == 0)
+            for (int i = keep + tid; i < n && i < a.x.kept_ld; i += T) kept[i] = 0.0f;
     }
-    __syncthreads();
-    for (int i = keep + tid; i < n && i < a.x.kept_ld; i += EVICT_T) kept[i] = 0.0f;
+    if constexpr (MOVE) {
+        __syncthreads();
+        constexpr int U = 2;
+        const int L = a.move.kv.head_dim / 8, W = T / L;
+        for (int64_t j = from + tid / L; j < to; j += U * W)
+            move_apart<U>(a.move, s, list - s * a.move.kv.kv_heads, 0, j, to, W, tid % L * 8, [&](int64_t j) { return slice[j - from]; });
+    }
+}
+
+template <int T, bool HELD>
+void launch_evict(hipStream_t s, EvictArgs a) {
+    const int64_t lists = a.move.b.nseq * a.move.kv.kv_heads;
+    // Few lists whose weights are not written over go to other pages in one launch.
+    if constexpr (HELD) {
+        if (a.x.to_table && a.x.kept != a.x.weights && lists <= EVICT_MOVES) {
+            a.groups = int(256 / lists);
+            a.per = int((a.x.keep + a.groups - 1) / a.groups);
+            a.groups = int((a.x.keep + a.per - 1) / a.per);
+            evict_kernel<T, true, true><<<dim3(unsigned(lists * a.groups)), dim3(T), unsigned(a.per) * 4, s>>>(a);
+            OMG_HIP(hipGetLastError());
+            return;
+        }
+    }
+    if (lists >= MAX_BLOCKS / (T / 256)) fail(E_CAPACITY, "kv_evict: too many lists for one call");
+    evict_kernel<T, HELD, false><<<dim3(unsigned(lists)), dim3(T), 0, s>>>(a);
+    OMG_HIP(hipGetLastError());
+    move_rows(s, a.move.kv, a.move.b, a.move.x);
 }
 
 }  // namespace
@@ -272,15 +324,14 @@ void launch_kv_evict(hipStream_t s, const PagedKv& kv, const PagedBatch& b, cons
     if (x.kept == x.weights && x.kept_ld != x.ldw) fail(E_INVALID, "kv_evict: kept_ld must be ldw in place");
     if (x.to_table && (x.to_ld <= 0 || x.to_ld > 0x3fffffff / kv.page))
         fail(E_INVALID, "kv_evict: to_ld out of range");
-    if (b.nseq * kv.kv_heads >= MAX_BLOCKS / (EVICT_T / 256)) fail(E_CAPACITY, "kv_evict: too many lists for one call");
-    EvictArgs a{b, x, kv.kv_heads, max_len};
-    const dim3 grid(unsigned(b.nseq * kv.kv_heads));
-    if (max_len <= CHOOSE_R * EVICT_T)
-        evict_kernel<true><<<grid, dim3(EVICT_T), 0, s>>>(a);
+    const KeepRows moves{x.rows, x.keep, x.keep, nullptr, 1, x.to_table, x.to_ld};
+    const EvictArgs a{KeepArgs{kv, b, moves, log2_of(kv.page), 0, 1, 1}, x, max_len, 1, int(x.keep)};
+    if (max_len <= CHOOSE_R * 512)
+        launch_evict<512, true>(s, a);
+    else if (max_len <= CHOOSE_R * 1024)
+        launch_evict<1024, true>(s, a);
     else
-        evict_kernel<false><<<grid, dim3(EVICT_T), 0, s>>>(a);
-    OMG_HIP(hipGetLastError());
-    move_rows(s, kv, b, KeepRows{x.rows, x.keep, x.keep, nullptr, 1, x.to_table, x.to_ld});
+        launch_evict<1024, false>(s, a);
 }
 
 }  // namespace omg

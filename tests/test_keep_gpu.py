@@ -301,6 +301,17 @@ def test_long_lists(n, keep):
         assert np.array_equal(got.view(np.int32), exp[2].view(np.int32))
 
 
+@pytest.mark.parametrize("nseq,kv_heads", [(1, 1), (4, 8), (3, 11), (9, 4)])
+@pytest.mark.parametrize("n,keep,recent,hd", [(300, 7, 2, 64), (4000, 1500, 900, 64), (6000, 3100, 1200, 128),
+                                              (1000, 999, 0, 512)])
+def test_choice_and_moves_in_one_launch_and_in_two(n, keep, recent, hd, nseq, kv_heads):
+    """Lists that many workgroups choose from, each moving a slice of the rows, and more lists than that."""
+    rng = np.random.default_rng(n + nseq)
+    lens = rng.integers(keep // 2, n, nseq)
+    lens[0] = n
+    Evict(rng, lens, kv_heads, hd, keep, recent, page=64, to=True, separate=True).test()
+
+
 def test_long_lists_of_equal_weights():
     rng = np.random.default_rng(17)
     c = Evict(rng, [140_000], 1, 64, 66_000, 5, page=256, weights=lambda w: np.ones_like(w))
