@@ -107,7 +107,8 @@ struct BlockArgs {
 // them: lane l of a step holds token l % 16 and dims of the quarter l / 16 of
 // the head, and blocks' means likewise, a run of 16 bytes at a time.  Bound by
 // the f64 products and the loads' latency before them: 64 tokens x 8 KV heads of
-// 128 on some 1,050 blocks 11.8 us, 12 x 4 of 256 on 126 9 us.
+// 128 on some 1,050 blocks 11.9 us, 12 x 4 of 256 on 126 8.1 us (its second half of
+// the means asked for behind the first half's products 8.7).
 template <typename T, int D>
 __global__ __launch_bounds__(256) void block_scores_kernel(BlockArgs x) {
     constexpr int Q = D / 4, DC = Q < 64 ? Q : 64;  // dims of a quarter, of them in LDS at once
@@ -160,6 +161,11 @@ __global__ __launch_bounds__(256) void block_scores_kernel(BlockArgs x) {
     const bool there = p >= 0 && p < a.kv.npages;
     const float* mean = x.means + ((there ? p : 0) * G + g) * D + lane / 16 * Q;
     doublex4 acc = {0.0, 0.0, 0.0, 0.0};
+    // (a page that is not there: the first page's means, and no score from them)
+    constexpr int N = DC < 32 ? DC : 32;  // dims whose means are under way
+    float4 m[N / 4];
+#pragma unroll
+    for (int d = 0; d < N; d += 4) m[d / 4] = *reinterpret_cast<const float4*>(mean + d);
     for (int c = 0; c < Q; c += DC) {
         if (c) __syncthreads();
         // A thread sums 8 dims of a token at a time over the heads.
@@ -182,13 +188,14 @@ __global__ __launch_bounds__(256) void block_scores_kernel(BlockArgs x) {
             for (int e = 0; e < 8; ++e) qs[(d + e) * WAVE + quarter * 16 + tok] = sum[e];
         }
         __syncthreads();
-        // (a page that is not there: the first page's means, and no score from them)
-#pragma unroll 1
-        for (int d0 = 0; d0 < DC; d0 += 32) {
-            constexpr int N = DC < 32 ? DC : 32;
-            float4 m[N / 4];
 #pragma unroll
-            for (int d = 0; d < N; d += 4) m[d / 4] = *reinterpret_cast<const float4*>(mean + c + d0 + d);
+        for (int d0 = 0; d0 < DC; d0 += N) {
+            float4 next[N / 4];
+            const bool more = c + d0 + N < Q;
+            if (more) {
+#pragma unroll
+                for (int d = 0; d < N; d += 4) next[d / 4] = *reinterpret_cast<const float4*>(mean + c + d0 + N + d);
+            }
 #pragma unroll
             for (int d = 0; d < N; d += 4) {
                 const double* q = qs + (d0 + d) * WAVE + lane;
@@ -196,6 +203,10 @@ __global__ __launch_bounds__(256) void block_scores_kernel(BlockArgs x) {
                 acc = __builtin_amdgcn_mfma_f64_16x16x4f64(double(m[d / 4].y), q[WAVE], acc, 0, 0, 0);
                 acc = __builtin_amdgcn_mfma_f64_16x16x4f64(double(m[d / 4].z), q[2 * WAVE], acc, 0, 0, 0);
                 acc = __builtin_amdgcn_mfma_f64_16x16x4f64(double(m[d / 4].w), q[3 * WAVE], acc, 0, 0, 0);
+            }
+            if (more) {
+#pragma unroll
+                for (int d = 0; d < N / 4; ++d) m[d] = next[d];
             }
         }
     }
@@ -221,11 +232,24 @@ __device__ inline int own_block(const BlockArgs& x, const SeqRow& at) {
     return x.np + int(row >> x.a.page_shift);
 }
 
+constexpr int CHOOSE_T = 256;
+
+// put(rank, block) for the blocks that a token takes, all threads of the
+// workgroup together; largest(n, k, hand) hands out the k best of the first n.
+template <typename L, typename F>
+__device__ inline void choose_blocks(const BlockArgs& x, int own, L largest, F put) {
+    const int tid = int(threadIdx.x), others = own < x.keep - 1 ? own : x.keep - 1;
+    if (others == own) {
+        for (int i = tid; i < own; i += CHOOSE_T) put(i, i);
+    } else {
+        largest(own, uint32_t(others), [&](int rank, int b, float) { put(rank, b); });
+    }
+    for (int i = others + tid; i < x.keep; i += CHOOSE_T) put(i, i == others ? own : -1);
+}
+
 // A workgroup a token and KV head, of 256 threads, so that many lists share a CU
 // (a step's 512 lists of 1,000 blocks: 9 us; 48 of 126: 5 to 6 us, the choice's
 // chain of barriers).
-constexpr int CHOOSE_T = 256;
-
 template <bool HELD>
 __global__ __launch_bounds__(CHOOSE_T) void block_choose_kernel(BlockArgs x) {
     typedef Choose<CHOOSE_T, HELD> C;
@@ -240,13 +264,8 @@ __global__ __launch_bounds__(CHOOSE_T) void block_choose_kernel(BlockArgs x) {
             for (int i = tid; i < x.keep; i += CHOOSE_T) to[i] = -1;
         return;
     }
-    const int others = own < x.keep - 1 ? own : x.keep - 1;
-    if (others == own) {
-        for (int i = tid; i < own; i += CHOOSE_T) to[i] = i;
-    } else {
-        C::run(shared, x.scores + list * x.blocks_ld, own, uint32_t(others), [&](int rank, int b, float) { to[rank] = b; });
-    }
-    for (int i = others + tid; i < x.keep; i += CHOOSE_T) to[i] = i == others ? own : -1;
+    auto largest = [&](int n, uint32_t k, auto hand) { C::run(shared, x.scores + list * x.blocks_ld, n, k, hand); };
+    choose_blocks(x, own, largest, [&](int rank, int b) { to[rank] = b; });
 }
 
 // --------------------------------------------------------------- attention
@@ -255,7 +274,9 @@ __global__ __launch_bounds__(CHOOSE_T) void block_choose_kernel(BlockArgs x) {
 // wave every fourth 16-key tile.  All rows see the same keys.  (512 lists of 64 x
 // 64 rows, 128-wide: 82 us, 1.1 GB through L2 and 270 MB from HBM; a second tile
 // a wave under way 85.)
-template <typename T, int D>
+// CHOOSE: the workgroup makes its list's choice itself, each split and part of the
+// heads again.
+template <typename T, int D, bool CHOOSE>
 __global__ __launch_bounds__(NW * 64, D == 512 ? 1 : D == 64 ? 4 : 2) void attention_blocks_kernel(BlockArgs x) {
     typedef Core<T, D, WAVES_KEYS> C;
     extern __shared__ __attribute__((aligned(1024))) unsigned char smem_raw[];
@@ -270,6 +291,9 @@ __global__ __launch_bounds__(NW * 64, D == 512 ? 1 : D == 64 ? 4 : 2) void atten
     id /= a.p.os;
     const int64_t tok = id / parts;
     const int head0 = int(id - tok * parts) * 16 + lane % 16;
+    const int64_t list = tok * G + g;
+    float score = 0.0f;  // CHOOSE: of few blocks the thread's, on its way before their number is known
+    if (CHOOSE && x.blocks_ld <= CHOOSE_T && tid < x.blocks_ld) score = x.scores[list * x.blocks_ld + tid];
     const SeqRow at = token_row(a.b, tok, lane);
     if (at.seq < 0) return;
     const int own = own_block(x, at);
@@ -279,8 +303,31 @@ __global__ __launch_bounds__(NW * 64, D == 512 ? 1 : D == 64 ? 4 : 2) void atten
 
     // Lane e: the page of the item's entry e and its rows that the token sees.
     const int e0 = split * x.chunk, count = imin(x.chunk, x.keep - e0);
-    const int32_t* list = x.chosen + (tok * G + g) * x.keep + e0;
-    const int block = lane < count ? list[lane] : -1;
+    int block = -1;
+    if constexpr (CHOOSE) {
+        typedef Choose<CHOOSE_T, true> Best;
+        static_assert(CHOOSE_T == NW * 64 && sizeof(typename Best::Shared) <= NW * 16 * D * 4, "the tiles' place");
+        auto& shared = *reinterpret_cast<typename Best::Shared*>(smem_raw);
+        __shared__ int taken[WAVE];
+        int32_t* to = x.chosen && split == 0 && id % parts == 0 ? x.chosen + list * x.keep : nullptr;
+        auto put = [&](int rank, int b) {
+            if (rank >= e0 && rank < e0 + count) taken[rank - e0] = b;
+            if (to) to[rank] = b;
+        };
+        if (own >= 0)
+            choose_blocks(x, own, [&](int n, uint32_t k, auto hand) {
+                if (x.blocks_ld <= CHOOSE_T)
+                    Best::run_few(shared, score, n, k, hand);
+                else
+                    Best::run(shared, x.scores + list * x.blocks_ld, n, k, hand);
+            }, put);
+        else
+            for (int i = tid; i < x.keep; i += CHOOSE_T) put(i, -1);
+        __syncthreads();
+        if (lane < count) block = taken[lane];
+    } else if (lane < count) {
+        block = x.chosen[list * x.keep + e0 + lane];
+    }
     int page = -1, rows = 0;
     if (block >= 0 && block <= own) {
         const int P = int(a.b.prefix_len), j = block - x.np;
@@ -324,8 +371,11 @@ void check_blocks(const PagedKv& kv, const PagedBatch& b, int heads, int64_t kee
     if (keep <= 0 || keep > 4096) fail(E_INVALID, "attention_blocks: blocks must be 1 to 4096");
 }
 
-// Entries are split over work items until these fill the chip's places (by
-// LDS), at least two at a time and at most a lane each.  (Lists of one token
+// Workgroups of attention_blocks_kernel that the chip takes at once, by LDS.
+int64_t places(int head_dim) { return 256 * (head_dim == 64 ? 4 : head_dim == 512 ? 1 : 2); }
+
+// Entries are split over work items until these fill the chip's places,
+// at least two at a time and at most a lane each.  (Lists of one token
 // each that start together stay together, and what one reads the next finds in
 // L2: 512 lists as 1,024 items 116 us, as 512 82.)
 BlockPlan plan_blocks(const PagedKv& kv, const PagedBatch& b, int heads, int64_t keep) {
@@ -333,9 +383,8 @@ BlockPlan plan_blocks(const PagedKv& kv, const PagedBatch& b, int heads, int64_t
     p.np = (b.prefix_len + kv.page - 1) / kv.page;
     p.blocks = p.np + b.max_pages;
     const int64_t hpg = heads / kv.kv_heads, items = b.t * kv.kv_heads * ((hpg + 15) / 16);
-    const int64_t places = 256 * (kv.head_dim == 64 ? 4 : kv.head_dim == 512 ? 1 : 2);
     const int64_t least = (keep + 63) / 64, most = std::min<int64_t>(64, (keep + 1) / 2);
-    const int64_t want = std::max(least, std::min(most, places / items));
+    const int64_t want = std::max(least, std::min(most, places(kv.head_dim) / items));
     p.chunk = int((keep + want - 1) / want);
     p.splits = int((keep + p.chunk - 1) / p.chunk);
     p.scores = up(b.t * kv.kv_heads * p.blocks * 4, 16);
@@ -344,8 +393,24 @@ BlockPlan plan_blocks(const PagedKv& kv, const PagedBatch& b, int heads, int64_t
     return p;
 }
 
+template <typename T, int D, bool CHOOSE>
+void launch_chosen(hipStream_t s, const BlockArgs& x, int64_t items) {
+    constexpr unsigned lds = NW * 16 * D * 4 + 2 * NW * 16 * 4;  // tiles of K and V a wave; their join
+    static std::atomic<uint64_t> lds_set{0};                     // the devices, once per instantiation
+    int device = 0;
+    OMG_HIP(hipGetDevice(&device));
+    const uint64_t bit = uint64_t(1) << (device & 63);
+    if (device > 63 || !(lds_set.load(std::memory_order_relaxed) & bit)) {
+        OMG_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(attention_blocks_kernel<T, D, CHOOSE>),
+                                    hipFuncAttributeMaxDynamicSharedMemorySize, int(lds)));
+        lds_set.fetch_or(bit, std::memory_order_relaxed);
+    }
+    attention_blocks_kernel<T, D, CHOOSE><<<dim3(unsigned(items)), dim3(NW * 64), lds, s>>>(x);
+    OMG_HIP(hipGetLastError());
+}
+
 template <typename T, int D>
-void launch_blocks_d(hipStream_t s, const BlockArgs& x, int64_t own_tiles) {
+void launch_blocks_d(hipStream_t s, BlockArgs x, int64_t own_tiles, int32_t* room) {
     const Args& a = x.a;
     const int64_t lists = a.b.t * a.kv.kv_heads;
     const int64_t scored = (x.prefix_items + own_tiles * x.own_chunks) * a.kv.kv_heads;
@@ -354,23 +419,20 @@ void launch_blocks_d(hipStream_t s, const BlockArgs& x, int64_t own_tiles) {
         fail(E_CAPACITY, "attention_blocks: too many work items");
     block_scores_kernel<T, D><<<dim3(unsigned(scored)), dim3(256), 0, s>>>(x);
     OMG_HIP(hipGetLastError());
-    if (x.blocks_ld <= CHOOSE_R * CHOOSE_T)
-        block_choose_kernel<true><<<dim3(unsigned(lists)), dim3(CHOOSE_T), 0, s>>>(x);
-    else
-        block_choose_kernel<false><<<dim3(unsigned(lists)), dim3(CHOOSE_T), 0, s>>>(x);
-    OMG_HIP(hipGetLastError());
-    constexpr unsigned lds = NW * 16 * D * 4 + 2 * NW * 16 * 4;  // tiles of K and V a wave; their join
-    static std::atomic<uint64_t> lds_set{0};                     // the devices, once per instantiation
-    int device = 0;
-    OMG_HIP(hipGetDevice(&device));
-    const uint64_t bit = uint64_t(1) << (device & 63);
-    if (device > 63 || !(lds_set.load(std::memory_order_relaxed) & bit)) {
-        OMG_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(attention_blocks_kernel<T, D>),
-                                    hipFuncAttributeMaxDynamicSharedMemorySize, int(lds)));
-        lds_set.fetch_or(bit, std::memory_order_relaxed);
+    // Work items that the chip takes at once choose for themselves (12 x 4 lists of
+    // 126 blocks: 18 us for 15.5 and 6, 512 of 1,050: 87 for 82 and 9).  More of them
+    // would hold the tiles' LDS through a chain of barriers, round by round (2,048 of
+    // 196: 114 us, in two launches 97 and 12).
+    const bool held = x.blocks_ld <= CHOOSE_R * CHOOSE_T;
+    if (held && items <= places(D)) {
+        launch_chosen<T, D, true>(s, x, items);
+    } else {
+        if (!x.chosen) x.chosen = room;
+        held ? block_choose_kernel<true><<<dim3(unsigned(lists)), dim3(CHOOSE_T), 0, s>>>(x)
+             : block_choose_kernel<false><<<dim3(unsigned(lists)), dim3(CHOOSE_T), 0, s>>>(x);
+        OMG_HIP(hipGetLastError());
+        launch_chosen<T, D, false>(s, x, items);
     }
-    attention_blocks_kernel<T, D><<<dim3(unsigned(items)), dim3(NW * 64), lds, s>>>(x);
-    OMG_HIP(hipGetLastError());
     if (!a.part_o) return;
     const int64_t rows = a.b.t * a.x.heads;
     if (a.p.slots() > 8)
@@ -381,12 +443,12 @@ void launch_blocks_d(hipStream_t s, const BlockArgs& x, int64_t own_tiles) {
 }
 
 template <typename T>
-void launch_blocks_t(hipStream_t s, const BlockArgs& x, int64_t own_tiles) {
+void launch_blocks_t(hipStream_t s, const BlockArgs& x, int64_t own_tiles, int32_t* room) {
     switch (x.a.kv.head_dim) {
-        case 64: return launch_blocks_d<T, 64>(s, x, own_tiles);
-        case 128: return launch_blocks_d<T, 128>(s, x, own_tiles);
-        case 256: return launch_blocks_d<T, 256>(s, x, own_tiles);
-        default: return launch_blocks_d<T, 512>(s, x, own_tiles);
+        case 64: return launch_blocks_d<T, 64>(s, x, own_tiles, room);
+        case 128: return launch_blocks_d<T, 128>(s, x, own_tiles, room);
+        case 256: return launch_blocks_d<T, 256>(s, x, own_tiles, room);
+        default: return launch_blocks_d<T, 512>(s, x, own_tiles, room);
     }
 }
 
@@ -443,12 +505,13 @@ void launch_attention_blocks(hipStream_t s, const PagedKv& kv, const PagedBatch&
     }
     k.means = means;
     k.scores = reinterpret_cast<float*>(room), k.blocks_ld = p.blocks;
-    k.chosen = chosen ? chosen : reinterpret_cast<int32_t*>(room + p.scores);
+    k.chosen = chosen;
     k.keep = int(keep), k.np = int(p.np), k.chunk = p.chunk;
     k.prefix_items = (b.t + 15) / 16 * ((p.np + 63) / 64);
     k.own_chunks = (b.max_pages + 63) / 64;
     const int64_t own_tiles = b.start ? b.t / 16 + b.nseq : b.nseq;
-    kv.dtype == ELEM_F16 ? launch_blocks_t<half_t>(s, k, own_tiles) : launch_blocks_t<bf16_t>(s, k, own_tiles);
+    int32_t* list = reinterpret_cast<int32_t*>(room + p.scores);
+    kv.dtype == ELEM_F16 ? launch_blocks_t<half_t>(s, k, own_tiles, list) : launch_blocks_t<bf16_t>(s, k, own_tiles, list);
 }
 
 }  // namespace omg

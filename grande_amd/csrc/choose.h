@@ -31,17 +31,50 @@ struct Choose {
     static constexpr int COPIES = 8, FEW = 128;
     static_assert(T >= 256 && T % 256 == 0, "a thread a bin");
     struct Shared {
-        uint32_t bins[COPIES * 256];
+        alignas(16) uint32_t bins[COPIES * 256];
         uint32_t cells[2 * CELLS];
         uint32_t few[FEW], sums[2 * (WAVES < 4 ? 4 : WAVES)], found[3], nfew;
     };
+
+    // The same for n <= T values, one a thread: how many lie over it, and of equal
+    // ones before it, says whether it is chosen.
+    template <typename F>
+    static __device__ void run_few(Shared& sh, float value, int n, uint32_t left, F hand) {
+        static_assert(T <= COPIES * 256);
+        const int tid = int(threadIdx.x), lane = tid % WAVE, wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
+        const uint32_t key = tid < n ? value_key(value) : 0;
+        const uint64_t before = (uint64_t(1) << lane) - 1;
+        sh.bins[tid] = key;
+        __syncthreads();
+        uint32_t order = 0;
+        for (int i = 0; i * WAVE < n; ++i) {  // (the keys behind the last one are over none and before none)
+            const uint4* cell = reinterpret_cast<const uint4*>(sh.bins + i * WAVE);
+            const uint32_t least = i < wave ? key : key + 1;  // (no key is 2^32 - 1)
+#pragma unroll
+            for (int j = 0; j < WAVE / 4; ++j) {
+                const uint4 k = cell[j];
+                order += (k.x >= least) + (k.y >= least) + (k.z >= least) + (k.w >= least);
+            }
+        }
+        uint64_t like = 0;  // the wave's
+#pragma unroll
+        for (int j = 0; j < WAVE; ++j) like |= uint64_t(uint32_t(__builtin_amdgcn_readlane(int(key), j)) == key) << j;
+        order += __popcll(like & before);
+        const uint64_t chosen = __ballot(tid < n && order < left);
+        if (lane == 0) sh.sums[wave] = __popcll(chosen);
+        __syncthreads();
+        int rank = __popcll(chosen & before);
+        for (int i = 0; i < wave; ++i) rank += sh.sums[i];
+        if (tid < n && order < left) hand(rank, tid, value);
+        __syncthreads();
+    }
 
     // hand(rank, place, value) for each chosen one of w[0 .. n), left <= n; the
     // list may be overwritten from its start on as they are handed out (a
     // chosen value's rank is at most its place, and all are read before).
     template <typename F>
     static __device__ void run(Shared& sh, const float* w, int n, uint32_t left, F hand) {
-        const int tid = int(threadIdx.x), lane = tid % WAVE, wave = tid / WAVE;
+        const int tid = int(threadIdx.x), lane = tid % WAVE, wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
         float held[R];
         if constexpr (HELD) {
 #pragma unroll
@@ -51,8 +84,8 @@ struct Choose {
         auto each = [&](auto f) {
             if constexpr (HELD) {
 #pragma unroll
-                for (int u = 0; u < R; ++u)
-                    if (tid + u * T < n) f(value_key(held[u]));
+                for (int u = 0; u < R; ++u)  // (a branch of the wave, then one of its lanes)
+                    if (wave * WAVE + u * T < n && tid + u * T < n) f(value_key(held[u]));
             } else {
                 for (int i0 = tid; i0 < n; i0 += R * T) {
                     float x[R];

@@ -594,7 +594,7 @@ class PagedKv(L.omg_paged_kv):
 
     def block_means(self, batch: PagedBatch, means_ptr: int, stream: int | None = None) -> None:
         """omg_dev_block_means: the mean keys of the pages that the step's new
-        rows are on, into means [npages][kv_heads][head_dim] (f32)."""
+        (or moved) rows are on, into means [npages][kv_heads][head_dim] (f32)."""
         L.check(L.lib().omg_dev_block_means(self, batch, means_ptr, stream))
 
     def attention_blocks_workspace(self, batch: PagedBatch, heads: int, blocks: int) -> int:

@@ -440,7 +440,9 @@ int omg_dev_attention_tree(const omg_paged_kv *kv, const omg_paged_batch *b, int
  * pages; omg_dev_block_means sets those of the pages that the batch's new rows
  * are on, over the rows up to lens[s] (64-bit sums, one rounding), and leaves
  * the others: one call behind each append keeps them, the prefix's by the call
- * that made it as a sequence of its own.
+ * that made it as a sequence of its own.  So does one behind rows that move: of
+ * a draft closed up by omg_dev_kv_keep the draft's batch with the lengths that
+ * are left, of an eviction one whose new rows are all that stay.
  *
  * A token's blocks are numbered through the prefix's pages, then its sequence's
  * own ones; score = sum over a KV head's query heads of q . mean (64-bit sums,

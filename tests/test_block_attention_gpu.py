@@ -164,6 +164,42 @@ def test_means_of_lengths_short_of_the_tokens_and_pages_outside_the_pool():
             assert bool((got[p] == 7.0).all())
 
 
+@pytest.mark.parametrize("evict", [False, True])
+def test_means_and_blocks_of_rows_that_have_moved(evict):
+    """An accepted path closed up over page borders, or an eviction: the means follow by a call whose new rows they are."""
+    rng = np.random.default_rng(25)
+    new, before, heads, kv_heads, hd = np.array([1, 40, 3, 37]), np.array([20, 30, 15, 64]), 4, 2, 64
+    c = BlockCall(rng, new, before, 100, heads, kv_heads, hd, 3)
+    c.all_means()
+    pool = c.pool
+    if evict:
+        keep, max_len = 45, pool.max_pages * pool.page
+        w = torch.rand(4 * kv_heads, max_len, device="cuda")
+        rows = torch.empty(4, kv_heads, keep, dtype=torch.int32, device="cuda")
+        c.kv.evict(c.batch, keep, 10, w.data_ptr(), max_len, rows.data_ptr())
+        left = np.minimum(pool.lens_host, keep)
+        moved = left
+    else:
+        rows = torch.full((4, 40), -1, dtype=torch.int32)
+        took = [np.sort(rng.choice(n, -(-n // 2), replace=False)) for n in new]
+        for s, x in enumerate(took):
+            rows[s, :len(x)] = torch.from_numpy(before[s] + x)
+        rows, first = rows.cuda(), torch.from_numpy(before.astype(np.int32)).cuda()
+        c.kv.keep(c.batch, rows.data_ptr(), 40, 40, first=first.data_ptr())
+        left = before + [len(x) for x in took]
+        moved = new
+    pool.lens.copy_(torch.from_numpy(left.astype(np.int32)))
+    start = torch.from_numpy(np.concatenate([[0], np.cumsum(moved)]).astype(np.int32)).cuda()
+    c.kv.block_means(pool.batch(int(moved.sum()), start), c.means.data_ptr())
+    torch.cuda.synchronize()
+    got = c.means.double().cpu()
+    for s in range(4):
+        for p, mean in mean_of(pool, pool.table_host[s], int(left[s]), pool.page).items():
+            assert bool(((got[p] - mean).abs() <= 2.0 ** -24 * mean.abs() + 2.0 ** -52).all()), (s, p)
+    if evict:
+        c.run().check()
+
+
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 @pytest.mark.parametrize("heads,kv_heads,hd", SHAPES + [(40, 1, 64), (36, 2, 128)])
 @pytest.mark.parametrize("nseq,prefix,blocks", [(1, 1000, 9), (9, 301, 6), (5, 0, 3), (20, 77, 40)])
@@ -202,6 +238,27 @@ def test_many_blocks_and_long_lists():
     c.run()
     torch.cuda.synchronize()
     assert torch.equal(first[0], c.out) and torch.equal(first[1], c.lse)
+
+
+@pytest.mark.parametrize("nseq,kv_heads,hd,blocks", [(64, 8, 128, 3), (57, 9, 128, 3), (32, 8, 512, 2), (43, 6, 512, 2),
+                                                     (128, 8, 64, 3), (129, 8, 64, 3)])
+def test_as_many_lists_as_the_chip_takes_at_once_and_more(nseq, kv_heads, hd, blocks):
+    """Where the attention's workgroups choose for themselves, and one list more."""
+    rng = np.random.default_rng(nseq + hd)
+    BlockCall(rng, [1] * nseq, rng.integers(0, 60, nseq), 90, kv_heads, kv_heads, hd, blocks).all_means().run().check()
+
+
+@pytest.mark.parametrize("give", [True, False])
+@pytest.mark.parametrize("prefix", [251 * 16, 252 * 16 + 3, 2043 * 16 + 1, 2044 * 16 + 1])
+def test_numbers_of_blocks_at_which_the_choice_changes(prefix, give):
+    """A block a thread, several in registers, and more; equal scores among them; without the caller's list too."""
+    rng = np.random.default_rng(prefix)
+    c = BlockCall(rng, [1, 1], [70, 9], prefix, 4, 2, 64, 30, give=give).all_means()
+    assert c.pool.max_pages == 5
+    c.run().check("as they come")
+    c.means.copy_((c.means * 2).round() / 2)
+    c.means[:, :, 1:] = 0
+    c.run().check("many alike")
 
 
 def test_all_blocks_are_plain_attention():
