@@ -455,9 +455,12 @@ int many_keys(int head_dim) { return head_dim == 512 ? 128 : 256; }
 // The splits of the queries of least time, by the rounds in which the places
 // that the chip has take the items with something to do (keys near a prompt's
 // end have few queries) and an item's tiles, three more for its start and end,
-// for sequences of the mean number of tokens.  (8,000 tokens x 8 heads of 256 on
-// 4 KV heads: 4 / 7 / 14 / 32 splits 244 / 172 / 216 / 220 us when it was 172; 7
-// is what this gives.)
+// for sequences of the mean number of tokens; of several, three quarters of the
+// items, since most are shorter than the table.  (8,000 tokens x 8 heads of 256 on
+// 4 KV heads: 4 / 7 / 16 / 32 splits 220 / 161 / 189 / 183 us, 7 is what this gives;
+// 600 x 8 of 512 on one, 150 tiles: 8 / 16 / 48 38 / 25 / 18; 9 x 200 tokens x 15 of 64
+// on 5: 1 / 2 / 8 / 32 29 / 20 / 14 / 18; 6 x 772 x 8 of 256 on 4, ragged: 1 / 3 / 12 67 / 44
+// / 64.)
 int splits(const PagedKv& kv, const PagedBatch& b, int heads) {
     if (few(kv, b, heads)) return 1;
     const int64_t max_len = b.max_pages * kv.page, keys = many_keys(kv.head_dim), blocks = (max_len + keys - 1) / keys;
@@ -466,13 +469,15 @@ int splits(const PagedKv& kv, const PagedBatch& b, int heads) {
     const double tile_us = 0.4 + kv.head_dim * 0.0057;
     int best = 1;
     double best_us = 1e30;
-    for (const int k : {1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 14, 16, 20, 24, 32}) {
-        if (k > 1 && tiles < 8 * k) break;
+    for (const int k : {1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 14, 16, 20, 24, 32, 48}) {
+        if (tiles < k) break;
         // Split c has tokens up to (c + 1) n / k, which see blocks up to theirs.
         int64_t items = 0;
         for (int c = 0; c < k; ++c) items += std::min(blocks, (base + (c + 1) * n / k) / keys + 1);
-        const double rounds = double((items * b.nseq * kv.kv_heads + places - 1) / places);
-        const double us = rounds * (double((tiles + k - 1) / k) + 3) * tile_us + (k > 1 ? 3 + 0.2 * k : 0);
+        items *= b.nseq * kv.kv_heads;
+        if (b.nseq > 1) items -= items / 4;
+        const double rounds = double((items + places - 1) / places);
+        const double us = rounds * (double((tiles + k - 1) / k) + 3) * tile_us + (k > 1 ? 5 + 0.2 * k : 0);
         if (us < best_us) best_us = us, best = k;
     }
     return best;
