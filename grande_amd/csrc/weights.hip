@@ -20,14 +20,12 @@
 //   64 sequences of 6,100 rows x 8 KV heads of 128 (bf16), one token each: 170 us,
 //     4.9 TB/s: the keys' bytes.
 //   12 sequences of 2,000 rows x 1 KV head of 256 (f16): 5.8 us: latency.
-//   a prompt of 8,000 tokens x 8 heads of 256 on 4 KV heads (f16): 164 us
-//     alone, 152 in a row, 800 to 860 TFLOP/s of the 1,154 that a product of 8,192^3
-//     reaches: the products (at
-//     this operand data the chip lowers its clock; the same MFMAs with nothing
-//     else take 130 us), and 15 % of the places idle, since prompts' last keys
-//     have few queries.  16 x 16 x 32 products draw less than 32 x 32 x 16 (from
-//     registers alone 2,050 and 1,700 TFLOP/s on random data): 174 -> 165 us, at
-//     128-wide heads 160 -> 132.
+//   a prompt of 8,000 tokens x 8 heads of 256 on 4 KV heads (f16): 149 us
+//     alone, 140 in a row, 880 to 940 TFLOP/s of the 1,154 that a product of 8,192^3
+//     reaches: the products (at this operand data the chip lowers its clock; the
+//     same MFMAs with nothing else take 130 us).  16 x 16 x 32 products draw less
+//     than 32 x 32 x 16 (from registers alone 2,050 and 1,700 TFLOP/s on random
+//     data): 174 -> 165 us when it was that, at 128-wide heads 160 -> 132.
 #include <algorithm>
 #include <atomic>
 #include <climits>
@@ -227,29 +225,35 @@ __global__ __launch_bounds__(256, 2) void weights_many_kernel(Args a) {
     float* log_sums = reinterpret_cast<float*>(smem_raw + M::BUFS * M::TILE * 2);  // [BUFS][4][64]
     const int lane = int(threadIdx.x) % WAVE, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / WAVE);
     const int G = a.kv.kv_heads, hpg = a.hpg;
-    // (KV heads fastest: the workgroups of one XCD share a few heads' queries)
+    // KV heads fastest: the workgroups of one XCD share a few heads' queries.  Blocks
+    // slowest: the longest items first, and a place's items in a row are not one
+    // sequence's (30 x 300 tokens x 32 heads of 128 53 -> 43 us, 114 x 382 x 8 of 256
+    // 97 -> 75).  A last split is short: not always the same XCD's.
     int64_t id = blockIdx.x;
     const int g = int(id % G);
     id /= G;
-    const int split = int(id % a.splits);
+    const int turn = int(id % a.splits);
     id /= a.splits;
-    const int block = int(id % a.blocks);
-    const int64_t s = id / a.blocks, list = s * G + g;
+    const int block = int(id / a.b.nseq), split = int((turn + id) % a.splits);
+    const int64_t s = id % a.b.nseq, list = s * G + g;
     const Seq q = sequence(a, s);
     const int kb = block * M::KEYS;
     if (kb >= q.len) return;
     const int k0 = kb + wave * 16 * NB, w = a.x.window;
-    // The split's tokens, those of them that see a key of the block.
-    const int per = (q.n + a.splits - 1) / a.splits;
-    int ta = split * per, tb = ta + per < q.n ? ta + per : q.n;
-    ta = ta > kb - q.base ? ta : kb - q.base;
+    // The tokens that see a key of the block, and the split's of them: whole
+    // query tiles, of the heads of TPT tokens or 32 heads of one, so that a lane's
+    // row is the same token and head past the tile's first in each.
+    const int heads = hpg < 32 ? hpg : 32, TPT = 32 / heads, parts = (hpg + 31) / 32;
+    int from = kb > q.base ? kb - q.base : 0, until = q.n;
     // (token rows outside the batch's are nobody's)
-    if (q.tok < 0 && ta < -q.tok) ta = -q.tok;
-    if (tb > a.b.t - q.tok) tb = int(a.b.t - q.tok);
+    if (q.tok < 0 && from < -q.tok) from = -q.tok;
+    if (until > a.b.t - q.tok) until = int(a.b.t - q.tok);
     if (w > 0) {
         const int64_t end = int64_t(kb) + M::KEYS - 1 + w - q.base;  // own < key + w
-        if (tb > end) tb = int(end < 0 ? 0 : end);
+        if (until > end) until = int(end < 0 ? 0 : end);
     }
+    const int per = until > from ? (until - from + a.splits * TPT - 1) / (a.splits * TPT) * TPT : 0;
+    const int ta = from + split * per, tb = ta + per < until ? ta + per : until;
     float sum[E];  // of key 16 (e / 4) + 4 (lane / 16) + e % 4 of the wave's
 #pragma unroll
     for (int e = 0; e < E; ++e) sum[e] = 0.0f;
@@ -265,9 +269,6 @@ __global__ __launch_bounds__(256, 2) void weights_many_kernel(Args a) {
             for (int st = 0; st < NS; ++st)
                 kf[j][st] = p ? *reinterpret_cast<const frag*>(p + 32 * st + 8 * (lane / 16)) : z;
         }
-        // A query tile: the heads of TPT tokens, or 32 heads of one, so that a
-        // lane's row is the same token and head past the tile's first in each.
-        const int heads = hpg < 32 ? hpg : 32, TPT = 32 / heads, parts = (hpg + 31) / 32;
         const int have = tb - ta, ntile = (have + TPT - 1) / TPT * parts;
         const int64_t tok0 = q.tok + ta;
         const char* qb = reinterpret_cast<const char*>(static_cast<const T*>(a.x.q) + tok0 * a.x.ldq + int64_t(g) * hpg * D);
@@ -452,32 +453,29 @@ bool few(const PagedKv& kv, const PagedBatch& b, int heads) { return b.t * (head
 
 int many_keys(int head_dim) { return head_dim == 512 ? 128 : 256; }
 
-// The splits of the queries of least time, by the rounds in which the places
-// that the chip has take the items with something to do (keys near a prompt's
-// end have few queries) and an item's tiles, three more for its start and end,
-// for sequences of the mean number of tokens; of several, three quarters of the
-// items, since most are shorter than the table.  (8,000 tokens x 8 heads of 256 on
-// 4 KV heads: 4 / 7 / 16 / 32 splits 220 / 161 / 189 / 183 us, 7 is what this gives;
-// 600 x 8 of 512 on one, 150 tiles: 8 / 16 / 48 38 / 25 / 18; 9 x 200 tokens x 15 of 64
-// on 5: 1 / 2 / 8 / 32 29 / 20 / 14 / 18; 6 x 772 x 8 of 256 on 4, ragged: 1 / 3 / 12 67 / 44
-// / 64.)
+// The splits of a key block's queries of least time: the longest item's tiles,
+// four more for its start and end, or all items' over the places that the chip
+// has and a quarter of one at the launch's end; for sequences of the mean number of
+// tokens, and of several three quarters of the items, since most are shorter than
+// the table.  (A split takes its part of the tokens that see the block, so that late
+// blocks' items, which come last, are short: of all tokens, 4,096 x 32 heads of 128
+// 127 us for 100, 8,000 x 8 of 256 on 4 KV heads 161 for 145.  Those 8,000: 4 / 6 / 10
+// / 16 / 32 splits 174 / 144 / 146 / 147 / 169, 10 is what this gives; 600 x 8 of 512 on
+// one: 8 / 16 / 48 37 / 25 / 18; 9 x 200 x 15 of 64 on 5: 1 / 2 / 8 / 48 30 / 21 / 14 / 18.)
 int splits(const PagedKv& kv, const PagedBatch& b, int heads) {
     if (few(kv, b, heads)) return 1;
     const int64_t max_len = b.max_pages * kv.page, keys = many_keys(kv.head_dim), blocks = (max_len + keys - 1) / keys;
     const int64_t n = (b.t + b.nseq - 1) / b.nseq, tiles = (n * (heads / kv.kv_heads) + 31) / 32;
-    const int64_t base = max_len - n, places = kv.head_dim == 64 ? 1024 : kv.head_dim == 128 ? 768 : 512;
+    // Blocks before the new tokens are seen by all of them, others by half.
+    const double seen = (blocks + double(std::max<int64_t>(max_len - n, 0)) / keys) / 2 * tiles, share = b.nseq > 1 ? 0.75 : 1.0;
+    const double per_place = share * b.nseq * kv.kv_heads / (kv.head_dim == 64 ? 1024 : kv.head_dim == 128 ? 768 : 512);
     const double tile_us = 0.4 + kv.head_dim * 0.0057;
     int best = 1;
     double best_us = 1e30;
     for (const int k : {1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 14, 16, 20, 24, 32, 48}) {
         if (tiles < k) break;
-        // Split c has tokens up to (c + 1) n / k, which see blocks up to theirs.
-        int64_t items = 0;
-        for (int c = 0; c < k; ++c) items += std::min(blocks, (base + (c + 1) * n / k) / keys + 1);
-        items *= b.nseq * kv.kv_heads;
-        if (b.nseq > 1) items -= items / 4;
-        const double rounds = double((items + places - 1) / places);
-        const double us = rounds * (double((tiles + k - 1) / k) + 3) * tile_us + (k > 1 ? 5 + 0.2 * k : 0);
+        const double longest = double((tiles + k - 1) / k) + 4, all = (seen + 4.0 * k * blocks) * per_place;
+        const double us = std::max(longest, all + longest / 4) * tile_us + (k > 1 ? 5 + 0.1 * k : 0);
         if (us < best_us) best_us = us, best = k;
     }
     return best;
