@@ -830,6 +830,7 @@ __global__ __launch_bounds__(NW * 64, TILE == WAVES_KEYS && D == 512 ? 1 : D == 
         C core;
         core.init(r.valid ? static_cast<const T*>(a.x.q) + tok * a.x.ldq + int64_t(head) * D : nullptr, lane);
         const Stream<T, D, TILE> st{a, g, wave, lane, smem};
+        [[maybe_unused]] int wb = 0, we = 0;  // MASKED with a window: the split's prefix keys
         if (whole || split < a.p.np) {
             int kb = whole ? 0 : split * a.p.chunk_p, ke = whole ? P : imin(P, kb + a.p.chunk_p);
             const int lo = first_seen(P, r.own, w);
@@ -840,7 +841,14 @@ __global__ __launch_bounds__(NW * 64, TILE == WAVES_KEYS && D == 512 ? 1 : D == 
                 __syncthreads();
                 if (r.valid) atomicMin(&first, lo);
                 __syncthreads();
-                kb = imax(kb, first == INT_MAX ? ke : first / 32 * 32);
+                if constexpr (MASKED) {
+                    // (what the tile sees of the prefix is split, not the prefix)
+                    const int from = uni(first == INT_MAX ? P : imin(P, first / 32 * 32));
+                    const int chunk = whole ? P - from : ((P - from + a.p.np - 1) / a.p.np + 31) / 32 * 32;
+                    wb = kb = imin(P, from + (whole ? 0 : split * chunk)), we = ke = imin(P, kb + chunk);
+                } else {
+                    kb = imax(kb, first == INT_MAX ? ke : first / 32 * 32);
+                }
                 __syncthreads();
             }
             if (kb < ke) st.run(core, a.b.prefix_table, (P - 1) >> a.page_shift, kb, ke, P, r.valid, lo, P);
@@ -876,6 +884,7 @@ __global__ __launch_bounds__(NW * 64, TILE == WAVES_KEYS && D == 512 ? 1 : D == 
         Keys in{g, 0, 0, 0, 0};
         if (whole || split < a.p.np)
             in.pb = whole ? 0 : split * a.p.chunk_p, in.pe = whole ? P : imin(P, in.pb + a.p.chunk_p);
+        if (MASKED && w > 0) in.pb = wb, in.pe = we;
         if (fused && (whole || split >= a.p.np))
             in.ob = whole ? 0 : (split - a.p.np) * a.p.chunk_o, in.oe = whole ? cap : imin(cap, in.ob + a.p.chunk_o);
         auto alone = [&](uint64_t rows, float lg) {

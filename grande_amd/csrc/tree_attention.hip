@@ -24,9 +24,14 @@ namespace {
 // for 2,100 tokens x 8 heads of 256, 132 items, 459 us, three 189; the best at 16
 // rows a wave 280.  70 tokens x 4 heads on 2,000 keys 17 us at 32 rows, 13 at
 // 16.)
-Plan plan_tree(const PagedKv& kv, const PagedBatch& b, int heads) {
+//
+// With a window the prefix counts as far as it reaches, in at most `most` slots (a
+// workspace's size does not hang on the window): 20 trees of 21 tokens x 15 heads of
+// 64 on 14,304 keys at 1,024 40 -> 24 us, where the splits were the prefix's.
+Plan plan_tree(const PagedKv& kv, const PagedBatch& b, int heads, int window = 0, int64_t most = INT64_MAX) {
     const Plan from = plan(kv, b, heads);
-    const int64_t hpg = heads / kv.kv_heads, rows = b.t * hpg, max_len = b.max_pages * kv.page, P = b.prefix_len;
+    const int64_t hpg = heads / kv.kv_heads, rows = b.t * hpg, max_len = b.max_pages * kv.page;
+    const int64_t P = window > 0 ? std::min<int64_t>(b.prefix_len, window) : b.prefix_len;
     const int D = kv.head_dim;
     const double slot_us = double(b.t) * heads * D * 8 / 4.5e6;
     auto chunk = [](int64_t keys, int64_t n) { return up((keys + n - 1) / n, 32); };
@@ -44,9 +49,10 @@ Plan plan_tree(const PagedKv& kv, const PagedBatch& b, int heads) {
         const double tile_us = (0.7 + D / 240.0) * (tile == WAVES_16 ? 0.55 : 1.0);
         const int64_t places = 256 * (D == 64 ? 4 : D == 128 ? 3 : D == 512 && !q.fused ? 1 : 2);
         auto tiles = [&](int64_t keys) { return double((keys + KT - 1) / KT) + 2; };
-        auto take = [&](const Plan& p, double most) {
+        auto take = [&](const Plan& p, double longest) {
             const int64_t nsplit = p.whole ? 1 : p.np + (p.fused ? p.os : 0);
-            const double us = double((base * nsplit + places - 1) / places) * most * tile_us +
+            if (p.slots() > most) return;
+            const double us = double((base * nsplit + places - 1) / places) * longest * tile_us +
                               (p.slots() > 1 ? 3.0 + slot_us * p.slots() : 0.0);
             if (us < best_us) best_us = us, best = p;
         };
@@ -91,7 +97,11 @@ void launch_attention_tree(hipStream_t s, const PagedKv& kv, const PagedBatch& b
     if (tree.words <= 0 || tree.words > (1 << 20)) fail(E_INVALID, "attention_tree: mask_ld must be 1 to 2^20 words");
     if (x.window > 0 && !tree.positions) fail(E_INVALID, "attention_tree: a window needs the tokens' positions");
     if (reinterpret_cast<uintptr_t>(tree.positions) % 4) fail(E_INVALID, "attention_tree: positions must be 4-byte aligned");
-    launch_attention<true>(s, kv, b, x, tree, plan_tree, workspace, bytes, "attention_tree");
+    auto planned = [&](const PagedKv& kv, const PagedBatch& b, int heads) {
+        const Plan p = plan_tree(kv, b, heads);
+        return x.window > 0 && p.tile != WAVES_KEYS ? plan_tree(kv, b, heads, x.window, p.slots()) : p;
+    };
+    launch_attention<true>(s, kv, b, x, tree, planned, workspace, bytes, "attention_tree");
 }
 
 }  // namespace omg

@@ -168,6 +168,25 @@ def test_windows_count_back_from_the_positions(heads, kv_heads, hd, new, before,
     TreeCall(rng, new, before, 0, heads, kv_heads, hd, window=window, bits=random_bits).run().check()
 
 
+@pytest.mark.parametrize("window", [1, 100, 700, 10_000])
+@pytest.mark.parametrize("heads,kv_heads,hd,new,before", [(4, 1, 256, [3, 9, 1], [40, 0, 130]), (8, 2, 64, [61, 40, 20], [5, 300, 0]),
+                                                          (8, 1, 512, [5, 7], [20, 9]), (16, 2, 128, [33] * 30, [3] * 30)])
+def test_windows_at_the_end_of_long_prefixes(heads, kv_heads, hd, new, before, window):
+    """The splits share out what a tile sees, from near its end to all of it; sums that f32 does not hold too."""
+    rng = np.random.default_rng(window + hd)
+    c = TreeCall(rng, new, before, 5003, heads, kv_heads, hd, window=window, dtype="bf16", page=64)
+    c.run().check()
+    for s in range(0, len(new), 2):  # (positions that lie far back see more)
+        c.pos_host[s] = c.pos_host[s] - rng.integers(0, 6000, len(c.pos_host[s]))
+    c.positions.copy_(torch.from_numpy(np.concatenate(c.pos_host).astype(np.int32)))
+    c.run().check("far back")
+    c.pool.v_raw.fill_(3.0e38)
+    c.run()
+    torch.cuda.synchronize()
+    v = float(torch.tensor(3.0e38, dtype=torch.bfloat16).double())
+    assert bool(((c.out[:, :heads * hd].double() - v).abs() <= 2 * half_step(torch.bfloat16) * v).all())
+
+
 def test_single_tokens_without_start():
     rng = np.random.default_rng(5)
     c = TreeCall(rng, [1] * 7, rng.integers(0, 50, 7), 20, 4, 2, 128, bits=random_bits)
