@@ -103,16 +103,18 @@ struct BlockArgs {
 };
 
 // 16 tokens (of any sequences: prefix blocks; of one: its own) x 64 blocks, 16
-// a wave.  The queries' sums lie in LDS in the order in which the lanes take
-// them: lane l of a step holds token l % 16 and dims of the quarter l / 16 of
-// the head, and blocks' means likewise, a run of 16 bytes at a time.  Bound by
-// the f64 products and the loads' latency before them: 64 tokens x 8 KV heads of
-// 128 on some 1,050 blocks 11.9 us, 12 x 4 of 256 on 126 8.1 us (its second half of
-// the means asked for behind the first half's products 8.7).
-template <typename T, int D>
+// a wave; FEW: x 16, a quarter of the head dims a wave.  The queries' sums lie in
+// LDS in the order in which the lanes take them: lane l of a step holds token l %
+// 16 and dims of the quarter l / 16 of the head, and blocks' means likewise, a run
+// of 16 bytes at a time.  Bound by the f64 products and the loads' latency before
+// them: 64 tokens x 8 KV heads of 128 on some 1,050 blocks 12 us, 12 x 4 of 256 on
+// 126 5.9.
+template <typename T, int D, bool FEW>
 __global__ __launch_bounds__(256) void block_scores_kernel(BlockArgs x) {
-    constexpr int Q = D / 4, DC = Q < 64 ? Q : 64;  // dims of a quarter, of them in LDS at once
-    __shared__ double qs[DC * WAVE];
+    constexpr int Q = D / 4, QW = FEW ? Q / 4 : Q;  // dims of a quarter, of them a wave's
+    constexpr int DC = FEW || Q < 64 ? Q : 64;      // of a quarter in LDS at once
+    constexpr int BW = FEW ? 16 : 64;               // blocks
+    __shared__ double qs[DC * WAVE > 1024 ? DC * WAVE : 1024];
     const Args& a = x.a;
     const int tid = int(threadIdx.x), lane = tid % WAVE, wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
     const int G = a.kv.kv_heads;
@@ -123,9 +125,9 @@ __global__ __launch_bounds__(256) void block_scores_kernel(BlockArgs x) {
     int64_t t0, t1, b0, nblocks, first;
     const int32_t* table;
     if (id < x.prefix_items) {
-        const int64_t chunks = (x.np + 63) / 64;
+        const int64_t chunks = (x.np + BW - 1) / BW;
         t0 = id / chunks * 16, t1 = t0 + 16 < a.b.t ? t0 + 16 : a.b.t;
-        b0 = id % chunks * 64, nblocks = x.np, first = 0, table = a.b.prefix_table;
+        b0 = id % chunks * BW, nblocks = x.np, first = 0, table = a.b.prefix_table;
     } else {
         id -= x.prefix_items;
         const int64_t i = id / x.own_chunks;
@@ -152,53 +154,61 @@ __global__ __launch_bounds__(256) void block_scores_kernel(BlockArgs x) {
         // (blocks up to the last token's own have a score that counts)
         const int64_t row = int64_t(a.b.lens[s]) - (end - (t1 - 1));
         const int64_t have = row < 0 ? 0 : (row >> a.page_shift) + 1;
-        b0 = id % x.own_chunks * 64, nblocks = have < a.b.max_pages ? have : a.b.max_pages, first = x.np;
+        b0 = id % x.own_chunks * BW, nblocks = have < a.b.max_pages ? have : a.b.max_pages, first = x.np;
         table = a.b.table + s * a.b.table_ld;
     }
     if (b0 >= nblocks) return;
-    const int64_t mine = b0 + wave * 16 + lane % 16;  // the block whose means the lane loads
+    b0 += FEW ? 0 : wave * 16;             // the wave's
+    const int64_t mine = b0 + lane % 16;  // the block whose means the lane loads
     const int64_t p = mine < nblocks ? table[mine] : -1;
     const bool there = p >= 0 && p < a.kv.npages;
-    const float* mean = x.means + ((there ? p : 0) * G + g) * D + lane / 16 * Q;
-    doublex4 acc = {0.0, 0.0, 0.0, 0.0};
     // (a page that is not there: the first page's means, and no score from them)
-    constexpr int N = DC < 32 ? DC : 32;  // dims whose means are under way
+    const float* mean = x.means + ((there ? p : 0) * G + g) * D + lane / 16 * Q + (FEW ? wave * QW : 0);
+    constexpr int N = QW < 32 ? QW : 32;  // dims whose means are under way
     float4 m[N / 4];
 #pragma unroll
     for (int d = 0; d < N; d += 4) m[d / 4] = *reinterpret_cast<const float4*>(mean + d);
+    doublex4 acc = {0.0, 0.0, 0.0, 0.0};
     for (int c = 0; c < Q; c += DC) {
         if (c) __syncthreads();
-        // A thread sums 8 dims of a token at a time over the heads.
-        for (int i = tid; i < 16 * 4 * (DC / 8); i += 256) {
-            const int tok = i % 16, quarter = i / 16 % 4, d = i / 64 * 8;
-            double sum[8] = {};
-            if (t0 + tok >= 0 && t0 + tok < t1) {
-                const T* q = static_cast<const T*>(a.x.q) + (t0 + tok) * a.x.ldq + int64_t(g) * a.hpg * D + quarter * Q + c + d;
-                for (int h0 = 0; h0 < a.hpg; h0 += 4) {
-                    float v[4][8];
+        // A thread sums 8 dims of a token over the heads, IT times.
+        constexpr int IT = DC < 32 ? 1 : DC / 32, HB = IT < 4 ? 4 : 2;
+        const int tok = tid % 16, quarter = tid / 16 % 4;
+        double sum[IT][8] = {};
+        if (t0 + tok >= 0 && t0 + tok < t1 && wave * 8 < DC) {
+            const T* q = static_cast<const T*>(a.x.q) + (t0 + tok) * a.x.ldq + int64_t(g) * a.hpg * D + quarter * Q + c + wave * 8;
+            for (int h0 = 0; h0 < a.hpg; h0 += HB) {
+                float v[IT][HB][8];
 #pragma unroll
-                    for (int h = 0; h < 4; ++h) load8(q + int64_t(h0 + h < a.hpg ? h0 + h : h0) * D, v[h]);
+                for (int i = 0; i < IT; ++i)
 #pragma unroll
-                    for (int h = 0; h < 4; ++h)
+                    for (int h = 0; h < HB; ++h) load8(q + int64_t(h0 + h < a.hpg ? h0 + h : h0) * D + 32 * i, v[i][h]);
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) sum[e] += h0 + h < a.hpg ? double(v[h][e]) : 0.0;
-                }
+                for (int i = 0; i < IT; ++i)
+#pragma unroll
+                    for (int h = 0; h < HB; ++h)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) sum[i][e] += h0 + h < a.hpg ? double(v[i][h][e]) : 0.0;
             }
+        }
+        if (wave * 8 < DC) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) qs[(d + e) * WAVE + quarter * 16 + tok] = sum[e];
+            for (int i = 0; i < IT; ++i)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) qs[(wave * 8 + 32 * i + e) * WAVE + quarter * 16 + tok] = sum[i][e];
         }
         __syncthreads();
 #pragma unroll
-        for (int d0 = 0; d0 < DC; d0 += N) {
+        for (int d0 = 0; d0 < (FEW ? QW : DC); d0 += N) {
             float4 next[N / 4];
-            const bool more = c + d0 + N < Q;
+            const bool more = c + d0 + N < QW;
             if (more) {
 #pragma unroll
                 for (int d = 0; d < N; d += 4) next[d / 4] = *reinterpret_cast<const float4*>(mean + c + d0 + N + d);
             }
 #pragma unroll
             for (int d = 0; d < N; d += 4) {
-                const double* q = qs + (d0 + d) * WAVE + lane;
+                const double* q = qs + ((FEW ? wave * QW : 0) + d0 + d) * WAVE + lane;
                 acc = __builtin_amdgcn_mfma_f64_16x16x4f64(double(m[d / 4].x), q[0], acc, 0, 0, 0);
                 acc = __builtin_amdgcn_mfma_f64_16x16x4f64(double(m[d / 4].y), q[WAVE], acc, 0, 0, 0);
                 acc = __builtin_amdgcn_mfma_f64_16x16x4f64(double(m[d / 4].z), q[2 * WAVE], acc, 0, 0, 0);
@@ -210,15 +220,26 @@ __global__ __launch_bounds__(256) void block_scores_kernel(BlockArgs x) {
             }
         }
     }
-    // The lane has blocks 4 r + lane / 16 of the wave's, token lane % 16.
+    // The lane has blocks 4 r + lane / 16 of the wave's, token lane % 16; FEW: the
+    // sum of all waves' for r = wave.
+    if constexpr (FEW) {
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < 4; ++r) qs[(wave * 4 + r) * WAVE + lane] = acc[r];
+        __syncthreads();
+        double v = 0.0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v += qs[(i * 4 + wave) * WAVE + lane];
+        acc[0] = v;
+    }
     const uint64_t gone = __ballot(!there) & 0xffff;
     const int64_t tok = t0 + lane % 16;
     if (tok < 0 || tok >= t1) return;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const int64_t b = b0 + wave * 16 + 4 * r + lane / 16;
-        if (b < nblocks)
-            x.scores[(tok * G + g) * x.blocks_ld + first + b] = gone >> (4 * r + lane / 16) & 1 ? 0.0f : float(acc[r]);
+    for (int i = 0; i < (FEW ? 1 : 4); ++i) {
+        const int of = 4 * (FEW ? wave : i) + lane / 16;
+        if (b0 + of < nblocks)
+            x.scores[(tok * G + g) * x.blocks_ld + first + b0 + of] = gone >> of & 1 ? 0.0f : float(acc[i]);
     }
 }
 
@@ -410,14 +431,24 @@ void launch_chosen(hipStream_t s, const BlockArgs& x, int64_t items) {
 }
 
 template <typename T, int D>
-void launch_blocks_d(hipStream_t s, BlockArgs x, int64_t own_tiles, int32_t* room) {
+void launch_blocks_d(hipStream_t s, BlockArgs x, int32_t* room) {
     const Args& a = x.a;
     const int64_t lists = a.b.t * a.kv.kv_heads;
-    const int64_t scored = (x.prefix_items + own_tiles * x.own_chunks) * a.kv.kv_heads;
     const int64_t items = lists * a.p.os * ((a.hpg + 15) / 16);
-    if (scored >= MAX_BLOCKS || items >= MAX_BLOCKS || lists >= MAX_BLOCKS)
+    const int64_t own_tiles = a.b.start ? a.b.t / 16 + a.b.nseq : a.b.nseq;
+    auto scored = [&](int blocks) {  // items of so many blocks each
+        x.prefix_items = (a.b.t + 15) / 16 * ((x.np + blocks - 1) / blocks);
+        x.own_chunks = (a.b.max_pages + blocks - 1) / blocks;
+        return (x.prefix_items + own_tiles * x.own_chunks) * a.kv.kv_heads;
+    };
+    // (56 items for 12 x 4 lists of 126 blocks, 256-wide, 8.1 us, of 16 blocks 5.8; 304
+    // 10.6 and 7.0, 768 14.0 and 14.1; 1,024 of 128-wide heads 11.8 and 15.)
+    const bool few = scored(64) < 768;
+    const int64_t scores = scored(few ? 16 : 64);
+    if (scores >= MAX_BLOCKS || items >= MAX_BLOCKS || lists >= MAX_BLOCKS)
         fail(E_CAPACITY, "attention_blocks: too many work items");
-    block_scores_kernel<T, D><<<dim3(unsigned(scored)), dim3(256), 0, s>>>(x);
+    few ? block_scores_kernel<T, D, true><<<dim3(unsigned(scores)), dim3(256), 0, s>>>(x)
+        : block_scores_kernel<T, D, false><<<dim3(unsigned(scores)), dim3(256), 0, s>>>(x);
     OMG_HIP(hipGetLastError());
     // Work items that the chip takes at once choose for themselves (12 x 4 lists of
     // 126 blocks: 18 us for 15.5 and 6, 512 of 1,050: 87 for 82 and 9).  More of them
@@ -443,12 +474,12 @@ void launch_blocks_d(hipStream_t s, BlockArgs x, int64_t own_tiles, int32_t* roo
 }
 
 template <typename T>
-void launch_blocks_t(hipStream_t s, const BlockArgs& x, int64_t own_tiles, int32_t* room) {
+void launch_blocks_t(hipStream_t s, const BlockArgs& x, int32_t* room) {
     switch (x.a.kv.head_dim) {
-        case 64: return launch_blocks_d<T, 64>(s, x, own_tiles, room);
-        case 128: return launch_blocks_d<T, 128>(s, x, own_tiles, room);
-        case 256: return launch_blocks_d<T, 256>(s, x, own_tiles, room);
-        default: return launch_blocks_d<T, 512>(s, x, own_tiles, room);
+        case 64: return launch_blocks_d<T, 64>(s, x, room);
+        case 128: return launch_blocks_d<T, 128>(s, x, room);
+        case 256: return launch_blocks_d<T, 256>(s, x, room);
+        default: return launch_blocks_d<T, 512>(s, x, room);
     }
 }
 
@@ -507,11 +538,8 @@ void launch_attention_blocks(hipStream_t s, const PagedKv& kv, const PagedBatch&
     k.scores = reinterpret_cast<float*>(room), k.blocks_ld = p.blocks;
     k.chosen = chosen;
     k.keep = int(keep), k.np = int(p.np), k.chunk = p.chunk;
-    k.prefix_items = (b.t + 15) / 16 * ((p.np + 63) / 64);
-    k.own_chunks = (b.max_pages + 63) / 64;
-    const int64_t own_tiles = b.start ? b.t / 16 + b.nseq : b.nseq;
     int32_t* list = reinterpret_cast<int32_t*>(room + p.scores);
-    kv.dtype == ELEM_F16 ? launch_blocks_t<half_t>(s, k, own_tiles, list) : launch_blocks_t<bf16_t>(s, k, own_tiles, list);
+    kv.dtype == ELEM_F16 ? launch_blocks_t<half_t>(s, k, list) : launch_blocks_t<bf16_t>(s, k, list);
 }
 
 }  // namespace omg

@@ -248,6 +248,16 @@ def test_as_many_lists_as_the_chip_takes_at_once_and_more(nseq, kv_heads, hd, bl
     BlockCall(rng, [1] * nseq, rng.integers(0, 60, nseq), 90, kv_heads, kv_heads, hd, blocks).all_means().run().check()
 
 
+@pytest.mark.parametrize("hd", [64, 128, 256, 512])
+@pytest.mark.parametrize("new", [[1] * 100, [20, 1, 3] * 33])
+def test_many_scores(new, hd):
+    """Launches of so many scores that a workgroup takes 64 blocks: the prefix's and sequences' of more than 64."""
+    rng = np.random.default_rng(hd + len(new))
+    before = rng.integers(0, 60, len(new))
+    before[7] = 1200
+    BlockCall(rng, new, before, 1100, 8, 8, hd, 4, dtype="bf16").all_means().run().check()
+
+
 @pytest.mark.parametrize("give", [True, False])
 @pytest.mark.parametrize("prefix", [251 * 16, 252 * 16 + 3, 2043 * 16 + 1, 2044 * 16 + 1])
 def test_numbers_of_blocks_at_which_the_choice_changes(prefix, give):
