@@ -396,7 +396,8 @@ void check_blocks(const PagedKv& kv, const PagedBatch& b, int heads, int64_t kee
 int64_t places(int head_dim) { return 256 * (head_dim == 64 ? 4 : head_dim == 512 ? 1 : 2); }
 
 // Entries are split over work items until these fill the chip's places,
-// at least two at a time and at most a lane each.  (Lists of one token
+// at least 128 rows at a time and at most an entry a lane.  (26 blocks of 128 rows of
+// 512: 13 items' launches 36 us in all, 26 32; 64 of 64 x 128 28 and 24.  Lists of one token
 // each that start together stay together, and what one reads the next finds in
 // L2: 512 lists as 1,024 items 116 us, as 512 82.)
 BlockPlan plan_blocks(const PagedKv& kv, const PagedBatch& b, int heads, int64_t keep) {
@@ -404,7 +405,7 @@ BlockPlan plan_blocks(const PagedKv& kv, const PagedBatch& b, int heads, int64_t
     p.np = (b.prefix_len + kv.page - 1) / kv.page;
     p.blocks = p.np + b.max_pages;
     const int64_t hpg = heads / kv.kv_heads, items = b.t * kv.kv_heads * ((hpg + 15) / 16);
-    const int64_t least = (keep + 63) / 64, most = std::min<int64_t>(64, (keep + 1) / 2);
+    const int64_t least = (keep + 63) / 64, most = std::min<int64_t>(64, std::max<int64_t>(1, keep * kv.page / 128));
     const int64_t want = std::max(least, std::min(most, places(kv.head_dim) / items));
     p.chunk = int((keep + want - 1) / want);
     p.splits = int((keep + p.chunk - 1) / p.chunk);
