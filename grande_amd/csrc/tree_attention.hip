@@ -4,11 +4,11 @@
 // masks (a word or two a lane, asked for a tile ahead).  Measured, and what bounds it:
 //   12 drafts of 4 to 8 tokens x 4 heads of 256 on 2,000 shared keys (f16): 12.4 us
 //     and the join's 4: latency.
-//   208 of 7 to 13 tokens x 8 heads of 256 on 8,000: 195 us and 17 for three slots'
-//     join alone, 197 in a row, 690 TFLOP/s: a wave's chain of product, softmax and
+//   208 of 7 to 13 tokens x 8 heads of 256 on 8,000: 195 us and 17 for the slots'
+//     join alone, 192 in a row, 710 TFLOP/s: a wave's chain of product, softmax and
 //     product, two waves a SIMD.
-//   16 trees of 31 to 61 tokens x 32 heads of 128 on 32,749 (bf16): 566 us and 22, 553
-//     in a row, 770 TFLOP/s: vector instructions 50 %, MFMAs 43 % of the SIMDs' cycles.
+//   16 trees of 31 to 61 tokens x 32 heads of 128 on 32,749 (bf16): 567 us and 17, 517
+//     in a row, 820 TFLOP/s: vector instructions 50 %, MFMAs 43 % of the SIMDs' cycles.
 #include "shared_attention.h"
 
 namespace omg {
@@ -18,8 +18,10 @@ namespace {
 // The tile and the splits of least time by a model of the launch: a work item
 // takes so long a tile of keys (a chain of dependent steps: hardly longer with
 // two or three workgroups on the CU) and two tiles' time besides; the places
-// that the chip has take items in rounds; a slot of partial results is written
-// and read.  Measured, for 32 and 16 rows a wave: 1.76 and 0.97 us a tile of
+// that the chip has take items one after the other, the last ones of them for half
+// a round (a whole round: 90 trees of 26 tokens x 32 heads of 128 on 1,323 + 590 keys in
+// three splits' rounds 172 us, in one item each 130); a slot of partial results is
+// written and read.  Measured, for 32 and 16 rows a wave: 1.76 and 0.97 us a tile of
 // 256-wide heads, 1.24 and 0.67 of 128-wide ones.  (One split of the 8,000 keys
 // for 2,100 tokens x 8 heads of 256, 132 items, 459 us, three 189; the best at 16
 // rows a wave 280.  70 tokens x 4 heads on 2,000 keys 17 us at 32 rows, 13 at
@@ -52,8 +54,8 @@ Plan plan_tree(const PagedKv& kv, const PagedBatch& b, int heads, int window = 0
         auto take = [&](const Plan& p, double longest) {
             const int64_t nsplit = p.whole ? 1 : p.np + (p.fused ? p.os : 0);
             if (p.slots() > most) return;
-            const double us = double((base * nsplit + places - 1) / places) * longest * tile_us +
-                              (p.slots() > 1 ? 3.0 + slot_us * p.slots() : 0.0);
+            const double full = double(base * nsplit) / places, rounds = full > 1.0 ? full + 0.5 : 1.0;
+            const double us = rounds * longest * tile_us + (p.slots() > 1 ? 3.0 + slot_us * p.slots() : 0.0);
             if (us < best_us) best_us = us, best = p;
         };
         if (!q.fused) {  // (the own keys' items as they are)
