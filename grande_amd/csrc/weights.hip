@@ -215,6 +215,79 @@ __device__ inline void wait_loads() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
 }
 
+// A work item: the key block of KEYS rows from kb on of a list, and the tokens [ta, tb) of
+// the sequence's, its split's of those that see a key of the block.
+struct Item {
+    int g, kb, split, ta, tb;
+    int64_t s, list;
+    Seq q;
+};
+template <int KEYS>
+__device__ inline Item item(const Args& a, int64_t id) {
+    Item x;
+    // KV heads fastest: the workgroups of one XCD share a few heads' queries.  Blocks
+    // slowest: the longest items first, and a place's items in a row are not one
+    // sequence's (30 x 300 tokens x 32 heads of 128 53 -> 43 us, 114 x 382 x 8 of 256
+    // 97 -> 75).  A last split is short: not always the same XCD's.
+    const int G = a.kv.kv_heads;
+    x.g = int(id % G);
+    id /= G;
+    const int turn = int(id % a.splits);
+    id /= a.splits;
+    x.kb = int(id / a.b.nseq) * KEYS, x.split = int((turn + id) % a.splits);
+    x.s = id % a.b.nseq, x.list = x.s * G + x.g;
+    x.q = sequence(a, x.s);
+    const int w = a.x.window, tile = 32 / (a.hpg < 32 ? a.hpg : 32);  // whole query tiles
+    int from = x.kb > x.q.base ? x.kb - x.q.base : 0, until = x.q.n;
+    // (token rows outside the batch's are nobody's)
+    if (x.q.tok < 0 && from < -x.q.tok) from = -x.q.tok;
+    if (until > a.b.t - x.q.tok) until = int(a.b.t - x.q.tok);
+    if (w > 0) {
+        const int64_t end = int64_t(x.kb) + KEYS - 1 + w - x.q.base;  // own < key + w
+        if (until > end) until = int(end < 0 ? 0 : end);
+    }
+    const int per = until > from ? (until - from + a.splits * tile - 1) / (a.splits * tile) * tile : 0;
+    x.ta = from + x.split * per, x.tb = x.ta + per < until ? x.ta + per : until;
+    return x;
+}
+
+// What a key gathers in a work item, with a row a lane and no row that does not see it:
+// until the sum is NaN.
+template <typename T, int D>
+__device__ inline float key_alone(int key, int lane) {
+    // (the item from the launch's arguments again: no register holds any of it until
+    // here; with them held, 8,000 tokens at a window of 512 took 56 us for 53)
+    uint64_t args = reinterpret_cast<uint64_t>(__builtin_amdgcn_kernarg_segment_ptr());
+    int id = int(blockIdx.x);
+    asm volatile("" : "+s"(args), "+s"(id));
+    const Args& a = *reinterpret_cast<const Args*>(args);
+    const Item it = item<Many<T, D>::KEYS>(a, id);
+    const T* k = key_row<T>(a, a.b.table + it.s * a.b.table_ld, key, it.g, D);
+    if (!k) return 0.0f;
+    float sum = 0.0f;
+#pragma unroll 1
+    for (int64_t r0 = int64_t(it.ta) * a.hpg, end = int64_t(it.tb) * a.hpg; r0 < end; r0 += WAVE) {
+        const int64_t r = r0 + lane, tok = r / a.hpg, own = it.q.base + tok, at = it.q.tok + tok;
+        const int head = it.g * a.hpg + int(r - tok * a.hpg);
+        const bool see = r < end && key <= own && (a.x.window == 0 || own - key < a.x.window);
+        const float nl = see ? negated(a.x.lse[at * a.x.heads + head]) : -INFINITY;
+        if (nl != -INFINITY) {
+            const T* x = static_cast<const T*>(a.x.q) + at * a.x.ldq + int64_t(head) * D;
+            float s = 0.0f;
+#pragma unroll 4
+            for (int c = 0; c < D; c += 8) {
+                float u[8], v[8];
+                load8(x + c, u), load8(k + c, v);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) s = fmaf(u[i], v[i], s);
+            }
+            sum += prob(s, a.x.scale, nl);
+        }
+        if (__any(sum != sum)) break;
+    }
+    return wave_sum(sum);
+}
+
 template <typename T, int D>
 __global__ __launch_bounds__(256, 2) void weights_many_kernel(Args a) {
     typedef typename Vec8<T>::type frag;
@@ -224,40 +297,17 @@ __global__ __launch_bounds__(256, 2) void weights_many_kernel(Args a) {
     T* smem = reinterpret_cast<T*>(smem_raw);  // BUFS query tiles
     float* log_sums = reinterpret_cast<float*>(smem_raw + M::BUFS * M::TILE * 2);  // [BUFS][4][64]
     const int lane = int(threadIdx.x) % WAVE, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / WAVE);
-    const int G = a.kv.kv_heads, hpg = a.hpg;
-    // KV heads fastest: the workgroups of one XCD share a few heads' queries.  Blocks
-    // slowest: the longest items first, and a place's items in a row are not one
-    // sequence's (30 x 300 tokens x 32 heads of 128 53 -> 43 us, 114 x 382 x 8 of 256
-    // 97 -> 75).  A last split is short: not always the same XCD's.
-    int64_t id = blockIdx.x;
-    const int g = int(id % G);
-    id /= G;
-    const int turn = int(id % a.splits);
-    id /= a.splits;
-    const int block = int(id / a.b.nseq), split = int((turn + id) % a.splits);
-    const int64_t s = id % a.b.nseq, list = s * G + g;
-    const Seq q = sequence(a, s);
-    const int kb = block * M::KEYS;
-    if (kb >= q.len) return;
-    const int k0 = kb + wave * 16 * NB, w = a.x.window;
-    // The tokens that see a key of the block, and the split's of them: whole
-    // query tiles, of the heads of TPT tokens or 32 heads of one, so that a lane's
-    // row is the same token and head past the tile's first in each.
+    const Item it = item<M::KEYS>(a, blockIdx.x);
+    const Seq q = it.q;
+    if (it.kb >= q.len) return;
+    const int g = it.g, hpg = a.hpg, kb = it.kb, k0 = kb + wave * 16 * NB, w = a.x.window, ta = it.ta, tb = it.tb;
+    // Query tiles of the heads of TPT tokens or 32 heads of one, so that a lane's row
+    // is the same token and head past the tile's first in each.
     const int heads = hpg < 32 ? hpg : 32, TPT = 32 / heads, parts = (hpg + 31) / 32;
-    int from = kb > q.base ? kb - q.base : 0, until = q.n;
-    // (token rows outside the batch's are nobody's)
-    if (q.tok < 0 && from < -q.tok) from = -q.tok;
-    if (until > a.b.t - q.tok) until = int(a.b.t - q.tok);
-    if (w > 0) {
-        const int64_t end = int64_t(kb) + M::KEYS - 1 + w - q.base;  // own < key + w
-        if (until > end) until = int(end < 0 ? 0 : end);
-    }
-    const int per = until > from ? (until - from + a.splits * TPT - 1) / (a.splits * TPT) * TPT : 0;
-    const int ta = from + split * per, tb = ta + per < until ? ta + per : until;
     float sum[E];  // of key 16 (e / 4) + 4 (lane / 16) + e % 4 of the wave's
 #pragma unroll
     for (int e = 0; e < E; ++e) sum[e] = 0.0f;
-    const int32_t* table = a.b.table + s * a.b.table_ld;
+    const int32_t* table = a.b.table + it.s * a.b.table_ld;
     if (ta < tb) {
         frag kf[NB][NS];
 #pragma unroll
@@ -421,11 +471,22 @@ __global__ __launch_bounds__(256, 2) void weights_many_kernel(Args a) {
         mine = lane % 16 == e ? v : mine;
     }
     const int e = lane % 16, key = k0 + 16 * (e / 4) + 4 * (lane / 16) + e % 4;
+    // Tiles that see the whole block add up all their rows: a zero for one that no token
+    // has or whose token sees nothing, but NaN where its score is infinite or NaN (an
+    // infinite key's with a row of zeros is).  So a key whose sum is NaN is taken again:
+    // 4,096 tokens x 7 heads of 256 with one such key in 1,000 98 us for 69, with nothing
+    // else 5.0 ms, where they are NaN themselves 1.3 ms.  (A choice for each probability
+    // instead takes 2 % of 256-wide, 3 % of 128-wide and 7 % of 64-wide heads' time, always.)
+    for (uint64_t again = __ballot(e < E && key < q.len && mine != mine); again; again &= again - 1) {
+        const int from = __builtin_ctzll(again);
+        const float v = key_alone<T, D>(__builtin_amdgcn_readlane(key, from), lane);
+        mine = lane == from ? v : mine;
+    }
     if (e >= E || key >= q.len || !key_row<T>(a, table, key, g, D)) return;
     if (a.part)
-        a.part[(split * a.b.nseq * G + list) * a.max_len + key] = mine;
+        a.part[(it.split * a.b.nseq * a.kv.kv_heads + it.list) * a.max_len + key] = mine;
     else
-        a.x.weights[list * a.x.ldw + key] += mine;
+        a.x.weights[it.list * a.x.ldw + key] += mine;
 }
 
 // The splits' sums, in their order.

@@ -467,8 +467,9 @@ int omg_dev_attention_blocks(const omg_paged_kv *kv, const omg_paged_batch *b, i
  * lets them, window included) and the query heads of KV head h; lse [t][heads]
  * is what that call gave (its prefix keys in it; minus infinity: a token that
  * sees nothing).  f32 sums in an order that the shapes fix.  A row's weight
- * hears from its own key alone, infinite and NaN ones too; rows from lens[s] on
- * and on pages outside the pool keep theirs.  ldw at least max_pages * page.
+ * hears from its own key alone, infinite and NaN ones too (a key whose scores
+ * hold these may take its tokens again one by one: right, and slower); rows from
+ * lens[s] on and on pages outside the pool keep theirs.  ldw at least max_pages * page.
  * Sizes, scale and workspace as there; ldq at most 2^24. */
 int64_t omg_dev_attention_weights_workspace(const omg_paged_kv *kv, const omg_paged_batch *b, int heads);
 int omg_dev_attention_weights(const omg_paged_kv *kv, const omg_paged_batch *b, int heads, const void *q, int64_t ldq,

@@ -303,3 +303,25 @@ def test_weights_of_attentions_own_log_sums_add_up_to_the_tokens():
         exp = torch.from_numpy(np.repeat(np.asarray(new)[:, None] * 4.0, 2, 1))
         # lse is off by 1e-6 + 2^-19 size (|score| sums below 64 here), a weight's sum rounds 200 times
         assert bool(((got - exp).abs() <= exp * (2e-4 + 200 * 2.0 ** -22)).all())
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads,hd", [(3, 1, 64), (8, 2, 128), (6, 2, 256), (7, 1, 512), (5, 5, 128), (40, 1, 64)])
+@pytest.mark.parametrize("new,before,window", [([1, 1, 1], [700, 3, 290], 0), ([701], [0], 0), ([650, 3, 667], [9, 290, 40], 0),
+                                               ([703, 690], [0, 33], 480)])
+def test_keys_of_infinite_elements_that_score_minus_infinity_weigh_nothing(new, before, window, heads, kv_heads, hd, dtype):
+    """exp(-inf) is 0, also from key blocks that whole tiles of tokens see, where
+    heads leave rows of a tile over, a last tile has few tokens, and tokens that
+    see nothing (a log sum of minus infinity) have queries of any kind."""
+    rng = np.random.default_rng(heads + hd + len(new) + window)
+    c = Weigh(rng, new, before, heads, kv_heads, hd, page=32, dtype=dtype, window=window)
+    for s, n in enumerate(c.pool.lens_host.tolist()):
+        for row in (0, 5, 40, 299, 300, n - 1):
+            if row < n:
+                c.pool.k[int(c.pool.table_host[s, row // 32]), row % kv_heads, row % 32, 7] = float("inf")
+    c.q[:, 7::hd] = -c.q[:, 7::hd].abs() - 1
+    idle = torch.from_numpy(rng.permutation(c.t)[:c.t // 5]).cuda()
+    c.lse[idle] = -np.inf
+    c.q[idle[0::3]] = float("nan")
+    c.q[idle[1::3]] = float("inf")
+    c.run().check()
