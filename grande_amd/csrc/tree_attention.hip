@@ -2,13 +2,15 @@
 // sequence's new rows, those that their masks name: the kernels of
 // shared_attention.h with MASKED.  Only tiles that hold new rows look at the
 // masks (a word or two a lane, asked for a tile ahead).  Measured, and what bounds it:
-//   12 drafts of 4 to 8 tokens x 4 heads of 256 on 2,000 shared keys (f16): 12.4 us
+//   12 drafts of 4 to 8 tokens x 4 heads of 256 on 2,000 shared keys (f16): 12.5 us
 //     and the join's 4: latency.
-//   208 of 7 to 13 tokens x 8 heads of 256 on 8,000: 195 us and 17 for the slots'
-//     join alone, 192 in a row, 710 TFLOP/s: a wave's chain of product, softmax and
-//     product, two waves a SIMD.
-//   16 trees of 31 to 61 tokens x 32 heads of 128 on 32,749 (bf16): 567 us and 17, 517
-//     in a row, 820 TFLOP/s: vector instructions 50 %, MFMAs 43 % of the SIMDs' cycles.
+//   208 of 7 to 13 tokens x 8 heads of 256 on 8,000: 192 to 201 us a call in a row,
+//     about 700 TFLOP/s (traced one by one 202 and, the slots' join, 17): a wave's
+//     chain of product, softmax and product, two waves a SIMD; MFMAs 39 % and vector
+//     instructions 35 % of the busy SIMDs' cycles, and 396 items on 512 places.
+//   16 trees of 31 to 61 tokens x 32 heads of 128 on 32,749 (bf16): 517 to 542 us a
+//     call in a row, cards differ, 800 TFLOP/s (traced one by one 563 to 612 and 17):
+//     vector instructions 50 %, MFMAs 42 % of the busy SIMDs' cycles.
 #include "shared_attention.h"
 
 namespace omg {

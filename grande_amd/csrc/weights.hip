@@ -20,12 +20,13 @@
 //   64 sequences of 6,100 rows x 8 KV heads of 128 (bf16), one token each: 170 us,
 //     4.9 TB/s: the keys' bytes.
 //   12 sequences of 2,000 rows x 1 KV head of 256 (f16): 5.8 us: latency.
-//   a prompt of 8,000 tokens x 8 heads of 256 on 4 KV heads (f16): 149 us
-//     alone, 140 in a row, 880 to 940 TFLOP/s of the 1,154 that a product of 8,192^3
-//     reaches: the products (at this operand data the chip lowers its clock; the
-//     same MFMAs with nothing else take 130 us).  16 x 16 x 32 products draw less
-//     than 32 x 32 x 16 (from registers alone 2,050 and 1,700 TFLOP/s on random
-//     data): 174 -> 165 us when it was that, at 128-wide heads 160 -> 132.
+//   a prompt of 8,000 tokens x 8 heads of 256 on 4 KV heads (f16): 148 us
+//     and the join's 5 alone, 141 a call in a row, 930 TFLOP/s of the 1,154 that a
+//     product of 8,192^3 reaches: MFMAs 48 % and vector instructions 53 % of the busy
+//     SIMDs' cycles.  On random data the chip lowers its clock, for 16 x 16 x 32
+//     products less than for 32 x 32 x 16 (from registers alone 1,990 and 1,660
+//     TFLOP/s, on zeros both 2,470): 174 -> 165 us when it was that, at 128-wide
+//     heads 160 -> 132.
 #include <algorithm>
 #include <atomic>
 #include <climits>
@@ -510,6 +511,9 @@ void check(const PagedKv& kv, const PagedBatch& b, int heads) {
     if (b.t * heads >= (1 << 26)) fail(E_INVALID, "attention_weights: t * heads must stay below 2^26");
 }
 
+// Few rows a sequence, in the mean: lengths lie on the device.  (A prompt among many
+// single tokens goes with these: 8,000 tokens and 300 single ones x 12 heads of 64 9.0 ms,
+// in a call each 0.12 and 0.18.)
 bool few(const PagedKv& kv, const PagedBatch& b, int heads) { return b.t * (heads / kv.kv_heads) <= 32 * b.nseq; }
 
 int many_keys(int head_dim) { return head_dim == 512 ? 128 : 256; }
@@ -551,8 +555,10 @@ template <typename T, int D>
 void launch_d(hipStream_t s, Args a) {
     const int64_t lists = a.b.nseq * a.kv.kv_heads;
     if (few(a.kv, a.b, a.x.heads)) {
-        // Chunks of 256 keys and more: 64 workgroups a CU are enough.  (512 lists of
-        // 8,192 rows: 32 / 16 / 8 of them 170 / 174 / 185 us.)
+        // Chunks of 64 keys (of 64-wide heads 128) and more: 64 workgroups a CU are
+        // enough.  (512 lists of 8,192 rows in 32 / 16 / 8 chunks 170 / 174 / 185 us.
+        // The table's rows are counted, not the sequences': the same lists in a table
+        // four times as wide, in chunks of 1,024, 476.)
         a.chunk = 4 * (D >= 128 ? 16 : 32);
         while (a.chunk < 4096 && lists * (a.max_len / a.chunk) > 16384) a.chunk *= 2;
         a.blocks = (a.max_len + a.chunk - 1) / a.chunk;

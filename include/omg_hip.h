@@ -470,7 +470,9 @@ int omg_dev_attention_blocks(const omg_paged_kv *kv, const omg_paged_batch *b, i
  * hears from its own key alone, infinite and NaN ones too (a key whose scores
  * hold these may take its tokens again one by one: right, and slower); rows from
  * lens[s] on and on pages outside the pool keep theirs.  ldw at least max_pages * page.
- * Sizes, scale and workspace as there; ldq at most 2^24. */
+ * Sizes, scale and workspace as there; ldq at most 2^24.  The launch is made for
+ * sequences with about alike numbers of tokens: a prompt's call of its own is many
+ * times faster than one with single tokens' sequences. */
 int64_t omg_dev_attention_weights_workspace(const omg_paged_kv *kv, const omg_paged_batch *b, int heads);
 int omg_dev_attention_weights(const omg_paged_kv *kv, const omg_paged_batch *b, int heads, const void *q, int64_t ldq,
                               const float *lse, float scale, int window, float *weights, int64_t ldw, void *workspace,
